@@ -199,7 +199,7 @@ def _eight_bits(x):
     pad = -n % BLOCK
     blocks = torch.cat([x, x.new_zeros((b, pad, d))], 1).view(b, -1, BLOCK, d)
     bits = blocks.abs().amax(2, keepdim=True).view(torch.int32)
-    # amax / scale lies in [64, 127.5): adding half a code's step to the mantissa moves on to the next exponent
+    # amax / scale lies in [63.75, 127.5): half a code's step added to the mantissa carries from 127.5 on
     exponent = torch.clamp(((bits + 0x10000) >> 23) - 6, min=1)
     scale = (exponent << 23).view(torch.float32)
     scale = torch.where(bits < 0x7F800000, scale, torch.full_like(scale, float("nan")))
