@@ -379,6 +379,111 @@ int mm_argmax_rows(const void* x, int64_t rows, int64_t n, int64_t stride, int32
 int mm_pair_scan(const float* a, const float* b, float* a_out, float* h_out, int64_t n,
                  void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Gated linear recurrence, one state a channel (no counterpart in the reference; it stands beside
+ * the selective scan, whose recurrence has dstate states a channel and no gate on its input):
+ *   r = sigmoid(a_gate)   i = sigmoid(x_gate)   a = exp(A[d] * r)
+ *   h_t = a_t * h_{t-1} + sqrt(1 - a_t^2) * i_t * x_t        (h = h0, or 0, before the first token)
+ *   y   = h * (z ? silu(z) : 1)
+ * A (dim,) fp32, <= 0 (a channel with A > 0 gives NaN where 1 - a^2 < 0); -inf is a = 0.
+ * x, a_gate, x_gate, z, y, dy: (batch, seqlen, dim) in dtype, strides of batch and time in elements
+ * (>= 0), unit channel stride.  States (batch, dim) contiguous fp32.  lengths (batch,), int32 or
+ * int64 (lengths_dtype), NULL = all seqlen: tokens from lengths[b] on (taken as clamped to
+ * [0, seqlen]) leave the state as it is, have y = 0 and gradients 0, and their inputs' values do
+ * not matter (they are read).  Arithmetic and states are fp32.  Outputs must not overlap inputs.
+ * seqlen 0: state_out is h0.
+ *
+ * Training: the forward call given block_states writes there the state before every 16th token,
+ * (batch, ceil(seqlen / 16), dim) contiguous fp32, from which the backward call recomputes the
+ * states of a block.  Given codes[k] and exps[k] (k = 0 x, 1 a_gate, 2 x_gate, 3 z; all of the present
+ * inputs or none), it also writes those inputs as 8-bit checkpoints (mm_act8_pack's format, tokens past
+ * a sequence's end as zeros), and the backward call that is given them reads them instead of x, a_gate,
+ * x_gate and z, which may then be NULL (z_present says whether there is a z). */
+#define MM_ACT8_BLOCK 16
+
+typedef struct mm_gated_scan_params {
+  const void* x;
+  const void* a_gate;
+  const void* x_gate;
+  const void* z;              /* NULL = no output gate */
+  const float* A;             /* (dim,) */
+  const float* h0;            /* (batch, dim); NULL = zeros */
+  const void* lengths;        /* (batch,); NULL = seqlen each */
+  void* y;                    /* forward */
+  float* state_out;           /* forward: the state after the last token; NULL = skip */
+  float* block_states;        /* forward: written (NULL = skip); backward: read */
+  int8_t* codes[4];           /* (batch, seqlen, dim) contiguous, or NULL */
+  uint8_t* exps[4];           /* (batch, ceil(seqlen / 16), dim) contiguous, or NULL */
+  const void* dy;             /* backward: gradient of y */
+  const float* dstate;        /* backward: gradient of state_out; NULL = zeros */
+  void* dx;                   /* backward: (batch, seqlen, dim) contiguous, dtype */
+  void* da_gate;
+  void* dx_gate;
+  void* dz;                   /* required where there is a z */
+  float* dA;                  /* (dim,) */
+  float* dh0;                 /* (batch, dim); NULL = skip */
+  void* workspace;            /* 256-byte aligned, no initial contents */
+  size_t workspace_bytes;
+  int64_t batch, seqlen, dim;
+  int64_t x_stride[2], a_gate_stride[2], x_gate_stride[2], z_stride[2], y_stride[2], dy_stride[2];
+  int32_t dtype;
+  int32_t lengths_dtype;      /* 0 int32, 1 int64 */
+  int32_t z_present;          /* backward from codes: the forward call had a z */
+  int32_t handoff_timeout_us; /* bound of a tile's wait for the tiles before it; 0 = 2 s (as mm_scan_params') */
+  int32_t* status;            /* optional: as mm_scan_params.status */
+} mm_gated_scan_params;
+
+/* Workspace bytes of the forward (backward = 0) or backward call; 0 when none is needed. */
+size_t mm_gated_scan_workspace_size(int64_t batch, int64_t seqlen, int64_t dim, int32_t backward);
+int mm_gated_scan_fwd(const mm_gated_scan_params* p, void* stream);
+/* Gradients of x, a_gate, x_gate, z, A and h0 given those of y and state_out.  With
+ * dh_t = dy_t silu(z_t) + a_{t+1} dh_{t+1} (dstate added after the last token), dl = dh (h_{t-1} a -
+ * i x a^2 / sqrt(1 - a^2)) -- the second term taken as 0 where a = 1 --:
+ *   dx = dh sqrt(1-a^2) i   dx_gate = dh sqrt(1-a^2) x i (1-i)   da_gate = dl A r (1-r)
+ *   dz = dy h silu'(z)      dA[d] = sum over batch and time of dl r      dh0 = a_1 dh_1
+ * The sums of dA are taken in a fixed order: calls repeat bit for bit. */
+int mm_gated_scan_bwd(const mm_gated_scan_params* p, void* stream);
+
+/* One token of the recurrence: state_out = a * state + sqrt(1 - a^2) * i * x (state_out may be state),
+ * y = state_out * silu(z).  state, state_out (batch, dim) contiguous fp32; the others (batch, dim) in
+ * dtype with batch strides and unit channel stride; z may be NULL. */
+int mm_gated_scan_step(const float* state, float* state_out, const void* x, const void* a_gate,
+                       const void* x_gate, const float* A, const void* z, void* y, int64_t batch,
+                       int64_t dim, int64_t x_stride_b, int64_t a_gate_stride_b,
+                       int64_t x_gate_stride_b, int64_t z_stride_b, int64_t y_stride_b,
+                       int32_t dtype, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Activations kept in 8 bits: blocks of MM_ACT8_BLOCK = 16 tokens of one channel (the last block of a
+ * sequence may be shorter) as int8 codes in [-127, 127] and one exponent byte e,
+ *   value = code * 2^(e - 127),
+ * with the smallest power of two that keeps |code| <= 127 (1 <= e <= 248), codes rounded to nearest
+ * even.  A block that holds an infinity or a NaN gets e = 255 and stands for NaNs.  x, y (batch, seqlen,
+ * dim) in dtype with strides of batch and time, unit channel stride; codes (batch, seqlen, dim), exps
+ * (batch, ceil(seqlen / 16), dim) contiguous.  Every value is exact in dtype (fp16's 65536 becomes 65504). */
+int mm_act8_pack(const void* x, int8_t* codes, uint8_t* exps, int64_t batch, int64_t seqlen,
+                 int64_t dim, const int64_t x_stride[2], int32_t dtype, void* stream);
+int mm_act8_unpack(const int8_t* codes, const uint8_t* exps, void* y, int64_t batch, int64_t seqlen,
+                   int64_t dim, const int64_t y_stride[2], int32_t dtype, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Backward pass of mm_causal_conv1d_fwd:
+ *   p[b,t,c] = bias[c] + sum_k w[c,k] x[b, t-(width-1)+k, c]     dp = dout * (apply_silu ? silu'(p) : 1)
+ *   dx[b,t,c] = sum_k w[c,k] dp[b, t+(width-1)-k, c]   dw[c,k] = sum_bt dp x[b, t-(width-1)+k, c]
+ *   dbias[c] = sum_bt dp
+ * x (x_dtype, strides (batch, time), unit channel stride) or, with x NULL, its 8-bit checkpoint x_codes
+ * and x_exps; dout in x_dtype, strides (batch, time), unit channel stride; weight (dim, width) with
+ * strides w_stride, bias (dim,) or NULL, in w_dtype.  dx (batch, seqlen, dim) contiguous in x_dtype,
+ * dw (dim, width) contiguous and dbias (dim,) in w_dtype; dx, or dw and dbias, or dbias may be NULL.
+ * Sums are fp32 or wider, in a fixed order.  width <= 8. */
+size_t mm_causal_conv1d_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_t dim, int64_t width);
+int mm_causal_conv1d_bwd(const void* x, const int8_t* x_codes, const uint8_t* x_exps,
+                         const void* weight, const void* bias, const void* dout, void* dx, void* dw,
+                         void* dbias, int64_t batch, int64_t seqlen, int64_t dim, int64_t width,
+                         const int64_t x_stride[2], const int64_t dout_stride[2],
+                         const int64_t w_stride[2], int32_t x_dtype, int32_t w_dtype,
+                         int32_t apply_silu, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,9 @@ include/mamba_mi355x.h); projections use torch GEMMs.  There is no CPU fallback.
 """
 
 from mamba_metal_amd._loader import load_kernel
+from mamba_metal_amd.act8 import Act8, act8_pack, act8_unpack
+from mamba_metal_amd.conv1d import causal_conv1d_train
+from mamba_metal_amd.gated_scan import gated_scan, gated_scan_step
 from mamba_metal_amd.generate import (GraphDecoder, GraphPrefill, generate, generate_fast,
                                       generate_fast_ids)
 from mamba_metal_amd.load_hf import load_mamba_hf
@@ -25,8 +28,14 @@ __all__ = [
     "load_mamba_hf",
     "selective_scan",
     # extensions beyond the reference's API
+    "Act8",
     "GraphDecoder",
     "GraphPrefill",
+    "act8_pack",
+    "act8_unpack",
+    "causal_conv1d_train",
+    "gated_scan",
+    "gated_scan_step",
     "generate_fast_ids",
     "init_weights_",
 ]

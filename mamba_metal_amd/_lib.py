@@ -79,6 +79,25 @@ class LinearParams(ctypes.Structure):
     ]
 
 
+class GatedScanParams(ctypes.Structure):
+    """Mirror of ``mm_gated_scan_params`` (include/mamba_mi355x.h)."""
+
+    _fields_ = [
+        ("x", _vp), ("a_gate", _vp), ("x_gate", _vp), ("z", _vp), ("A", _vp), ("h0", _vp),
+        ("lengths", _vp), ("y", _vp), ("state_out", _vp), ("block_states", _vp),
+        ("codes", _vp * 4), ("exps", _vp * 4), ("dy", _vp), ("dstate", _vp), ("dx", _vp),
+        ("da_gate", _vp), ("dx_gate", _vp), ("dz", _vp), ("dA", _vp), ("dh0", _vp),
+        ("workspace", _vp), ("workspace_bytes", _sz),
+        ("batch", _i64), ("seqlen", _i64), ("dim", _i64),
+        ("x_stride", _i64a2), ("a_gate_stride", _i64a2), ("x_gate_stride", _i64a2),
+        ("z_stride", _i64a2), ("y_stride", _i64a2), ("dy_stride", _i64a2),
+        ("dtype", _i32), ("lengths_dtype", _i32), ("z_present", _i32),
+        ("handoff_timeout_us", _i32), ("status", _vp),
+    ]
+
+
+ACT8_BLOCK = 16   # MM_ACT8_BLOCK
+
 _SIGNATURES = {
     "mm_abi_version": ([], ctypes.c_int),
     "mm_last_error": ([], ctypes.c_char_p),
@@ -112,6 +131,15 @@ _SIGNATURES = {
     "mm_prefill_linear": ([_vp] * 4 + [_i64] * 6 + [_i32, _vp], ctypes.c_int),
     "mm_argmax_rows": ([_vp, _i64, _i64, _i64, _i32, _vp, _vp], ctypes.c_int),
     "mm_pair_scan": ([_vp] * 4 + [_i64, _vp], ctypes.c_int),
+    "mm_gated_scan_workspace_size": ([_i64, _i64, _i64, _i32], _sz),
+    "mm_gated_scan_fwd": ([ctypes.POINTER(GatedScanParams), _vp], ctypes.c_int),
+    "mm_gated_scan_bwd": ([ctypes.POINTER(GatedScanParams), _vp], ctypes.c_int),
+    "mm_gated_scan_step": ([_vp] * 8 + [_i64] * 7 + [_i32, _vp], ctypes.c_int),
+    "mm_act8_pack": ([_vp] * 3 + [_i64] * 3 + [_i64a2, _i32, _vp], ctypes.c_int),
+    "mm_act8_unpack": ([_vp] * 3 + [_i64] * 3 + [_i64a2, _i32, _vp], ctypes.c_int),
+    "mm_causal_conv1d_bwd_workspace_size": ([_i64] * 4, _sz),
+    "mm_causal_conv1d_bwd": (
+        [_vp] * 9 + [_i64] * 4 + [_i64a2, _i64a2, _i64a2, _i32, _i32, _i32, _vp, _sz, _vp], ctypes.c_int),
 }
 
 # Every symbol include/mamba_mi355x.h declares (checked by the CPU ABI tests).

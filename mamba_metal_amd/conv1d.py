@@ -5,13 +5,16 @@
 captures the conv state of mamba_block.py:118-127 in the same pass.
 ``conv_step`` replaces the window shift / dot / bias / SiLU of
 mamba_block.py:170-177, updating the resident conv state in place.
+``causal_conv1d_train`` is ``causal_conv1d`` with gradients (the reference has none).
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from mamba_metal_amd import _lib
+from mamba_metal_amd.act8 import Act8, act8_pack, channels_last
 
 
 def _w2d(weight):
@@ -79,3 +82,73 @@ def conv_step(conv_state, x, weight, bias=None, *, apply_silu=True, out=None):
             1 if apply_silu else 0, _lib.stream_of(dev))
     _lib.check(st, "mm_decode_conv_step")
     return out
+
+
+def _conv1d_backward(x, packed, weight, bias, dout, apply_silu, want_dx, want_dw):
+    """Gradients of x, weight and bias; x as a tensor, or its 8-bit codes in ``packed``."""
+    lib = _lib.load()
+    dev = weight.device
+    batch, seqlen, dim = dout.shape
+    w, ws = _w2d(weight)
+    width = w.shape[1]
+    dx = torch.empty((batch, seqlen, dim), dtype=dout.dtype, device=dev) if want_dx else None
+    dw = torch.empty((dim, width), dtype=w.dtype, device=dev) if want_dw else None
+    db = torch.empty((dim,), dtype=w.dtype, device=dev) if want_dw and bias is not None else None
+    nbytes = lib.mm_causal_conv1d_bwd_workspace_size(batch, seqlen, dim, width) if want_dw else 0
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    two = _lib._i64a2
+    with _lib.on_device(dev):
+        st = lib.mm_causal_conv1d_bwd(
+            _lib.ptr(x), None if packed is None else packed.codes.data_ptr(),
+            None if packed is None else packed.exps.data_ptr(), w.data_ptr(), _lib.ptr(bias), dout.data_ptr(),
+            _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), batch, seqlen, dim, width,
+            two(*x.stride()[:2]) if x is not None else two(0, 0), two(*dout.stride()[:2]), ws,
+            _lib.dtype_code(dout.dtype), _lib.dtype_code(w.dtype), 1 if apply_silu else 0, _lib.ptr(work), nbytes,
+            _lib.stream_of(dev))
+    _lib.check(st, "mm_causal_conv1d_bwd")
+    return dx, None if dw is None else dw.view(weight.shape), db
+
+
+class _CausalConv1d(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, apply_silu, checkpoint):
+        out = causal_conv1d(x, weight, bias, apply_silu=apply_silu)
+        ctx.meta = (x.dtype, x.shape, apply_silu)
+        if checkpoint == "int8":
+            packed = act8_pack(x)
+            ctx.save_for_backward(weight, bias, packed.codes, packed.exps)
+        else:
+            ctx.save_for_backward(weight, bias, x)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        dtype, shape, apply_silu = ctx.meta
+        weight, bias, *kept = ctx.saved_tensors
+        x, packed = (kept[0], None) if len(kept) == 1 else (None, Act8(*kept, shape, dtype))
+        if dout.dtype != dtype or (dout.stride(-1) != 1 and shape[2] > 1):
+            dout = dout.to(dtype).contiguous()
+        need = ctx.needs_input_grad
+        dx, dw, db = _conv1d_backward(x, packed, weight, bias, dout, apply_silu, need[0], need[1] or need[2])
+        return dx, dw, db, None, None
+
+
+def causal_conv1d_train(x, weight, bias=None, *, apply_silu=True, checkpoint="full"):
+    """``causal_conv1d`` with gradients of x, weight and bias.
+
+    x (batch, seqlen, dim) with unit channel stride, weight (dim, 1, width) or (dim, width), width <= 8.
+    ``checkpoint`` says how x is kept for the backward pass: "full", as it is, or "int8", as 8-bit codes
+    (``act8_pack``); the gradients are then those at the values that the codes stand for.  Sums over batch
+    and time are taken in float32 and wider, in a fixed order."""
+    if x.dim() != 3:
+        raise ValueError(f"x must be (batch, seqlen, dim), got {tuple(x.shape)}")
+    channels_last(x, "x")
+    w, _ = _w2d(weight)
+    if w.dim() != 2 or w.shape[0] != x.shape[2] or not 1 <= w.shape[1] <= 8:
+        raise ValueError(f"weight must be ({x.shape[2]}, 1, width) with width 1 to 8, got {tuple(weight.shape)}")
+    if checkpoint not in ("full", "int8"):
+        raise ValueError(f"checkpoint must be 'full' or 'int8', got {checkpoint!r}")
+    _lib.dtype_code(x.dtype)
+    _lib.dtype_code(weight.dtype)
+    return _CausalConv1d.apply(x, weight, bias, apply_silu, checkpoint)
