@@ -412,8 +412,8 @@ typedef struct mm_gated_scan_params {
   void* y;                    /* forward */
   float* state_out;           /* forward: the state after the last token; NULL = skip */
   float* block_states;        /* forward: written (NULL = skip); backward: read */
-  int8_t* codes[4];           /* (batch, seqlen, dim) contiguous, or NULL */
-  uint8_t* exps[4];           /* (batch, ceil(seqlen / 16), dim) contiguous, or NULL */
+  int8_t* codes[4];           /* mm_act8_pack's, or NULL */
+  uint8_t* exps[4];
   const void* dy;             /* backward: gradient of y */
   const float* dstate;        /* backward: gradient of state_out; NULL = zeros */
   void* dx;                   /* backward: (batch, seqlen, dim) contiguous, dtype */
@@ -459,8 +459,9 @@ int mm_gated_scan_step(const float* state, float* state_out, const void* x, cons
  *   value = code * 2^(e - 127),
  * with the smallest power of two that keeps |code| <= 127 (1 <= e <= 248), codes rounded to nearest
  * even.  A block that holds an infinity or a NaN gets e = 255 and stands for NaNs.  x, y (batch, seqlen,
- * dim) in dtype with strides of batch and time, unit channel stride; codes (batch, seqlen, dim), exps
- * (batch, ceil(seqlen / 16), dim) contiguous.  Every value is exact in dtype (fp16's 65536 becomes 65504). */
+ * dim) in dtype with strides of batch and time, unit channel stride; codes (batch, ceil(seqlen / 16), dim, 16)
+ * (zeros past seqlen, 16-byte aligned), exps (batch, ceil(seqlen / 16), dim), both contiguous.  Every value is
+ * exact in dtype (fp16's 65536 becomes 65504). */
 int mm_act8_pack(const void* x, int8_t* codes, uint8_t* exps, int64_t batch, int64_t seqlen,
                  int64_t dim, const int64_t x_stride[2], int32_t dtype, void* stream);
 int mm_act8_unpack(const int8_t* codes, const uint8_t* exps, void* y, int64_t batch, int64_t seqlen,

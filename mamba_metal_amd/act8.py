@@ -23,8 +23,9 @@ BLOCK = _lib.ACT8_BLOCK
 
 @dataclass
 class Act8:
-    """An activation in 8 bits: ``codes`` (batch, seqlen, dim) int8, ``exps`` (batch, ceil(seqlen / 16),
-    dim) uint8, both contiguous, value = codes * 2^(exps - 127); the shape and dtype it had."""
+    """An activation in 8 bits: ``codes`` (batch, ceil(seqlen / 16), dim, 16) int8, a channel's 16 tokens
+    side by side, and ``exps`` (batch, ceil(seqlen / 16), dim) uint8, both contiguous, value =
+    codes * 2^(exps - 127); the shape and dtype it had."""
 
     codes: torch.Tensor
     exps: torch.Tensor
@@ -45,8 +46,9 @@ def channels_last(t, name):
 def empty_like(x, shape=None) -> Act8:
     """Uninitialised codes for x (batch, seqlen, dim)."""
     b, n, d = x.shape
-    return Act8(torch.empty((b, n, d), dtype=torch.int8, device=x.device),
-                torch.empty((b, -(-n // BLOCK), d), dtype=torch.uint8, device=x.device),
+    nblk = -(-n // BLOCK)
+    return Act8(torch.empty((b, nblk, d, BLOCK), dtype=torch.int8, device=x.device),
+                torch.empty((b, nblk, d), dtype=torch.uint8, device=x.device),
                 x.shape if shape is None else shape, x.dtype)
 
 
@@ -75,12 +77,15 @@ def act8_unpack(packed: Act8, dtype: torch.dtype | None = None, out: torch.Tenso
         raise TypeError(f"out is {out.dtype}, not {dtype}")
     dtype = out.dtype if out is not None else dtype or packed.dtype
     code = _lib.dtype_code(dtype)
-    b, n, d = packed.codes.shape
+    if len(packed.shape) not in (2, 3):
+        raise ValueError(f"an activation is (batch, seqlen, dim) or (seqlen, dim), not {tuple(packed.shape)}")
+    b, n, d = packed.shape if len(packed.shape) == 3 else (1, *packed.shape)
+    nblk = -(-n // BLOCK)
     if packed.codes.dtype != torch.int8 or packed.exps.dtype != torch.uint8 \
-            or packed.exps.shape != (b, -(-n // BLOCK), d) \
+            or packed.codes.shape != (b, nblk, d, BLOCK) or packed.exps.shape != (b, nblk, d) \
             or not packed.codes.is_contiguous() or not packed.exps.is_contiguous():
-        raise ValueError("codes must be contiguous int8 (batch, seqlen, dim), exps contiguous uint8 "
-                         "(batch, ceil(seqlen / 16), dim)")
+        raise ValueError("codes must be contiguous int8 (batch, ceil(seqlen / 16), dim, 16), exps contiguous "
+                         "uint8 (batch, ceil(seqlen / 16), dim)")
     if out is not None:
         if out.shape != packed.shape:
             raise ValueError(f"out is {tuple(out.shape)}, the activation {tuple(packed.shape)}")

@@ -21,15 +21,16 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const void* x, int8_t* c
   for (int k = 0; k < kBlk; ++k) {
     const int64_t t = t0 + k < seqlen ? t0 + k : seqlen - 1;
     v[k] = ld<DT>(x, b * xsb + t * xst + d);
-    const uint32_t m = abs_bits(v[k]);
-    top = m > top ? m : top;
+    if (t0 + k >= seqlen) v[k] = 0.0f;
+    top = max(top, abs_bits(v[k]));
   }
   const uint32_t e = exponent_of(top);
   const float inv = inv_scale(e);
   exps[id] = static_cast<uint8_t>(e);
+  uint32_t w[kBlk / 4];
 #pragma unroll
-  for (int k = 0; k < kBlk; ++k)
-    if (t0 + k < seqlen) codes[(b * seqlen + t0 + k) * dim + d] = code_of(v[k], inv);
+  for (int k = 0; k < kBlk; k += 4) w[k / 4] = code4(v[k], v[k + 1], v[k + 2], v[k + 3], inv);
+  *reinterpret_cast<uint4*>(codes + id * kBlk) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <int DT>
@@ -41,15 +42,10 @@ __global__ __launch_bounds__(kThreads) void unpack_kernel(const int8_t* codes, c
   if (id >= total) return;
   const int64_t d = id % dim, row = id / dim, b = row / nblk, t0 = row % nblk * kBlk;
   const float scale = scale_of(exps[id]);
-  int8_t c[kBlk];
+  const uint4 w = *reinterpret_cast<const uint4*>(codes + id * kBlk);
 #pragma unroll
   for (int k = 0; k < kBlk; ++k) {
-    const int64_t t = t0 + k < seqlen ? t0 + k : seqlen - 1;
-    c[k] = codes[(b * seqlen + t) * dim + d];
-  }
-#pragma unroll
-  for (int k = 0; k < kBlk; ++k) {
-    float v = static_cast<float>(c[k]) * scale;
+    float v = value_of(w, k, scale);
     // fp16's largest numbers round to a code that stands for 65536
     if (DT == MM_F16 && fabsf(v) == 65536.0f) v = v < 0.0f ? -65504.0f : 65504.0f;
     if (t0 + k < seqlen) st<DT>(y, b * ysb + (t0 + k) * yst + d, v);
@@ -63,8 +59,9 @@ static int check(const void* x, const void* codes, const void* exps, int64_t bat
   if (batch == 0 || seqlen == 0 || dim == 0) return MM_OK;
   if (!x || !codes || !exps || !stride)
     return fail(MM_ERR_NULL_POINTER, "the tensor, its strides, codes and exps are required");
+  if (!aligned(codes, kBlk)) return fail(MM_ERR_LAYOUT, "codes are not 16-byte aligned");
   if (stride[0] < 0 || stride[1] < 0) return fail(MM_ERR_LAYOUT, "negative stride");
-  if (ceil_div(seqlen, kBlk) > INT64_MAX / batch / dim ||
+  if (ceil_div(seqlen, kBlk) > INT64_MAX / kBlk / 4 / batch / dim ||
       ceil_div(batch * ceil_div(seqlen, kBlk) * dim, kThreads) > 0x7fffffff)
     return fail(MM_ERR_SHAPE, "too many blocks");
   return MM_OK;

@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "act8.h"
+#include "reduce_rows.h"
 
 namespace mm {
 namespace convb {
@@ -32,6 +33,7 @@ struct Params {
   int32_t w_dtype, silu;
 };
 
+__device__ __forceinline__ int64_t round_up_dev(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 __device__ __forceinline__ float ld_any(const void* p, int64_t i, int32_t dt) {
   return dt == MM_F32 ? ld<MM_F32>(p, i) : dt == MM_F16 ? ld<MM_F16>(p, i) : ld<MM_BF16>(p, i);
 }
@@ -43,62 +45,95 @@ __device__ __forceinline__ void st_any(void* p, int64_t i, float v, int32_t dt) 
 
 template <int DT, int K, bool C8>
 __global__ __launch_bounds__(kThreads) void conv1d_bwd_kernel(const Params p) {
-  const int64_t d = static_cast<int64_t>(blockIdx.x % p.ncb) * kThreads + threadIdx.x;
+  using T = typename Ty<DT>::T;
+  constexpr int kB = act8::kBlk, H = K - 1;  // tokens loaded at once; history
+  const uint32_t d = (blockIdx.x % p.ncb) * 64 + (threadIdx.x & 63);
   if (d >= p.dim) return;
   const int64_t row = blockIdx.x / p.ncb;  // of all sequences' runs
   const int64_t b = row / p.nruns, t0 = row % p.nruns * kRun;
   const int64_t t1 = t0 + kRun < p.seqlen ? t0 + kRun : p.seqlen;
-  const int64_t nblk = (p.seqlen + act8::kBlk - 1) / act8::kBlk;
-  float w[K], dw[K], xw[K], dpw[K];  // xw[k] = x[t - (K-1) + k], dpw likewise
+  const int64_t nblk = (p.seqlen + kB - 1) / kB;
+  const T* const xb = static_cast<const T*>(p.x) + b * p.xs0;
+  const T* const yb = static_cast<const T*>(p.dout) + b * p.ds0;
+  T* const dxb = static_cast<T*>(p.dx) + b * p.seqlen * p.dim;
+  float w[K], dw[K];
   const float bias = p.bias ? ld_any(p.bias, d, p.w_dtype) : 0.0f;
   float db = 0.0f;
-  float scale = 0.0f;
-  auto load_x = [&](int64_t t) __attribute__((always_inline)) {  // 0 <= t < seqlen
-    if constexpr (C8) {
-      scale = act8::scale_of(p.exps[(b * nblk + t / act8::kBlk) * p.dim + d]);
-      return scale * static_cast<float>(p.codes[(b * p.seqlen + t) * p.dim + d]);
-    } else {
-      return ld<DT>(p.x, b * p.xs0 + t * p.xs1 + d);
-    }
-  };
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     w[k] = ld_any(p.w, d * p.ws0 + k * p.ws1, p.w_dtype);
     dw[k] = 0.0f;
-    dpw[k] = 0.0f;
-    const int64_t t = t0 - K + k;  // the window before the first token
-    xw[k] = t >= 0 ? load_x(t) : 0.0f;
   }
-  for (int64_t t = t0; t < t1 + K - 1; ++t) {
+  // x[t0 + k], k < n, of the 16 tokens from t0 on (a block's); tokens past the sequence read its last one
+  auto load_x = [&](float* x, int64_t t0, int k0, int n) __attribute__((always_inline)) {
+    if constexpr (C8) {
+      const int64_t o = (b * nblk + t0 / kB) * p.dim + d;
+      const uint4 q = *reinterpret_cast<const uint4*>(p.codes + o * kB);
+      const float scale = act8::scale_of(p.exps[o]);
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) {
-      xw[k] = xw[k + 1];
-      dpw[k] = dpw[k + 1];
-    }
-    float dp = 0.0f;
-    if (t < p.seqlen) {
-      xw[K - 1] = load_x(t);
-      dp = ld<DT>(p.dout, b * p.ds0 + t * p.ds1 + d);
-      if (p.silu) {
-        float v = bias;
+      for (int k = 0; k < n; ++k) x[k] = act8::value_of(q, k0 + k, scale);
+    } else {
 #pragma unroll
-        for (int k = 0; k < K; ++k) v = __builtin_fmaf(w[k], xw[k], v);
-        const float s = rcp_hw(1.0f + exp2_hw(-v * kLog2e));
-        dp *= s * __builtin_fmaf(v, 1.0f - s, 1.0f);
+      for (int k = 0; k < n; ++k) {
+        const int64_t t = t0 + k0 + k;
+        x[k] = Ty<DT>::f(xb[(t < p.seqlen ? t : p.seqlen - 1) * p.xs1 + d]);
       }
     }
-    dpw[K - 1] = dp;
-    if (t < t1) {
-      db += dp;
+  };
+  auto slope = [&](float v) __attribute__((always_inline)) {  // silu'
+    const float s = rcp_hw(1.0f + exp2_hw(-v * kLog2e));
+    return s * __builtin_fmaf(v, 1.0f - s, 1.0f);
+  };
+  float x[H + kB], dp[H + kB];  // tokens t - H .. t + 15
 #pragma unroll
-      for (int k = 0; k < K; ++k) dw[k] = __builtin_fmaf(dp, xw[k], dw[k]);
+  for (int k = 0; k < H; ++k) x[k] = dp[k] = 0.0f;
+  if (H > 0 && t0 > 0) load_x(x, t0 - kB, kB - H, H);
+  // tokens t + k0, k0 < n: p, dp, the sums (`own` tokens only) and dx of H tokens earlier
+  auto tokens = [&](int64_t t, auto n_c, auto own_c) __attribute__((always_inline)) {
+    constexpr int n = decltype(n_c)::value;
+    constexpr bool own = decltype(own_c)::value;
+    float dy[n];
+#pragma unroll
+    for (int k = 0; k < n; ++k) dy[k] = Ty<DT>::f(yb[(t + k < p.seqlen ? t + k : p.seqlen - 1) * p.ds1 + d]);
+    load_x(x + H, t, 0, n);
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      float v = bias;
+#pragma unroll
+      for (int q = 0; q < K; ++q) v = __builtin_fmaf(w[q], x[k + q], v);
+      const float s = p.silu ? slope(v) : 1.0f;
+      dp[H + k] = t + k < p.seqlen ? dy[k] * s : 0.0f;
+      if constexpr (own) {
+        db += dp[H + k];
+#pragma unroll
+        for (int q = 0; q < K; ++q) dw[q] = __builtin_fmaf(dp[H + k], t + k < p.seqlen ? x[k + q] : 0.0f, dw[q]);
+      }
+      const int64_t o = t + k - H;
+      if (p.dx != nullptr && o >= t0 && o < t1) {
+        float u = 0.0f;
+#pragma unroll
+        for (int q = 0; q < K; ++q) u = __builtin_fmaf(w[q], dp[H + k - q], u);
+        dxb[o * p.dim + d] = Ty<DT>::from(u);
+      }
     }
-    const int64_t o = t - (K - 1);
-    if (p.dx != nullptr && o >= t0) {
-      float v = 0.0f;
 #pragma unroll
-      for (int k = 0; k < K; ++k) v = __builtin_fmaf(w[k], dpw[K - 1 - k], v);
-      st<DT>(p.dx, (b * p.seqlen + o) * p.dim + d, v);
+    for (int k = 0; k < H; ++k) x[k] = x[n + k], dp[k] = dp[n + k];
+  };
+  for (int64_t t = t0; t < t1; t += kB) tokens(t, std::integral_constant<int, kB>{}, std::true_type{});
+  // the last H tokens' dx: up to H tokens of the next run, or zeros
+  if constexpr (H > 0) {
+    const int64_t end = round_up_dev(t1, kB);
+    if (end < p.seqlen) {
+      tokens(end, std::integral_constant<int, H>{}, std::false_type{});
+    } else if (p.dx != nullptr) {
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        const int64_t o = end + k - H;
+        float u = 0.0f;
+#pragma unroll
+        for (int q = k + 1; q < K; ++q) u = __builtin_fmaf(w[q], dp[H + k - q], u);
+        if (o >= t0 && o < t1) dxb[o * p.dim + d] = Ty<DT>::from(u);
+      }
     }
   }
   if (p.part != nullptr) {
@@ -109,27 +144,14 @@ __global__ __launch_bounds__(kThreads) void conv1d_bwd_kernel(const Params p) {
   }
 }
 
-// dw[c, k] and dbias[c] from the runs' sums: 64 columns of [K + 1][dim] by 4 row groups a workgroup.
-constexpr int kGroups = 4;
-__global__ __launch_bounds__(64 * kGroups) void reduce_kernel(const float* part, void* dw, void* dbias, int64_t rows,
-                                                              int64_t dim, int width, int32_t w_dtype) {
-  __shared__ double s_part[kGroups][64];
-  const int64_t cols = (width + 1) * dim, c = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 63);
-  const int g = threadIdx.x >> 6;
-  double s = 0.0;
-  if (c < cols)
-    for (int64_t r = g; r < rows; r += kGroups) s += part[r * cols + c];
-  s_part[g][threadIdx.x & 63] = s;
-  __syncthreads();
-  if (g != 0 || c >= cols) return;
-#pragma unroll
-  for (int k = 1; k < kGroups; ++k) s += s_part[k][threadIdx.x & 63];
-  const int64_t k = c / dim, d = c % dim;
-  if (k == width) {
-    if (dbias != nullptr) st_any(dbias, d, static_cast<float>(s), w_dtype);
-  } else {
-    st_any(dw, d * width + k, static_cast<float>(s), w_dtype);
-  }
+// dw[c, k] and dbias[c] from the runs' sums, rows of [K + 1][dim].
+__global__ __launch_bounds__(64 * rows::kGroups) void reduce_kernel(const float* part, void* dw, void* dbias, int64_t nrows,
+                                                                  int64_t dim, int width, int32_t w_dtype) {
+  rows::sum_columns(part, nrows, (width + 1) * dim, nrows, [&](int64_t c, double s) {
+    const int64_t k = c / dim, d = c % dim;
+    if (k < width) st_any(dw, d * width + k, static_cast<float>(s), w_dtype);
+    else if (dbias != nullptr) st_any(dbias, d, static_cast<float>(s), w_dtype);
+  });
 }
 
 static bool sizes_ok(int64_t batch, int64_t seqlen, int64_t dim) {
@@ -146,7 +168,7 @@ size_t mm_causal_conv1d_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_
   using namespace mm;
   using namespace mm::convb;
   if (!sizes_ok(batch, seqlen, dim) || width < 1 || width > kMaxW) return 0;
-  return static_cast<size_t>(batch * ceil_div(seqlen, kRun) * (width + 1) * dim * 4);
+  return static_cast<size_t>(rows::floats(batch * ceil_div(seqlen, kRun), (width + 1) * dim) * 4);
 }
 
 int mm_causal_conv1d_bwd(const void* x, const int8_t* x_codes, const uint8_t* x_exps,
@@ -163,7 +185,7 @@ int mm_causal_conv1d_bwd(const void* x, const int8_t* x_codes, const uint8_t* x_
   if (!sizes_ok(batch, seqlen, dim)) return fail(MM_ERR_SHAPE, "too many elements");
   if (!valid_dtype(x_dtype) || !valid_dtype(w_dtype)) return fail(MM_ERR_DTYPE, "bad dtype");
   const bool c8 = x == nullptr;
-  const int64_t nruns = ceil_div(seqlen, kRun), rows = batch * nruns;
+  const int64_t nruns = ceil_div(seqlen, kRun), nrun_rows = batch * nruns;
   if (batch > 0 && seqlen > 0 && dim > 0) {
     if (c8 ? !x_codes || !x_exps : !x_stride)
       return fail(MM_ERR_NULL_POINTER, "x and its strides, or x_codes and x_exps, are required");
@@ -173,15 +195,16 @@ int mm_causal_conv1d_bwd(const void* x, const int8_t* x_codes, const uint8_t* x_
         w_stride[0] < 0 || w_stride[1] < 0)
       return fail(MM_ERR_LAYOUT, "negative stride");
   }
-  if (rows > 0x7fffffff / ceil_div(dim > 0 ? dim : 1, kThreads)) return fail(MM_ERR_SHAPE, "too many elements");
+  if (nrun_rows > 0x7fffffff / ceil_div(dim > 0 ? dim : 1, kThreads)) return fail(MM_ERR_SHAPE, "too many elements");
   if (dbias && !dw) return fail(MM_ERR_NULL_POINTER, "dbias needs dw");
   if (dim == 0 || (!dx && !dw)) return MM_OK;
   const size_t need = dw ? mm_causal_conv1d_bwd_workspace_size(batch, seqlen, dim, width) : 0;
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(MM_ERR_WORKSPACE, "workspace of %zu bytes needed", need);
+  if (c8 && !aligned(x_codes, act8::kBlk)) return fail(MM_ERR_LAYOUT, "x_codes are not 16-byte aligned");
   if (need > 0 && !aligned(workspace, 256)) return fail(MM_ERR_WORKSPACE, "workspace is not 256-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (rows > 0) {
+  if (nrun_rows > 0) {
     Params p{};
     p.x = x;
     p.codes = x_codes;
@@ -200,7 +223,7 @@ int mm_causal_conv1d_bwd(const void* x, const int8_t* x_codes, const uint8_t* x_
     p.w_dtype = w_dtype;
     p.silu = apply_silu != 0;
     p.ncb = static_cast<uint32_t>(ceil_div(dim, kThreads));
-    const dim3 grid(static_cast<unsigned>(p.ncb * rows));
+    const dim3 grid(static_cast<unsigned>(p.ncb * nrun_rows));
 #define MM_CB1(D, K, C) hipLaunchKernelGGL((conv1d_bwd_kernel<D, K, C>), grid, dim3(kThreads), 0, s, p)
 #define MM_CB2(D, K) \
   if (c8) MM_CB1(D, K, true); else MM_CB1(D, K, false); break
@@ -227,9 +250,11 @@ int mm_causal_conv1d_bwd(const void* x, const int8_t* x_codes, const uint8_t* x_
     if (e != MM_OK) return e;
   }
   if (!dw) return MM_OK;
-  const int64_t blocks = ceil_div((width + 1) * dim, 64);
-  hipLaunchKernelGGL(reduce_kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kGroups), 0, s,
-                     static_cast<const float*>(workspace), dw, dbias, rows, dim, static_cast<int>(width), w_dtype);
+  const int64_t cols = (width + 1) * dim;
+  int64_t nrows = nrun_rows;
+  const float* part = rows::reduce_first(static_cast<float*>(workspace), nrows, cols, s);
+  hipLaunchKernelGGL(reduce_kernel, dim3(static_cast<unsigned>(ceil_div(cols, 64))), dim3(64 * rows::kGroups), 0, s, part, dw,
+                     dbias, nrows, dim, static_cast<int>(width), w_dtype);
   return check_launch("causal_conv1d_bwd_reduce");
 }
 

@@ -33,7 +33,10 @@ def test_values(dev, dtype, shape):
     packed = act8_pack(x)
     got = check(x, packed)
     finite = torch.isfinite(x).cpu()
-    assert packed.codes.abs().max() <= 127 and packed.codes.shape == shape
+    b, n, d = shape
+    assert packed.codes.abs().max() <= 127 and packed.codes.shape == (b, -(-n // 16), d, 16)
+    if n % 16:  # past the sequence
+        assert not packed.codes[:, -1, :, n % 16:].any()
     # half a step of the block's power of two; the largest magnitude is at least 63.75 steps (127.5 of the next
     # smaller power of two, which it no longer fits), so half a step is at most 1/127.5 of it
     err = (got.cpu().double() - x.cpu().double()).abs()
@@ -78,7 +81,7 @@ def test_shapes_and_strides(dev):
     act8_unpack(packed, out=out[:, 5:55, 50:250])
     assert torch.equal(out[:, 5:55, 50:250], act8_unpack(packed, torch.float32))
     assert not out[:, :5].any() and not out[:, 55:].any() and not out[..., :50].any() and not out[..., 250:].any()
-    assert packed.nbytes == 3 * 50 * 200 + 3 * 4 * 200
+    assert packed.nbytes == 3 * 4 * 200 * 17
 
 
 @pytest.mark.parametrize("shape", [(0, 5, 4), (2, 0, 4), (2, 5, 0)])

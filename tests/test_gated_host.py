@@ -79,11 +79,14 @@ def test_act8_refuses():
                    (z3(3, 2).t(), ValueError), (z3(2, 3), ValueError)):
         with pytest.raises(err):
             act8_pack(x)
-    codes, exps = torch.zeros((1, 20, 3), dtype=torch.int8), torch.zeros((1, 2, 3), dtype=torch.uint8)
-    good = Act8(codes, exps, codes.shape, torch.float32)
-    for packed, kw, err in ((Act8(codes, exps[:, :1], codes.shape, torch.float32), {}, ValueError),
-                            (Act8(codes.float(), exps, codes.shape, torch.float32), {}, ValueError),
-                            (Act8(codes, exps.char(), codes.shape, torch.float32), {}, ValueError),
+    codes, exps = torch.zeros((1, 2, 3, 16), dtype=torch.int8), torch.zeros((1, 2, 3), dtype=torch.uint8)
+    shape = torch.Size((1, 20, 3))
+    good = Act8(codes, exps, shape, torch.float32)
+    for packed, kw, err in ((Act8(codes, exps[:, :1], shape, torch.float32), {}, ValueError),
+                            (Act8(codes, exps, torch.Size((1, 40, 3)), torch.float32), {}, ValueError),
+                            (Act8(codes, exps, torch.Size((20,)), torch.float32), {}, ValueError),
+                            (Act8(codes.float(), exps, shape, torch.float32), {}, ValueError),
+                            (Act8(codes, exps.char(), shape, torch.float32), {}, ValueError),
                             (good, dict(dtype=torch.int8), TypeError),
                             (good, dict(out=z3(1, 20, 4)), ValueError),
                             (good, dict(out=z3(1, 3, 20).transpose(1, 2)), ValueError),
