@@ -32,22 +32,57 @@ __device__ __forceinline__ float inv_scale(uint32_t e) {
 __device__ __forceinline__ float scale_of(uint32_t e) {
   return e == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(e << 23);
 }
-__device__ __forceinline__ int code_of(float x, float inv) {
-  float q = __builtin_rintf(x * inv);
-  q = fminf(fmaxf(q, -127.0f), 127.0f);  // (a NaN, in a block of them, gives -127: any code will do)
-  return static_cast<int>(q);
+
+// Codes of a lane's 16 values, the first in the lowest byte, and their exponent byte.  x / scale + 1.5 * 2^23 in
+// one multiply-add is rounded to a whole number, ties to even, and has the code in its lowest byte.  (Only the
+// largest exponent leaves room for a code of 128: there values are cut to 127 first.)
+__device__ __forceinline__ uint4 pack16(const float (&v)[kBlk], uint32_t& e) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < kBlk; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+  e = exponent_of(top);
+  const float inv = inv_scale(e);
+  uint32_t w[kBlk / 4];
+  auto codes = [&](auto value) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < kBlk; k += 4) {
+      uint32_t c[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) c[q] = __float_as_uint(__builtin_fmaf(value(v[k + q]), inv, 12582912.0f));
+      // bytes 0 of two words: select 0 is the second operand's lowest byte, 4 the first's, 0xc zero
+      const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u);
+      w[k / 4] = lo | hi << 16;
+    }
+  };
+  if (__any(e == 248u)) {
+    const float most = 127.0f * __uint_as_float(248u << 23);
+    codes([&](float x) __attribute__((always_inline)) { return e == 248u ? fminf(fmaxf(x, -most), most) : x; });
+  } else {
+    codes([](float x) __attribute__((always_inline)) { return x; });
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// Codes of four values, the first in the lowest byte.
-__device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, float inv) {
-  return (static_cast<uint32_t>(code_of(a, inv)) & 0xffu) | (static_cast<uint32_t>(code_of(b, inv)) & 0xffu) << 8 |
-         (static_cast<uint32_t>(code_of(c, inv)) & 0xffu) << 16 | static_cast<uint32_t>(code_of(d, inv)) << 24;
-}
-// Value k of a block's 16 codes.
-__device__ __forceinline__ float value_of(const uint4& w, int k, float scale) {
-  const uint32_t v = k < 4 ? w.x : k < 8 ? w.y : k < 12 ? w.z : w.w;
-  return static_cast<float>(static_cast<int8_t>(v >> (8 * (k % 4)))) * scale;
-}
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// A lane's block of 16 codes: loaded, prepared once, read value by value.
+struct Block {
+  uint4 w;
+  uint32_t e;
+  float scale;
+  // codes and exps of a row of blocks (wave-uniform), the lane's channel
+  __device__ __forceinline__ void load(const int8_t* codes, const uint8_t* exps, uint32_t d) {
+    w = *reinterpret_cast<const uint4*>(codes + static_cast<uint64_t>(d) * kBlk);
+    e = exps[d];
+  }
+  // code + 128 as unsigned bytes, which convert to float in one instruction
+  __device__ __forceinline__ void prepare() {
+    w.x ^= 0x80808080u, w.y ^= 0x80808080u, w.z ^= 0x80808080u, w.w ^= 0x80808080u;
+    scale = scale_of(e);
+  }
+  __device__ __forceinline__ float value(int k) const {
+    const uint32_t v = k < 4 ? w.x : k < 8 ? w.y : k < 12 ? w.z : w.w;
+    return (static_cast<float>((v >> (8 * (k % 4))) & 0xffu) - 128.0f) * scale;
+  }
+};
 
 }  // namespace act8
 }  // namespace mm

@@ -16,21 +16,15 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const void* x, int8_t* c
   if (id >= total) return;
   const int64_t d = id % dim, row = id / dim, b = row / nblk, t0 = row % nblk * kBlk;
   float v[kBlk];
-  uint32_t top = 0;
 #pragma unroll
   for (int k = 0; k < kBlk; ++k) {
     const int64_t t = t0 + k < seqlen ? t0 + k : seqlen - 1;
     v[k] = ld<DT>(x, b * xsb + t * xst + d);
     if (t0 + k >= seqlen) v[k] = 0.0f;
-    top = max(top, abs_bits(v[k]));
   }
-  const uint32_t e = exponent_of(top);
-  const float inv = inv_scale(e);
+  uint32_t e;
+  *reinterpret_cast<uint4*>(codes + id * kBlk) = pack16(v, e);
   exps[id] = static_cast<uint8_t>(e);
-  uint32_t w[kBlk / 4];
-#pragma unroll
-  for (int k = 0; k < kBlk; k += 4) w[k / 4] = code4(v[k], v[k + 1], v[k + 2], v[k + 3], inv);
-  *reinterpret_cast<uint4*>(codes + id * kBlk) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <int DT>
@@ -41,11 +35,12 @@ __global__ __launch_bounds__(kThreads) void unpack_kernel(const int8_t* codes, c
   const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (id >= total) return;
   const int64_t d = id % dim, row = id / dim, b = row / nblk, t0 = row % nblk * kBlk;
-  const float scale = scale_of(exps[id]);
-  const uint4 w = *reinterpret_cast<const uint4*>(codes + id * kBlk);
+  Block w;
+  w.load(codes + (id - d) * kBlk, exps + (id - d), static_cast<uint32_t>(d));
+  w.prepare();
 #pragma unroll
   for (int k = 0; k < kBlk; ++k) {
-    float v = value_of(w, k, scale);
+    float v = w.value(k);
     // fp16's largest numbers round to a code that stands for 65536
     if (DT == MM_F16 && fabsf(v) == 65536.0f) v = v < 0.0f ? -65504.0f : 65504.0f;
     if (t0 + k < seqlen) st<DT>(y, b * ysb + (t0 + k) * yst + d, v);

@@ -67,11 +67,12 @@ __global__ __launch_bounds__(kThreads) void conv1d_bwd_kernel(const Params p) {
   // x[t0 + k], k < n, of the 16 tokens from t0 on (a block's); tokens past the sequence read its last one
   auto load_x = [&](float* x, int64_t t0, int k0, int n) __attribute__((always_inline)) {
     if constexpr (C8) {
-      const int64_t o = (b * nblk + t0 / kB) * p.dim + d;
-      const uint4 q = *reinterpret_cast<const uint4*>(p.codes + o * kB);
-      const float scale = act8::scale_of(p.exps[o]);
+      const int64_t o = (b * nblk + t0 / kB) * p.dim;
+      act8::Block q;
+      q.load(p.codes + o * kB, p.exps + o, d);
+      q.prepare();
 #pragma unroll
-      for (int k = 0; k < n; ++k) x[k] = act8::value_of(q, k0 + k, scale);
+      for (int k = 0; k < n; ++k) x[k] = q.value(k0 + k);
     } else {
 #pragma unroll
       for (int k = 0; k < n; ++k) {

@@ -2,16 +2,16 @@
 //
 //   r = sigmoid(a_gate)  i = sigmoid(x_gate)  a = exp(A r)  h_t = a h_{t-1} + sqrt(1 - a^2) i x
 //
-// One pass over the data, whatever the shape.  A workgroup takes a tile of W x 16 tokens by 64 C channels
-// (lane = C channels, wave = 16 tokens): it loads all of the tile at once, turns it into the pairs (a, b)
+// One pass over the data, whatever the shape.  A workgroup takes a tile of W x 16 tokens by 64 channels
+// (lane = channel, wave = 16 tokens): it loads all of the tile at once, turns it into the pairs (a, b)
 // of h = a h + b in registers, composes them to one pair a wave and, through LDS, one pair (P, Q) a tile and
 // channel, gets the state h before its first token, and runs the recurrence again from there to the outputs:
 // two multiply-adds a token and channel for time in parallel.  The state comes from the tiles before it in
 // the same channels: a tile publishes (P, Q) as soon as it has them and its last state as soon as it
 // knows it; a tile waits for the nearest kWindow - 1 tiles' pairs or states and the next one's state and
 // folds them, first tile first.  The state after tile k is P_k h + Q_k by the same operation for whoever
-// folds it, so results do not depend on who was there first.  Tiles are claimed from a counter, in order of
-// time, so that what a tile waits for is always running or done.
+// folds it, so results do not depend on who was there first.  Workgroups claim the tiles of their strip of
+// channels from its counter, in order of time, so that what a tile waits for is always running or done.
 //
 // The backward pass is the same in reverse: dh_t = g_t + c, c <- a_t dh_t, with each wave's 16 states
 // recomputed from the stored state before its first token.
@@ -28,21 +28,31 @@ constexpr int kMaxWaves = 16;        // of a forward tile
 constexpr int kMaxWavesBwd = 8;      // of a backward tile
 constexpr int kWindow = 16;          // tiles that a tile looks back at
 constexpr int kStepThreads = 64;
+#ifndef BWD_EU
+#define BWD_EU 4
+#endif
+
 
 __device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp2_hw(-x * kLog2e)); }
 // a = exp(l) and beta^2 = 1 - a^2 for l = A r <= 0.  Next to a = 1 both come from q = 1 - a, taken from its
-// series -l (1 + l/2 + l^2/6 + ... + l^5/720) (the first dropped term is 5e-8 of q at l = -1/4): 1 - a^2 keeps
-// its precision, and a's rounding leans to no side, where the hardware exponential's would add up over the
-// thousands of tokens that such a channel remembers.  Below, q >= 0.22 is 1 - a to a few 1e-7.
+// series -l (1 + l/2 + l^2/6 + ...): 1 - a^2 keeps its precision, and a's rounding leans to no side, where the
+// hardware exponential's would add up over the thousands of tokens that such a channel remembers.  fp32: from
+// l = -1/4 on, to l^5/720 (the first dropped term is 5e-8 of q there; below, 1 - a is good to a few 1e-7).
+// 16-bit types: from l = -1/16 on, to l^3/24 (1e-7; below, 1 - a is good to 2e-6, a thousandth of their half
+// step), two multiply-adds less.
+template <int DT>
 __device__ __forceinline__ void decay(float l, float& a, float& beta2) {
-  float s = 1.0f / 720.0f;
-  s = __builtin_fmaf(s, l, 1.0f / 120.0f);
-  s = __builtin_fmaf(s, l, 1.0f / 24.0f);
+  constexpr bool wide = DT == MM_F32;
+  float s = wide ? 1.0f / 720.0f : 1.0f / 24.0f;
+  if constexpr (wide) {
+    s = __builtin_fmaf(s, l, 1.0f / 120.0f);
+    s = __builtin_fmaf(s, l, 1.0f / 24.0f);
+  }
   s = __builtin_fmaf(s, l, 1.0f / 6.0f);
   s = __builtin_fmaf(s, l, 0.5f);
   s = __builtin_fmaf(s, l, 1.0f);
   const float e = exp2_hw(l * kLog2e);
-  const bool near = l > -0.25f;
+  const bool near = l > (wide ? -0.25f : -0.0625f);
   const float q = near ? -l * s : 1.0f - e;
   a = near ? 1.0f - q : e;
   beta2 = q * (1.0f + a);
@@ -58,34 +68,61 @@ __device__ __forceinline__ int64_t length_of(const mm_gated_scan_params& p, int6
 }
 
 
-// ------------------------------------------------------------------------------ C neighbouring channels
-template <int DT, int C>
-struct Ch {
+// ------------------------------------------------------------------------------ memory
+// Rows of a tensor: a wave-uniform address that moves on by a row, and a lane's 32-bit offset into it (dim is at
+// most 2^30, an element at most 4 bytes), so that an access takes no vector address arithmetic.
+template <int DT>
+struct Rows {
   using T = typename Ty<DT>::T;
-  typedef T V __attribute__((ext_vector_type(C)));
-  __device__ static __forceinline__ V load(const T* p) { return *reinterpret_cast<const V*>(p); }
-  __device__ static __forceinline__ void store(T* p, const float (&v)[C]) {
-    V o;
-#pragma unroll
-    for (int c = 0; c < C; ++c) o[c] = cvt<DT>(v[c]);
-    *reinterpret_cast<V*>(p) = o;
-  }
-  template <int D>
-  __device__ static __forceinline__ T cvt(float x) {
-    if constexpr (D == MM_BF16) return __builtin_bit_cast(unsigned short, static_cast<__bf16>(x));  // v_cvt_pk_bf16_f32
-    else return Ty<DT>::from(x);
+  typedef __attribute__((address_space(1))) char Byte;  // (the asm below would lose that it is global memory)
+  typedef __attribute__((address_space(1))) T Elem;
+  Byte* p;
+  int64_t step;  // bytes
+  __device__ __forceinline__ Rows(const void* base, const int64_t* stride, int64_t b, int64_t t)
+      : p((Byte*)const_cast<void*>(base) + (b * stride[0] + t * stride[1]) * static_cast<int64_t>(sizeof(T))),
+        step(stride[1] * static_cast<int64_t>(sizeof(T))) {}
+  __device__ __forceinline__ Rows(void* base, int64_t row, int64_t dim)  // contiguous
+      : p((Byte*)base + row * dim * static_cast<int64_t>(sizeof(T))),
+        step(dim * static_cast<int64_t>(sizeof(T))) {}
+  __device__ __forceinline__ T load(uint32_t off) const { return *(const Elem*)(p + off); }
+  __device__ __forceinline__ void store(uint32_t off, T v) const { *(Elem*)(p + off) = v; }
+  __device__ __forceinline__ void next(bool more = true) {
+    p += more ? step : 0;
+    // a running address, not a product a row, and no more than one ahead of its access: SGPRs are few
+    asm("" : "+s"(p));
+    __builtin_amdgcn_sched_barrier(0);
   }
 };
 
+// Takes v as computed here: the compiler otherwise moves what only the outputs need past the wait, and holds its
+// several operands in registers over it instead (backward pass: 240 registers, or 180 spilled ones).
+__device__ __forceinline__ void keep(float& v) { asm volatile("" : "+v"(v)); }
+
+// Two tokens' outputs, rounded to nearest even (bf16: one v_cvt_pk_bf16_f32 for both).
+template <int DT>
+__device__ __forceinline__ void round2(float x, float y, typename Ty<DT>::T& a, typename Ty<DT>::T& b) {
+  if constexpr (DT == MM_BF16) {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const uint32_t v = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), bf2));
+    a = static_cast<unsigned short>(v);
+    b = static_cast<unsigned short>(v >> 16);
+  } else {
+    a = Ty<DT>::from(x);
+    b = Ty<DT>::from(y);
+  }
+}
+
 // ------------------------------------------------------------------------------ the tiles' hand-off
-// Workspace: [control: ticket, error][a pair of words for each tile and channel].  A word is a float and a tag
+// Workspace: [control: an expired wait, then each strip's next turn, a line each][a pair of words for each tile
+// and channel].  One counter for all tiles bounded the forward pass at about 25 ns a tile.  A word is a float and a tag
 // in one 64-bit access, so a reader that sees the tag has the value: no fence, no cache write-back.
-constexpr int kControlBytes = 256;
+constexpr int kControlBytes = 128;
 constexpr uint32_t kPair = 1, kState = 2;  // tags: (P, Q) so far, the state after the tile
 
 struct Handoff {
-  uint32_t* control;       // [0] tickets, [1] an expired wait
-  unsigned long long* word; // [tile][2: Q or state, P][64 C]
+  uint32_t* control;
+  unsigned long long* word; // [tile][2: Q or state, P][64]
   uint64_t spin_ticks;
   int32_t* status;
 };
@@ -99,65 +136,87 @@ __device__ __forceinline__ unsigned long long peek(const unsigned long long* w) 
 }
 
 __device__ __forceinline__ bool peek_error(const Handoff& hd) {
-  return __hip_atomic_load(&hd.control[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
+  return __hip_atomic_load(&hd.control[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
 }
 
-// The tile's claim: tickets count tiles in order of their turn, all channels of a turn first.
+// The tile's claim: a workgroup's strip of channels is fixed, its turn in time the next of its strip.
 struct Claim {
   uint32_t strip, turn;
 };
 __device__ __forceinline__ Claim claim(const Handoff& hd, uint32_t nstrips, uint32_t nturns) {
-  __shared__ uint32_t s_ticket;
-  uint32_t ticket = blockIdx.x;
+  __shared__ uint32_t s_turn;
+  uint32_t turn = 0;
+  const uint32_t strip = blockIdx.x % nstrips;
   if (nturns > 1) {
-    if (threadIdx.x == 0) s_ticket = atomicAdd(&hd.control[0], 1u);
+    if (threadIdx.x == 0) s_turn = atomicAdd(&hd.control[(1 + strip) * (kControlBytes / 4)], 1u);
     __syncthreads();
-    ticket = __builtin_amdgcn_readfirstlane(s_ticket);
+    turn = __builtin_amdgcn_readfirstlane(s_turn);
   }
-  return {ticket % nstrips, ticket / nstrips};
+  return {strip, turn};
 }
 
-// What wave w of `waves` does between its tile's composition and the state before the tile: wave 0 publishes
-// the tile's pair, and the waves fetch the kWindow tiles before it into s_back[distance - 1], a pair, or a
-// state with P = -1 (a product of decays is never negative).  The wait is bounded by wall-clock time and
-// sets the status word if it expires, which is not expected: the tiles waited for are running or done.
-template <int C>
+// What a wave does between its tile's composition and the state before the tile: the waves fetch the kWindow
+// tiles before it into s_back[distance - 1], a pair, or a state with P = -1 (a product of decays is never
+// negative).  A wave's tiles are polled together, so that it takes one round trip where all are there.  The wait
+// is bounded by wall-clock time and sets the status word if it expires, which is not expected: the tiles waited
+// for are running or done.  At least kMinWaves waves.
+constexpr int kMinWaves = 4, kPolls = kWindow / kMinWaves;
 __device__ __forceinline__ void look_back(const Handoff& hd, uint32_t turn, uint32_t strip, uint32_t nstrips, int wave,
-                                          int waves, float2 (&s_back)[kWindow][64 * C]) {
+                                          int waves, float2 (&s_back)[kWindow][64]) {
   const int lane = threadIdx.x & 63;
-  for (int j = wave; j < kWindow && static_cast<uint32_t>(j) < turn; j += waves) {
-    const unsigned long long* w =
-        hd.word + (static_cast<uint64_t>(turn - 1 - j) * nstrips + strip) * (2 * 64 * C) + lane * C;
-    const bool last = j == kWindow - 1;  // this one's state is needed
-    const uint64_t t_start = wall_clock64();
+  const unsigned long long* w[kPolls];
+  unsigned long long q[kPolls], pw[kPolls];
+  bool need[kPolls];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float2 v = make_float2(-1.0f, 0.0f);
-      for (;;) {
-        const unsigned long long q = peek(w + c), pw = peek(w + 64 * C + c);
-        const uint32_t tag = static_cast<uint32_t>(q >> 32);
-        v.y = __uint_as_float(static_cast<uint32_t>(q));
-        if (tag == kState) {
-          v.x = -1.0f;
-          break;
-        }
-        if (tag == kPair && !last && static_cast<uint32_t>(pw >> 32) == kPair) {
-          v.x = __uint_as_float(static_cast<uint32_t>(pw));
-          break;
-        }
-        // one expired wait of the call makes the others return at once
-        if (wall_clock64() - t_start > hd.spin_ticks || peek_error(hd)) {
-          __hip_atomic_store(&hd.control[1], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          if (hd.status != nullptr)
-            __hip_atomic_fetch_or(hd.status, MM_SCAN_STATUS_HANDOFF_TIMEOUT, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          v = make_float2(-1.0f, 0.0f);
-          break;
-        }
-        __builtin_amdgcn_s_sleep(1);
-      }
-      s_back[j][lane * C + c] = v;
-    }
+  for (int k = 0; k < kPolls; ++k) {
+    const int j = wave + k * waves;
+    need[k] = j < kWindow && static_cast<uint32_t>(j) < turn;
+    w[k] = hd.word + (static_cast<uint64_t>(need[k] ? turn - 1 - j : turn) * nstrips + strip) * 128 + lane;
   }
+  const uint64_t t_start = wall_clock64();
+  for (;;) {
+#pragma unroll
+    for (int k = 0; k < kPolls; ++k)
+      if (need[k]) q[k] = peek(w[k]), pw[k] = peek(w[k] + 64);
+    bool again = false;
+#pragma unroll
+    for (int k = 0; k < kPolls; ++k) {
+      if (!need[k]) continue;
+      const int j = wave + k * waves;
+      const uint32_t tag = static_cast<uint32_t>(q[k] >> 32);
+      // the farthest tile's state is needed, of the others the pair will do
+      const bool pair = tag == kPair && j != kWindow - 1 && static_cast<uint32_t>(pw[k] >> 32) == kPair;
+      if (__all(tag == kState || pair)) {
+        s_back[j][lane] = make_float2(tag == kState ? -1.0f : __uint_as_float(static_cast<uint32_t>(pw[k])),
+                                      __uint_as_float(static_cast<uint32_t>(q[k])));
+        need[k] = false;
+      } else {
+        again = true;
+      }
+    }
+    if (!again) break;
+    // one expired wait of the call makes the others return at once
+    if (wall_clock64() - t_start > hd.spin_ticks || peek_error(hd)) {
+      __hip_atomic_store(&hd.control[0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (hd.status != nullptr)
+        __hip_atomic_fetch_or(hd.status, MM_SCAN_STATUS_HANDOFF_TIMEOUT, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (int k = 0; k < kPolls; ++k)
+        if (need[k]) s_back[wave + k * waves][lane] = make_float2(-1.0f, 0.0f);
+      break;
+    }
+    __builtin_amdgcn_s_sleep(1);
+  }
+}
+// The state before the tile from what look_back fetched, first tile first.
+__device__ __forceinline__ float fold_back(uint32_t turn, const float2 (&s_back)[kWindow][64]) {
+  const int lane = threadIdx.x & 63, far = turn < kWindow ? static_cast<int>(turn) : kWindow;
+  float h = 0.0f;
+  for (int j = far - 1; j >= 0; --j) {
+    const float2 v = s_back[j][lane];
+    h = v.x < 0.0f ? v.y : __builtin_fmaf(v.x, h, v.y);
+  }
+  return h;
 }
 
 __global__ __launch_bounds__(256) void clear_kernel(uint4* p, int64_t n) {
@@ -169,207 +228,171 @@ struct Launch {
   mm_gated_scan_params p;
   Handoff hd;
   float* dA_part;
-  uint32_t nstrips, nturns, ncb;  // strips of 64 C channels of a sequence, tiles of a strip, strips a sequence
+  uint32_t nstrips, nturns, ncb;  // strips of 64 channels of a sequence, tiles of a strip, strips a sequence
   int32_t waves;
 };
 
 // ------------------------------------------------------------------------------ forward
-template <int DT, int C, bool Z, bool P8>
+// A token's state is h_t = E_t h + H_t for the state h before the wave, E and H the products and sums so far: E, H
+// and the gate's input are what is kept in registers over the wait.
+template <int DT, bool Z, bool P8>
 __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
-  using V = typename Ch<DT, C>::V;
   using T = typename Ty<DT>::T;
   constexpr int N = Z ? 4 : 3;
-  __shared__ float2 s_pair[kMaxWaves][64 * C];
-  __shared__ float2 s_back[kWindow][64 * C];
+  __shared__ float2 s_pair[kMaxWaves][64];
+  __shared__ float2 s_back[kWindow][64];
   const mm_gated_scan_params& p = k.p;
   const Claim cl = claim(k.hd, k.nstrips, k.nturns);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t b = cl.strip / k.ncb;
-  const uint32_t d = (cl.strip % k.ncb) * (64 * C) + lane * C;
-  const bool live = d < p.dim;           // with C = 2 dim is even
-  const uint32_t dd = live ? d : 0;      // loads of the other lanes stay in bounds
+  // lanes past the last channel do what the last one's does, stores and all
+  const uint32_t d = min((cl.strip % k.ncb) * 64 + lane, static_cast<uint32_t>(p.dim - 1));
+  const uint32_t off = d * static_cast<uint32_t>(sizeof(T));
   const int64_t len = length_of(p, b), nblk = (p.seqlen + kBlk - 1) / kBlk;
   const int64_t blk = static_cast<int64_t>(cl.turn) * k.waves + wave, t0 = blk * kBlk;
-  const bool here = t0 < p.seqlen;       // the wave has tokens
+  const bool here = t0 < p.seqlen;  // the wave has tokens
 
-  // pairs (a, b), and the gate's inputs for later
-  float a[kBlk][C], bu[kBlk][C];
-  V zr[Z ? kBlk : 1];
-  float P[C], Q[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) P[c] = 1.0f, Q[c] = 0.0f;
+  float E[kBlk], H[kBlk];
+  T zr[Z ? kBlk : 1];
+  float P = 1.0f, Q = 0.0f;
   auto load_all = [&](auto full_c) __attribute__((always_inline)) {
     constexpr bool full = decltype(full_c)::value;
-    const T* src[4] = {static_cast<const T*>(p.x) + b * p.x_stride[0], static_cast<const T*>(p.a_gate) + b * p.a_gate_stride[0],
-                       static_cast<const T*>(p.x_gate) + b * p.x_gate_stride[0],
-                       Z ? static_cast<const T*>(p.z) + b * p.z_stride[0] : nullptr};
-    const int64_t st[4] = {p.x_stride[1], p.a_gate_stride[1], p.x_gate_stride[1], Z ? p.z_stride[1] : 0};
-    V raw[N][kBlk];
+    Rows<DT> in[4] = {{p.x, p.x_stride, b, t0}, {p.a_gate, p.a_gate_stride, b, t0}, {p.x_gate, p.x_gate_stride, b, t0},
+                      {Z ? p.z : p.x, Z ? p.z_stride : p.x_stride, b, t0}};
+    T raw[N][kBlk];
 #pragma unroll
     for (int t = 0; t < kBlk; ++t) {
-      const int64_t tt = full || t0 + t < p.seqlen ? t0 + t : p.seqlen - 1;
 #pragma unroll
-      for (int j = 0; j < N; ++j) raw[j][t] = Ch<DT, C>::load(src[j] + tt * st[j] + dd);
+      for (int j = 0; j < N; ++j) {
+        raw[j][t] = in[j].load(off);
+        in[j].next(full || t0 + t + 1 < p.seqlen);
+      }
     }
+    const float A = rate_of(p.A[d]);
     if constexpr (!full) {
 #pragma unroll
       for (int t = 0; t < kBlk; ++t)
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-#pragma unroll
-          for (int c = 0; c < C; ++c) raw[j][t][c] = t0 + t < len ? raw[j][t][c] : static_cast<T>(0);
+        for (int j = 0; j < N; ++j) raw[j][t] = t0 + t < len ? raw[j][t] : static_cast<T>(0);
     }
     if constexpr (P8) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
+        float v[kBlk];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          uint32_t top = 0;
-#pragma unroll
-          for (int t = 0; t < kBlk; ++t) top = max(top, act8::abs_bits(Ty<DT>::f(raw[j][t][c])));
-          const uint32_t e = act8::exponent_of(top);
-          const float inv = act8::inv_scale(e);
-          uint32_t w[kBlk / 4];
-#pragma unroll
-          for (int t = 0; t < kBlk; t += 4) w[t / 4] = act8::code4(Ty<DT>::f(raw[j][t][c]), Ty<DT>::f(raw[j][t + 1][c]),
-                                                                    Ty<DT>::f(raw[j][t + 2][c]), Ty<DT>::f(raw[j][t + 3][c]), inv);
-          if (live) {
-            const int64_t o = (b * nblk + blk) * p.dim + d + c;
-            *reinterpret_cast<uint4*>(p.codes[j] + o * kBlk) = make_uint4(w[0], w[1], w[2], w[3]);
-            p.exps[j][o] = static_cast<uint8_t>(e);
-          }
-        }
+        for (int t = 0; t < kBlk; ++t) v[t] = Ty<DT>::f(raw[j][t]);
+        uint32_t e;
+        const uint4 w = act8::pack16(v, e);
+        const int64_t o = (b * nblk + blk) * p.dim;
+        *reinterpret_cast<uint4*>(p.codes[j] + o * kBlk + static_cast<uint64_t>(d) * kBlk) = w;
+        (p.exps[j] + o)[d] = static_cast<uint8_t>(e);
       }
     }
-    float A[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) A[c] = rate_of(p.A[dd + c]);
 #pragma unroll
     for (int t = 0; t < kBlk; ++t) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        float beta2;
-        decay(A[c] * sigmoid_f(Ty<DT>::f(raw[1][t][c])), a[t][c], beta2);
-        bu[t][c] = __builtin_amdgcn_sqrtf(beta2) * (sigmoid_f(Ty<DT>::f(raw[2][t][c])) * Ty<DT>::f(raw[0][t][c]));
-        if constexpr (!full) {
-          a[t][c] = t0 + t < len ? a[t][c] : 1.0f;
-          bu[t][c] = t0 + t < len ? bu[t][c] : 0.0f;
-        }
-        P[c] *= a[t][c];
-        Q[c] = __builtin_fmaf(a[t][c], Q[c], bu[t][c]);
+      float a, beta2;
+      decay<DT>(A * sigmoid_f(Ty<DT>::f(raw[1][t])), a, beta2);
+      float bu = __builtin_amdgcn_sqrtf(beta2) * (sigmoid_f(Ty<DT>::f(raw[2][t])) * Ty<DT>::f(raw[0][t]));
+      if constexpr (!full) {
+        a = t0 + t < len ? a : 1.0f;
+        bu = t0 + t < len ? bu : 0.0f;
       }
+      E[t] = P = P * a;
+      H[t] = Q = __builtin_fmaf(a, Q, bu);
+      keep(E[t]);
+      keep(H[t]);
       if constexpr (Z) zr[t] = raw[3][t];
     }
   };
-  const bool full = t0 + kBlk <= len;
+  const bool full = t0 + kBlk <= len, some = here && (P8 || t0 < len);
   if (full) load_all(std::true_type{});
-  else if (here && (P8 || t0 < len)) load_all(std::false_type{});
+  else if (some) load_all(std::false_type{});
 
-  // the state before the tile
-  float h[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    s_pair[wave][lane * C + c] = make_float2(P[c], Q[c]);
-    h[c] = 0.0f;
+  // the state before the tile, and before the wave
+  float h = 0.0f;
+  if (k.waves > 1) {
+    s_pair[wave][lane] = make_float2(P, Q);
+    __syncthreads();
   }
-  __syncthreads();
-  float tp[C], tq[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) tp[c] = 1.0f, tq[c] = 0.0f;
-  unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * (2 * 64 * C) + lane * C;
-  if (k.nturns > 1 && wave == 0) {
+  float tp = 1.0f, tq = 0.0f;
+  unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 128 + lane;
+  const bool more = cl.turn + 1 < k.nturns;
+  if (more && wave == 0) {
     for (int w = 0; w < k.waves; ++w) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const float2 v = s_pair[w][lane * C + c];
-        tp[c] *= v.x;
-        tq[c] = __builtin_fmaf(v.x, tq[c], v.y);
-      }
+      const float2 v = s_pair[w][lane];
+      tp *= v.x;
+      tq = __builtin_fmaf(v.x, tq, v.y);
     }
-    if (cl.turn > 0 && cl.turn + 1 < k.nturns) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        publish(mine + 64 * C + c, tp[c], kPair);
-        publish(mine + c, tq[c], kPair);
-      }
+    if (cl.turn > 0) {
+      publish(mine + 64, tp, kPair);
+      publish(mine, tq, kPair);
     }
   }
   if (cl.turn == 0) {
-    if (p.h0 != nullptr) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) h[c] = p.h0[b * p.dim + dd + c];
-    }
+    if (p.h0 != nullptr) h = p.h0[b * p.dim + d];
   } else {
-    look_back<C>(k.hd, cl.turn, cl.strip, k.nstrips, wave, k.waves, s_back);
+    look_back(k.hd, cl.turn, cl.strip, k.nstrips, wave, k.waves, s_back);
     __syncthreads();
-    const int far = cl.turn < kWindow ? static_cast<int>(cl.turn) : kWindow;
-    for (int j = far - 1; j >= 0; --j) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const float2 v = s_back[j][lane * C + c];
-        h[c] = v.x < 0.0f ? v.y : __builtin_fmaf(v.x, h[c], v.y);
-      }
-    }
+    h = fold_back(cl.turn, s_back);
   }
-  if (k.nturns > 1 && wave == 0 && cl.turn + 1 < k.nturns) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) publish(mine + c, __builtin_fmaf(tp[c], h[c], tq[c]), kState);
-  }
-  // the state before the wave
+  if (more && wave == 0) publish(mine, __builtin_fmaf(tp, h, tq), kState);
   for (int w = 0; w < wave; ++w) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const float2 v = s_pair[w][lane * C + c];
-      h[c] = __builtin_fmaf(v.x, h[c], v.y);
-    }
+    const float2 v = s_pair[w][lane];
+    h = __builtin_fmaf(v.x, h, v.y);
   }
-  if (here && live && p.block_states != nullptr) {
-    float* const o = p.block_states + (b * nblk + blk) * p.dim + d;
-#pragma unroll
-    for (int c = 0; c < C; ++c) o[c] = h[c];
-  }
+  if (here && p.block_states != nullptr) (p.block_states + (b * nblk + blk) * p.dim)[d] = h;
 
-  // the recurrence and the outputs
-  T* const yb = static_cast<T*>(p.y) + b * p.y_stride[0];
-  if (full) {
+  float last = h;
+  auto finish = [&](auto full_c) __attribute__((always_inline)) {
+    constexpr bool full = decltype(full_c)::value;
+    Rows<DT> out(p.y, p.y_stride, b, t0);
 #pragma unroll
-    for (int t = 0; t < kBlk; ++t) {
-      float y[C];
+    for (int t = 0; t < kBlk; t += 2) {
+      float y[2];
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        h[c] = __builtin_fmaf(a[t][c], h[c], bu[t][c]);
-        y[c] = Z ? h[c] * silu_f(Ty<DT>::f(zr[Z ? t : 0][c])) : h[c];
-      }
-      if (live) Ch<DT, C>::store(yb + (t0 + t) * p.y_stride[1] + d, y);
-    }
-  } else if (here) {
-#pragma unroll
-    for (int t = 0; t < kBlk; ++t) {
-      const bool in = t0 + t < len;
-      float y[C];
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if (in) h[c] = __builtin_fmaf(a[t][c], h[c], bu[t][c]);
-        y[c] = Z ? h[c] * silu_f(Ty<DT>::f(zr[Z ? t : 0][c])) : h[c];
+      for (int c = 0; c < 2; ++c) {
+        const bool in = full || t0 + t + c < len;
+        last = in ? __builtin_fmaf(E[t + c], h, H[t + c]) : last;
+        y[c] = last;
+        if constexpr (Z) {
+          const float z = Ty<DT>::f(zr[t + c]);
+          y[c] *= z * sigmoid_f(z);
+        }
         y[c] = in ? y[c] : 0.0f;
       }
-      if (live && t0 + t < p.seqlen) Ch<DT, C>::store(yb + (t0 + t) * p.y_stride[1] + d, y);
-    }
-  }
-  // (by the wave of the last block: the state is y's last one, bit for bit)
-  if (p.state_out != nullptr && live && blk == (nblk > 0 ? nblk - 1 : 0)) {
+      T v[2];
+      round2<DT>(y[0], y[1], v[0], v[1]);
 #pragma unroll
-    for (int c = 0; c < C; ++c) p.state_out[b * p.dim + d + c] = h[c];
+      for (int c = 0; c < 2; ++c) {
+        if (full || t0 + t + c < p.seqlen) out.store(off, v[c]);
+        out.next();
+      }
+    }
+  };
+  if (full) {
+    finish(std::true_type{});
+  } else if (here) {
+    if (!some) {
+#pragma unroll
+      for (int t = 0; t < kBlk; ++t) {
+        E[t] = H[t] = 0.0f;
+        if constexpr (Z) zr[t] = static_cast<T>(0);
+      }
+    }
+    finish(std::false_type{});
   }
+  // (by the wave of the last block: the state is the last token's, bit for bit)
+  if (p.state_out != nullptr && blk == (nblk > 0 ? nblk - 1 : 0)) p.state_out[b * p.dim + d] = last;
 }
 
 // ------------------------------------------------------------------------------ backward
-// Turn 0 is the last tile of a sequence.  Of a token, what needs dh is dh times a number that does not:
-//   dx = dh c1, c1 = i beta            dx_gate = dh c2, c2 = beta u (1 - i)
-//   da_gate = dh c3, c3 = f l (1 - r)  dA += dh c4, c4 = f r      with f = h_{t-1} a - u a^2 / beta
-// so these four, a and g are all that is kept in registers over the wait.
+// Turn 0 is the last tile of a sequence.  With c what comes from the tokens after the wave, dh_t = E_t c + G_t, E
+// and G the products and sums of the recurrence in reverse.  What needs dh is dh times a number that does not:
+//   dx = dh c1, c1 = i beta    dx_gate = dh c2, c2 = beta u (1 - i)    da_gate = dh c3, c3 = f l (1 - r)
+// with f = h_{t-1} a - u a^2 / beta, and dA is c (sum of E f r) + (sum of G f r): five numbers a token and two more
+// are all that is kept in registers over the wait.
 template <int DT, bool Z, bool C8>
-__global__ __launch_bounds__(64 * kMaxWavesBwd, 2) void bwd_kernel(const Launch k) {
+__global__ __launch_bounds__(64 * kMaxWavesBwd, BWD_EU) void bwd_kernel(const Launch k) {
   using T = typename Ty<DT>::T;
   constexpr int N = Z ? 4 : 3;
   __shared__ float2 s_pair[kMaxWavesBwd][64];
@@ -379,165 +402,200 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, 2) void bwd_kernel(const Launch 
   const Claim cl = claim(k.hd, k.nstrips, k.nturns);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t b = cl.strip / k.ncb;
-  const uint32_t d = (cl.strip % k.ncb) * 64 + lane;
-  const bool live = d < p.dim;
-  const uint32_t dd = live ? d : 0;
+  const uint32_t d = min((cl.strip % k.ncb) * 64 + lane, static_cast<uint32_t>(p.dim - 1));
+  const uint32_t off = d * static_cast<uint32_t>(sizeof(T));
   const int64_t len = length_of(p, b), nblk = (p.seqlen + kBlk - 1) / kBlk;
   const int64_t blk = static_cast<int64_t>(k.nturns - 1 - cl.turn) * k.waves + wave, t0 = blk * kBlk;
   const bool here = t0 < p.seqlen;
-  const int64_t row = (b * p.seqlen + t0) * p.dim;  // of the gradients
+  const int64_t row = b * p.seqlen + t0;  // of the gradients
 
-  float a[kBlk], g[kBlk], c1[kBlk], c2[kBlk], c3[kBlk], c4[kBlk];
-  float P = 1.0f, Q = 0.0f;
+  float E[kBlk], G[kBlk], c1[kBlk], c2[kBlk], c3[kBlk];
+  float P = 1.0f, Q = 0.0f, dA_c = 0.0f, dA_0 = 0.0f;
   auto load_all = [&](auto full_c) __attribute__((always_inline)) {
     constexpr bool full = decltype(full_c)::value;
-    const T* src[5] = {};
-    int64_t st[5] = {};
-    src[4] = static_cast<const T*>(p.dy) + b * p.dy_stride[0];
-    st[4] = p.dy_stride[1];
-    uint4 code[C8 ? N : 1];
-    float scale[C8 ? N : 1];
+    act8::Block code[C8 ? N : 1];
     T raw[C8 ? 1 : N][kBlk], dyr[kBlk];
+    Rows<DT> dyp(p.dy, p.dy_stride, b, t0);
     if constexpr (C8) {
+      const int64_t o = (b * nblk + blk) * p.dim;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int64_t o = (b * nblk + blk) * p.dim + dd;
-        code[j] = *reinterpret_cast<const uint4*>(p.codes[j] + o * kBlk);
-        scale[j] = act8::scale_of(p.exps[j][o]);
-      }
+      for (int j = 0; j < N; ++j) code[j].load(p.codes[j] + o * kBlk, p.exps[j] + o, d);
     } else {
-      src[0] = static_cast<const T*>(p.x) + b * p.x_stride[0], st[0] = p.x_stride[1];
-      src[1] = static_cast<const T*>(p.a_gate) + b * p.a_gate_stride[0], st[1] = p.a_gate_stride[1];
-      src[2] = static_cast<const T*>(p.x_gate) + b * p.x_gate_stride[0], st[2] = p.x_gate_stride[1];
-      if constexpr (Z) src[3] = static_cast<const T*>(p.z) + b * p.z_stride[0], st[3] = p.z_stride[1];
+      Rows<DT> in[4] = {{p.x, p.x_stride, b, t0}, {p.a_gate, p.a_gate_stride, b, t0}, {p.x_gate, p.x_gate_stride, b, t0},
+                        {Z ? p.z : p.x, Z ? p.z_stride : p.x_stride, b, t0}};
+#pragma unroll
+      for (int t = 0; t < kBlk; ++t)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          raw[j][t] = in[j].load(off);
+          in[j].next(full || t0 + t + 1 < p.seqlen);
+        }
     }
 #pragma unroll
     for (int t = 0; t < kBlk; ++t) {
-      const int64_t tt = full || t0 + t < p.seqlen ? t0 + t : p.seqlen - 1;
-      if constexpr (!C8) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) raw[j][t] = src[j][tt * st[j] + dd];
-      }
-      dyr[t] = src[4][tt * st[4] + dd];
+      dyr[t] = dyp.load(off);
+      dyp.next(full || t0 + t + 1 < p.seqlen);
     }
-    const float A = rate_of(p.A[dd]);
-    float h = p.block_states[(b * nblk + blk) * p.dim + dd];
+    const float A = rate_of(p.A[d]);
+    float h = (p.block_states + (b * nblk + blk) * p.dim)[d];
+    if constexpr (C8) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) code[j].prepare();
+    }
     auto value = [&](int j, int t) __attribute__((always_inline)) {
       float v;
-      if constexpr (C8) v = act8::value_of(code[j], t, scale[j]);
+      if constexpr (C8) v = code[j].value(t);
       else v = Ty<DT>::f(raw[j][t]);
       return full || t0 + t < len ? v : 0.0f;
     };
+    float a[kBlk], c4[kBlk];
+    Rows<DT> dzp(p.dz, row, p.dim);
 #pragma unroll
-    for (int t = 0; t < kBlk; ++t) {
-      const bool in = full || t0 + t < len;
-      const float x = value(0, t), r = sigmoid_f(value(1, t)), i = sigmoid_f(value(2, t)), l = A * r;
-      float beta2;
-      decay(l, a[t], beta2);
-      // 1 / beta, or 0 at a = 1, where the root has no slope (and where beta^2 is below the smallest normal
-      // number, whose reciprocal root the instruction takes as infinite; a NaN stays one)
-      const float ib = fabsf(beta2) < 1.17549435e-38f ? 0.0f : __builtin_amdgcn_rsqf(beta2);
-      const float beta = beta2 * ib, u = i * x, hp = h;
-      const float f = __builtin_fmaf(hp, a[t], -u * (a[t] * a[t] * ib));
-      c1[t] = i * beta;
-      c2[t] = beta * u * (1.0f - i);
-      c3[t] = f * l * (1.0f - r);
-      c4[t] = f * r;
-      h = __builtin_fmaf(a[t], h, beta * u);
-      g[t] = Ty<DT>::f(dyr[t]);
-      if constexpr (Z) {
-        const float z = value(3, t), s = sigmoid_f(z), zs = z * s;
-        const float dz = g[t] * h * __builtin_fmaf(zs, 1.0f - s, s);
-        if (live && (full || t0 + t < p.seqlen))
-          static_cast<T*>(p.dz)[row + t * p.dim + d] = Ch<DT, 1>::template cvt<DT>(in ? dz : 0.0f);
-        g[t] *= zs;
+    for (int t = 0; t < kBlk; t += 2) {
+      float dz[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int tt = t + c;
+        const bool in = full || t0 + tt < len;
+        const float x = value(0, tt), r = sigmoid_f(value(1, tt)), i = sigmoid_f(value(2, tt)), l = A * r;
+        float beta2;
+        decay<DT>(l, a[tt], beta2);
+        // 1 / beta, or 0 at a = 1, where the root has no slope (and where beta^2 is below the smallest normal
+        // number, whose reciprocal root the instruction takes as infinite; a NaN stays one)
+        const float ib = fabsf(beta2) < 1.17549435e-38f ? 0.0f : __builtin_amdgcn_rsqf(beta2);
+        const float beta = beta2 * ib, u = i * x, bu = beta * u;
+        const float f = __builtin_fmaf(h, a[tt], -u * (a[tt] * a[tt] * ib));
+        c1[tt] = i * beta;
+        c2[tt] = __builtin_fmaf(-bu, i, bu);
+        c4[tt] = f * r;
+        c3[tt] = f * __builtin_fmaf(-l, r, l);
+        const float hn = __builtin_fmaf(a[tt], h, bu);
+        h = in ? hn : h;
+        G[tt] = Ty<DT>::f(dyr[tt]);
+        if constexpr (Z) {
+          const float z = value(3, tt), s = sigmoid_f(z), zs = z * s;
+          dz[c] = in ? G[tt] * h * __builtin_fmaf(zs, 1.0f - s, s) : 0.0f;
+          G[tt] *= zs;
+        }
+        if constexpr (!full) {
+          a[tt] = in ? a[tt] : 1.0f;
+          G[tt] = in ? G[tt] : 0.0f;
+          c1[tt] = in ? c1[tt] : 0.0f;
+          c2[tt] = in ? c2[tt] : 0.0f;
+          c3[tt] = in ? c3[tt] : 0.0f;
+          c4[tt] = in ? c4[tt] : 0.0f;
+        }
       }
-      if constexpr (!full) {
-        a[t] = in ? a[t] : 1.0f;
-        h = in ? h : hp;
-        g[t] = in ? g[t] : 0.0f;
-        c1[t] = in ? c1[t] : 0.0f;
-        c2[t] = in ? c2[t] : 0.0f;
-        c3[t] = in ? c3[t] : 0.0f;
-        c4[t] = in ? c4[t] : 0.0f;
+      if constexpr (Z) {
+        T v[2];
+        round2<DT>(dz[0], dz[1], v[0], v[1]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (full || t0 + t + c < p.seqlen) dzp.store(off, v[c]);
+          dzp.next();
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        keep(c1[t + c]);
+        keep(c2[t + c]);
+        keep(c3[t + c]);
+        keep(c4[t + c]);
       }
     }
 #pragma unroll
     for (int t = kBlk - 1; t >= 0; --t) {
+      E[t] = P;
+      G[t] += Q;
+      dA_c = __builtin_fmaf(P, c4[t], dA_c);
+      dA_0 = __builtin_fmaf(G[t], c4[t], dA_0);
       P *= a[t];
-      Q = a[t] * (Q + g[t]);
+      Q = a[t] * G[t];
     }
   };
   const bool full = t0 + kBlk <= len, some = here && t0 < len;
   if (full) load_all(std::true_type{});
   else if (some) load_all(std::false_type{});
 
-  s_pair[wave][lane] = make_float2(P, Q);
-  __syncthreads();
+  if (k.waves > 1) {
+    s_pair[wave][lane] = make_float2(P, Q);
+    __syncthreads();
+  }
   float tp = 1.0f, tq = 0.0f, carry = 0.0f;
   unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 128 + lane;
-  if (k.nturns > 1 && wave == 0) {
+  const bool more = cl.turn + 1 < k.nturns;
+  if (more && wave == 0) {
     for (int w = k.waves - 1; w >= 0; --w) {
       const float2 v = s_pair[w][lane];
       tp *= v.x;
       tq = __builtin_fmaf(v.x, tq, v.y);
     }
-    if (cl.turn > 0 && cl.turn + 1 < k.nturns) {
+    if (cl.turn > 0) {
       publish(mine + 64, tp, kPair);
       publish(mine, tq, kPair);
     }
   }
   if (cl.turn == 0) {
-    if (p.dstate != nullptr) carry = p.dstate[b * p.dim + dd];
+    if (p.dstate != nullptr) carry = p.dstate[b * p.dim + d];
   } else {
-    look_back<1>(k.hd, cl.turn, cl.strip, k.nstrips, wave, k.waves, s_back);
+    look_back(k.hd, cl.turn, cl.strip, k.nstrips, wave, k.waves, s_back);
     __syncthreads();
-    const int far = cl.turn < kWindow ? static_cast<int>(cl.turn) : kWindow;
-    for (int j = far - 1; j >= 0; --j) {
-      const float2 v = s_back[j][lane];
-      carry = v.x < 0.0f ? v.y : __builtin_fmaf(v.x, carry, v.y);
-    }
+    carry = fold_back(cl.turn, s_back);
   }
-  if (k.nturns > 1 && wave == 0 && cl.turn + 1 < k.nturns) publish(mine, __builtin_fmaf(tp, carry, tq), kState);
+  if (more && wave == 0) publish(mine, __builtin_fmaf(tp, carry, tq), kState);
   for (int w = k.waves - 1; w > wave; --w) {
     const float2 v = s_pair[w][lane];
     carry = __builtin_fmaf(v.x, carry, v.y);
   }
 
-  float dA = 0.0f;
-  T* const dx = static_cast<T*>(p.dx) + row;
-  T* const da = static_cast<T*>(p.da_gate) + row;
-  T* const dg = static_cast<T*>(p.dx_gate) + row;
-  auto out = [&](int t, float v1, float v2, float v3) __attribute__((always_inline)) {
-    dx[t * p.dim + d] = Ch<DT, 1>::template cvt<DT>(v1);
-    dg[t * p.dim + d] = Ch<DT, 1>::template cvt<DT>(v2);
-    da[t * p.dim + d] = Ch<DT, 1>::template cvt<DT>(v3);
-  };
-  if (some) {
+  auto finish = [&](auto full_c) __attribute__((always_inline)) {
+    constexpr bool full = decltype(full_c)::value;
+    Rows<DT> o[3] = {{p.dx, row, p.dim}, {p.dx_gate, row, p.dim}, {p.da_gate, row, p.dim}};
 #pragma unroll
-    for (int t = kBlk - 1; t >= 0; --t) {
-      const float dh = g[t] + carry;
-      carry = full || t0 + t < len ? a[t] * dh : carry;
-      dA = __builtin_fmaf(dh, c4[t], dA);
-      if (live && (full || t0 + t < p.seqlen)) {
-        const bool in = full || t0 + t < len;  // (0 times an infinite dh is not 0)
-        out(t, in ? dh * c1[t] : 0.0f, in ? dh * c2[t] : 0.0f, in ? dh * c3[t] : 0.0f);
+    for (int t = 0; t < kBlk; t += 2) {
+      float v[3][2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const bool in = full || t0 + t + c < len;  // (0 times an infinite dh is not 0)
+        const float dh = __builtin_fmaf(E[t + c], carry, G[t + c]);
+        v[0][c] = in ? dh * c1[t + c] : 0.0f;
+        v[1][c] = in ? dh * c2[t + c] : 0.0f;
+        v[2][c] = in ? dh * c3[t + c] : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        T w[2];
+        round2<DT>(v[j][0], v[j][1], w[0], w[1]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (full || t0 + t + c < p.seqlen) o[j].store(off, w[c]);
+          o[j].next();
+        }
       }
     }
-  } else if (here && live) {
+  };
+  if (full) {
+    finish(std::true_type{});
+  } else if (some) {
+    finish(std::false_type{});
+  } else if (here) {
+    Rows<DT> o[4] = {{p.dx, row, p.dim}, {p.dx_gate, row, p.dim}, {p.da_gate, row, p.dim}, {Z ? p.dz : p.dx, row, p.dim}};
+    for (int64_t t = t0; t < t0 + kBlk && t < p.seqlen; ++t) {
 #pragma unroll
-    for (int t = 0; t < kBlk; ++t) {
-      if (t0 + t >= p.seqlen) break;
-      out(t, 0.0f, 0.0f, 0.0f);
-      if constexpr (Z) static_cast<T*>(p.dz)[row + t * p.dim + d] = Ch<DT, 1>::template cvt<DT>(0.0f);
+      for (int j = 0; j < N; ++j) {
+        o[j].store(off, static_cast<T>(0));
+        o[j].next();
+      }
     }
   }
-  if (p.dh0 != nullptr && live && cl.turn + 1 == k.nturns && wave == 0) p.dh0[b * p.dim + d] = carry;
+  const float dA = some ? __builtin_fmaf(dA_c, carry, dA_0) : 0.0f;
+  if (p.dh0 != nullptr && cl.turn + 1 == k.nturns && wave == 0) p.dh0[b * p.dim + d] = __builtin_fmaf(P, carry, Q);
   s_dA[wave][lane] = dA;
   __syncthreads();
-  if (wave == 0 && live) {
-    for (int w = 1; w < k.waves; ++w) dA += s_dA[w][lane];
-    k.dA_part[(b * k.nturns + cl.turn) * p.dim + d] = dA;
+  if (wave == 0) {
+    float sum = dA;
+    for (int w = 1; w < k.waves; ++w) sum += s_dA[w][lane];
+    k.dA_part[(b * k.nturns + cl.turn) * p.dim + d] = sum;
   }
 }
 
@@ -553,7 +611,7 @@ __global__ __launch_bounds__(kStepThreads) void step_kernel(const float* state, 
   const int64_t d = static_cast<int64_t>(blockIdx.x) * kStepThreads + threadIdx.x, b = blockIdx.y;
   if (d >= dim) return;
   float a, beta2;
-  decay(rate_of(A[d]) * sigmoid_f(ld<DT>(a_gate, b * as + d)), a, beta2);
+  decay<DT>(rate_of(A[d]) * sigmoid_f(ld<DT>(a_gate, b * as + d)), a, beta2);
   const float u = sigmoid_f(ld<DT>(x_gate, b * gs + d)) * ld<DT>(x, b * xs + d);
   const float h = __builtin_fmaf(a, state[b * dim + d], __builtin_sqrtf(beta2) * u);
   state_out[b * dim + d] = h;
@@ -562,8 +620,7 @@ __global__ __launch_bounds__(kStepThreads) void step_kernel(const float* state, 
 
 #ifndef TW
 #define TW 8
-#define TWB 8
-#define MM_C2 0
+#define TWB 4
 #endif
 constexpr int kTileWaves = TW, kTileWavesBwd = TWB;         // of the tiles of longer sequences
 constexpr int kMaxBatch = 65535;  // grid y
@@ -629,18 +686,19 @@ static int check_workspace(const mm_gated_scan_params* p, size_t need) {
 // ------------------------------------------------------------------------------ shapes of a call
 struct Shape {
   int waves;
-  int64_t ncb, nstrips, nturns, handoff_bytes;
+  int64_t ncb, nstrips, nturns, control_bytes, handoff_bytes;
 };
-// C channels a lane.  Sequences of up to `most` blocks of 16 tokens are one tile: no hand-off, one launch.
-static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, int C, bool backward) {
+// Sequences of up to `most` blocks of 16 tokens are one tile: no hand-off, one launch.
+static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward) {
   const int most = backward ? kMaxWavesBwd : kMaxWaves;
   const int64_t nblk = ceil_div(seqlen > 0 ? seqlen : 1, kBlk);
   Shape s;
   s.waves = nblk <= most ? static_cast<int>(nblk) : backward ? kTileWavesBwd : kTileWaves;
-  s.ncb = ceil_div(dim, 64 * C);
+  s.ncb = ceil_div(dim, 64);
   s.nstrips = batch * s.ncb;
   s.nturns = ceil_div(nblk, s.waves);
-  s.handoff_bytes = s.nturns > 1 ? kControlBytes + s.nturns * s.nstrips * (2 * 64 * C * 8) : 0;
+  s.control_bytes = kControlBytes * (1 + s.nstrips);
+  s.handoff_bytes = s.nturns > 1 ? s.control_bytes + s.nturns * s.nstrips * (2 * 64 * 8) : 0;
   return s;
 }
 static int64_t dA_bytes(const Shape& s, int64_t batch, int64_t dim) { return round_up(rows::floats(batch * s.nturns, dim) * 4, 256); }
@@ -649,7 +707,7 @@ static int prepare(Launch& k, const mm_gated_scan_params* p, const Shape& s, cha
   if (s.nstrips * s.nturns > 0x7fffffff) return fail(MM_ERR_SHAPE, "too many elements");
   k.p = *p;
   k.hd.control = reinterpret_cast<uint32_t*>(handoff);
-  k.hd.word = reinterpret_cast<unsigned long long*>(handoff + kControlBytes);
+  k.hd.word = reinterpret_cast<unsigned long long*>(handoff + s.control_bytes);
   k.hd.status = p->status;
   if (s.nturns > 1) {
     static DeviceCache cache;
@@ -676,17 +734,6 @@ static int prepare(Launch& k, const mm_gated_scan_params* p, const Shape& s, cha
   return MM_OK;
 }
 
-// Whether lanes may take two neighbouring channels: pairs of them are aligned in every tensor.
-static bool pairs_ok(const mm_gated_scan_params* p) {
-  const int64_t vb = 2 * dtype_size(p->dtype);
-  const void* ptr[5] = {p->x, p->a_gate, p->x_gate, p->z, p->y};
-  const int64_t* st[5] = {p->x_stride, p->a_gate_stride, p->x_gate_stride, p->z_stride, p->y_stride};
-  if (p->dim % 2 != 0) return false;
-  for (int k = 0; k < 5; ++k)
-    if (ptr[k] && (!aligned(ptr[k], vb) || st[k][0] % 2 != 0 || st[k][1] % 2 != 0)) return false;
-  return true;
-}
-
 }  // namespace gscan
 }  // namespace mm
 
@@ -695,10 +742,8 @@ extern "C" {
 size_t mm_gated_scan_workspace_size(int64_t batch, int64_t seqlen, int64_t dim, int32_t backward) {
   using namespace mm::gscan;
   if (batch <= 0 || seqlen < 0 || dim <= 0 || !sizes_ok(batch, seqlen, dim)) return 0;
-  const Shape s = shape_of(batch, seqlen, dim, 1, backward != 0);
-  if (backward) return static_cast<size_t>(dA_bytes(s, batch, dim) + s.handoff_bytes);
-  const Shape s2 = shape_of(batch, seqlen, dim, 2, false);
-  return static_cast<size_t>(s2.handoff_bytes > s.handoff_bytes ? s2.handoff_bytes : s.handoff_bytes);
+  const Shape s = shape_of(batch, seqlen, dim, backward != 0);
+  return static_cast<size_t>((backward ? dA_bytes(s, batch, dim) : 0) + s.handoff_bytes);
 }
 
 int mm_gated_scan_fwd(const mm_gated_scan_params* p, void* stream) {
@@ -716,27 +761,24 @@ int mm_gated_scan_fwd(const mm_gated_scan_params* p, void* stream) {
   }
   if ((e = check_workspace(p, mm_gated_scan_workspace_size(p->batch, p->seqlen, p->dim, 0))) != MM_OK) return e;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int C = pairs_ok(p) && MM_C2 ? 2 : 1;
-  const Shape s = shape_of(p->batch, p->seqlen, p->dim, C, false);
+  const Shape s = shape_of(p->batch, p->seqlen, p->dim, false);
   Launch k{};
   if ((e = prepare(k, p, s, static_cast<char*>(p->workspace), st)) != MM_OK) return e;
   const dim3 grid(static_cast<unsigned>(s.nstrips * s.nturns)), block(64 * s.waves);
   const bool p8 = p->codes[0] != nullptr && p->seqlen > 0;
-#define MM_GS1(D, C, Z, P8) hipLaunchKernelGGL((fwd_kernel<D, C, Z, P8>), grid, block, 0, st, k)
-#define MM_GS2(D, C, Z) \
-  if (p8) MM_GS1(D, C, Z, true); else MM_GS1(D, C, Z, false)
-#define MM_GS3(D, C) \
-  if (p->z) { MM_GS2(D, C, true); } else { MM_GS2(D, C, false); }
-#define MM_GS(D) \
-  if (C == 2) { MM_GS3(D, 2) } else { MM_GS3(D, 1) }
+#define MM_GS1(D, Z, P8) hipLaunchKernelGGL((fwd_kernel<D, Z, P8>), grid, block, 0, st, k)
+#define MM_GS(D)                                                 \
+  if (p8) {                                                      \
+    if (p->z) MM_GS1(D, true, true); else MM_GS1(D, false, true);   \
+  } else {                                                       \
+    if (p->z) MM_GS1(D, true, false); else MM_GS1(D, false, false); \
+  }
   switch (p->dtype) {
     case MM_F32: MM_GS(MM_F32); break;
     case MM_F16: MM_GS(MM_F16); break;
     default: MM_GS(MM_BF16); break;
   }
 #undef MM_GS
-#undef MM_GS3
-#undef MM_GS2
 #undef MM_GS1
   return check_launch("gated_scan_fwd");
 }
@@ -760,7 +802,7 @@ int mm_gated_scan_bwd(const mm_gated_scan_params* p, void* stream) {
   }
   if ((e = check_workspace(p, mm_gated_scan_workspace_size(p->batch, p->seqlen, p->dim, 1))) != MM_OK) return e;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const Shape s = shape_of(p->batch, p->seqlen, p->dim, 1, true);
+  const Shape s = shape_of(p->batch, p->seqlen, p->dim, true);
   Launch k{};
   k.dA_part = static_cast<float*>(p->workspace);
   if ((e = prepare(k, p, s, static_cast<char*>(p->workspace) + dA_bytes(s, p->batch, p->dim), st)) != MM_OK) return e;
