@@ -73,14 +73,10 @@ struct Block {
     w = *reinterpret_cast<const uint4*>(codes + static_cast<uint64_t>(d) * kBlk);
     e = exps[d];
   }
-  // code + 128 as unsigned bytes, which convert to float in one instruction
-  __device__ __forceinline__ void prepare() {
-    w.x ^= 0x80808080u, w.y ^= 0x80808080u, w.z ^= 0x80808080u, w.w ^= 0x80808080u;
-    scale = scale_of(e);
-  }
+  __device__ __forceinline__ void prepare() { scale = scale_of(e); }
   __device__ __forceinline__ float value(int k) const {
     const uint32_t v = k < 4 ? w.x : k < 8 ? w.y : k < 12 ? w.z : w.w;
-    return (static_cast<float>((v >> (8 * (k % 4))) & 0xffu) - 128.0f) * scale;
+    return static_cast<float>(static_cast<int8_t>(v >> (8 * (k % 4)))) * scale;
   }
 };
 

@@ -25,7 +25,7 @@ namespace gscan {
 
 constexpr int kBlk = MM_ACT8_BLOCK;  // tokens of a wave
 constexpr int kMaxWaves = 16;        // of a forward tile
-constexpr int kMaxWavesBwd = 8;      // of a backward tile
+constexpr int kMaxWavesBwd = 4;      // of a backward tile
 constexpr int kWindow = 16;          // tiles that a tile looks back at
 constexpr int kStepThreads = 64;
 #ifndef BWD_EU
@@ -53,8 +53,10 @@ __device__ __forceinline__ void decay(float l, float& a, float& beta2) {
   s = __builtin_fmaf(s, l, 1.0f);
   const float e = exp2_hw(l * kLog2e);
   const bool near = l > (wide ? -0.25f : -0.0625f);
-  const float q = near ? -l * s : 1.0f - e;
-  a = near ? 1.0f - q : e;
+  const float q_near = -l * s, q_far = 1.0f - e;  // (both by name: as operands of ?: they became branches)
+  const float q = near ? q_near : q_far;
+  const float a_near = 1.0f - q;
+  a = near ? a_near : e;
   beta2 = q * (1.0f + a);
 }
 // A as the kernels use it: A r stays finite at A = -inf (a = 0 all the same, and 0 * l = 0), a NaN stays.
@@ -139,20 +141,25 @@ __device__ __forceinline__ bool peek_error(const Handoff& hd) {
   return __hip_atomic_load(&hd.control[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
 }
 
-// The tile's claim: a workgroup's strip of channels is fixed, its turn in time the next of its strip.
+// The tile's claim: a workgroup's strip of channels is fixed, its turn in time the next of its strip.  Workgroups
+// go to the chip's 8 dies in turn: with per_die > 0 each die takes per_die neighbouring strips, whose rows share
+// DRAM pages and lines (16-row tiles of 128-byte rows: 4.65 -> 5.25 TB/s of plain copying); strips past the last
+// have no tile.
 struct Claim {
   uint32_t strip, turn;
 };
-__device__ __forceinline__ Claim claim(const Handoff& hd, uint32_t nstrips, uint32_t nturns) {
+constexpr uint32_t kDies = 8;
+__device__ __forceinline__ bool claim(const Handoff& hd, uint32_t nstrips, uint32_t per_die, uint32_t nturns, Claim& cl) {
   __shared__ uint32_t s_turn;
-  uint32_t turn = 0;
-  const uint32_t strip = blockIdx.x % nstrips;
+  cl.turn = 0;
+  cl.strip = per_die ? blockIdx.x % kDies * per_die + blockIdx.x / kDies % per_die : blockIdx.x % nstrips;
+  if (cl.strip >= nstrips) return false;
   if (nturns > 1) {
-    if (threadIdx.x == 0) s_turn = atomicAdd(&hd.control[(1 + strip) * (kControlBytes / 4)], 1u);
+    if (threadIdx.x == 0) s_turn = atomicAdd(&hd.control[(1 + cl.strip) * (kControlBytes / 4)], 1u);
     __syncthreads();
-    turn = __builtin_amdgcn_readfirstlane(s_turn);
+    cl.turn = __builtin_amdgcn_readfirstlane(s_turn);
   }
-  return {strip, turn};
+  return true;
 }
 
 // What a wave does between its tile's composition and the state before the tile: the waves fetch the kWindow
@@ -228,6 +235,7 @@ struct Launch {
   mm_gated_scan_params p;
   Handoff hd;
   float* dA_part;
+  uint32_t per_die;               // claim's
   uint32_t nstrips, nturns, ncb;  // strips of 64 channels of a sequence, tiles of a strip, strips a sequence
   int32_t waves;
 };
@@ -242,7 +250,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
   __shared__ float2 s_pair[kMaxWaves][64];
   __shared__ float2 s_back[kWindow][64];
   const mm_gated_scan_params& p = k.p;
-  const Claim cl = claim(k.hd, k.nstrips, k.nturns);
+  Claim cl;
+  if (!claim(k.hd, k.nstrips, k.per_die, k.nturns, cl)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t b = cl.strip / k.ncb;
   // lanes past the last channel do what the last one's does, stores and all
@@ -297,10 +306,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
         a = t0 + t < len ? a : 1.0f;
         bu = t0 + t < len ? bu : 0.0f;
       }
-      E[t] = P = P * a;
-      H[t] = Q = __builtin_fmaf(a, Q, bu);
-      keep(E[t]);
-      keep(H[t]);
+      P *= a;
+      Q = __builtin_fmaf(a, Q, bu);
+      keep(P);
+      keep(Q);
+      E[t] = P;
+      H[t] = Q;
       if constexpr (Z) zr[t] = raw[3][t];
     }
   };
@@ -397,9 +408,12 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, BWD_EU) void bwd_kernel(const La
   constexpr int N = Z ? 4 : 3;
   __shared__ float2 s_pair[kMaxWavesBwd][64];
   __shared__ float2 s_back[kWindow][64];
+  // A lane's own f r, and c3 of the first 12 tokens: 28 registers less, which 4 waves a SIMD do not have
+  __shared__ float4 s_c4[kMaxWavesBwd][kBlk / 4][64], s_c3[kMaxWavesBwd][3][64];
   __shared__ float s_dA[kMaxWavesBwd][64];
   const mm_gated_scan_params& p = k.p;
-  const Claim cl = claim(k.hd, k.nstrips, k.nturns);
+  Claim cl;
+  if (!claim(k.hd, k.nstrips, k.per_die, k.nturns, cl)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t b = cl.strip / k.ncb;
   const uint32_t d = min((cl.strip % k.ncb) * 64 + lane, static_cast<uint32_t>(p.dim - 1));
@@ -448,7 +462,7 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, BWD_EU) void bwd_kernel(const La
       else v = Ty<DT>::f(raw[j][t]);
       return full || t0 + t < len ? v : 0.0f;
     };
-    float a[kBlk], c4[kBlk];
+    float a[kBlk], c4[4];
     Rows<DT> dzp(p.dz, row, p.dim);
 #pragma unroll
     for (int t = 0; t < kBlk; t += 2) {
@@ -462,12 +476,13 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, BWD_EU) void bwd_kernel(const La
         decay<DT>(l, a[tt], beta2);
         // 1 / beta, or 0 at a = 1, where the root has no slope (and where beta^2 is below the smallest normal
         // number, whose reciprocal root the instruction takes as infinite; a NaN stays one)
-        const float ib = fabsf(beta2) < 1.17549435e-38f ? 0.0f : __builtin_amdgcn_rsqf(beta2);
+        const float root = __builtin_amdgcn_rsqf(beta2);
+        const float ib = fabsf(beta2) < 1.17549435e-38f ? 0.0f : root;
         const float beta = beta2 * ib, u = i * x, bu = beta * u;
         const float f = __builtin_fmaf(h, a[tt], -u * (a[tt] * a[tt] * ib));
         c1[tt] = i * beta;
         c2[tt] = __builtin_fmaf(-bu, i, bu);
-        c4[tt] = f * r;
+        c4[tt % 4] = f * r;
         c3[tt] = f * __builtin_fmaf(-l, r, l);
         const float hn = __builtin_fmaf(a[tt], h, bu);
         h = in ? hn : h;
@@ -483,7 +498,7 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, BWD_EU) void bwd_kernel(const La
           c1[tt] = in ? c1[tt] : 0.0f;
           c2[tt] = in ? c2[tt] : 0.0f;
           c3[tt] = in ? c3[tt] : 0.0f;
-          c4[tt] = in ? c4[tt] : 0.0f;
+          c4[tt % 4] = in ? c4[tt % 4] : 0.0f;
         }
       }
       if constexpr (Z) {
@@ -499,16 +514,24 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, BWD_EU) void bwd_kernel(const La
       for (int c = 0; c < 2; ++c) {
         keep(c1[t + c]);
         keep(c2[t + c]);
-        keep(c3[t + c]);
-        keep(c4[t + c]);
+        if (t >= 12) keep(c3[t + c]);
+      }
+      if (t % 4 == 2) {
+        s_c4[wave][t / 4][lane] = make_float4(c4[0], c4[1], c4[2], c4[3]);
+        if (t < 12) s_c3[wave][t / 4][lane] = make_float4(c3[t - 2], c3[t - 1], c3[t], c3[t + 1]);
       }
     }
+    float4 q4[kBlk / 4];
+#pragma unroll
+    for (int t = 0; t < kBlk / 4; ++t) q4[t] = s_c4[wave][t][lane];
 #pragma unroll
     for (int t = kBlk - 1; t >= 0; --t) {
       E[t] = P;
       G[t] += Q;
-      dA_c = __builtin_fmaf(P, c4[t], dA_c);
-      dA_0 = __builtin_fmaf(G[t], c4[t], dA_0);
+      const float4 q = q4[t / 4];
+      const float c = t % 4 == 0 ? q.x : t % 4 == 1 ? q.y : t % 4 == 2 ? q.z : q.w;
+      dA_c = __builtin_fmaf(P, c, dA_c);
+      dA_0 = __builtin_fmaf(G[t], c, dA_0);
       P *= a[t];
       Q = a[t] * G[t];
     }
@@ -551,6 +574,11 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, BWD_EU) void bwd_kernel(const La
   auto finish = [&](auto full_c) __attribute__((always_inline)) {
     constexpr bool full = decltype(full_c)::value;
     Rows<DT> o[3] = {{p.dx, row, p.dim}, {p.dx_gate, row, p.dim}, {p.da_gate, row, p.dim}};
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {
+      const float4 q = s_c3[wave][t][lane];
+      c3[4 * t] = q.x, c3[4 * t + 1] = q.y, c3[4 * t + 2] = q.z, c3[4 * t + 3] = q.w;
+    }
 #pragma unroll
     for (int t = 0; t < kBlk; t += 2) {
       float v[3][2];
@@ -686,7 +714,7 @@ static int check_workspace(const mm_gated_scan_params* p, size_t need) {
 // ------------------------------------------------------------------------------ shapes of a call
 struct Shape {
   int waves;
-  int64_t ncb, nstrips, nturns, control_bytes, handoff_bytes;
+  int64_t ncb, per_die, tiles, nstrips, nturns, control_bytes, handoff_bytes;
 };
 // Sequences of up to `most` blocks of 16 tokens are one tile: no hand-off, one launch.
 static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward) {
@@ -697,6 +725,10 @@ static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward)
   s.ncb = ceil_div(dim, 64);
   s.nstrips = batch * s.ncb;
   s.nturns = ceil_div(nblk, s.waves);
+  // neighbouring strips on one die where that leaves no more than an eighth of the workgroups without a tile
+  s.per_die = ceil_div(s.nstrips, int64_t{kDies});
+  if (8 * kDies * s.per_die > 9 * s.nstrips) s.per_die = 0;
+  s.tiles = s.nturns * (s.per_die ? kDies * s.per_die : s.nstrips);
   s.control_bytes = kControlBytes * (1 + s.nstrips);
   s.handoff_bytes = s.nturns > 1 ? s.control_bytes + s.nturns * s.nstrips * (2 * 64 * 8) : 0;
   return s;
@@ -704,7 +736,7 @@ static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward)
 static int64_t dA_bytes(const Shape& s, int64_t batch, int64_t dim) { return round_up(rows::floats(batch * s.nturns, dim) * 4, 256); }
 
 static int prepare(Launch& k, const mm_gated_scan_params* p, const Shape& s, char* handoff, hipStream_t stream) {
-  if (s.nstrips * s.nturns > 0x7fffffff) return fail(MM_ERR_SHAPE, "too many elements");
+  if (s.tiles > 0x7fffffff) return fail(MM_ERR_SHAPE, "too many elements");
   k.p = *p;
   k.hd.control = reinterpret_cast<uint32_t*>(handoff);
   k.hd.word = reinterpret_cast<unsigned long long*>(handoff + s.control_bytes);
@@ -730,6 +762,7 @@ static int prepare(Launch& k, const mm_gated_scan_params* p, const Shape& s, cha
   k.nstrips = static_cast<uint32_t>(s.nstrips);
   k.nturns = static_cast<uint32_t>(s.nturns);
   k.ncb = static_cast<uint32_t>(s.ncb);
+  k.per_die = static_cast<uint32_t>(s.per_die);
   k.waves = s.waves;
   return MM_OK;
 }
@@ -764,7 +797,7 @@ int mm_gated_scan_fwd(const mm_gated_scan_params* p, void* stream) {
   const Shape s = shape_of(p->batch, p->seqlen, p->dim, false);
   Launch k{};
   if ((e = prepare(k, p, s, static_cast<char*>(p->workspace), st)) != MM_OK) return e;
-  const dim3 grid(static_cast<unsigned>(s.nstrips * s.nturns)), block(64 * s.waves);
+  const dim3 grid(static_cast<unsigned>(s.tiles)), block(64 * s.waves);
   const bool p8 = p->codes[0] != nullptr && p->seqlen > 0;
 #define MM_GS1(D, Z, P8) hipLaunchKernelGGL((fwd_kernel<D, Z, P8>), grid, block, 0, st, k)
 #define MM_GS(D)                                                 \
@@ -806,7 +839,7 @@ int mm_gated_scan_bwd(const mm_gated_scan_params* p, void* stream) {
   Launch k{};
   k.dA_part = static_cast<float*>(p->workspace);
   if ((e = prepare(k, p, s, static_cast<char*>(p->workspace) + dA_bytes(s, p->batch, p->dim), st)) != MM_OK) return e;
-  const dim3 grid(static_cast<unsigned>(s.nstrips * s.nturns)), block(64 * s.waves);
+  const dim3 grid(static_cast<unsigned>(s.tiles)), block(64 * s.waves);
 #define MM_GS1(D, Z, C) hipLaunchKernelGGL((bwd_kernel<D, Z, C>), grid, block, 0, st, k)
 #define MM_GS(D)                                            \
   if (c8) {                                                 \
