@@ -485,6 +485,15 @@ int mm_causal_conv1d_bwd(const void* x, const int8_t* x_codes, const uint8_t* x_
                          const int64_t w_stride[2], int32_t x_dtype, int32_t w_dtype,
                          int32_t apply_silu, void* workspace, size_t workspace_bytes, void* stream);
 
+/* mm_causal_conv1d_fwd that also keeps its input as an 8-bit checkpoint (mm_act8_pack's x_codes and x_exps) for
+ * mm_causal_conv1d_bwd, in the same pass over x.  x: strides (batch, time), unit channel stride; out (batch, seqlen,
+ * dim) contiguous, the same bits as mm_causal_conv1d_fwd's; weight and bias as there. */
+int mm_causal_conv1d_fwd_act8(const void* x, const void* weight, const void* bias, void* out,
+                              int8_t* x_codes, uint8_t* x_exps, int64_t batch, int64_t seqlen,
+                              int64_t dim, int64_t width, const int64_t x_stride[2],
+                              const int64_t w_stride[2], int32_t x_dtype, int32_t w_dtype,
+                              int32_t apply_silu, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

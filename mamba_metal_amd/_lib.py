@@ -137,6 +137,8 @@ _SIGNATURES = {
     "mm_gated_scan_step": ([_vp] * 8 + [_i64] * 7 + [_i32, _vp], ctypes.c_int),
     "mm_act8_pack": ([_vp] * 3 + [_i64] * 3 + [_i64a2, _i32, _vp], ctypes.c_int),
     "mm_act8_unpack": ([_vp] * 3 + [_i64] * 3 + [_i64a2, _i32, _vp], ctypes.c_int),
+    "mm_causal_conv1d_fwd_act8": (
+        [_vp] * 6 + [_i64] * 4 + [_i64a2, _i64a2, _i32, _i32, _i32, _vp], ctypes.c_int),
     "mm_causal_conv1d_bwd_workspace_size": ([_i64] * 4, _sz),
     "mm_causal_conv1d_bwd": (
         [_vp] * 9 + [_i64] * 4 + [_i64a2, _i64a2, _i64a2, _i32, _i32, _i32, _vp, _sz, _vp], ctypes.c_int),

@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from mamba_metal_amd import _lib
-from mamba_metal_amd.act8 import Act8, act8_pack, channels_last
+from mamba_metal_amd.act8 import Act8, channels_last, empty_like
 
 
 def _w2d(weight):
@@ -109,15 +109,31 @@ def _conv1d_backward(x, packed, weight, bias, dout, apply_silu, want_dx, want_dw
     return dx, None if dw is None else dw.view(weight.shape), db
 
 
+def _conv1d_act8(x, weight, bias, apply_silu):
+    """causal_conv1d's output and x's 8-bit codes, in one pass over x."""
+    lib = _lib.load()
+    dev = _lib.require_cuda(x, weight, bias)
+    w, ws = _w2d(weight)
+    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    packed = empty_like(x)
+    with _lib.on_device(dev):
+        st = lib.mm_causal_conv1d_fwd_act8(
+            x.data_ptr(), w.data_ptr(), _lib.ptr(bias), out.data_ptr(), packed.codes.data_ptr(),
+            packed.exps.data_ptr(), *x.shape, w.shape[1], (_lib._i64a2)(*x.stride()[:2]), ws,
+            _lib.dtype_code(x.dtype), _lib.dtype_code(w.dtype), 1 if apply_silu else 0, _lib.stream_of(dev))
+    _lib.check(st, "mm_causal_conv1d_fwd_act8")
+    return out, packed
+
+
 class _CausalConv1d(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, apply_silu, checkpoint):
-        out = causal_conv1d(x, weight, bias, apply_silu=apply_silu)
         ctx.meta = (x.dtype, x.shape, apply_silu)
         if checkpoint == "int8":
-            packed = act8_pack(x)
+            out, packed = _conv1d_act8(x, weight, bias, apply_silu)
             ctx.save_for_backward(weight, bias, packed.codes, packed.exps)
         else:
+            out = causal_conv1d(x, weight, bias, apply_silu=apply_silu)
             ctx.save_for_backward(weight, bias, x)
         return out
 
@@ -151,4 +167,6 @@ def causal_conv1d_train(x, weight, bias=None, *, apply_silu=True, checkpoint="fu
         raise ValueError(f"checkpoint must be 'full' or 'int8', got {checkpoint!r}")
     _lib.dtype_code(x.dtype)
     _lib.dtype_code(weight.dtype)
+    if bias is not None and (bias.shape != (x.shape[2],) or bias.dtype != weight.dtype or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous (dim,) tensor of the weight's dtype")
     return _CausalConv1d.apply(x, weight, bias, apply_silu, checkpoint)

@@ -105,13 +105,17 @@ def test_act8_refuses():
     (dict(checkpoint="half"), ValueError),
     (dict(x=z3(2, 5, 4, dtype=torch.float64)), TypeError),
     (dict(weight=z3(4, 1, 4, dtype=torch.float64)), TypeError),
+    (dict(bias=z3(5)), ValueError),
+    (dict(bias=z3(4, dtype=torch.float16)), ValueError),
+    (dict(bias=z3(8)[::2]), ValueError),
     (dict(), ValueError),
+    (dict(checkpoint="int8"), ValueError),
 ])
 def test_conv_refuses(kw, err):
-    a = dict(x=z3(2, 5, 4), weight=z3(4, 1, 4), checkpoint="full")
+    a = dict(x=z3(2, 5, 4), weight=z3(4, 1, 4), checkpoint="full", bias=None)
     a.update(kw)
     with pytest.raises(err):
-        causal_conv1d_train(a["x"], a["weight"], checkpoint=a["checkpoint"])
+        causal_conv1d_train(a["x"], a["weight"], a["bias"], checkpoint=a["checkpoint"])
 
 
 # ------------------------------------------------------------------------------ the C entry points
@@ -231,3 +235,22 @@ def conv(lib, **over):
 ])
 def test_conv_c_refuses(lib, over, status):
     assert conv(lib, **over) == status
+
+
+def conv_fwd(lib, **over):
+    two = _lib._i64a2
+    a = dict(x=FAKE, w=FAKE, b=None, out=FAKE, codes=FAKE, exps=FAKE, batch=2, seqlen=100, dim=64, width=4,
+             xs=two(6400, 64), ws=two(4, 1), xdt=0, wdt=0, silu=1)
+    a.update(over)
+    return lib.mm_causal_conv1d_fwd_act8(*a.values(), None)
+
+
+def test_conv_fwd_act8_c_refuses(lib):
+    for k in ("x", "w", "out", "codes", "exps"):
+        assert conv_fwd(lib, **{k: None}) == _lib.ERR_NULL_POINTER, k
+    assert conv_fwd(lib, width=9) == _lib.ERR_SHAPE
+    assert conv_fwd(lib, dim=-1) == _lib.ERR_SHAPE
+    assert conv_fwd(lib, wdt=3) == _lib.ERR_DTYPE
+    assert conv_fwd(lib, codes=FAKE + 8) == _lib.ERR_LAYOUT
+    assert conv_fwd(lib, xs=(_lib._i64a2)(-1, 64)) == _lib.ERR_LAYOUT
+    assert conv_fwd(lib, seqlen=0, x=None) == _lib.OK
