@@ -19,6 +19,7 @@ namespace convb {
 
 constexpr int kThreads = 256;
 constexpr int kB = act8::kBlk;  // tokens loaded at once
+constexpr int kS = 8;             // tokens in registers at once, backward
 constexpr int kMaxW = 8;
 
 struct Params {
@@ -36,9 +37,11 @@ struct Params {
   int32_t w_dtype, silu;
 };
 
-// Tokens of a run: 64, and fewer where that leaves the chip with less than 8 waves a CU.
-static int64_t run_of(int64_t batch, int64_t seqlen, int64_t dim) {
-  int64_t run = 64;
+// Tokens of a run: 64 forward, 128 backward, where tokens done twice and partial sums are one in so many (8 x 2048 x
+// 5120: 64 114 + 7 us with the sum, 128 107 + 4, 256 107 + 4), and fewer where that leaves the chip with less
+// than 8 waves a CU.
+static int64_t run_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward) {
+  int64_t run = backward ? 128 : 64;
   while (run > kB && batch * ceil_div(seqlen, run) * ceil_div(dim, 64) < 2048) run /= 2;
   return run;
 }
@@ -105,46 +108,50 @@ __global__ __launch_bounds__(kThreads) void conv1d_bwd_kernel(const Params p) {
     w[k] = ld_any(p.w, d * p.ws0 + k * p.ws1, p.w_dtype);
     dw[k] = 0.0f;
   }
-  // x[t + k0 + k], k < n, of the block of 16 tokens from t on
-  auto load_x = [&](float* x, int64_t t, auto k0_c, auto n_c) __attribute__((always_inline)) {
-    constexpr int k0 = decltype(k0_c)::value, n = decltype(n_c)::value;
-    if constexpr (C8) {
-      const int64_t o = (b * at.nblk + t / kB) * p.dim;
-      act8::Block q;
-      q.load(p.codes + o * kB, p.exps + o, d);
-      q.prepare();
-#pragma unroll
-      for (int k = 0; k < n; ++k) x[k] = q.value(k0 + k);
-    } else {
-      load_rows<DT, n>(x, p.x, p.xs, b, t + k0, p.seqlen, off);
-    }
-  };
   using std::integral_constant;
-  float x[H + kB], dp[H + kB];  // tokens t - H .. t + 15
+  // Tokens t - H .. t + kS - 1: half a block at a time, so that eight waves a SIMD have the registers.
+  float x[H + kS], dp[H + kS];
 #pragma unroll
   for (int k = 0; k < H; ++k) x[k] = dp[k] = 0.0f;
-  if (H > 0 && at.t0 > 0) load_x(x, at.t0 - kB, integral_constant<int, kB - H>{}, integral_constant<int, H>{});
-  // tokens t + k, k < n: p, dp, the sums (`own` tokens only) and dx of H tokens earlier
-  auto tokens = [&](int64_t t, auto n_c, auto own_c) __attribute__((always_inline)) {
-    constexpr int n = decltype(n_c)::value;
+  act8::Block xc;  // the block of 16 tokens
+  auto fetch = [&](int64_t t) __attribute__((always_inline)) {
+    const int64_t o = (b * at.nblk + t / kB) * p.dim;
+    xc.load(p.codes + o * kB, p.exps + o, d);
+    xc.prepare();
+  };
+  if (H > 0 && at.t0 > 0) {
+    if constexpr (C8) {
+      fetch(at.t0 - kB);
+#pragma unroll
+      for (int k = 0; k < H; ++k) x[k] = xc.value(kB - H + k);
+    } else {
+      load_rows<DT, H>(x, p.x, p.xs, b, at.t0 - H, p.seqlen, off);
+    }
+  }
+  // tokens t + k, k < n, from the block's token k0 on: p, dp, the sums (`own` tokens only) and dx of H tokens earlier
+  auto tokens = [&](int64_t t, auto k0_c, auto n_c, auto own_c) __attribute__((always_inline)) {
+    constexpr int k0 = decltype(k0_c)::value, n = decltype(n_c)::value;
     constexpr bool own = decltype(own_c)::value;
     float dy[n];
     load_rows<DT, n>(dy, p.dout, p.ds, b, t, p.seqlen, off);
-    load_x(x + H, t, integral_constant<int, 0>{}, n_c);
+    if constexpr (C8) {
+#pragma unroll
+      for (int k = 0; k < n; ++k) x[H + k] = xc.value(k0 + k);
+    } else {
+      load_rows<DT, n>(x + H, p.x, p.xs, b, t, p.seqlen, off);
+    }
     Rows<DT> out(p.dx, b * p.seqlen + t - H, p.dim);
     auto walk = [&](auto whole_c) __attribute__((always_inline)) {
       constexpr bool whole = decltype(whole_c)::value;  // all tokens and their dx are the run's
 #pragma unroll
       for (int k = 0; k < n; ++k) {
         const bool in = whole || t + k < p.seqlen;
-        float s = 1.0f;
-        if (p.silu) {  // silu'
-          float v = bias;
+        float v = bias;
 #pragma unroll
-          for (int q = 0; q < K; ++q) v = __builtin_fmaf(w[q], x[k + q], v);
-          s = rcp_hw(1.0f + exp2_hw(-v * kLog2e));
-          s *= __builtin_fmaf(v, 1.0f - s, 1.0f);
-        }
+        for (int q = 0; q < K; ++q) v = __builtin_fmaf(w[q], x[k + q], v);
+        float s = rcp_hw(1.0f + exp2_hw(-v * kLog2e));
+        s *= __builtin_fmaf(v, 1.0f - s, 1.0f);  // silu'
+        s = p.silu ? s : 1.0f;
         dp[H + k] = in ? dy[k] * s : 0.0f;
         if constexpr (own) {
           db += dp[H + k];
@@ -152,31 +159,35 @@ __global__ __launch_bounds__(kThreads) void conv1d_bwd_kernel(const Params p) {
           for (int q = 0; q < K; ++q) dw[q] = __builtin_fmaf(dp[H + k], in ? x[k + q] : 0.0f, dw[q]);
         }
         const int64_t o = t + k - H;
-        if (whole || (o >= at.t0 && o < at.t1)) {
-          if (p.dx != nullptr) {
-            float u = 0.0f;
+        if (p.dx != nullptr && (whole || (o >= at.t0 && o < at.t1))) {
+          float u = 0.0f;
 #pragma unroll
-            for (int q = 0; q < K; ++q) u = __builtin_fmaf(w[q], dp[H + k - q], u);
-            T v, unused;
-            round2<DT>(u, 0.0f, v, unused);
-            out.store(off, v);
-          }
+          for (int q = 0; q < K; ++q) u = __builtin_fmaf(w[q], dp[H + k - q], u);
+          T r, unused;
+          round2<DT>(u, 0.0f, r, unused);
+          out.store(off, r);
         }
         out.next();
       }
     };
-    if (t - H >= at.t0 && t + n <= p.seqlen && t + n - H <= at.t1) walk(std::true_type{});
+    const bool whole = t - H >= at.t0 && t + n <= p.seqlen && t + n - H <= at.t1;
+    if (whole) walk(std::true_type{});
     else walk(std::false_type{});
 #pragma unroll
     for (int k = 0; k < H; ++k) x[k] = x[n + k], dp[k] = dp[n + k];
   };
-  for (int64_t t = at.t0; t < at.t1; t += kB) tokens(t, integral_constant<int, kB>{}, std::true_type{});
+  for (int64_t t = at.t0; t < at.t1; t += kB) {
+    if constexpr (C8) fetch(t);
+    tokens(t, integral_constant<int, 0>{}, integral_constant<int, kS>{}, std::true_type{});
+    if (t + kS < at.t1) tokens(t + kS, integral_constant<int, kS>{}, integral_constant<int, kS>{}, std::true_type{});
+  }
   // the last H tokens' dx: up to H tokens of the next run, or zeros
   if constexpr (H > 0) {
-    const int64_t end = (at.t1 + kB - 1) / kB * kB;
+    const int64_t end = (at.t1 + kS - 1) / kS * kS;  // of the tokens walked
     if (p.dx != nullptr) {
       if (end < p.seqlen) {
-        tokens(end, integral_constant<int, H>{}, std::false_type{});
+        if constexpr (C8) fetch(end);
+        tokens(end, integral_constant<int, 0>{}, integral_constant<int, H>{}, std::false_type{});
       } else {
         Rows<DT> out(p.dx, b * p.seqlen + end - H, p.dim);
 #pragma unroll
@@ -268,7 +279,7 @@ static bool sizes_ok(int64_t batch, int64_t seqlen, int64_t dim) {
 static int prepare(Params& p, const void* x, const int8_t* codes, const uint8_t* exps, const void* weight, const void* bias,
                    const void* dout, int64_t batch, int64_t seqlen, int64_t dim, int64_t width, const int64_t x_stride[2],
                    const int64_t dout_stride[2], const int64_t w_stride[2], int32_t x_dtype, int32_t w_dtype,
-                   int32_t apply_silu) {
+                   int32_t apply_silu, bool backward) {
   if (batch < 0 || seqlen < 0 || dim < 0) return fail(MM_ERR_SHAPE, "negative size");
   if (width < 1 || width > kMaxW) return fail(MM_ERR_SHAPE, "width=%lld not in 1..%d", (long long)width, kMaxW);
   if (!sizes_ok(batch, seqlen, dim)) return fail(MM_ERR_SHAPE, "too many elements");
@@ -290,7 +301,7 @@ static int prepare(Params& p, const void* x, const int8_t* codes, const uint8_t*
   p.dout = dout;
   p.seqlen = seqlen;
   p.dim = dim;
-  p.run = run_of(batch, seqlen, dim);
+  p.run = run_of(batch, seqlen, dim, backward);
   p.nruns = ceil_div(seqlen, p.run);
   for (int k = 0; k < 2; ++k) p.xs[k] = x ? x_stride[k] : 0, p.ds[k] = dout_stride[k];
   p.ws0 = w_stride[0], p.ws1 = w_stride[1];
@@ -329,7 +340,7 @@ size_t mm_causal_conv1d_bwd_workspace_size(int64_t batch, int64_t seqlen, int64_
   using namespace mm;
   using namespace mm::convb;
   if (!sizes_ok(batch, seqlen, dim) || width < 1 || width > kMaxW) return 0;
-  return static_cast<size_t>(rows::floats(batch * ceil_div(seqlen, run_of(batch, seqlen, dim)), (width + 1) * dim) * 4);
+  return static_cast<size_t>(rows::floats(batch * ceil_div(seqlen, run_of(batch, seqlen, dim, true)), (width + 1) * dim) * 4);
 }
 
 int mm_causal_conv1d_bwd(const void* x, const int8_t* x_codes, const uint8_t* x_exps,
@@ -343,7 +354,7 @@ int mm_causal_conv1d_bwd(const void* x, const int8_t* x_codes, const uint8_t* x_
   clear_error();
   Params p{};
   int e = prepare(p, x, x ? nullptr : x_codes, x ? nullptr : x_exps, weight, bias, dout, batch, seqlen, dim, width, x_stride,
-                  dout_stride, w_stride, x_dtype, w_dtype, apply_silu);
+                  dout_stride, w_stride, x_dtype, w_dtype, apply_silu, true);
   if (e != MM_OK) return e;
   if (dbias && !dw) return fail(MM_ERR_NULL_POINTER, "dbias needs dw");
   if (dim == 0 || (!dx && !dw)) return MM_OK;
@@ -383,7 +394,7 @@ int mm_causal_conv1d_fwd_act8(const void* x, const void* weight, const void* bia
   Params p{};
   const int64_t out_stride[2] = {0, 0};  // contiguous
   const int e = prepare(p, x, x_codes, x_exps, weight, bias, out, batch, seqlen, dim, width, x_stride, out_stride, w_stride,
-                        x_dtype, w_dtype, apply_silu);
+                        x_dtype, w_dtype, apply_silu, false);
   if (e != MM_OK || batch == 0 || seqlen == 0 || dim == 0) return e;
   if (!x || !x_codes) return fail(MM_ERR_NULL_POINTER, "x, x_codes and x_exps are required");
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -25,13 +25,12 @@ namespace mm {
 namespace gscan {
 
 constexpr int kBlk = MM_ACT8_BLOCK;  // tokens of a wave
-constexpr int kMaxWaves = 16;        // of a forward tile
-constexpr int kMaxWavesBwd = 4;      // of a backward tile
+// Waves of a tile.  Forward 16 where they hold the whole sequence (one tile, no hand-off), else 8: with 4 a sequence
+// has twice the tiles to hand on (1 x 32768 x 64 29 -> 51 us, 1 x 8192 x 5120 111 -> 114), and 5 or 6 load the SIMDs
+// unevenly (133 us).  Backward 4, so that four workgroups share a CU's registers and LDS.
+constexpr int kMaxWaves = 16, kTileWaves = 8, kMaxWavesBwd = 4;
 constexpr int kWindow = 16;          // tiles that a tile looks back at
 constexpr int kStepThreads = 64;
-#ifndef BWD_EU
-#define BWD_EU 4
-#endif
 
 
 __device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp2_hw(-x * kLog2e)); }
@@ -118,12 +117,30 @@ __device__ __forceinline__ bool claim(const Handoff& hd, uint32_t nstrips, uint3
   return true;
 }
 
+// f of the lane's pairs v[lo] .. v[hi - 1], or in reverse, eight LDS reads in flight at a time.
+__device__ __forceinline__ float2 lane_pair(const float2 (*v)[64], int j) { return v[j][threadIdx.x & 63]; }
+template <bool BACK, typename F>
+__device__ __forceinline__ void each_pair(const float2 (*v)[64], int lo, int hi, F f) {  // lo .. hi - 1, or hi - 1 .. lo
+  for (int j0 = 0; j0 < hi - lo; j0 += 8) {
+    float2 q[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int j = j0 + k < hi - lo ? j0 + k : 0;
+      q[k] = lane_pair(v, BACK ? hi - 1 - j : lo + j);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (j0 + k < hi - lo) f(q[k]);
+  }
+}
+
 // What a wave does between its tile's composition and the state before the tile: the waves fetch the kWindow
 // tiles before it into s_back[distance - 1], a pair, or a state with P = -1 (a product of decays is never
 // negative).  A wave's tiles are polled together, so that it takes one round trip where all are there.  The wait
 // is bounded by wall-clock time and sets the status word if it expires, which is not expected: the tiles waited
 // for are running or done.  At least kMinWaves waves.
 constexpr int kMinWaves = 4, kPolls = kWindow / kMinWaves;
+constexpr uint64_t kLongWait = 10000;  // ticks, 100 us
 __device__ __forceinline__ void look_back(const Handoff& hd, uint32_t turn, uint32_t strip, uint32_t nstrips, int wave,
                                           int waves, float2 (&s_back)[kWindow][64]) {
   const int lane = threadIdx.x & 63;
@@ -158,8 +175,10 @@ __device__ __forceinline__ void look_back(const Handoff& hd, uint32_t turn, uint
       }
     }
     if (!again) break;
-    // one expired wait of the call makes the others return at once
-    if (wall_clock64() - t_start > hd.spin_ticks || peek_error(hd)) {
+    // one expired wait of the call makes the others return soon (a look at its word is another round trip, so only
+    // a wait that is already long takes it)
+    const uint64_t waited = wall_clock64() - t_start;
+    if (waited > hd.spin_ticks || (waited > kLongWait && peek_error(hd))) {
       __hip_atomic_store(&hd.control[0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       if (hd.status != nullptr)
         __hip_atomic_fetch_or(hd.status, MM_SCAN_STATUS_HANDOFF_TIMEOUT, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -173,12 +192,11 @@ __device__ __forceinline__ void look_back(const Handoff& hd, uint32_t turn, uint
 }
 // The state before the tile from what look_back fetched, first tile first.
 __device__ __forceinline__ float fold_back(uint32_t turn, const float2 (&s_back)[kWindow][64]) {
-  const int lane = threadIdx.x & 63, far = turn < kWindow ? static_cast<int>(turn) : kWindow;
   float h = 0.0f;
-  for (int j = far - 1; j >= 0; --j) {
-    const float2 v = s_back[j][lane];
-    h = v.x < 0.0f ? v.y : __builtin_fmaf(v.x, h, v.y);
-  }
+  each_pair<true>(s_back, 0, turn < kWindow ? static_cast<int>(turn) : kWindow, [&](const float2& v) __attribute__((always_inline)) {
+    const float joined = __builtin_fmaf(v.x, h, v.y);
+    h = v.x < 0.0f ? v.y : joined;
+  });
   return h;
 }
 
@@ -285,11 +303,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
   unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 128 + lane;
   const bool more = cl.turn + 1 < k.nturns;
   if (more && wave == 0) {
-    for (int w = 0; w < k.waves; ++w) {
-      const float2 v = s_pair[w][lane];
+    each_pair<false>(s_pair, 0, k.waves, [&](const float2& v) __attribute__((always_inline)) {
       tp *= v.x;
       tq = __builtin_fmaf(v.x, tq, v.y);
-    }
+    });
     if (cl.turn > 0) {
       publish(mine + 64, tp, kPair);
       publish(mine, tq, kPair);
@@ -303,10 +320,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
     h = fold_back(cl.turn, s_back);
   }
   if (more && wave == 0) publish(mine, __builtin_fmaf(tp, h, tq), kState);
-  for (int w = 0; w < wave; ++w) {
-    const float2 v = s_pair[w][lane];
-    h = __builtin_fmaf(v.x, h, v.y);
-  }
+  each_pair<false>(s_pair, 0, wave, [&](const float2& v) __attribute__((always_inline)) { h = __builtin_fmaf(v.x, h, v.y); });
   if (here && p.block_states != nullptr) (p.block_states + (b * nblk + blk) * p.dim)[d] = h;
 
   float last = h;
@@ -359,7 +373,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
 // with f = h_{t-1} a - u a^2 / beta, and dA is c (sum of E f r) + (sum of G f r): five numbers a token and two more
 // are all that is kept in registers over the wait.
 template <int DT, bool Z, bool C8>
-__global__ __launch_bounds__(64 * kMaxWavesBwd, BWD_EU) void bwd_kernel(const Launch k) {
+__global__ __launch_bounds__(64 * kMaxWavesBwd, 4) void bwd_kernel(const Launch k) {
   using T = typename Ty<DT>::T;
   constexpr int N = Z ? 4 : 3;
   __shared__ float2 s_pair[kMaxWavesBwd][64];
@@ -504,11 +518,10 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, BWD_EU) void bwd_kernel(const La
   unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 128 + lane;
   const bool more = cl.turn + 1 < k.nturns;
   if (more && wave == 0) {
-    for (int w = k.waves - 1; w >= 0; --w) {
-      const float2 v = s_pair[w][lane];
+    each_pair<true>(s_pair, 0, k.waves, [&](const float2& v) __attribute__((always_inline)) {
       tp *= v.x;
       tq = __builtin_fmaf(v.x, tq, v.y);
-    }
+    });
     if (cl.turn > 0) {
       publish(mine + 64, tp, kPair);
       publish(mine, tq, kPair);
@@ -522,10 +535,7 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, BWD_EU) void bwd_kernel(const La
     carry = fold_back(cl.turn, s_back);
   }
   if (more && wave == 0) publish(mine, __builtin_fmaf(tp, carry, tq), kState);
-  for (int w = k.waves - 1; w > wave; --w) {
-    const float2 v = s_pair[w][lane];
-    carry = __builtin_fmaf(v.x, carry, v.y);
-  }
+  each_pair<true>(s_pair, wave + 1, k.waves, [&](const float2& v) __attribute__((always_inline)) { carry = __builtin_fmaf(v.x, carry, v.y); });
 
   auto finish = [&](auto full_c) __attribute__((always_inline)) {
     constexpr bool full = decltype(full_c)::value;
@@ -602,11 +612,6 @@ __global__ __launch_bounds__(kStepThreads) void step_kernel(const float* state, 
   st<DT>(y, b * ys + d, z ? h * silu_f(ld<DT>(z, b * zs + d)) : h);
 }
 
-#ifndef TW
-#define TW 8
-#define TWB 4
-#endif
-constexpr int kTileWaves = TW, kTileWavesBwd = TWB;         // of the tiles of longer sequences
 constexpr int kMaxBatch = 65535;  // grid y
 
 // Sizes whose products below stay within 64 bits: the element count, times what a workspace takes of each.
@@ -677,7 +682,7 @@ static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward)
   const int most = backward ? kMaxWavesBwd : kMaxWaves;
   const int64_t nblk = ceil_div(seqlen > 0 ? seqlen : 1, kBlk);
   Shape s;
-  s.waves = nblk <= most ? static_cast<int>(nblk) : backward ? kTileWavesBwd : kTileWaves;
+  s.waves = nblk <= most ? static_cast<int>(nblk) : backward ? kMaxWavesBwd : kTileWaves;
   s.ncb = ceil_div(dim, 64);
   s.nstrips = batch * s.ncb;
   s.nturns = ceil_div(nblk, s.waves);
