@@ -10,123 +10,141 @@ input carries no gate.  Arithmetic and states are float32 for every dtype.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from mamba_metal_amd import _lib
-from mamba_metal_amd.act8 import BLOCK, Act8, channels_last, empty_like
+from mamba_metal_amd.act8 import BLOCK, channels_last
 from mamba_metal_amd.selective_scan import _status_word
 
 CHECKPOINTS = ("full", "int8")
-_INPUTS = ("x", "a_gate", "x_gate", "z")
+_two = _lib._i64a2
 
 
-def _strides2(t):
-    s = t.stride()
-    return (_lib._i64a2)(s[0], s[1])
-
-
-def _params(tensors, A, h0, lengths, dtype, shape, dev) -> _lib.GatedScanParams:
+def _params(A, lengths, dtype, shape, dev) -> _lib.GatedScanParams:
     p = _lib.GatedScanParams()
-    for name, t in zip(_INPUTS, tensors):
-        if t is not None:
-            setattr(p, name, t.data_ptr())
-            setattr(p, f"{name}_stride", _strides2(t))
-    p.A, p.h0, p.lengths = A.data_ptr(), _lib.ptr(h0), _lib.ptr(lengths)
+    p.A = A.data_ptr()
+    if lengths is not None:
+        p.lengths = lengths.data_ptr()
+        p.lengths_dtype = 1 if lengths.dtype == torch.int64 else 0
     p.batch, p.seqlen, p.dim = shape
     p.dtype = _lib.dtype_code(dtype)
-    p.lengths_dtype = 1 if lengths is not None and lengths.dtype == torch.int64 else 0
     p.status = _status_word(dev).data_ptr()
     return p
 
 
-def _set_codes(p, packed):
-    for k, c in enumerate(packed):
-        p.codes[k], p.exps[k] = c.codes.data_ptr(), c.exps.data_ptr()
+def _set_inputs(p, x, a_gate, x_gate, z):
+    p.x, p.x_stride = x.data_ptr(), _two(*x.stride()[:2])
+    p.a_gate, p.a_gate_stride = a_gate.data_ptr(), _two(*a_gate.stride()[:2])
+    p.x_gate, p.x_gate_stride = x_gate.data_ptr(), _two(*x_gate.stride()[:2])
+    if z is not None:
+        p.z, p.z_stride = z.data_ptr(), _two(*z.stride()[:2])
+
+
+def _set_codes(p, codes, exps):
+    """codes (inputs, batch, blocks, dim, 16) and exps (inputs, batch, blocks, dim): act8_pack's of each input."""
+    n = len(codes)
+    if codes.numel():
+        step = exps.numel() // n
+        c, e = codes.data_ptr(), exps.data_ptr()
+        for k in range(n):
+            p.codes[k], p.exps[k] = c + k * step * BLOCK, e + k * step
 
 
 def _call(name, p, backward, dev):
     lib = _lib.load()
     nbytes = lib.mm_gated_scan_workspace_size(p.batch, p.seqlen, p.dim, backward)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    p.workspace, p.workspace_bytes = _lib.ptr(ws), nbytes
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
     with _lib.on_device(dev):
-        st = getattr(lib, name)(ctypes.byref(p), _lib.stream_of(dev))
+        st = getattr(lib, name)(p, _lib.stream_of(dev))
     _lib.check(st, name)
 
 
-def _forward(x, a_gate, x_gate, A, z, h0, lengths, want_state, train, checkpoint):
+def _forward(dev, x, a_gate, x_gate, A, z, h0, lengths, want_state, train, checkpoint):
     """y, the final state (or None) and, for training, the block states and the inputs' 8-bit codes."""
-    dev = _lib.require_cuda(x, a_gate, x_gate, A, z, h0, lengths)
     b, n, d = x.shape
-    p = _params((x, a_gate, x_gate, z), A, h0, lengths, x.dtype, x.shape, dev)
+    p = _params(A, lengths, x.dtype, (b, n, d), dev)
+    _set_inputs(p, x, a_gate, x_gate, z)
     y = torch.empty((b, n, d), dtype=x.dtype, device=dev)
-    p.y, p.y_stride = y.data_ptr(), _strides2(y)
-    f32 = {"dtype": torch.float32, "device": dev}
-    state = torch.empty((b, d), **f32) if want_state else None
-    p.state_out = _lib.ptr(state)
-    blocks, packed = None, []
+    p.y, p.y_stride = y.data_ptr(), _two(n * d, d)
+    state = blocks = codes = exps = None
+    if h0 is not None:
+        p.h0 = h0.data_ptr()
+    if want_state:
+        state = torch.empty((b, d), dtype=torch.float32, device=dev)
+        p.state_out = state.data_ptr()
     if train:
-        blocks = torch.empty((b, -(-n // BLOCK), d), **f32)
+        nblk = -(-n // BLOCK)
+        blocks = torch.empty((b, nblk, d), dtype=torch.float32, device=dev)
         p.block_states = blocks.data_ptr()
         if checkpoint == "int8":
-            packed = [empty_like(t) for t in (x, a_gate, x_gate, z) if t is not None]
-            _set_codes(p, packed)
+            k = 3 if z is None else 4
+            codes = torch.empty((k, b, nblk, d, BLOCK), dtype=torch.int8, device=dev)
+            exps = torch.empty((k, b, nblk, d), dtype=torch.uint8, device=dev)
+            _set_codes(p, codes, exps)
     _call("mm_gated_scan_fwd", p, 0, dev)
-    return y, state, blocks, packed
+    return y, state, blocks, codes, exps
 
 
-def _backward(tensors, packed, A, lengths, blocks, dtype, shape, gated, dy, dstate, want_dh0):
-    dev = blocks.device
+def _backward(dev, inputs, codes, exps, A, lengths, blocks, dtype, shape, gated, dy, dstate, want_dh0):
+    """Gradients of x, a_gate, x_gate, z (or None), A and h0 (or None); ``inputs`` or their codes."""
     b, n, d = shape
-    p = _params(tensors, A, None, lengths, dtype, shape, dev)
+    p = _params(A, lengths, dtype, shape, dev)
     p.block_states = blocks.data_ptr()
-    _set_codes(p, packed)
-    p.z_present = 1 if gated else 0
+    if codes is not None:
+        _set_codes(p, codes, exps)
+        p.z_present = 1 if gated else 0
+    else:
+        _set_inputs(p, *inputs)
     if dy is None:  # only the final state was used
         dy = torch.zeros((1, 1, d), dtype=dtype, device=dev).expand(b, n, d)
     elif dy.dtype != dtype or (dy.stride(-1) != 1 and d > 1):
         dy = dy.to(dtype).contiguous()
-    p.dy, p.dy_stride = dy.data_ptr(), _strides2(dy)
+    p.dy, p.dy_stride = dy.data_ptr(), _two(*dy.stride()[:2])
     if dstate is not None:
         dstate = dstate.contiguous()
         p.dstate = dstate.data_ptr()
-    grads = [torch.empty((b, n, d), dtype=dtype, device=dev) if k < 3 or gated else None for k in range(4)]
-    p.dx, p.da_gate, p.dx_gate, p.dz = (_lib.ptr(t) for t in grads)
+    dx = torch.empty((b, n, d), dtype=dtype, device=dev)
+    da, dg = torch.empty_like(dx), torch.empty_like(dx)
+    p.dx, p.da_gate, p.dx_gate = dx.data_ptr(), da.data_ptr(), dg.data_ptr()
+    dz = dh0 = None
+    if gated:
+        dz = torch.empty_like(dx)
+        p.dz = dz.data_ptr()
     dA = (torch.empty if b else torch.zeros)((d,), dtype=torch.float32, device=dev)
-    dh0 = torch.empty((b, d), dtype=torch.float32, device=dev) if want_dh0 else None
-    p.dA, p.dh0 = dA.data_ptr(), _lib.ptr(dh0)
+    p.dA = dA.data_ptr()
+    if want_dh0:
+        dh0 = torch.empty((b, d), dtype=torch.float32, device=dev)
+        p.dh0 = dh0.data_ptr()
     _call("mm_gated_scan_bwd", p, 1, dev)
-    return grads, dA, dh0
+    return dx, da, dg, dA, dz, dh0
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, a_gate, x_gate, A, z, h0, lengths, checkpoint):
-        y, state, blocks, packed = _forward(x, a_gate, x_gate, A, z, h0, lengths, True, True, checkpoint)
-        ctx.meta = (x.dtype, x.shape, z is not None, len(packed))
+    def forward(ctx, dev, x, a_gate, x_gate, A, z, h0, lengths, want_state, checkpoint):
+        y, state, blocks, codes, exps = _forward(dev, x, a_gate, x_gate, A, z, h0, lengths, want_state, True, checkpoint)
+        ctx.meta = (dev, x.dtype, x.shape, z is not None)
         ctx.set_materialize_grads(False)
-        kept = [t for c in packed for t in (c.codes, c.exps)] if packed else [x, a_gate, x_gate, z]
-        ctx.save_for_backward(A, lengths, blocks, *kept)
-        return y, state
+        if codes is not None:
+            ctx.save_for_backward(A, lengths, blocks, codes, exps)
+        else:
+            ctx.save_for_backward(A, lengths, blocks, x, a_gate, x_gate, z)
+        return (y, state) if want_state else y
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dy, dstate):
+    def backward(ctx, dy, dstate=None):
         if dy is None and dstate is None:
-            return (None,) * 8
-        dtype, shape, gated, npacked = ctx.meta
+            return (None,) * 10
+        dev, dtype, shape, gated = ctx.meta
         A, lengths, blocks, *kept = ctx.saved_tensors
-        if npacked:
-            packed = [Act8(kept[2 * k], kept[2 * k + 1], shape, dtype) for k in range(npacked)]
-            tensors = ()
-        else:
-            packed, tensors = (), kept
-        (dx, da, dg, dz), dA, dh0 = _backward(tensors, packed, A, lengths, blocks, dtype, shape, gated, dy, dstate,
-                                              ctx.needs_input_grad[5])
-        return dx, da, dg, dA, dz, dh0, None, None
+        inputs, codes, exps = (None, *kept) if len(kept) == 2 else (kept, None, None)
+        grads = _backward(dev, inputs, codes, exps, A, lengths, blocks, dtype, shape, gated, dy, dstate,
+                          ctx.needs_input_grad[6])
+        return None, *grads, None, None, None
 
 
 def _f32(t):
@@ -159,27 +177,33 @@ def gated_scan(x: torch.Tensor, a_gate: torch.Tensor, x_gate: torch.Tensor, A: t
     if x.dim() != 3:
         raise ValueError(f"x must be (batch, seqlen, dim), got {tuple(x.shape)}")
     b, _, d = x.shape
-    for name, t in (("x", x), ("a_gate", a_gate), ("x_gate", x_gate), ("z", z)):
-        if t is None:
-            continue
-        if t.shape != x.shape:
-            raise ValueError(f"{name} is {tuple(t.shape)}, x {tuple(x.shape)}")
-        if t.dtype != x.dtype:
-            raise TypeError(f"{name} is {t.dtype}, x {x.dtype}")
-        channels_last(t, name)
+    _check_alike(x, (("a_gate", a_gate), ("x_gate", x_gate), ("z", z)))
     _lib.dtype_code(x.dtype)
     _check_rest(A, h0, lengths, b, d)
     if checkpoint not in CHECKPOINTS:
         raise ValueError(f"checkpoint must be one of {CHECKPOINTS}, got {checkpoint!r}")
-    _lib.require_cuda(x, a_gate, x_gate, A, z, h0, lengths)
+    dev = _lib.require_cuda(x, a_gate, x_gate, A, z, h0, lengths)
     A = _f32(A).contiguous()
     h0 = None if h0 is None else _f32(h0).contiguous()
     lengths = None if lengths is None else lengths.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, a_gate, x_gate, A, z, h0)):
-        y, state = _GatedScan.apply(x, a_gate, x_gate, A, z, h0, lengths, checkpoint)
-    else:
-        y, state, _, _ = _forward(x, a_gate, x_gate, A, z, h0, lengths, return_state, False, checkpoint)
+        return _GatedScan.apply(dev, x, a_gate, x_gate, A, z, h0, lengths, return_state, checkpoint)
+    y, state, *_ = _forward(dev, x, a_gate, x_gate, A, z, h0, lengths, return_state, False, checkpoint)
     return (y, state) if return_state else y
+
+
+def _check_alike(x, others):
+    """x has unit channel stride, and the others its shape, its dtype and that."""
+    shape, dtype = x.shape, x.dtype
+    channels_last(x, "x")
+    for name, t in others:
+        if t is None:
+            continue
+        if t.shape != shape:
+            raise ValueError(f"{name} is {tuple(t.shape)}, x {tuple(shape)}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} is {t.dtype}, x {dtype}")
+        channels_last(t, name)
 
 
 def _check_rest(A, h0, lengths, b, d):
@@ -210,25 +234,20 @@ def gated_scan_step(state: torch.Tensor, x: torch.Tensor, a_gate: torch.Tensor, 
     if x.dim() != 2:
         raise ValueError(f"x must be (batch, dim), got {tuple(x.shape)}")
     b, d = x.shape
-    for name, t in (("x", x), ("a_gate", a_gate), ("x_gate", x_gate), ("z", z), ("out", out)):
-        if t is None:
-            continue
-        if t.shape != x.shape:
-            raise ValueError(f"{name} is {tuple(t.shape)}, x {tuple(x.shape)}")
-        if t.dtype != x.dtype:
-            raise TypeError(f"{name} is {t.dtype}, x {x.dtype}")
-        channels_last(t, name)
+    _check_alike(x, (("a_gate", a_gate), ("x_gate", x_gate), ("z", z), ("out", out)))
     for name, t in (("state", state), ("state_out", state_out)):
         if t is not None and (t.shape != (b, d) or t.dtype != torch.float32 or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous float32 {(b, d)}")
     code = _lib.dtype_code(x.dtype)
     _check_rest(A, None, None, b, d)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (state, x, a_gate, x_gate, A, z)):
+    if torch.is_grad_enabled() and (state.requires_grad or x.requires_grad or a_gate.requires_grad
+                                    or x_gate.requires_grad or A.requires_grad or (z is not None and z.requires_grad)):
         raise RuntimeError("gated_scan_step has no gradient: call it under no_grad or inference_mode, "
                            "or train through gated_scan")
     dev = _lib.require_cuda(state, x, a_gate, x_gate, A, z, state_out, out)
     lib = _lib.load()
-    A = _f32(A).contiguous()
+    if A.dtype != torch.float32 or not A.is_contiguous():
+        A = A.float().contiguous()
     if out is None:
         out = torch.empty((b, d), dtype=x.dtype, device=dev)
     with _lib.on_device(dev):
