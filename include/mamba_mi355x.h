@@ -390,8 +390,8 @@ int mm_pair_scan(const float* a, const float* b, float* a_out, float* h_out, int
  * (>= 0), unit channel stride.  States (batch, dim) contiguous fp32.  lengths (batch,), int32 or
  * int64 (lengths_dtype), NULL = all seqlen: tokens from lengths[b] on (taken as clamped to
  * [0, seqlen]) leave the state as it is, have y = 0 and gradients 0, and their inputs' values do
- * not matter (they are read).  Arithmetic and states are fp32.  Outputs must not overlap inputs.
- * seqlen 0: state_out is h0.
+ * not matter (they may be read).  Arithmetic and states are fp32.  Outputs must not overlap inputs.
+ * seqlen 0: state_out is h0.  batch at most 65535.
  *
  * Training: the forward call given block_states writes there the state before every 16th token,
  * (batch, ceil(seqlen / 16), dim) contiguous fp32, from which the backward call recomputes the

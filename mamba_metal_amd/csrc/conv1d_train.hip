@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kThreads) void conv1d_fwd_act8_kernel(const Params 
 // dw[c, k] and dbias[c] from the runs' sums, rows of [K + 1][dim].
 __global__ __launch_bounds__(64 * rows::kGroups) void reduce_kernel(const float* part, void* dw, void* dbias, int64_t nrows,
                                                                   int64_t dim, int width, int32_t w_dtype) {
-  rows::sum_columns(part, nrows, (width + 1) * dim, nrows, [&](int64_t c, double s) {
+  rows::sum_columns(part, nrows, (width + 1) * dim, blockIdx.x, 0, nrows, [&](int64_t c, double s) {
     const int64_t k = c / dim, d = c % dim;
     if (k < width) st_any(dw, d * width + k, static_cast<float>(s), w_dtype);
     else if (dbias != nullptr) st_any(dbias, d, static_cast<float>(s), w_dtype);

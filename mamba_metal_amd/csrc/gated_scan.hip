@@ -594,7 +594,7 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, 4) void bwd_kernel(const Launch 
 }
 
 __global__ __launch_bounds__(64 * rows::kGroups) void dA_kernel(const float* part, float* dA, int64_t nrows, int64_t dim) {
-  rows::sum_columns(part, nrows, dim, nrows, [&](int64_t c, double s) { dA[c] = static_cast<float>(s); });
+  rows::sum_columns(part, nrows, dim, blockIdx.x, 0, nrows, [&](int64_t c, double s) { dA[c] = static_cast<float>(s); });
 }
 
 template <int DT>

@@ -83,10 +83,17 @@ def test_strides(dev):
 
 
 @pytest.mark.parametrize("shape", [(0, 5, 4), (2, 0, 4), (2, 5, 0)])
-def test_empty(dev, shape):
+@pytest.mark.parametrize("checkpoint", ["full", "int8"])
+def test_empty(dev, shape, checkpoint):
     f = rand(5, *shape, 4, torch.float32, dev)
-    y, got = train(f)
+    y, got = train(f, checkpoint=checkpoint)
     assert y.shape == shape and got["x"].shape == shape and not got["weight"].any() and not got["bias"].any()
+
+
+def test_many_rows_of_partial_sums(dev):
+    """Enough runs that the sums' rows go through two passes."""
+    f = rand(10, 700, 17, 9, 4, torch.float32, dev)
+    check(f, *train(f))
 
 
 def test_nan_stays_in_its_channel(dev):

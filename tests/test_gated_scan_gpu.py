@@ -355,6 +355,88 @@ def test_two_graphs_share_nothing(dev):
             assert torch.equal(w[0], o[0]) and torch.equal(w[1], o[1])
 
 
+def test_offsets_past_32_bits(dev):
+    """More than 2^31 outputs; the inputs are one token broadcast over time, so h_t = b (1 - a^t) / (1 - a)."""
+    n, d = 530_000, 4096
+    g = torch.Generator().manual_seed(45)
+    token = {k: torch.randn((1, 1, d), generator=g).to(torch.bfloat16).to(dev) for k in ("x", "a_gate", "x_gate")}
+    leaves = {k: v.expand(1, n, d) for k, v in token.items()}
+    A = (-0.1 - torch.rand(d, generator=g)).to(dev).requires_grad_(True)
+    y, state = gated_scan(leaves["x"], leaves["a_gate"], leaves["x_gate"], A, return_state=True, checkpoint="int8")
+    assert y.numel() > 2 ** 31
+    c = ref.Case(*(t.expand(1, 400, d) for t in token.values()), A)
+    wy, ey, wh, eh = c.forward()
+    ref.close(y[:, :400], wy, ey, torch.bfloat16, "first tokens")
+    r, i, l, a, beta, u, *_ = c.elements()
+    assert (1 - a).min() > 0.009
+    limit = (beta * u / (1 - a))[:, :1]
+    # a token adds at most 10 u of error to a and the state, the state remembers 1 / (1 - a) < 112 of them, and b has
+    # 25 u of its own: 1150 u < 1e-4; bf16 half a step, 2^-8
+    assert ((state[:, None].cpu().double() - limit).abs() <= 1e-4 * limit.abs() + 1e-30).all()
+    assert torch.equal(y[:, -1], state.to(torch.bfloat16))
+    # gradient of the last token alone: 2000 tokens before it a^t < 2e-8 of it is left
+    dy = torch.zeros((1, n, d), dtype=torch.bfloat16, device=dev)
+    dy[:, -1] = 1.0
+    dA, = torch.autograd.grad(y, A, dy)
+    tail = ref.Case(*(t.expand(1, 2000, d) for t in token.values()), A, h0=limit[:, 0])
+    want, bound = tail.backward(torch.cat([torch.zeros((1, 1999, d)), torch.ones((1, 1, d))], 1), eight=True)["A"]
+    # the reference starts from the limit, the kernel from its state: 1e-4 of each token's part
+    assert ((dA.cpu().double() - want).abs() <= bound + 2e-4 * want.abs()).all()
+
+
+def test_expired_waits_end_the_call(dev):
+    """A wait bound of a microsecond, from the C interface: the call ends, and says so where it gave up."""
+    b, n, d = 2, 6000, 128
+    f = rand(46, b, n, d, torch.float32, dev, z=False)
+    want, _ = gated_scan(f["x"], f["a_gate"], f["x_gate"], f["A"], return_state=True)
+    y, status = torch.empty_like(want), torch.zeros(1, dtype=torch.int32, device=dev)
+    lib, p = _lib.load(), _lib.GatedScanParams()
+    for k in ("x", "a_gate", "x_gate"):
+        setattr(p, k, f[k].data_ptr())
+        setattr(p, f"{k}_stride", (_lib._i64a2)(n * d, d))
+    p.A, p.y, p.y_stride, p.status = f["A"].data_ptr(), y.data_ptr(), (_lib._i64a2)(n * d, d), status.data_ptr()
+    p.batch, p.seqlen, p.dim, p.handoff_timeout_us = b, n, d, 1
+    nbytes = lib.mm_gated_scan_workspace_size(b, n, d, 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+    _lib.check(lib.mm_gated_scan_fwd(p, _lib.stream_of(dev)), "mm_gated_scan_fwd")
+    torch.cuda.synchronize()
+    assert status.item() in (0, _lib.SCAN_STATUS_HANDOFF_TIMEOUT)
+    if status.item() == 0:
+        assert torch.equal(y, want)
+    # the next call is a good one again, in the same workspace
+    p.handoff_timeout_us = 0
+    status.zero_()
+    _lib.check(lib.mm_gated_scan_fwd(p, _lib.stream_of(dev)), "mm_gated_scan_fwd")
+    torch.cuda.synchronize()
+    assert status.item() == 0 and torch.equal(y, want)
+
+
+def test_many_rows_of_partial_sums(dev):
+    """Enough tiles that dA's rows go through two passes."""
+    f = rand(47, 40, 900, 10, torch.float32, dev)
+    y, state, got = train(f)
+    check_grads(case(f), f, got, torch.float32)
+
+
+def test_no_second_derivative(dev):
+    f = rand(48, 1, 20, 64, torch.float32, dev)
+    x = f["x"].clone().requires_grad_(True)
+    y = gated_scan(x, f["a_gate"], f["x_gate"], f["A"])
+    dx, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
+def test_backward_twice_with_a_kept_graph(dev):
+    f = rand(49, 2, 300, 70, torch.float16, dev)
+    leaves = {k: f[k].clone().requires_grad_(True) for k in ("x", "a_gate", "x_gate", "A", "z")}
+    y = gated_scan(leaves["x"], leaves["a_gate"], leaves["x_gate"], leaves["A"], z=leaves["z"], checkpoint="int8")
+    first = torch.autograd.grad(y, list(leaves.values()), f["dy"], retain_graph=True)
+    again = torch.autograd.grad(y, list(leaves.values()), f["dy"])
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
 def test_saved_inputs_are_guarded(dev):
     """An input changed between the passes is an error, as for any torch operator; codes do not care."""
     f = rand(50, 1, 20, 64, torch.float32, dev)
