@@ -71,27 +71,27 @@ __device__ __forceinline__ int64_t length_of(const mm_gated_scan_params& p, int6
 
 
 // ------------------------------------------------------------------------------ the tiles' hand-off
-// Workspace: [control: an expired wait, then each strip's next turn, a line each][a pair of words for each tile
-// and channel].  One counter for all tiles bounded the forward pass at about 25 ns a tile.  A word is a float and a tag
-// in one 64-bit access, so a reader that sees the tag has the value: no fence, no cache write-back.
+// Workspace: [control: an expired wait, then each strip's next turn, a line each][a word for each tile and channel].
+// One counter for all tiles bounded the forward pass at about 25 ns a tile.  A word is the pair (P, Q), or (-1, the
+// state after the tile): a product of decays is never negative.  It is one 64-bit access, so a reader has both or
+// neither: no fence, no cache write-back.  All zeros is a word that is not there yet, and a P of 0 is written as -0.
 constexpr int kControlBytes = 128;
-constexpr uint32_t kPair = 1, kState = 2;  // tags: (P, Q) so far, the state after the tile
+constexpr int kWordsBytes = 64 * 8;  // of a tile
 
 struct Handoff {
   uint32_t* control;
-  unsigned long long* word; // [tile][2: Q or state, P][64]
+  unsigned long long* word; // [tile][64]
   uint64_t spin_ticks;
   int32_t* status;
 };
 
-__device__ __forceinline__ void publish(unsigned long long* w, float v, uint32_t tag) {
-  __hip_atomic_store(w, static_cast<unsigned long long>(tag) << 32 | __float_as_uint(v), __ATOMIC_RELAXED,
+__device__ __forceinline__ void publish(unsigned long long* w, float p, float q) {
+  __hip_atomic_store(w, static_cast<unsigned long long>(__float_as_uint(p)) << 32 | __float_as_uint(q), __ATOMIC_RELAXED,
                      __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ unsigned long long peek(const unsigned long long* w) {
   return __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-
 __device__ __forceinline__ bool peek_error(const Handoff& hd) {
   return __hip_atomic_load(&hd.control[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
 }
@@ -135,8 +135,7 @@ __device__ __forceinline__ void each_pair(const float2 (*v)[64], int lo, int hi,
 }
 
 // What a wave does between its tile's composition and the state before the tile: the waves fetch the kWindow
-// tiles before it into s_back[distance - 1], a pair, or a state with P = -1 (a product of decays is never
-// negative).  A wave's tiles are polled together, so that it takes one round trip where all are there.  The wait
+// tiles before it into s_back[distance - 1], a pair or a state (P = -1).  A wave's tiles are polled together, so that it takes one round trip where all are there.  The wait
 // is bounded by wall-clock time and sets the status word if it expires, which is not expected: the tiles waited
 // for are running or done.  At least kMinWaves waves.
 constexpr int kMinWaves = 4, kPolls = kWindow / kMinWaves;
@@ -145,30 +144,28 @@ __device__ __forceinline__ void look_back(const Handoff& hd, uint32_t turn, uint
                                           int waves, float2 (&s_back)[kWindow][64]) {
   const int lane = threadIdx.x & 63;
   const unsigned long long* w[kPolls];
-  unsigned long long q[kPolls], pw[kPolls];
+  unsigned long long q[kPolls];
   bool need[kPolls];
 #pragma unroll
   for (int k = 0; k < kPolls; ++k) {
     const int j = wave + k * waves;
     need[k] = j < kWindow && static_cast<uint32_t>(j) < turn;
-    w[k] = hd.word + (static_cast<uint64_t>(need[k] ? turn - 1 - j : turn) * nstrips + strip) * 128 + lane;
+    w[k] = hd.word + (static_cast<uint64_t>(need[k] ? turn - 1 - j : turn) * nstrips + strip) * 64 + lane;
   }
   const uint64_t t_start = wall_clock64();
   for (;;) {
 #pragma unroll
     for (int k = 0; k < kPolls; ++k)
-      if (need[k]) q[k] = peek(w[k]), pw[k] = peek(w[k] + 64);
+      if (need[k]) q[k] = peek(w[k]);
     bool again = false;
 #pragma unroll
     for (int k = 0; k < kPolls; ++k) {
       if (!need[k]) continue;
       const int j = wave + k * waves;
-      const uint32_t tag = static_cast<uint32_t>(q[k] >> 32);
+      const float pk = __uint_as_float(static_cast<uint32_t>(q[k] >> 32));
       // the farthest tile's state is needed, of the others the pair will do
-      const bool pair = tag == kPair && j != kWindow - 1 && static_cast<uint32_t>(pw[k] >> 32) == kPair;
-      if (__all(tag == kState || pair)) {
-        s_back[j][lane] = make_float2(tag == kState ? -1.0f : __uint_as_float(static_cast<uint32_t>(pw[k])),
-                                      __uint_as_float(static_cast<uint32_t>(q[k])));
+      if (__all(j == kWindow - 1 ? pk < 0.0f : q[k] >> 32 != 0)) {
+        s_back[j][lane] = make_float2(pk, __uint_as_float(static_cast<uint32_t>(q[k])));
         need[k] = false;
       } else {
         again = true;
@@ -300,17 +297,15 @@ __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
     __syncthreads();
   }
   float tp = 1.0f, tq = 0.0f;
-  unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 128 + lane;
+  unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 64 + lane;
   const bool more = cl.turn + 1 < k.nturns;
   if (more && wave == 0) {
     each_pair<false>(s_pair, 0, k.waves, [&](const float2& v) __attribute__((always_inline)) {
       tp *= v.x;
       tq = __builtin_fmaf(v.x, tq, v.y);
     });
-    if (cl.turn > 0) {
-      publish(mine + 64, tp, kPair);
-      publish(mine, tq, kPair);
-    }
+    tp = tp == 0.0f ? -0.0f : tp;
+    if (cl.turn > 0) publish(mine, tp, tq);
   }
   if (cl.turn == 0) {
     if (p.h0 != nullptr) h = p.h0[b * p.dim + d];
@@ -319,7 +314,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
     __syncthreads();
     h = fold_back(cl.turn, s_back);
   }
-  if (more && wave == 0) publish(mine, __builtin_fmaf(tp, h, tq), kState);
+  if (more && wave == 0) publish(mine, -1.0f, __builtin_fmaf(tp, h, tq));
   each_pair<false>(s_pair, 0, wave, [&](const float2& v) __attribute__((always_inline)) { h = __builtin_fmaf(v.x, h, v.y); });
   if (here && p.block_states != nullptr) (p.block_states + (b * nblk + blk) * p.dim)[d] = h;
 
@@ -515,17 +510,15 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, 4) void bwd_kernel(const Launch 
     __syncthreads();
   }
   float tp = 1.0f, tq = 0.0f, carry = 0.0f;
-  unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 128 + lane;
+  unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 64 + lane;
   const bool more = cl.turn + 1 < k.nturns;
   if (more && wave == 0) {
     each_pair<true>(s_pair, 0, k.waves, [&](const float2& v) __attribute__((always_inline)) {
       tp *= v.x;
       tq = __builtin_fmaf(v.x, tq, v.y);
     });
-    if (cl.turn > 0) {
-      publish(mine + 64, tp, kPair);
-      publish(mine, tq, kPair);
-    }
+    tp = tp == 0.0f ? -0.0f : tp;
+    if (cl.turn > 0) publish(mine, tp, tq);
   }
   if (cl.turn == 0) {
     if (p.dstate != nullptr) carry = p.dstate[b * p.dim + d];
@@ -534,7 +527,7 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, 4) void bwd_kernel(const Launch 
     __syncthreads();
     carry = fold_back(cl.turn, s_back);
   }
-  if (more && wave == 0) publish(mine, __builtin_fmaf(tp, carry, tq), kState);
+  if (more && wave == 0) publish(mine, -1.0f, __builtin_fmaf(tp, carry, tq));
   each_pair<true>(s_pair, wave + 1, k.waves, [&](const float2& v) __attribute__((always_inline)) { carry = __builtin_fmaf(v.x, carry, v.y); });
 
   auto finish = [&](auto full_c) __attribute__((always_inline)) {
@@ -691,7 +684,7 @@ static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward)
   if (8 * kDies * s.per_die > 9 * s.nstrips) s.per_die = 0;
   s.tiles = s.nturns * (s.per_die ? kDies * s.per_die : s.nstrips);
   s.control_bytes = kControlBytes * (1 + s.nstrips);
-  s.handoff_bytes = s.nturns > 1 ? s.control_bytes + s.nturns * s.nstrips * (2 * 64 * 8) : 0;
+  s.handoff_bytes = s.nturns > 1 ? s.control_bytes + s.nturns * s.nstrips * kWordsBytes : 0;
   return s;
 }
 static int64_t dA_bytes(const Shape& s, int64_t batch, int64_t dim) { return round_up(rows::floats(batch * s.nturns, dim) * 4, 256); }
