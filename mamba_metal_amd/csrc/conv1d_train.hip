@@ -8,6 +8,10 @@
 // blocks of 16 tokens, all of a block loaded at once, with the last K - 1 values of x and dp in registers, and
 // recomputes p.  A run's last dx need dp of the K - 1 tokens after it, which are computed again.  A run's sums
 // for dw and dbias go to the workspace; another kernel adds the runs up in a fixed order, in double.
+//
+// bf16 8 x 2048 x 5120, width 4, 8-bit checkpoint: forward with the codes 81 us (5.3 TB/s, memory), backward 107 + 5 us
+// (4.0 TB/s; 31 vector instructions an element keep the units 80% busy).  The next block's loads ahead of this one's
+// arithmetic change nothing.
 #include <type_traits>
 
 #include "act8.h"
