@@ -391,6 +391,7 @@ int mm_pair_scan(const float* a, const float* b, float* a_out, float* h_out, int
  * int64 (lengths_dtype), NULL = all seqlen: tokens from lengths[b] on (taken as clamped to
  * [0, seqlen]) leave the state as it is, have y = 0 and gradients 0, and their inputs' values do
  * not matter (they may be read).  Arithmetic and states are fp32.  Outputs must not overlap inputs.
+ * A state that became infinite stays infinite or becomes NaN (products of decays may vanish before it).
  * seqlen 0: state_out is h0.  batch at most 65535.
  *
  * Training: the forward call given block_states writes there the state before every 16th token,

@@ -10,7 +10,7 @@
 // for dw and dbias go to the workspace; another kernel adds the runs up in a fixed order, in double.
 //
 // bf16 8 x 2048 x 5120, width 4, 8-bit checkpoint: forward with the codes 81 us (5.3 TB/s, memory), backward 107 + 5 us
-// (4.0 TB/s; 31 vector instructions an element keep the units 80% busy).  The next block's loads ahead of this one's
+// (4.0 TB/s; 32 vector instructions an element keep the units 83% busy).  The next block's loads ahead of this one's
 // arithmetic change nothing.
 #include <type_traits>
 

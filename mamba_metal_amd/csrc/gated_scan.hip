@@ -16,7 +16,7 @@
 // The backward pass is the same in reverse: dh_t = g_t + c, c <- a_t dh_t, with each wave's 16 states
 // recomputed from the stored state before its first token.
 //
-// Bound by memory, then by vector instructions (49 an element forward with the output gate, 75 backward).  bf16 with
+// Bound by memory, then by vector instructions (50 an element forward with the output gate, 77 backward).  bf16 with
 // the output gate: forward 1 x 8192 x 5120 109 us (3.8 TB/s; 4.99 is what a large copy reaches; without the wait for the
 // states before a tile 98), backward 8 x 2048 x 5120 367 us (4.2 TB/s), 4 x 8192 x 5120 with 8-bit checkpoints 642
 // forward and 626 backward (3.8 and 3.9 TB/s).
@@ -294,32 +294,36 @@ __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
   if (full) load_all(std::true_type{});
   else if (some) load_all(std::false_type{});
 
-  // the state before the tile, and before the wave
+  // The state before the tile, and before the wave.  A tile past the sequence's end has none to pass on: the tiles
+  // after it are past it too, and the final state is written where the last token is.
   float h = 0.0f;
-  if (k.waves > 1) {
-    s_pair[wave][lane] = make_float2(P, Q);
-    __syncthreads();
+  const bool past = cl.turn > 0 && static_cast<int64_t>(cl.turn) * k.waves * kBlk >= len;
+  if (!past) {
+    if (k.waves > 1) {
+      s_pair[wave][lane] = make_float2(P, Q);
+      __syncthreads();
+    }
+    float tp = 1.0f, tq = 0.0f;
+    unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 64 + lane;
+    const bool more = cl.turn + 1 < k.nturns;
+    if (more && wave == 0) {
+      each_pair<false>(s_pair, 0, k.waves, [&](const float2& v) __attribute__((always_inline)) {
+        tp *= v.x;
+        tq = __builtin_fmaf(v.x, tq, v.y);
+      });
+      tp = tp == 0.0f ? -0.0f : tp;
+      if (cl.turn > 0) publish(mine, tp, tq);
+    }
+    if (cl.turn == 0) {
+      if (p.h0 != nullptr) h = p.h0[b * p.dim + d];
+    } else {
+      look_back(k.hd, cl.turn, cl.strip, k.nstrips, wave, k.waves, s_back);
+      __syncthreads();
+      h = fold_back(cl.turn, s_back);
+    }
+    if (more && wave == 0) publish(mine, -1.0f, __builtin_fmaf(tp, h, tq));
+    each_pair<false>(s_pair, 0, wave, [&](const float2& v) __attribute__((always_inline)) { h = __builtin_fmaf(v.x, h, v.y); });
   }
-  float tp = 1.0f, tq = 0.0f;
-  unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 64 + lane;
-  const bool more = cl.turn + 1 < k.nturns;
-  if (more && wave == 0) {
-    each_pair<false>(s_pair, 0, k.waves, [&](const float2& v) __attribute__((always_inline)) {
-      tp *= v.x;
-      tq = __builtin_fmaf(v.x, tq, v.y);
-    });
-    tp = tp == 0.0f ? -0.0f : tp;
-    if (cl.turn > 0) publish(mine, tp, tq);
-  }
-  if (cl.turn == 0) {
-    if (p.h0 != nullptr) h = p.h0[b * p.dim + d];
-  } else {
-    look_back(k.hd, cl.turn, cl.strip, k.nstrips, wave, k.waves, s_back);
-    __syncthreads();
-    h = fold_back(cl.turn, s_back);
-  }
-  if (more && wave == 0) publish(mine, -1.0f, __builtin_fmaf(tp, h, tq));
-  each_pair<false>(s_pair, 0, wave, [&](const float2& v) __attribute__((always_inline)) { h = __builtin_fmaf(v.x, h, v.y); });
   if (here && p.block_states != nullptr) (p.block_states + (b * nblk + blk) * p.dim)[d] = h;
 
   float last = h;
@@ -361,8 +365,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
     }
     finish(std::false_type{});
   }
-  // (by the wave of the last block: the state is the last token's, bit for bit)
-  if (p.state_out != nullptr && blk == (nblk > 0 ? nblk - 1 : 0)) p.state_out[b * p.dim + d] = last;
+  // (by the wave of the last token: the state is that token's, bit for bit)
+  if (p.state_out != nullptr && blk == (len > 0 ? (len - 1) / kBlk : 0)) p.state_out[b * p.dim + d] = last;
 }
 
 // ------------------------------------------------------------------------------ backward
@@ -509,30 +513,36 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, 4) void bwd_kernel(const Launch 
   if (full) load_all(std::true_type{});
   else if (some) load_all(std::false_type{});
 
-  if (k.waves > 1) {
+  // what comes from the tokens after the tile, and after the wave: past the sequence's end just dstate
+  float carry = 0.0f;
+  const bool past = static_cast<int64_t>(k.nturns - 1 - cl.turn) * k.waves * kBlk >= len;
+  if ((past || cl.turn == 0) && p.dstate != nullptr) carry = p.dstate[b * p.dim + d];
+  if (!past && k.waves > 1) {
     s_pair[wave][lane] = make_float2(P, Q);
     __syncthreads();
   }
-  float tp = 1.0f, tq = 0.0f, carry = 0.0f;
+  float tp = 1.0f, tq = 0.0f;
   unsigned long long* const mine = k.hd.word + (static_cast<uint64_t>(cl.turn) * k.nstrips + cl.strip) * 64 + lane;
   const bool more = cl.turn + 1 < k.nturns;
-  if (more && wave == 0) {
-    each_pair<true>(s_pair, 0, k.waves, [&](const float2& v) __attribute__((always_inline)) {
-      tp *= v.x;
-      tq = __builtin_fmaf(v.x, tq, v.y);
-    });
-    tp = tp == 0.0f ? -0.0f : tp;
-    if (cl.turn > 0) publish(mine, tp, tq);
-  }
-  if (cl.turn == 0) {
-    if (p.dstate != nullptr) carry = p.dstate[b * p.dim + d];
+  if (past) {
+    if (more && wave == 0) publish(mine, -1.0f, carry);
   } else {
-    look_back(k.hd, cl.turn, cl.strip, k.nstrips, wave, k.waves, s_back);
-    __syncthreads();
-    carry = fold_back(cl.turn, s_back);
+    if (more && wave == 0) {
+      each_pair<true>(s_pair, 0, k.waves, [&](const float2& v) __attribute__((always_inline)) {
+        tp *= v.x;
+        tq = __builtin_fmaf(v.x, tq, v.y);
+      });
+      tp = tp == 0.0f ? -0.0f : tp;
+      if (cl.turn > 0) publish(mine, tp, tq);
+    }
+    if (cl.turn > 0) {
+      look_back(k.hd, cl.turn, cl.strip, k.nstrips, wave, k.waves, s_back);
+      __syncthreads();
+      carry = fold_back(cl.turn, s_back);
+    }
+    if (more && wave == 0) publish(mine, -1.0f, __builtin_fmaf(tp, carry, tq));
+    each_pair<true>(s_pair, wave + 1, k.waves, [&](const float2& v) __attribute__((always_inline)) { carry = __builtin_fmaf(v.x, carry, v.y); });
   }
-  if (more && wave == 0) publish(mine, -1.0f, __builtin_fmaf(tp, carry, tq));
-  each_pair<true>(s_pair, wave + 1, k.waves, [&](const float2& v) __attribute__((always_inline)) { carry = __builtin_fmaf(v.x, carry, v.y); });
 
   auto finish = [&](auto full_c) __attribute__((always_inline)) {
     constexpr bool full = decltype(full_c)::value;

@@ -166,6 +166,9 @@ def gated_scan(x: torch.Tensor, a_gate: torch.Tensor, x_gate: torch.Tensor, A: t
     Returns y (batch, seqlen, dim), contiguous, in x's dtype; with ``return_state`` also the state after
     each sequence's last token, (batch, dim) float32.
 
+    Not-a-numbers and infinities stay in their sequence and channel and reach all later tokens there (an infinite
+    state may become NaN).
+
     Gradients flow to x, a_gate, x_gate, z, A and h0 (once, not twice).  For them a call that needs any keeps
     the state before every 16th token and, with ``checkpoint="full"``, its inputs as they are; with
     ``checkpoint="int8"`` the inputs as 8-bit codes (``act8_pack``), and the gradients are those at the values

@@ -96,7 +96,7 @@ def test_rates(dev, dtype, rates):
 
 @pytest.mark.parametrize("lengths_dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("checkpoint", ["full", "int8"])
-@pytest.mark.parametrize("n", [40, 700])
+@pytest.mark.parametrize("n", [40, 700, 2900])
 def test_lengths(dev, lengths_dtype, checkpoint, n):
     """Padded batches: empty slots, single tokens, ends inside a block and on its border, whole ones, lengths out
     of range; what padding holds (here NaNs and infinities) does not matter."""
