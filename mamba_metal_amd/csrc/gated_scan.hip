@@ -101,19 +101,26 @@ __device__ __forceinline__ bool peek_error(const Handoff& hd) {
 }
 
 // The tile's claim: a workgroup's strip of channels is fixed, its turn in time the next of its strip.  Workgroups
-// go to the chip's 8 dies in turn: with per_die > 0 each die takes per_die neighbouring strips, whose rows share
-// DRAM pages and lines (16-row tiles of 128-byte rows: 4.65 -> 5.25 TB/s of plain copying); strips past the last
-// have no tile.
+// go to the chip's 8 dies in turn: with per_die > 0 each die takes per_die neighbouring strips out of every `span`,
+// whose rows share DRAM pages and lines (16-row tiles of 128-byte rows: 4.65 -> 5.25 TB/s of plain copying); strips
+// past the span's last have no tile.
 struct Claim {
   uint32_t strip, turn;
 };
 constexpr uint32_t kDies = 8;
-__device__ __forceinline__ bool claim(const Handoff& hd, uint32_t nstrips, uint32_t per_die, uint32_t nturns, Claim& cl) {
+struct Spread {
+  uint32_t nstrips, nturns, per_die, span;
+};
+__device__ __forceinline__ bool claim(const Handoff& hd, const Spread& sp, Claim& cl) {
   __shared__ uint32_t s_turn;
   cl.turn = 0;
-  cl.strip = per_die ? blockIdx.x % kDies * per_die + blockIdx.x / kDies % per_die : blockIdx.x % nstrips;
-  if (cl.strip >= nstrips) return false;
-  if (nturns > 1) {
+  cl.strip = blockIdx.x % sp.nstrips;
+  if (sp.per_die) {
+    const uint32_t j = blockIdx.x / kDies, s = blockIdx.x % kDies * sp.per_die + j % sp.per_die;
+    if (s >= sp.span) return false;
+    cl.strip = j / sp.per_die * sp.span % sp.nstrips + s;
+  }
+  if (sp.nturns > 1) {
     if (threadIdx.x == 0) s_turn = atomicAdd(&hd.control[(1 + cl.strip) * (kControlBytes / 4)], 1u);
     __syncthreads();
     cl.turn = __builtin_amdgcn_readfirstlane(s_turn);
@@ -210,7 +217,7 @@ struct Launch {
   mm_gated_scan_params p;
   Handoff hd;
   float* dA_part;
-  uint32_t per_die;               // claim's
+  Spread spread;
   uint32_t nstrips, nturns, ncb;  // strips of 64 channels of a sequence, tiles of a strip, strips a sequence
   int32_t waves;
 };
@@ -226,7 +233,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void fwd_kernel(const Launch k) {
   __shared__ float2 s_back[kWindow][64];
   const mm_gated_scan_params& p = k.p;
   Claim cl;
-  if (!claim(k.hd, k.nstrips, k.per_die, k.nturns, cl)) return;
+  if (!claim(k.hd, k.spread, cl)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t b = cl.strip / k.ncb;
   // lanes past the last channel do what the last one's does, stores and all
@@ -386,7 +393,7 @@ __global__ __launch_bounds__(64 * kMaxWavesBwd, 4) void bwd_kernel(const Launch 
   __shared__ float s_dA[kMaxWavesBwd][64];
   const mm_gated_scan_params& p = k.p;
   Claim cl;
-  if (!claim(k.hd, k.nstrips, k.per_die, k.nturns, cl)) return;
+  if (!claim(k.hd, k.spread, cl)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t b = cl.strip / k.ncb;
   const uint32_t d = min((cl.strip % k.ncb) * 64 + lane, static_cast<uint32_t>(p.dim - 1));
@@ -682,10 +689,10 @@ static int check_workspace(const mm_gated_scan_params* p, size_t need) {
 // ------------------------------------------------------------------------------ shapes of a call
 struct Shape {
   int waves;
-  int64_t ncb, per_die, tiles, nstrips, nturns, control_bytes, handoff_bytes;
+  int64_t ncb, per_die, span, tiles, nstrips, nturns, control_bytes, handoff_bytes;
 };
 // Sequences of up to `most` blocks of 16 tokens are one tile: no hand-off, one launch.
-static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward) {
+static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward, bool ragged = false) {
   const int most = backward ? kMaxWavesBwd : kMaxWaves;
   const int64_t nblk = ceil_div(seqlen > 0 ? seqlen : 1, kBlk);
   Shape s;
@@ -693,10 +700,19 @@ static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward)
   s.ncb = ceil_div(dim, 64);
   s.nstrips = batch * s.ncb;
   s.nturns = ceil_div(nblk, s.waves);
-  // neighbouring strips on one die where that leaves no more than an eighth of the workgroups without a tile
-  s.per_die = ceil_div(s.nstrips, int64_t{kDies});
-  if (8 * kDies * s.per_die > 9 * s.nstrips) s.per_die = 0;
-  s.tiles = s.nturns * (s.per_die ? kDies * s.per_die : s.nstrips);
+  // Neighbouring strips of every sequence on one die, so that ragged sequences spread over all of them, or, where a
+  // sequence's do not divide well and all have one length, of all sequences; either where it leaves no more than an
+  // eighth of the workgroups without a tile.
+  s.per_die = 0;
+  s.span = s.nstrips;
+  for (int64_t span : {s.ncb, ragged ? s.ncb : s.nstrips}) {
+    const int64_t n = ceil_div(span, int64_t{kDies});
+    if (8 * kDies * n > 9 * span) continue;
+    s.per_die = n;
+    s.span = span;
+    break;
+  }
+  s.tiles = s.nturns * (s.per_die ? s.nstrips / s.span * kDies * s.per_die : s.nstrips);
   s.control_bytes = kControlBytes * (1 + s.nstrips);
   s.handoff_bytes = s.nturns > 1 ? s.control_bytes + s.nturns * s.nstrips * kWordsBytes : 0;
   return s;
@@ -730,7 +746,7 @@ static int prepare(Launch& k, const mm_gated_scan_params* p, const Shape& s, cha
   k.nstrips = static_cast<uint32_t>(s.nstrips);
   k.nturns = static_cast<uint32_t>(s.nturns);
   k.ncb = static_cast<uint32_t>(s.ncb);
-  k.per_die = static_cast<uint32_t>(s.per_die);
+  k.spread = {k.nstrips, k.nturns, static_cast<uint32_t>(s.per_die), static_cast<uint32_t>(s.span)};
   k.waves = s.waves;
   return MM_OK;
 }
@@ -762,7 +778,7 @@ int mm_gated_scan_fwd(const mm_gated_scan_params* p, void* stream) {
   }
   if ((e = check_workspace(p, mm_gated_scan_workspace_size(p->batch, p->seqlen, p->dim, 0))) != MM_OK) return e;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const Shape s = shape_of(p->batch, p->seqlen, p->dim, false);
+  const Shape s = shape_of(p->batch, p->seqlen, p->dim, false, p->lengths != nullptr);
   Launch k{};
   if ((e = prepare(k, p, s, static_cast<char*>(p->workspace), st)) != MM_OK) return e;
   const dim3 grid(static_cast<unsigned>(s.tiles)), block(64 * s.waves);
@@ -803,7 +819,7 @@ int mm_gated_scan_bwd(const mm_gated_scan_params* p, void* stream) {
   }
   if ((e = check_workspace(p, mm_gated_scan_workspace_size(p->batch, p->seqlen, p->dim, 1))) != MM_OK) return e;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const Shape s = shape_of(p->batch, p->seqlen, p->dim, true);
+  const Shape s = shape_of(p->batch, p->seqlen, p->dim, true, p->lengths != nullptr);
   Launch k{};
   k.dA_part = static_cast<float*>(p->workspace);
   if ((e = prepare(k, p, s, static_cast<char*>(p->workspace) + dA_bytes(s, p->batch, p->dim), st)) != MM_OK) return e;
