@@ -18,8 +18,8 @@
 //
 // Bound by memory, then by vector instructions (50 an element forward with the output gate, 77 backward).  bf16 with
 // the output gate: forward 1 x 8192 x 5120 109 us (3.8 TB/s; 4.99 is what a large copy reaches; without the wait for the
-// states before a tile 98), backward 8 x 2048 x 5120 367 us (4.2 TB/s), 4 x 8192 x 5120 with 8-bit checkpoints 642
-// forward and 626 backward (3.8 and 3.9 TB/s).
+// states before a tile 98), backward 8 x 2048 x 5120 350 us (4.4 TB/s), 4 x 8192 x 5120 with 8-bit checkpoints 643
+// forward and 624 backward (3.8 and 3.9 TB/s).
 #include <type_traits>
 
 #include "act8.h"
@@ -684,7 +684,6 @@ static int check_workspace(const mm_gated_scan_params* p, size_t need) {
   if (!aligned(p->workspace, 256)) return fail(MM_ERR_WORKSPACE, "workspace is not 256-byte aligned");
   return MM_OK;
 }
-
 
 // ------------------------------------------------------------------------------ shapes of a call
 struct Shape {
