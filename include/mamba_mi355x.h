@@ -387,7 +387,7 @@ int mm_pair_scan(const float* a, const float* b, float* a_out, float* h_out, int
  *   y   = h * (z ? silu(z) : 1)
  * A (dim,) fp32, <= 0 (a channel with A > 0 gives NaN where 1 - a^2 < 0); -inf is a = 0.
  * x, a_gate, x_gate, z, y, dy: (batch, seqlen, dim) in dtype, strides of batch and time in elements
- * (>= 0), unit channel stride.  States (batch, dim) contiguous fp32.  lengths (batch,), int32 or
+ * (>= 0; rows of y must not overlap), unit channel stride.  States (batch, dim) contiguous fp32.  lengths (batch,), int32 or
  * int64 (lengths_dtype), NULL = all seqlen: tokens from lengths[b] on (taken as clamped to
  * [0, seqlen]) leave the state as it is, have y = 0 and gradients 0, and their inputs' values do
  * not matter (they may be read).  Arithmetic and states are fp32.  Outputs must not overlap inputs.

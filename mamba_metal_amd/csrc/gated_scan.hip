@@ -772,6 +772,8 @@ int mm_gated_scan_fwd(const mm_gated_scan_params* p, void* stream) {
     if ((e = check_inputs(p, true, p->z != nullptr)) != MM_OK) return e;
     if (!p->y) return fail(MM_ERR_NULL_POINTER, "y is required");
     if ((e = check_strides(p->y_stride, "y")) != MM_OK) return e;
+    if ((p->batch > 1 && p->y_stride[0] < p->dim) || (p->seqlen > 1 && p->y_stride[1] < p->dim))
+      return fail(MM_ERR_LAYOUT, "rows of y overlap");
   } else if (!p->A) {
     return fail(MM_ERR_NULL_POINTER, "A is required");
   }
@@ -862,6 +864,7 @@ int mm_gated_scan_step(const float* state, float* state_out, const void* x, cons
     return fail(MM_ERR_NULL_POINTER, "state, state_out, x, a_gate, x_gate, A and y are required");
   if (x_stride_b < 0 || a_gate_stride_b < 0 || x_gate_stride_b < 0 || (z && z_stride_b < 0) || y_stride_b < 0)
     return fail(MM_ERR_LAYOUT, "negative stride");
+  if (batch > 1 && y_stride_b < dim) return fail(MM_ERR_LAYOUT, "rows of y overlap");
   const dim3 grid(static_cast<unsigned>(ceil_div(dim, kStepThreads)), static_cast<unsigned>(batch));
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define MM_GS(D)                                                                                       \

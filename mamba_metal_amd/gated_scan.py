@@ -67,7 +67,7 @@ def _forward(dev, x, a_gate, x_gate, A, z, h0, lengths, want_state, train, check
     b, n, d = x.shape
     p = _params(A, lengths, x.dtype, (b, n, d), dev)
     _set_inputs(p, x, a_gate, x_gate, z)
-    y = torch.empty((b, n, d), dtype=x.dtype, device=dev)
+    y = x.new_empty((b, n, d))
     p.y, p.y_stride = y.data_ptr(), _two(n * d, d)
     state = blocks = codes = exps = None
     if h0 is not None:
@@ -106,12 +106,11 @@ def _backward(dev, inputs, codes, exps, A, lengths, blocks, dtype, shape, gated,
     if dstate is not None:
         dstate = dstate.contiguous()
         p.dstate = dstate.data_ptr()
-    dx = torch.empty((b, n, d), dtype=dtype, device=dev)
-    da, dg = torch.empty_like(dx), torch.empty_like(dx)
+    dx, da, dg = (dy.new_empty((b, n, d)) for _ in range(3))
     p.dx, p.da_gate, p.dx_gate = dx.data_ptr(), da.data_ptr(), dg.data_ptr()
     dz = dh0 = None
     if gated:
-        dz = torch.empty_like(dx)
+        dz = dy.new_empty((b, n, d))
         p.dz = dz.data_ptr()
     dA = (torch.empty if b else torch.zeros)((d,), dtype=torch.float32, device=dev)
     p.dA = dA.data_ptr()
@@ -252,7 +251,7 @@ def gated_scan_step(state: torch.Tensor, x: torch.Tensor, a_gate: torch.Tensor, 
     if A.dtype != torch.float32 or not A.is_contiguous():
         A = A.float().contiguous()
     if out is None:
-        out = torch.empty((b, d), dtype=x.dtype, device=dev)
+        out = x.new_empty((b, d))
     with _lib.on_device(dev):
         st = lib.mm_gated_scan_step(
             state.data_ptr(), state.data_ptr() if state_out is None else state_out.data_ptr(), x.data_ptr(),

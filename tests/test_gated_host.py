@@ -158,6 +158,8 @@ def test_gated_scan_c_refuses(lib, over, status):
 @pytest.mark.parametrize("name,over,status", [
     ("fwd", dict(y=None), _lib.ERR_NULL_POINTER),
     ("fwd", dict(y_stride=(_lib._i64a2)(0, -64)), _lib.ERR_LAYOUT),
+    ("fwd", dict(y_stride=(_lib._i64a2)(0, 64)), _lib.ERR_LAYOUT),
+    ("fwd", dict(y_stride=(_lib._i64a2)(64, 0)), _lib.ERR_LAYOUT),
     ("bwd", dict(dy=None), _lib.ERR_NULL_POINTER),
     ("bwd", dict(dx=None), _lib.ERR_NULL_POINTER),
     ("bwd", dict(z=FAKE), _lib.ERR_NULL_POINTER),  # dz missing
@@ -192,6 +194,7 @@ def test_step_c_refuses(lib):
     assert step(lib, batch=-1) == _lib.ERR_SHAPE
     assert step(lib, dtype=9) == _lib.ERR_DTYPE
     assert step(lib, xs=-1) == _lib.ERR_LAYOUT
+    assert step(lib, ys=63) == _lib.ERR_LAYOUT
     assert step(lib, batch=0, x=None) == _lib.OK
 
 
@@ -204,6 +207,8 @@ def test_act8_c_refuses(lib):
         assert f(FAKE, FAKE, FAKE, 1, 1, 64, two, 5, None) == _lib.ERR_DTYPE
         assert f(FAKE, FAKE, FAKE, 1, 1, 64, (_lib._i64a2)(-1, 0), 0, None) == _lib.ERR_LAYOUT
         assert f(None, None, None, 0, 1, 64, two, 0, None) == _lib.OK
+    assert lib.mm_act8_unpack(FAKE, FAKE, FAKE, 2, 1, 64, (_lib._i64a2)(0, 64), 0, None) == _lib.ERR_LAYOUT
+    assert lib.mm_act8_unpack(FAKE, FAKE, FAKE, 1, 2, 64, (_lib._i64a2)(64, 32), 0, None) == _lib.ERR_LAYOUT
 
 
 def conv(lib, **over):
