@@ -18,8 +18,8 @@
 //
 // Bound by memory, then by vector instructions (50 an element forward with the output gate, 77 backward).  bf16 with
 // the output gate: forward 1 x 8192 x 5120 109 us (3.8 TB/s; 4.99 is what a large copy reaches; without the wait for the
-// states before a tile 98), backward 8 x 2048 x 5120 350 us (4.4 TB/s), 4 x 8192 x 5120 with 8-bit checkpoints 643
-// forward and 624 backward (3.8 and 3.9 TB/s).
+// states before a tile 98), backward 8 x 2048 x 5120 350 us (4.4 TB/s), 4 x 8192 x 5120 with 8-bit checkpoints 601
+// forward and 624 backward (4.0 and 3.9 TB/s).
 #include <type_traits>
 
 #include "act8.h"
@@ -30,10 +30,13 @@ namespace mm {
 namespace gscan {
 
 constexpr int kBlk = MM_ACT8_BLOCK;  // tokens of a wave
-// Waves of a tile.  Forward 16 where they hold the whole sequence (one tile, no hand-off), else 8: with 4 a sequence
-// has twice the tiles to hand on (1 x 32768 x 64 29 -> 51 us, 1 x 8192 x 5120 111 -> 114), and 5 or 6 load the SIMDs
-// unevenly (133 us).  Backward 4, so that four workgroups share a CU's registers and LDS.
-constexpr int kMaxWaves = 16, kTileWaves = 8, kMaxWavesBwd = 4;
+// Waves of a tile.  Forward 16 where they hold the whole sequence (one tile, no hand-off).  Longer ones: 4 from
+// kManyStrips strips of channels on, where more and smaller workgroups overlap loads, arithmetic and waits better, else
+// 8, since with few strips the chain of tiles counts, which 4 make twice as long (us with 8 and 4; 1 strip of 32768
+// tokens 29, 51; 16 102, 105; 32 188, 195; 80 427, 431; 160 of 16384 423, 414; 256 of 2048 96.5, 93; 320 of 8192 with
+// codes 640, 600).  5 or 6 load the SIMDs unevenly (a fifth slower).  Backward 4, so that four workgroups share a CU's
+// registers and LDS.
+constexpr int kMaxWaves = 16, kTileWaves = 8, kManyTileWaves = 4, kManyStrips = 128, kMaxWavesBwd = 4;
 constexpr int kWindow = 16;          // tiles that a tile looks back at
 constexpr int kStepThreads = 64;
 
@@ -695,9 +698,10 @@ static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward,
   const int most = backward ? kMaxWavesBwd : kMaxWaves;
   const int64_t nblk = ceil_div(seqlen > 0 ? seqlen : 1, kBlk);
   Shape s;
-  s.waves = nblk <= most ? static_cast<int>(nblk) : backward ? kMaxWavesBwd : kTileWaves;
   s.ncb = ceil_div(dim, 64);
   s.nstrips = batch * s.ncb;
+  const int tile = backward ? kMaxWavesBwd : s.nstrips >= kManyStrips ? kManyTileWaves : kTileWaves;
+  s.waves = nblk <= most ? static_cast<int>(nblk) : tile;
   s.nturns = ceil_div(nblk, s.waves);
   // Neighbouring strips of every sequence on one die, so that ragged sequences spread over all of them, or, where a
   // sequence's do not divide well and all have one length, of all sequences; either where it leaves no more than an

@@ -14,9 +14,9 @@ from mamba_metal_amd.selective_scan import reset_scan_status, scan_status
 pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
-# lengths of one token, around a block of 16 tokens, around tiles of time, widths around 64 lanes
+# lengths of one token, around a block of 16 tokens, around tiles of time, widths around 64 lanes, many sequences
 SIZES = [(1, 1, 1), (2, 2, 3), (3, 16, 64), (2, 17, 65), (1, 33, 130), (2, 129, 66), (1, 600, 200), (1, 1021, 70),
-         (2, 2600, 64)]
+         (2, 2600, 64), (129, 300, 9)]
 
 
 def rand(seed, b, n, d, dtype, dev, z=True, h0=False, rates=1.0):
