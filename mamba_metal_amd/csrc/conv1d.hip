@@ -47,13 +47,13 @@ __device__ __forceinline__ float ld_any(const void* p, int64_t i, int32_t dt) {
   return dt == MM_F32 ? ld<MM_F32>(p, i) : dt == MM_F16 ? ld<MM_F16>(p, i) : ld<MM_BF16>(p, i);
 }
 
-// K = compile-time width; K == 0 means "runtime width <= kMaxW" using a zero-padded
-// kMaxW-tap window (taps aligned to the newest input).
-template <int DT, int K, bool VEC, bool UNI>
+// W = width, each its own kernel: a window of kMaxW taps with leading zeros for the other widths than 2 to 4
+// multiplied tokens outside the window by 0, which is NaN where they are infinite or NaN (and took longer: 64 x 512 x
+// 5120 bf16 at width 1 280 us, 134 now, at width 8 316 and 203).
+template <int DT, int W, bool VEC, bool UNI>
 __global__ __launch_bounds__(kBlock) void conv1d_kernel(const Params p) {
   using T = typename Ty<DT>::T;
   using V8 = typename Ty<DT>::V8;
-  constexpr int W = K > 0 ? K : kMaxW;
   constexpr int U = VEC ? kU : 1;
   // UNI: a wave is 64 neighbouring channel groups of one run, so the run's indexes are wave-uniform
   // (scalar registers and arithmetic: with a run per thread their divisions and products were
@@ -73,8 +73,6 @@ __global__ __launch_bounds__(kBlock) void conv1d_kernel(const Params p) {
   const decltype(run) nchunks = p.nchunks;  // (a 32-bit one cost a strided fp32 call 3 to 7%)
   const int64_t b = run / nchunks, chunk = run % nchunks;
   const int64_t c0 = cg * kCV;
-  const int off = W - static_cast<int>(K > 0 ? K : p.width);  // leading zero taps (K == 0)
-
   const int64_t t_begin = chunk * p.tc;
   const int64_t t_end = std::min<int64_t>(t_begin + p.tc, p.seqlen);
 
@@ -99,9 +97,9 @@ __global__ __launch_bounds__(kBlock) void conv1d_kernel(const Params p) {
     }
   };
   // (after the taps at widths 2 and 3: fp32 3 x 777 x 2048 14.8 -> 13.7 us and 17.1 -> 15.2)
-  if constexpr (K == 4 || K == 0) load_first();
+  if constexpr (W == 1 || W >= 4) load_first();
 
-  // Taps (zero-padded at the old end when K == 0) and bias ((dim,) contiguous, w_dtype).
+  // Taps and bias ((dim,) contiguous, w_dtype).
   // Every load is unconditional, from a clamped in-bounds address, and masked afterwards:
   // guarded loads compiled to one branch and one vmcnt(0) wait per tap (~40 dependent
   // round trips per thread, most of a short sequence's time).  The dtype dispatch is
@@ -114,10 +112,7 @@ __global__ __launch_bounds__(kBlock) void conv1d_kernel(const Params p) {
       const int64_t c = c0 + j;
       const int64_t cc = c < p.dim ? c : 0;
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const int kk = k - off;
-        w[j][k] = ld<WDT>(p.w, cc * p.ws0 + (kk >= 0 ? kk : 0) * p.ws1);
-      }
+      for (int k = 0; k < W; ++k) w[j][k] = ld<WDT>(p.w, cc * p.ws0 + k * p.ws1);
       bias[j] = ld<WDT>(p.bias != nullptr ? p.bias : p.w, p.bias != nullptr ? cc : 0);
     }
   };
@@ -141,7 +136,7 @@ __global__ __launch_bounds__(kBlock) void conv1d_kernel(const Params p) {
     }
   };
   bool taps_done = false;
-  if constexpr (K == 4) {
+  if constexpr (W == 4) {
     if (p.w_vec) {
       if (p.w_dtype == MM_F32) load_taps_vec(std::integral_constant<int, MM_F32>{});
       else if (p.w_dtype == MM_F16) load_taps_vec(std::integral_constant<int, MM_F16>{});
@@ -158,11 +153,11 @@ __global__ __launch_bounds__(kBlock) void conv1d_kernel(const Params p) {
   for (int j = 0; j < kCV; ++j) {
     const bool cin = c0 + j < p.dim;
 #pragma unroll
-    for (int k = 0; k < W; ++k) w[j][k] = (cin && k >= off) ? w[j][k] : 0.0f;
+    for (int k = 0; k < W; ++k) w[j][k] = cin ? w[j][k] : 0.0f;
     bias[j] = (cin && p.bias != nullptr) ? bias[j] : 0.0f;
   }
 
-  if constexpr (K == 2 || K == 3) load_first();
+  if constexpr (W == 2 || W == 3) load_first();
 
   // Strided path: x[b, t, c0 .. c0 + 7] (t >= 0) element by element; channels past dim read
   // channel 0 and count as zero.
@@ -238,24 +233,20 @@ __global__ __launch_bounds__(kBlock) void conv1d_kernel(const Params p) {
     // at the last step the window win[0..W-2] ++ xn holds x[t-(W-1) .. t], zeros
     // where the index is negative.
     if (p.state != nullptr && t == p.seqlen - 1) {
-      const int width = static_cast<int>(p.width);
 #pragma unroll
       for (int j = 0; j < kCV; ++j) {
         const int64_t c = c0 + j;
         if (c >= p.dim) continue;
-        T* sp = static_cast<T*>(p.state) + (b * p.dim + c) * width;
+        T* sp = static_cast<T*>(p.state) + (b * p.dim + c) * W;
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-          const int kk = k - (W - width);
-          if (kk >= 0) sp[kk] = Ty<DT>::from(k == W - 1 ? xn[j] : win[k][j]);
-        }
+        for (int k = 0; k < W; ++k) sp[k] = Ty<DT>::from(k == W - 1 ? xn[j] : win[k][j]);
       }
     }
 #pragma unroll
     for (int k = 0; k + 1 < W - 1; ++k)
 #pragma unroll
       for (int j = 0; j < kCV; ++j) win[k][j] = win[k + 1][j];
-    if (W > 1) {
+    if constexpr (W > 1) {
 #pragma unroll
       for (int j = 0; j < kCV; ++j) win[W - 2][j] = xn[j];
     }
@@ -270,10 +261,14 @@ void launch_dt(const Params& p, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(blocks));
 #define MM_CONV_W(V, U)                                                                         \
   switch (p.width) {                                                                          \
+    case 1: hipLaunchKernelGGL((conv1d_kernel<DT, 1, V, U>), grid, dim3(kBlock), 0, s, p); break; \
     case 2: hipLaunchKernelGGL((conv1d_kernel<DT, 2, V, U>), grid, dim3(kBlock), 0, s, p); break; \
     case 3: hipLaunchKernelGGL((conv1d_kernel<DT, 3, V, U>), grid, dim3(kBlock), 0, s, p); break; \
     case 4: hipLaunchKernelGGL((conv1d_kernel<DT, 4, V, U>), grid, dim3(kBlock), 0, s, p); break; \
-    default: hipLaunchKernelGGL((conv1d_kernel<DT, 0, V, U>), grid, dim3(kBlock), 0, s, p); break; \
+    case 5: hipLaunchKernelGGL((conv1d_kernel<DT, 5, V, U>), grid, dim3(kBlock), 0, s, p); break; \
+    case 6: hipLaunchKernelGGL((conv1d_kernel<DT, 6, V, U>), grid, dim3(kBlock), 0, s, p); break; \
+    case 7: hipLaunchKernelGGL((conv1d_kernel<DT, 7, V, U>), grid, dim3(kBlock), 0, s, p); break; \
+    default: hipLaunchKernelGGL((conv1d_kernel<DT, 8, V, U>), grid, dim3(kBlock), 0, s, p); break; \
   }
   if (p.uni) {
     MM_CONV_W(true, true)
@@ -419,10 +414,12 @@ int mm_causal_conv1d_fwd(const void* x, const void* weight, const void* bias, vo
   // / 16.4, 8 x 1024 x 2048 23.6 / 21.9 / 18.9 / 17.1, 64 x 512 x 5120 179 / 154 / 139 / 140.
   // The flat range spends more per run and wants more waves, and runs of 8 at least: 4 x 2048 x 1032
   // 14.9 us at 8 steps, 16.0 at 16; so do taps that are not read as vectors (1 x 2048 x 1536 at
-  // width 3 8.2 us at 8 steps, 8.6 at 4, at width 8 20.9 and 27.1).  Strided x: up to 256 steps, each
+  // width 3 8.2 us at 8 steps, 8.6 at 4).  Strided x: up to 256 steps, each
   // of a run's loads being a line of its own (64 x 512 x 5120 along time 3.3 ms, 3.5 at 32 steps).
   const int64_t least = p.uni && p.w_vec ? kU : 2 * kU;
-  const int64_t few = !p.vec_ok ? 262143 : p.uni ? 65536 : 131072;
+  // Wide windows re-read more lines a run and have fewer waves to hide it: strided x along time at width 8, 262143
+  // and 65535 threads: 8 x 1024 x 2048 fp16 506 -> 369 us, 4 x 2048 x 1536 fp32 306 -> 269.
+  const int64_t few = !p.vec_ok ? (width > 4 ? 65535 : 262143) : p.uni ? 65536 : 131072;
   int64_t tc = p.vec_ok ? 32 : 256;
   while (tc > least && batch * p.ncg * ceil_div(seqlen, tc) <= few) tc /= 2;
   // In place: one run per sequence, which reads every step before it writes it (a run's history is
