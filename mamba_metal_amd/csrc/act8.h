@@ -35,7 +35,8 @@ __device__ __forceinline__ float scale_of(uint32_t e) {
 
 // Codes of a lane's 16 values, the first in the lowest byte, and their exponent byte.  x / scale + 1.5 * 2^23 in
 // one multiply-add is rounded to a whole number, ties to even, and has the code in its lowest byte.  (Only the
-// largest exponent leaves room for a code of 128: there values are cut to 127 first.)
+// largest exponent leaves room for a code of 128: there values are cut to 127 first.  A broken block's codes are
+// zeros: a NaN would leave its own lowest byte.)
 __device__ __forceinline__ uint4 pack16(const float (&v)[kBlk], uint32_t& e) {
   uint32_t top = 0;
 #pragma unroll
@@ -54,9 +55,12 @@ __device__ __forceinline__ uint4 pack16(const float (&v)[kBlk], uint32_t& e) {
       w[k / 4] = lo | hi << 16;
     }
   };
-  if (__any(e == 248u)) {
+  if (__any(e >= 248u)) {
     const float most = 127.0f * __uint_as_float(248u << 23);
-    codes([&](float x) __attribute__((always_inline)) { return e == 248u ? fminf(fmaxf(x, -most), most) : x; });
+    codes([&](float x) __attribute__((always_inline)) {
+      const float cut = e == 248u ? fminf(fmaxf(x, -most), most) : x;
+      return e == 255u ? 0.0f : cut;
+    });
   } else {
     codes([](float x) __attribute__((always_inline)) { return x; });
   }
