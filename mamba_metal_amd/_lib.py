@@ -17,6 +17,7 @@ import threading
 from pathlib import Path
 
 import torch  # noqa: F401  (must be loaded before the HIP library; see module docstring)
+from torch.autograd import forward_ad
 
 LIB_NAME = "libmamba_mi355x.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
@@ -210,6 +211,16 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """Raises where a tensor carries a tangent of forward-mode differentiation, which a library call would drop.
+    (The level is looked at first: without one, as almost always, that is all there is to do.)"""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -58,6 +58,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
         raise ValueError(f"act8_pack takes (batch, seqlen, dim) or (seqlen, dim), got {tuple(x.shape)}")
     code = _lib.dtype_code(x.dtype)
     channels_last(x, "x")
+    _lib.refuse_tangents("act8_pack", x)
     dev = _lib.require_cuda(x)
     lib = _lib.load()
     x3 = x if x.dim() == 3 else x[None]

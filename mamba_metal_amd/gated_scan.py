@@ -168,7 +168,7 @@ def gated_scan(x: torch.Tensor, a_gate: torch.Tensor, x_gate: torch.Tensor, A: t
     Not-a-numbers and infinities stay in their sequence and channel and reach all later tokens there (an infinite
     state may become NaN).
 
-    Gradients flow to x, a_gate, x_gate, z, A and h0 (once, not twice).  For them a call that needs any keeps
+    Gradients flow to x, a_gate, x_gate, z, A and h0 (once, not twice, and not in forward mode).  For them a call that needs any keeps
     the state before every 16th token and, with ``checkpoint="full"``, its inputs as they are; with
     ``checkpoint="int8"`` the inputs as 8-bit codes (``act8_pack``), and the gradients are those at the values
     that the codes stand for.  At a = 1 (A = 0, or a gate so far down that A r vanishes), where the square
@@ -184,6 +184,7 @@ def gated_scan(x: torch.Tensor, a_gate: torch.Tensor, x_gate: torch.Tensor, A: t
     _check_rest(A, h0, lengths, b, d)
     if checkpoint not in CHECKPOINTS:
         raise ValueError(f"checkpoint must be one of {CHECKPOINTS}, got {checkpoint!r}")
+    _lib.refuse_tangents("gated_scan", x, a_gate, x_gate, A, z, h0)
     dev = _lib.require_cuda(x, a_gate, x_gate, A, z, h0, lengths)
     A = _f32(A).contiguous()
     h0 = None if h0 is None else _f32(h0).contiguous()
@@ -232,7 +233,8 @@ def gated_scan_step(state: torch.Tensor, x: torch.Tensor, a_gate: torch.Tensor, 
 
     state (batch, dim) contiguous float32 is updated in place, or left as it is where ``state_out`` (the same
     kind of tensor) is given.  x, a_gate, x_gate, z: (batch, dim) of one dtype with unit channel stride; A
-    (dim,).  Not differentiable: a tensor that requires a gradient is refused while gradients are on."""
+    (dim,).  Not differentiable: a tensor that requires a gradient is refused while gradients are on, and one
+    with a tangent always."""
     if x.dim() != 2:
         raise ValueError(f"x must be (batch, dim), got {tuple(x.shape)}")
     b, d = x.shape
@@ -246,6 +248,7 @@ def gated_scan_step(state: torch.Tensor, x: torch.Tensor, a_gate: torch.Tensor, 
                                     or x_gate.requires_grad or A.requires_grad or (z is not None and z.requires_grad)):
         raise RuntimeError("gated_scan_step has no gradient: call it under no_grad or inference_mode, "
                            "or train through gated_scan")
+    _lib.refuse_tangents("gated_scan_step", state, x, a_gate, x_gate, A, z)
     dev = _lib.require_cuda(state, x, a_gate, x_gate, A, z, state_out, out)
     lib = _lib.load()
     if A.dtype != torch.float32 or not A.is_contiguous():
