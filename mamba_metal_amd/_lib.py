@@ -213,9 +213,21 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def refuse_tangents(name: str, *tensors) -> None:
-    """Raises where a tensor carries a tangent of forward-mode differentiation, which a library call would drop.
-    (The level is looked at first: without one, as almost always, that is all there is to do.)"""
+_is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+
+
+def refuse_transforms(name: str, *tensors) -> None:
+    """Raises where a library call would go missing without a word: while torch records a program (it would hold the
+    call's empty output alone), and where a tensor carries a tangent of forward-mode differentiation.  (A few tenths of
+    a microsecond where neither is going on.)"""
+    if _is_tracing():
+        raise RuntimeError(f"{name} cannot be recorded by torch.jit.trace")
+    if _modes is None or _modes() > 0:
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+        if get_proxy_mode() is not None:
+            raise RuntimeError(f"{name} cannot be recorded by make_fx")
     if getattr(forward_ad, "_current_level", 0) < 0:
         return
     for t in tensors:

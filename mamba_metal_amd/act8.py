@@ -58,7 +58,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
         raise ValueError(f"act8_pack takes (batch, seqlen, dim) or (seqlen, dim), got {tuple(x.shape)}")
     code = _lib.dtype_code(x.dtype)
     channels_last(x, "x")
-    _lib.refuse_tangents("act8_pack", x)
+    _lib.refuse_transforms("act8_pack", x)
     dev = _lib.require_cuda(x)
     lib = _lib.load()
     x3 = x if x.dim() == 3 else x[None]
@@ -91,6 +91,7 @@ def act8_unpack(packed: Act8, dtype: torch.dtype | None = None, out: torch.Tenso
         if out.shape != packed.shape:
             raise ValueError(f"out is {tuple(out.shape)}, the activation {tuple(packed.shape)}")
         channels_last(out, "out")
+    _lib.refuse_transforms("act8_unpack", out)
     dev = _lib.require_cuda(packed.codes, packed.exps, out)
     lib = _lib.load()
     if out is None:

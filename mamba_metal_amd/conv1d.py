@@ -169,4 +169,5 @@ def causal_conv1d_train(x, weight, bias=None, *, apply_silu=True, checkpoint="fu
     _lib.dtype_code(weight.dtype)
     if bias is not None and (bias.shape != (x.shape[2],) or bias.dtype != weight.dtype or not bias.is_contiguous()):
         raise ValueError("bias must be a contiguous (dim,) tensor of the weight's dtype")
+    _lib.refuse_transforms("causal_conv1d_train", x, weight, bias)
     return _CausalConv1d.apply(x, weight, bias, apply_silu, checkpoint)

@@ -184,7 +184,7 @@ def gated_scan(x: torch.Tensor, a_gate: torch.Tensor, x_gate: torch.Tensor, A: t
     _check_rest(A, h0, lengths, b, d)
     if checkpoint not in CHECKPOINTS:
         raise ValueError(f"checkpoint must be one of {CHECKPOINTS}, got {checkpoint!r}")
-    _lib.refuse_tangents("gated_scan", x, a_gate, x_gate, A, z, h0)
+    _lib.refuse_transforms("gated_scan", x, a_gate, x_gate, A, z, h0)
     dev = _lib.require_cuda(x, a_gate, x_gate, A, z, h0, lengths)
     A = _f32(A).contiguous()
     h0 = None if h0 is None else _f32(h0).contiguous()
@@ -248,7 +248,7 @@ def gated_scan_step(state: torch.Tensor, x: torch.Tensor, a_gate: torch.Tensor, 
                                     or x_gate.requires_grad or A.requires_grad or (z is not None and z.requires_grad)):
         raise RuntimeError("gated_scan_step has no gradient: call it under no_grad or inference_mode, "
                            "or train through gated_scan")
-    _lib.refuse_tangents("gated_scan_step", state, x, a_gate, x_gate, A, z)
+    _lib.refuse_transforms("gated_scan_step", state, x, a_gate, x_gate, A, z)
     dev = _lib.require_cuda(state, x, a_gate, x_gate, A, z, state_out, out)
     lib = _lib.load()
     if A.dtype != torch.float32 or not A.is_contiguous():

@@ -6,7 +6,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fw
 
-from mamba_metal_amd import act8_pack, gated_scan, gated_scan_step
+from mamba_metal_amd import act8_pack, causal_conv1d_train, gated_scan, gated_scan_step
 
 Z3 = torch.zeros((2, 5, 4))
 Z2 = torch.zeros((2, 4))
@@ -25,7 +25,9 @@ def step(**kw):
 
 CALLS = [(scan, "x", Z3), (scan, "a_gate", Z3), (scan, "x_gate", Z3), (scan, "A", torch.zeros(4)), (scan, "z", Z3),
          (scan, "h0", Z2), (step, "state", Z2), (step, "x", Z2), (step, "a_gate", Z2), (step, "x_gate", Z2),
-         (step, "A", torch.zeros(4)), (step, "z", Z2), (lambda x: act8_pack(x), "x", Z3)]
+         (step, "A", torch.zeros(4)), (step, "z", Z2), (lambda x: act8_pack(x), "x", Z3),
+         (lambda x: causal_conv1d_train(x, torch.zeros((4, 1, 2))), "x", Z3),
+         (lambda w: causal_conv1d_train(Z3, w, checkpoint="int8"), "w", torch.zeros((4, 1, 2)))]
 
 
 @pytest.mark.parametrize("no_grad", [False, True])
