@@ -160,8 +160,8 @@ def causal_conv1d_train(x, weight, bias=None, *, apply_silu=True, checkpoint="fu
     if x.dim() != 3:
         raise ValueError(f"x must be (batch, seqlen, dim), got {tuple(x.shape)}")
     channels_last(x, "x")
-    w, _ = _w2d(weight)
-    if w.dim() != 2 or w.shape[0] != x.shape[2] or not 1 <= w.shape[1] <= 8:
+    shape = tuple(weight.shape)
+    if len(shape) not in (2, 3) or shape[0] != x.shape[2] or shape[1:-1] not in ((), (1,)) or not 1 <= shape[-1] <= 8:
         raise ValueError(f"weight must be ({x.shape[2]}, 1, width) with width 1 to 8, got {tuple(weight.shape)}")
     if checkpoint not in ("full", "int8"):
         raise ValueError(f"checkpoint must be 'full' or 'int8', got {checkpoint!r}")
