@@ -53,11 +53,16 @@ def empty_like(x, shape=None) -> Act8:
 
 
 def act8_pack(x: torch.Tensor) -> Act8:
-    """x (batch, seqlen, dim) or (seqlen, dim), float32 / float16 / bfloat16 with unit channel stride."""
+    """x (batch, seqlen, dim) or (seqlen, dim), float32 / float16 / bfloat16 with unit channel stride.
+
+    Not differentiable: a tensor that requires a gradient is refused while gradients are on (in the pack hook of
+    ``torch.autograd.graph.saved_tensors_hooks`` they are off), and one with a tangent always."""
     if x.dim() not in (2, 3):
         raise ValueError(f"act8_pack takes (batch, seqlen, dim) or (seqlen, dim), got {tuple(x.shape)}")
     code = _lib.dtype_code(x.dtype)
     channels_last(x, "x")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("act8_pack has no gradient: call it under no_grad, or on x.detach()")
     _lib.refuse_transforms("act8_pack", x)
     dev = _lib.require_cuda(x)
     lib = _lib.load()

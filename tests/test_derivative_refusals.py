@@ -50,3 +50,18 @@ def test_other_tensors_at_a_level_are_not():
 def test_jvp_is_refused():
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(lambda x: scan(x=x), (Z3,), (Z3,))
+
+
+def test_packing_cuts_no_gradient():
+    """A tensor that requires a gradient is refused while gradients are on, and goes on otherwise: under no_grad,
+    detached, and in the pack hook of autograd's saved tensors."""
+    x = Z3.clone().requires_grad_(True)
+    for t in (x, x * 1):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            act8_pack(t)
+        for go in (lambda: act8_pack(t.detach()), torch.no_grad()(lambda: act8_pack(t))):
+            with pytest.raises(ValueError, match="need GPU"):
+                go()
+    with pytest.raises(ValueError, match="need GPU"):
+        with torch.autograd.graph.saved_tensors_hooks(act8_pack, lambda p: p):
+            x.exp()
