@@ -78,7 +78,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
 def act8_unpack(packed: Act8, dtype: torch.dtype | None = None, out: torch.Tensor | None = None):
     """The values that ``packed`` stands for, in its dtype unless another is given (or out's).
 
-    ``out``, when given, has packed's shape and unit channel stride."""
+    ``out``, when given, has packed's shape, unit channel stride and rows that do not overlap."""
     if out is not None and dtype is not None and out.dtype != dtype:
         raise TypeError(f"out is {out.dtype}, not {dtype}")
     dtype = out.dtype if out is not None else dtype or packed.dtype

@@ -144,8 +144,7 @@ int mm_act8_unpack(const int8_t* codes, const uint8_t* exps, void* y, int64_t ba
   clear_error();
   const int e = check(y, codes, exps, batch, seqlen, dim, y_stride, dtype);
   if (e != MM_OK || batch == 0 || seqlen == 0 || dim == 0) return e;
-  if ((batch > 1 && y_stride[0] < dim) || (seqlen > 1 && y_stride[1] < dim))
-    return fail(MM_ERR_LAYOUT, "rows of y overlap");
+  if (rows_overlap(batch, seqlen, dim, y_stride)) return fail(MM_ERR_LAYOUT, "rows of y overlap");
   const uint32_t nblk = static_cast<uint32_t>(ceil_div(seqlen, kBlk));
   const int threads = threads_of(dim);
   const uint32_t ncb = static_cast<uint32_t>(ceil_div(dim, threads));

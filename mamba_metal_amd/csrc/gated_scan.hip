@@ -776,8 +776,7 @@ int mm_gated_scan_fwd(const mm_gated_scan_params* p, void* stream) {
     if ((e = check_inputs(p, true, p->z != nullptr)) != MM_OK) return e;
     if (!p->y) return fail(MM_ERR_NULL_POINTER, "y is required");
     if ((e = check_strides(p->y_stride, "y")) != MM_OK) return e;
-    if ((p->batch > 1 && p->y_stride[0] < p->dim) || (p->seqlen > 1 && p->y_stride[1] < p->dim))
-      return fail(MM_ERR_LAYOUT, "rows of y overlap");
+    if (rows_overlap(p->batch, p->seqlen, p->dim, p->y_stride)) return fail(MM_ERR_LAYOUT, "rows of y overlap");
   } else if (!p->A) {
     return fail(MM_ERR_NULL_POINTER, "A is required");
   }

@@ -30,6 +30,23 @@ inline bool aligned(const void* p, int64_t bytes) {
   return (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes)) == 0;
 }
 
+// Whether two of a tensor's n[0] x n[1] rows of dim elements, strides s >= 0, share an element.  Nested strides are
+// seen at once; else row j of the larger stride can only meet the two rows of the smaller one next to it.
+inline bool rows_overlap(int64_t n0, int64_t n1, int64_t dim, const int64_t s[2]) {
+  if ((n0 > 1 && s[0] < dim) || (n1 > 1 && s[1] < dim)) return true;
+  if (n0 <= 1 || n1 <= 1) return false;
+  const bool first = s[0] < s[1];  // the smaller stride is the first
+  const int64_t na = first ? n0 : n1, nb = first ? n1 : n0, sa = s[first ? 0 : 1], sb = s[first ? 1 : 0];
+  const __int128 end = static_cast<__int128>(na - 1) * sa + dim;
+  for (int64_t j = 1; j < nb; ++j) {
+    const __int128 at = static_cast<__int128>(j) * sb;
+    if (at >= end) return false;
+    const int64_t i = static_cast<int64_t>(at / sa), r = static_cast<int64_t>(at % sa);
+    if ((i < na && r < dim) || (i + 1 < na && sa - r < dim)) return true;
+  }
+  return false;
+}
+
 // Per-device cache of a launch constant (CU count, resident workgroups per CU of one
 // kernel).  The value is computed on first use on each device and published with an
 // atomic store; racing threads compute and store the same value, so no lock is needed.

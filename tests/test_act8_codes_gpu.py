@@ -33,3 +33,26 @@ def test_codes_of_a_broken_block(dev, huge):
         assert torch.isnan(back[0, 16:32, ::5][:, :len(BITS)]).all()
         if huge:  # cut to 127 steps of the largest power of two
             assert packed.codes[0, 1, 3, 4] == 127 and packed.exps[0, 1, 3] == 248
+
+
+@pytest.mark.parametrize("n,strides", [(20, (70, 210)), (2, (140, 70)), (2, (140, 210)), (3, (331, 90))])
+def test_unpack_into_rows_between_others(dev, n, strides):
+    """Time outside the batch, inside it, and rows of one sequence between those of another; the rest stays."""
+    b, d = 3, 70
+    packed = act8_pack(torch.randn((b, n, d), generator=torch.Generator().manual_seed(2)).to(dev))
+    store = torch.full(((b - 1) * strides[0] + (n - 1) * strides[1] + d + 5,), 9.0, device=dev)
+    out = store.as_strided((b, n, d), (*strides, 1))
+    act8_unpack(packed, out=out)
+    assert torch.equal(out, act8_unpack(packed))
+    covered = torch.zeros_like(store, dtype=torch.bool)
+    covered.as_strided((b, n, d), (*strides, 1)).fill_(True)
+    assert covered.sum() == b * n * d and (store[~covered] == 9.0).all()
+
+
+def test_unpack_into_rows_that_overlap(dev):
+    packed = act8_pack(torch.ones((3, 4, 70), device=dev))
+    store = torch.full((2000,), 9.0, device=dev)
+    for strides in ((70, 70), (140, 70), (210, 139), (69, 300)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            act8_unpack(packed, out=store.as_strided((3, 4, 70), (*strides, 1)))
+    assert (store == 9.0).all()
