@@ -23,20 +23,13 @@
 #include <type_traits>
 
 #include "act8.h"
+#include "gated_tiles.h"
 #include "reduce_rows.h"
 #include "row_io.h"
 
 namespace mm {
 namespace gscan {
 
-constexpr int kBlk = MM_ACT8_BLOCK;  // tokens of a wave
-// Waves of a tile.  Forward 16 where they hold the whole sequence (one tile, no hand-off).  Longer ones: 4 from
-// kManyStrips strips of channels on, where more and smaller workgroups overlap loads, arithmetic and waits better, else
-// 8, since with few strips the chain of tiles counts, which 4 make twice as long (us with 8 and 4; 1 strip of 32768
-// tokens 29, 51; 16 102, 105; 32 188, 195; 80 427, 431; 160 of 16384 423, 414; 256 of 2048 96.5, 93; 320 of 8192 with
-// codes 640, 600).  5 or 6 load the SIMDs unevenly (a fifth slower).  Backward 4, so that four workgroups share a CU's
-// registers and LDS.
-constexpr int kMaxWaves = 16, kTileWaves = 8, kManyTileWaves = 4, kManyStrips = 128, kMaxWavesBwd = 4;
 constexpr int kWindow = 16;          // tiles that a tile looks back at
 constexpr int kStepThreads = 64;
 
@@ -82,9 +75,6 @@ __device__ __forceinline__ int64_t length_of(const mm_gated_scan_params& p, int6
 // One counter for all tiles bounded the forward pass at about 25 ns a tile.  A word is the pair (P, Q), or (-1, the
 // state after the tile): a product of decays is never negative.  It is one 64-bit access, so a reader has both or
 // neither: no fence, no cache write-back.  All zeros is a word that is not there yet, and a P of 0 is written as -0.
-constexpr int kControlBytes = 128;
-constexpr int kWordsBytes = 64 * 8;  // of a tile
-
 struct Handoff {
   uint32_t* control;
   unsigned long long* word; // [tile][64]
@@ -103,25 +93,18 @@ __device__ __forceinline__ bool peek_error(const Handoff& hd) {
   return __hip_atomic_load(&hd.control[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
 }
 
-// The tile's claim: a workgroup's strip of channels is fixed, its turn in time the next of its strip.  Workgroups
-// go to the chip's 8 dies in turn: with per_die > 0 each die takes per_die neighbouring strips out of every `span`,
-// whose rows share DRAM pages and lines (16-row tiles of 128-byte rows: 4.65 -> 5.25 TB/s of plain copying); strips
-// past the span's last have no tile.
+// The tile's claim: the workgroup's strip, its turn in time the next of its strip.
 struct Claim {
   uint32_t strip, turn;
-};
-constexpr uint32_t kDies = 8;
-struct Spread {
-  uint32_t nstrips, nturns, per_die, span;
 };
 __device__ __forceinline__ bool claim(const Handoff& hd, const Spread& sp, Claim& cl) {
   __shared__ uint32_t s_turn;
   cl.turn = 0;
   cl.strip = blockIdx.x % sp.nstrips;
   if (sp.per_die) {
-    const uint32_t j = blockIdx.x / kDies, s = blockIdx.x % kDies * sp.per_die + j % sp.per_die;
+    const uint32_t j = blockIdx.x / kDies, s = place_of(blockIdx.x % kDies, j, sp);
     if (s >= sp.span) return false;
-    cl.strip = j / sp.per_die * sp.span % sp.nstrips + s;
+    cl.strip = span_of(j, sp) + s;
   }
   if (sp.nturns > 1) {
     if (threadIdx.x == 0) s_turn = atomicAdd(&hd.control[(1 + cl.strip) * (kControlBytes / 4)], 1u);
@@ -688,38 +671,6 @@ static int check_workspace(const mm_gated_scan_params* p, size_t need) {
   return MM_OK;
 }
 
-// ------------------------------------------------------------------------------ shapes of a call
-struct Shape {
-  int waves;
-  int64_t ncb, per_die, span, tiles, nstrips, nturns, control_bytes, handoff_bytes;
-};
-// Sequences of up to `most` blocks of 16 tokens are one tile: no hand-off, one launch.
-static Shape shape_of(int64_t batch, int64_t seqlen, int64_t dim, bool backward, bool ragged = false) {
-  const int most = backward ? kMaxWavesBwd : kMaxWaves;
-  const int64_t nblk = ceil_div(seqlen > 0 ? seqlen : 1, kBlk);
-  Shape s;
-  s.ncb = ceil_div(dim, 64);
-  s.nstrips = batch * s.ncb;
-  const int tile = backward ? kMaxWavesBwd : s.nstrips >= kManyStrips ? kManyTileWaves : kTileWaves;
-  s.waves = nblk <= most ? static_cast<int>(nblk) : tile;
-  s.nturns = ceil_div(nblk, s.waves);
-  // Neighbouring strips of every sequence on one die, so that ragged sequences spread over all of them, or, where a
-  // sequence's do not divide well and all have one length, of all sequences; either where it leaves no more than an
-  // eighth of the workgroups without a tile.
-  s.per_die = 0;
-  s.span = s.nstrips;
-  for (int64_t span : {s.ncb, ragged ? s.ncb : s.nstrips}) {
-    const int64_t n = ceil_div(span, int64_t{kDies});
-    if (8 * kDies * n > 9 * span) continue;
-    s.per_die = n;
-    s.span = span;
-    break;
-  }
-  s.tiles = s.nturns * (s.per_die ? s.nstrips / s.span * kDies * s.per_die : s.nstrips);
-  s.control_bytes = kControlBytes * (1 + s.nstrips);
-  s.handoff_bytes = s.nturns > 1 ? s.control_bytes + s.nturns * s.nstrips * kWordsBytes : 0;
-  return s;
-}
 static int64_t dA_bytes(const Shape& s, int64_t batch, int64_t dim) { return round_up(rows::floats(batch * s.nturns, dim) * 4, 256); }
 
 static int prepare(Launch& k, const mm_gated_scan_params* p, const Shape& s, char* handoff, hipStream_t stream) {
