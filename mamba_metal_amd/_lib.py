@@ -213,6 +213,24 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_hooks = getattr(torch._C._autograd, "_top_saved_tensors_default_hooks", None)
+
+
+def hooked() -> bool:
+    """Whether hooks on saved tensors are on (``torch.autograd.graph.saved_tensors_hooks``, ``save_on_cpu``)."""
+    return _hooks is None or _hooks(False) is not None
+
+
+def saved(t, dtype, shape, device, rows=False):
+    """A backward pass's saved tensor after hooks, which can hand back anything: another type, shape or device than was
+    saved raises, since a kernel would read past its end.  Contiguous; with ``rows``, for an activation, with unit channel
+    stride."""
+    if t is None or t.dtype != dtype or t.shape != shape or t.get_device() != device.index:
+        raise RuntimeError(f"a saved tensor came back as {None if t is None else (t.dtype, tuple(t.shape), str(t.device))}, "
+                           f"not as {(dtype, tuple(shape), str(device))}")
+    return t if rows and (t.stride(-1) == 1 or shape[-1] == 1) else t.contiguous()
+
+
 _is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
 _modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
 

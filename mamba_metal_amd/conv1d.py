@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from mamba_metal_amd import _lib
-from mamba_metal_amd.act8 import Act8, channels_last, empty_like
+from mamba_metal_amd.act8 import BLOCK, Act8, channels_last, empty_like
 
 
 def _w2d(weight):
@@ -125,10 +125,24 @@ def _conv1d_act8(x, weight, bias, apply_silu):
     return out, packed
 
 
+def _checked(saved, dev, dtype, shape, w_dtype, w_shape, has_bias):
+    """The saved tensors, where hooks may have changed them."""
+    (b, n, d), (weight, bias, *kept) = shape, saved
+    if has_bias:
+        bias = _lib.saved(bias, w_dtype, (d,), dev)
+    if len(kept) == 1:
+        kept = (_lib.saved(kept[0], dtype, shape, dev, rows=True),)
+    else:
+        nblk = -(-n // BLOCK)
+        kept = (_lib.saved(kept[0], torch.int8, (b, nblk, d, BLOCK), dev), _lib.saved(kept[1], torch.uint8, (b, nblk, d), dev))
+    return _lib.saved(weight, w_dtype, w_shape, dev), bias, *kept
+
+
 class _CausalConv1d(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, apply_silu, checkpoint):
-        ctx.meta = (x.dtype, x.shape, apply_silu)
+        ctx.meta = (x.device, x.dtype, x.shape, apply_silu,
+                    _lib.hooked() and (weight.dtype, weight.shape, bias is not None))
         if checkpoint == "int8":
             out, packed = _conv1d_act8(x, weight, bias, apply_silu)
             ctx.save_for_backward(weight, bias, packed.codes, packed.exps)
@@ -140,8 +154,11 @@ class _CausalConv1d(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        dtype, shape, apply_silu = ctx.meta
-        weight, bias, *kept = ctx.saved_tensors
+        dev, dtype, shape, apply_silu, hooked = ctx.meta
+        saved = ctx.saved_tensors
+        if hooked:
+            saved = _checked(saved, dev, dtype, shape, *hooked)
+        weight, bias, *kept = saved
         x, packed = (kept[0], None) if len(kept) == 1 else (None, Act8(*kept, shape, dtype))
         if dout.dtype != dtype or (dout.stride(-1) != 1 and shape[2] > 1):
             dout = dout.to(dtype).contiguous()

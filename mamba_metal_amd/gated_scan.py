@@ -121,11 +121,26 @@ def _backward(dev, inputs, codes, exps, A, lengths, blocks, dtype, shape, gated,
     return dx, da, dg, dA, dz, dh0
 
 
+def _checked(saved, dev, dtype, shape, gated, lengths_dtype):
+    """The saved tensors, where hooks may have changed them."""
+    (b, n, d), (A, lengths, blocks, *kept) = shape, saved
+    nblk, k = -(-n // BLOCK), 4 if gated else 3
+    if lengths_dtype is not None:
+        lengths = _lib.saved(lengths, lengths_dtype, (b,), dev)
+    if len(kept) == 2:
+        kept = (_lib.saved(kept[0], torch.int8, (k, b, nblk, d, BLOCK), dev),
+                _lib.saved(kept[1], torch.uint8, (k, b, nblk, d), dev))
+    else:
+        kept = [_lib.saved(t, dtype, shape, dev, rows=True) for t in kept[:k]] + [None] * (4 - k)
+    return _lib.saved(A, torch.float32, (d,), dev), lengths, _lib.saved(blocks, torch.float32, (b, nblk, d), dev), *kept
+
+
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, dev, x, a_gate, x_gate, A, z, h0, lengths, want_state, checkpoint):
         y, state, blocks, codes, exps = _forward(dev, x, a_gate, x_gate, A, z, h0, lengths, want_state, True, checkpoint)
-        ctx.meta = (dev, x.dtype, x.shape, z is not None)
+        ctx.meta = (dev, x.dtype, x.shape, z is not None,
+                    _lib.hooked() and (None if lengths is None else lengths.dtype,))
         ctx.set_materialize_grads(False)
         if codes is not None:
             ctx.save_for_backward(A, lengths, blocks, codes, exps)
@@ -138,8 +153,11 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dy, dstate=None):
         if dy is None and dstate is None:
             return (None,) * 10
-        dev, dtype, shape, gated = ctx.meta
-        A, lengths, blocks, *kept = ctx.saved_tensors
+        dev, dtype, shape, gated, hooked = ctx.meta
+        saved = ctx.saved_tensors
+        if hooked:
+            saved = _checked(saved, dev, dtype, shape, gated, *hooked)
+        A, lengths, blocks, *kept = saved
         inputs, codes, exps = (None, *kept) if len(kept) == 2 else (kept, None, None)
         grads = _backward(dev, inputs, codes, exps, A, lengths, blocks, dtype, shape, gated, dy, dstate,
                           ctx.needs_input_grad[6])
