@@ -459,10 +459,10 @@ int mm_gated_scan_step(const float* state, float* state_out, const void* x, cons
  * sequence may be shorter) as int8 codes in [-127, 127] and one exponent byte e,
  *   value = code * 2^(e - 127),
  * with the smallest power of two that keeps |code| <= 127 (1 <= e <= 248), codes rounded to nearest
- * even.  A block that holds an infinity or a NaN gets e = 255 and stands for NaNs.  x, y (batch, seqlen,
+ * even.  A block that holds an infinity or a NaN gets e = 255 and codes of 0 and stands for NaNs.  x, y (batch, seqlen,
  * dim) in dtype with strides of batch and time, unit channel stride; codes (batch, ceil(seqlen / 16), dim, 16)
  * (zeros past seqlen, 16-byte aligned), exps (batch, ceil(seqlen / 16), dim), both contiguous.  Every value is
- * exact in dtype (fp16's 65536 becomes 65504). */
+ * exact in the dtype that was packed (fp16's 65536 becomes 65504); another one rounds it.  Rows of y must not overlap. */
 int mm_act8_pack(const void* x, int8_t* codes, uint8_t* exps, int64_t batch, int64_t seqlen,
                  int64_t dim, const int64_t x_stride[2], int32_t dtype, void* stream);
 int mm_act8_unpack(const int8_t* codes, const uint8_t* exps, void* y, int64_t batch, int64_t seqlen,

@@ -3,7 +3,8 @@
 ``act8_pack(x)`` turns an activation (batch, seqlen, dim) into whole numbers of at most 127 and one
 power of two for each block of 16 tokens of a channel: 1.06 bytes an element instead of 2 or 4, off by
 at most half a step of the block's power of two, 1/127.5 of the block's largest magnitude at worst.
-``act8_unpack`` gives back the values that the codes stand for, which every dtype here holds exactly.
+``act8_unpack`` gives back the values that the codes stand for, which the activation's own dtype holds exactly (but for
+float16's largest numbers, whose code stands for 65536: they come back as 65504); another dtype rounds them.
 ``gated_scan`` and ``causal_conv1d_train`` with ``checkpoint="int8"`` keep their inputs this way and
 read the codes in their backward kernels; these two functions are for any other activation.
 

@@ -3,8 +3,8 @@
 // A block's scale is 2^(e - 127) for its exponent byte e, the smallest power of two that keeps the codes
 // within 127: with m = max |x| over the block, m / scale lies in [63.75, 127.5), so a code is off by at most
 // half a step, m / 127.5 at worst.  A power of two costs up to one bit against m / 127 and makes everything
-// exact: x / scale and code * scale round nowhere, a code times its scale is a bf16 or fp16 number, and
-// the scale takes one byte.  Blocks run along time because a layer's outlier channels then keep their
+// exact: x / scale and code * scale round nowhere, a code times its scale is a number of the activation's own type
+// (but for fp16's largest, whose code stands for 65536), and the scale takes one byte.  Blocks run along time because a layer's outlier channels then keep their
 // scale to themselves, and because the kernels hold a channel's 16 tokens in one lane: no reduction
 // crosses lanes.  A block's 16 codes are 16 contiguous bytes, blocks of neighbouring channels next to each
 // other, so that a lane moves a block in one access and a wave 1 KB.  e = 255 marks a block that held an infinity or a NaN: it stands for NaNs.

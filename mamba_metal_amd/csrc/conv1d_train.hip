@@ -9,8 +9,8 @@
 // recomputes p.  A run's last dx need dp of the K - 1 tokens after it, which are computed again.  A run's sums
 // for dw and dbias go to the workspace; another kernel adds the runs up in a fixed order, in double.
 //
-// bf16 8 x 2048 x 5120, width 4, 8-bit checkpoint: forward with the codes 81 us (5.3 TB/s, memory), backward 107 + 5 us
-// (4.0 TB/s; 32 vector instructions an element keep the units 83% busy).  The next block's loads ahead of this one's
+// bf16 8 x 2048 x 5120, width 4, 8-bit checkpoint: forward with the codes 81 us (5.3 TB/s, memory), backward 107 + 4 us
+// (4.0 TB/s; 32 vector instructions an element keep the units 84% busy).  The next block's loads ahead of this one's
 // arithmetic change nothing.
 #include <type_traits>
 
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kThreads) void conv1d_bwd_kernel(const Params p) {
     dw[k] = 0.0f;
   }
   using std::integral_constant;
-  // Tokens t - H .. t + kS - 1: half a block at a time, so that eight waves a SIMD have the registers.
+  // Tokens t - H .. t + kS - 1: half a block at a time, for the registers (6 waves a SIMD at width 4, 4 at width 8).
   float x[H + kS], dp[H + kS];
 #pragma unroll
   for (int k = 0; k < H; ++k) x[k] = dp[k] = 0.0f;

@@ -16,10 +16,10 @@
 // The backward pass is the same in reverse: dh_t = g_t + c, c <- a_t dh_t, with each wave's 16 states
 // recomputed from the stored state before its first token.
 //
-// Bound by memory, then by vector instructions (50 an element forward with the output gate, 77 backward).  bf16 with
-// the output gate: forward 1 x 8192 x 5120 109 us (3.8 TB/s; 4.99 is what a large copy reaches; without the wait for the
-// states before a tile 98), backward 8 x 2048 x 5120 350 us (4.4 TB/s), 4 x 8192 x 5120 with 8-bit checkpoints 601
-// forward and 624 backward (4.0 and 3.9 TB/s).
+// Bound by memory, then by vector instructions (51 an element forward with the output gate, 78 backward).  bf16 with
+// the output gate, us in passes one after another: forward 1 x 8192 x 5120 110 (3.8 TB/s; 4.99 is what a large copy
+// reaches; without the wait for the states before a tile 98), 8 x 2048 x 5120 forward 240 and backward 343 (3.6 and 4.5
+// TB/s), 4 x 8192 x 5120 with 8-bit checkpoints 548 and 562 (4.4 and 4.3 TB/s).
 #include <type_traits>
 
 #include "act8.h"
@@ -39,8 +39,8 @@ __device__ __forceinline__ float sigmoid_f(float x) { return rcp_hw(1.0f + exp2_
 // series -l (1 + l/2 + l^2/6 + ...): 1 - a^2 keeps its precision, and a's rounding leans to no side, where the
 // hardware exponential's would add up over the thousands of tokens that such a channel remembers.  fp32: from
 // l = -1/4 on, to l^5/720 (the first dropped term is 5e-8 of q there; below, 1 - a is good to a few 1e-7).
-// 16-bit types: from l = -1/16 on, to l^3/24 (1e-7; below, 1 - a is good to 2e-6, a thousandth of their half
-// step), two multiply-adds less.
+// 16-bit types: from l = -1/16 on, to l^3/24 (1e-7; below, 1 - a is good to 2e-6, a 2000th of bf16's half step, a
+// 250th of fp16's), two multiply-adds less.
 template <int DT>
 __device__ __forceinline__ void decay(float l, float& a, float& beta2) {
   constexpr bool wide = DT == MM_F32;
