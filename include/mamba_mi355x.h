@@ -495,6 +495,69 @@ int mm_causal_conv1d_fwd_act8(const void* x, const void* weight, const void* bia
                               const int64_t w_stride[2], int32_t x_dtype, int32_t w_dtype,
                               int32_t apply_silu, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Linear attention with a decay for each head (no counterpart in the reference; it stands beside the selective scan and
+ * the gated recurrence, whose states are a channel's, not a head's outer products):
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T      y_t = scale * S_t^T q_t        (S = h0, or 0, before the first token)
+ * q, k: (batch, seqlen, groups, key_dim), v, y, dy: (batch, seqlen, heads, value_dim) in dtype, unit channel stride,
+ * strides of batch, time and head in elements (>= 0); y, dq, dk, dv contiguous.  Head h uses q and k of group
+ * h / (heads / groups).  log_decay g: (batch, seqlen, heads) with three strides (0 for what all share), <= 0 (-inf
+ * forgets; above 0 the state grows until it overflows).  States (batch, heads, key_dim, value_dim) contiguous fp32.
+ * lengths as in mm_gated_scan_params: tokens from lengths[b] on leave the state as it is, have y = 0 and gradients 0,
+ * and their inputs do not matter.  key_dim <= 128, value_dim <= 1024.  Sums and states are fp32; 16-bit types round
+ * the scores of a run of 64 tokens and the state that meets q, each once, to dtype before their products.
+ *
+ * Training: the forward call given run_states (mm_decay_attention_states_size bytes, 256-byte aligned) writes there, in
+ * dtype, the states that the backward call reads.  Sums are taken in a fixed order: calls repeat bit for bit. */
+typedef struct mm_decay_attention_params {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* log_decay;
+  const float* h0;            /* NULL = zeros */
+  const void* lengths;        /* (batch,); NULL = seqlen each */
+  void* y;                    /* forward */
+  float* state_out;           /* forward: the state after the last token; NULL = skip */
+  void* run_states;           /* forward: written (NULL = skip); backward: read */
+  const void* dy;             /* backward: gradient of y */
+  const float* dstate;        /* backward: gradient of state_out; NULL = zeros */
+  void* dq;
+  void* dk;
+  void* dv;
+  float* dlog_decay;          /* (batch, seqlen, heads) contiguous fp32; NULL = skip */
+  float* dlog_decay_heads;    /* (heads,) fp32: its sums over batch and time, dlog_decay NULL; NULL = skip */
+  float* dh0;                 /* NULL = skip */
+  void* workspace;            /* 256-byte aligned, no initial contents */
+  size_t workspace_bytes;
+  int64_t batch, seqlen, heads, groups, key_dim, value_dim;
+  int64_t q_stride[3], k_stride[3], v_stride[3], log_decay_stride[3], dy_stride[3];
+  float scale;
+  int32_t dtype;
+  int32_t log_decay_dtype;
+  int32_t lengths_dtype;      /* 0 int32, 1 int64 */
+} mm_decay_attention_params;
+
+size_t mm_decay_attention_states_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t key_dim,
+                                      int64_t value_dim, int32_t dtype);
+/* Workspace bytes of the forward (backward = 0) or backward call; 0 when none is needed. */
+size_t mm_decay_attention_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t groups,
+                                         int64_t key_dim, int64_t value_dim, int32_t dtype, int32_t backward);
+int mm_decay_attention_fwd(const mm_decay_attention_params* p, void* stream);
+/* With dS_t = exp(g_{t+1}) dS_{t+1} + scale q_t dy_t^T (dstate after the last token): dq_t = scale S_t dy_t,
+ * dk_t = dS_t v_t (both summed over a group's heads), dv_t = dS_t^T k_t, dlog_decay_t = exp(g_t) <dS_t, S_{t-1}>,
+ * dh0 = exp(g_1) dS_1. */
+int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream);
+
+/* One token: state_out = exp(g) state + k v^T (state_out may be state), y = scale * state_out^T q.  Strides of batch
+ * and head in elements, unit channel stride; the states contiguous. */
+int mm_decay_attention_step(const float* state, float* state_out, const void* q, const void* k,
+                            const void* v, const void* log_decay, void* y, int64_t batch,
+                            int64_t heads, int64_t groups, int64_t key_dim, int64_t value_dim,
+                            const int64_t q_stride[2], const int64_t k_stride[2],
+                            const int64_t v_stride[2], const int64_t log_decay_stride[2],
+                            const int64_t y_stride[2], float scale, int32_t dtype,
+                            int32_t log_decay_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ include/mamba_mi355x.h); projections use torch GEMMs.  There is no CPU fallback.
 from mamba_metal_amd._loader import load_kernel
 from mamba_metal_amd.act8 import Act8, act8_pack, act8_unpack
 from mamba_metal_amd.conv1d import causal_conv1d_train
+from mamba_metal_amd.decay_attention import decay_attention, decay_attention_step
 from mamba_metal_amd.gated_scan import gated_scan, gated_scan_step
 from mamba_metal_amd.generate import (GraphDecoder, GraphPrefill, generate, generate_fast,
                                       generate_fast_ids)
@@ -34,6 +35,8 @@ __all__ = [
     "act8_pack",
     "act8_unpack",
     "causal_conv1d_train",
+    "decay_attention",
+    "decay_attention_step",
     "gated_scan",
     "gated_scan_step",
     "generate_fast_ids",

@@ -97,6 +97,20 @@ class GatedScanParams(ctypes.Structure):
     ]
 
 
+class DecayAttentionParams(ctypes.Structure):
+    """Mirror of ``mm_decay_attention_params`` (include/mamba_mi355x.h)."""
+
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("log_decay", _vp), ("h0", _vp), ("lengths", _vp), ("y", _vp),
+        ("state_out", _vp), ("run_states", _vp), ("dy", _vp), ("dstate", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+        ("dlog_decay", _vp), ("dlog_decay_heads", _vp), ("dh0", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+        ("batch", _i64), ("seqlen", _i64), ("heads", _i64), ("groups", _i64), ("key_dim", _i64), ("value_dim", _i64),
+        ("q_stride", _i64a3), ("k_stride", _i64a3), ("v_stride", _i64a3), ("log_decay_stride", _i64a3),
+        ("dy_stride", _i64a3), ("scale", ctypes.c_float), ("dtype", _i32), ("log_decay_dtype", _i32),
+        ("lengths_dtype", _i32),
+    ]
+
+
 ACT8_BLOCK = 16   # MM_ACT8_BLOCK
 
 _SIGNATURES = {
@@ -136,6 +150,12 @@ _SIGNATURES = {
     "mm_gated_scan_fwd": ([ctypes.POINTER(GatedScanParams), _vp], ctypes.c_int),
     "mm_gated_scan_bwd": ([ctypes.POINTER(GatedScanParams), _vp], ctypes.c_int),
     "mm_gated_scan_step": ([_vp] * 8 + [_i64] * 7 + [_i32, _vp], ctypes.c_int),
+    "mm_decay_attention_states_size": ([_i64] * 5 + [_i32], _sz),
+    "mm_decay_attention_workspace_size": ([_i64] * 6 + [_i32] * 2, _sz),
+    "mm_decay_attention_fwd": ([ctypes.POINTER(DecayAttentionParams), _vp], ctypes.c_int),
+    "mm_decay_attention_bwd": ([ctypes.POINTER(DecayAttentionParams), _vp], ctypes.c_int),
+    "mm_decay_attention_step": (
+        [_vp] * 7 + [_i64] * 5 + [_i64a2] * 5 + [ctypes.c_float, _i32, _i32, _vp], ctypes.c_int),
     "mm_act8_pack": ([_vp] * 3 + [_i64] * 3 + [_i64a2, _i32, _vp], ctypes.c_int),
     "mm_act8_unpack": ([_vp] * 3 + [_i64] * 3 + [_i64a2, _i32, _vp], ctypes.c_int),
     "mm_causal_conv1d_fwd_act8": (

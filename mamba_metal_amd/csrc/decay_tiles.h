@@ -1,0 +1,217 @@
+// Tiles of decaying linear attention: matrix-core operands read from shared memory, and a run's decays.
+//
+// All products are 16 x 16 tiles with fp32 accumulators.  Lane l = 16 g + i (g = l / 16) holds of an operand the row
+// (or column) i and kE of the kStep elements of the sum, and of an accumulator column i, rows 4 g .. 4 g + 3.  Which
+// elements of the sum a lane holds is free as long as both operands agree:
+//   row order   k = kE g + j                            one 16-byte read of a row
+//   acc order   k = 4 g + j, and 16 + 4 g + (j - 4)     the rows of two accumulator tiles, so that an accumulator is an
+//                                                       operand of the next product without leaving its registers
+// (fp32 operands: kE = 4, and the two orders are one).
+#pragma once
+
+#include "mm_common.h"
+
+namespace mm {
+namespace dattn {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kRun = 64;    // tokens a run
+constexpr int kVBlock = 64; // value channels a workgroup
+constexpr int kMaxDk = 128;
+
+template <int DT>
+struct Op {
+  using T = typename Ty<DT>::T;
+  static constexpr bool kWide = DT == MM_F32;
+  static constexpr int kE = kWide ? 4 : 8;      // elements of an operand in a lane
+  static constexpr int kStep = 4 * kE;          // elements of the sum an operand covers
+  static constexpr int kTiles = kWide ? 1 : 2;  // accumulator tiles an operand is made of
+  static constexpr int kPad = kWide ? 4 : 16;   // of a row in shared memory: transposed reads without bank conflicts
+};
+
+template <int DT>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (DT == MM_F16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  } else if constexpr (DT == MM_BF16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+    return c;
+  }
+}
+
+// Two fp32 values as a pair of T in one word (round to nearest even).
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == MM_BF16) {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), bf2));
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, (h2{static_cast<_Float16>(a), static_cast<_Float16>(b)}));
+  }
+}
+template <int DT>
+__device__ __forceinline__ void unpack2(uint32_t v, float& a, float& b) {
+  if constexpr (DT == MM_BF16) {
+    a = __uint_as_float(v << 16);
+    b = __uint_as_float(v & 0xffff0000u);
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 h = __builtin_bit_cast(h2, v);
+    a = static_cast<float>(h[0]);
+    b = static_cast<float>(h[1]);
+  }
+}
+
+// An operand in acc order of kTiles accumulator tiles.
+template <int DT>
+__device__ __forceinline__ u32x4 from_acc(const f32x4* t) {
+  if constexpr (Op<DT>::kWide) return __builtin_bit_cast(u32x4, t[0]);
+  else
+    return u32x4{pack2<DT>(t[0][0], t[0][1]), pack2<DT>(t[0][2], t[0][3]), pack2<DT>(t[1][0], t[1][1]),
+                 pack2<DT>(t[1][2], t[1][3])};
+}
+
+// Row r0 + i of a tile in shared memory, elements k0 on, in row order.
+template <int DT>
+__device__ __forceinline__ u32x4 row_operand(const typename Ty<DT>::T* tile, int ld, int r0, int k0, int lane) {
+  return *reinterpret_cast<const u32x4*>(tile + (r0 + (lane & 15)) * ld + k0 + Op<DT>::kE * (lane >> 4));
+}
+// ... in acc order.
+template <int DT>
+__device__ __forceinline__ u32x4 row_operand_acc(const typename Ty<DT>::T* tile, int ld, int r0, int k0, int lane) {
+  const typename Ty<DT>::T* const p = tile + (r0 + (lane & 15)) * ld + k0 + 4 * (lane >> 4);
+  if constexpr (Op<DT>::kWide) {
+    return *reinterpret_cast<const u32x4*>(p);
+  } else {
+    const u32x2 a = *reinterpret_cast<const u32x2*>(p), b = *reinterpret_cast<const u32x2*>(p + 16);
+    return u32x4{a[0], a[1], b[0], b[1]};
+  }
+}
+// Four elements of column c0 + i of rows r0 + 4 g on, 16-bit types: the transposing read, in which each group of 16
+// lanes reads 4 rows of 16 elements, 8 bytes a lane, and gets a column each.
+template <int DT>
+__device__ __forceinline__ u32x2 column4(const typename Ty<DT>::T* tile, int ld, int r0, int c0, int lane) {
+  const typename Ty<DT>::T* const p = tile + (r0 + 4 * (lane >> 4) + ((lane & 15) >> 2)) * ld + c0 + 4 * (lane & 3);
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4*)const_cast<typename Ty<DT>::T*>(p)));
+}
+// Column c0 + i, rows k0 on, in acc order: an operand whose sum runs over a tile's rows.
+template <int DT>
+__device__ __forceinline__ u32x4 column_operand(const typename Ty<DT>::T* tile, int ld, int k0, int c0, int lane) {
+  if constexpr (Op<DT>::kWide) {
+    u32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = __float_as_uint(tile[(k0 + 4 * (lane >> 4) + j) * ld + c0 + (lane & 15)]);
+    return v;
+  } else {
+    const u32x2 a = column4<DT>(tile, ld, k0, c0, lane), b = column4<DT>(tile, ld, k0 + 16, c0, lane);
+    return u32x4{a[0], a[1], b[0], b[1]};
+  }
+}
+
+// Rows of a (batch, seqlen, heads, width) tensor of one head, as a workgroup of 256 stages them: 64 rows of W elements,
+// 16 bytes a thread and step, held in registers between the load and the write to shared memory.
+template <int DT, int W>
+struct Staged {
+  using T = typename Ty<DT>::T;
+  static constexpr int kE = Op<DT>::kE;
+  static constexpr int kUnits = W / kE;                 // 16-byte units of a row
+  static constexpr int kSteps = kRun * kUnits / 256;
+  u32x4 v[kSteps];
+  // Rows r >= rows and elements >= width come as zeros.  vec: 16-byte aligned rows and a width that 16 bytes divide.
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int width, bool vec) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int u = s * 256 + static_cast<int>(threadIdx.x), r = u / kUnits, e = u % kUnits * kE;
+      v[s] = u32x4{0, 0, 0, 0};
+      if (r < rows && e < width) {
+        const T* const p = base + r * stride + e;
+        if (vec) {
+          v[s] = *reinterpret_cast<const u32x4*>(p);
+        } else {
+          T t[kE];
+#pragma unroll
+          for (int j = 0; j < kE; ++j) t[j] = e + j < width ? p[j] : static_cast<T>(0);
+          __builtin_memcpy(&v[s], t, 16);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* tile) const {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int u = s * 256 + static_cast<int>(threadIdx.x), r = u / kUnits, e = u % kUnits * kE;
+      *reinterpret_cast<u32x4*>(tile + r * (W + Op<DT>::kPad) + e) = v[s];
+    }
+  }
+};
+
+// A run's decays: c_t, the running sum of the log decays to token t and with it, in log2 units.  Sums are 64-bit and
+// kept as two floats, so that a difference is exact to fp32 however far both lie down.
+struct Decays {
+  float hi[kRun], lo[kRun];
+  float into[kRun];    // exp(c_t): what the state before the run still counts at t
+  float onward[kRun];  // exp(c_last - c_t): what token t still counts at the run's end
+  float whole;         // exp(c_last)
+};
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// Inclusive sum over the lanes up to each.
+__device__ __forceinline__ double prefix_sum(double v) {
+  v += dpp_or_zero<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8 within 16 lanes
+  v += dpp_or_zero<0x112, 0xF>(v);
+  v += dpp_or_zero<0x114, 0xF>(v);
+  v += dpp_or_zero<0x118, 0xF>(v);
+  v += dpp_or_zero<0x142, 0xA>(v);  // lane 15 of each row to the next, rows 1 and 3
+  v += dpp_or_zero<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
+  return v;
+}
+
+// g: lane t's log decay.  One that vanishes in fp32 anyway (exp(-1000) = 0, as for -inf) is cut off, so that sums stay
+// finite and later differences exact.
+__device__ __forceinline__ void run_decays(Decays& d, float g, int lane) {
+  g = g < -1000.0f ? -1000.0f : g;
+  const double c = prefix_sum(static_cast<double>(g)) * 1.4426950408889634;
+  const float hi = static_cast<float>(c);
+  const double last = __shfl(c, 63, 64);
+  d.hi[lane] = hi;
+  d.lo[lane] = static_cast<float>(c - hi);
+  d.into[lane] = exp2_acc(hi) * (1.0f + static_cast<float>(c - hi) * kLn2);
+  const double rest = last - c;
+  const float rh = static_cast<float>(rest);
+  d.onward[lane] = exp2_acc(rh) * (1.0f + static_cast<float>(rest - rh) * kLn2);
+  if (lane == 63) d.whole = exp2_acc(hi) * (1.0f + static_cast<float>(c - hi) * kLn2);
+}
+
+// exp(c_t - c_s)
+template <int DT>
+__device__ __forceinline__ float between(float hi_t, float lo_t, float hi_s, float lo_s) {
+  const float x = (hi_t - hi_s) + (lo_t - lo_s);
+  const float e = exp2_decay<DT>(x);
+  return DT == MM_F32 && x != x ? x : e;  // (exp2_acc's clamp would lose a NaN)
+}
+
+template <int GT>
+__device__ __forceinline__ float load_g(const void* g, int64_t i) { return ld<GT>(g, i); }
+
+}  // namespace dattn
+}  // namespace mm

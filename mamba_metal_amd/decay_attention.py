@@ -1,0 +1,247 @@
+"""Linear attention with a decay for each head, over long sequences and token by token.
+
+    S_t = exp(g_t) S_{t-1} + k_t v_t^T          y_t = scale S_t^T q_t
+
+``decay_attention`` runs it over (batch, seqlen, heads) and is differentiable; ``decay_attention_step`` is its single
+token.  It stands beside ``selective_scan`` and ``gated_scan``, whose states belong to a channel; here a head has a
+(key_dim, value_dim) state, and neighbouring heads may share their q and k.  States and sums are float32 for every dtype.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from mamba_metal_amd import _lib
+from mamba_metal_amd.act8 import channels_last
+
+MAX_KEY_DIM = 128     # MM_DECAY_MAX_KEY_DIM
+MAX_VALUE_DIM = 1024  # MM_DECAY_MAX_VALUE_DIM
+_two, _three = _lib._i64a2, _lib._i64a3
+
+
+def _params(q, k, v, g, lengths, scale, dev):
+    p = _lib.DecayAttentionParams()
+    p.batch, p.seqlen, p.groups, p.key_dim = q.shape
+    p.heads, p.value_dim = v.shape[2:]
+    p.q, p.q_stride = q.data_ptr(), _three(*q.stride()[:3])
+    p.k, p.k_stride = k.data_ptr(), _three(*k.stride()[:3])
+    p.v, p.v_stride = v.data_ptr(), _three(*v.stride()[:3])
+    p.log_decay = g.data_ptr()
+    p.log_decay_stride = _three(0, 0, g.stride(0)) if g.dim() == 1 else _three(*g.stride())
+    if lengths is not None:
+        p.lengths = lengths.data_ptr()
+        p.lengths_dtype = 1 if lengths.dtype == torch.int64 else 0
+    p.scale = scale
+    p.dtype, p.log_decay_dtype = _lib.dtype_code(q.dtype), _lib.dtype_code(g.dtype)
+    return p
+
+
+def _call(name, p, backward, dev):
+    lib = _lib.load()
+    nbytes = lib.mm_decay_attention_workspace_size(p.batch, p.seqlen, p.heads, p.groups, p.key_dim, p.value_dim, p.dtype,
+                                                   backward)
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+    with _lib.on_device(dev):
+        st = getattr(lib, name)(p, _lib.stream_of(dev))
+    _lib.check(st, name)
+
+
+def _states_bytes(q, v):
+    return _lib.load().mm_decay_attention_states_size(q.shape[0], q.shape[1], v.shape[2], q.shape[3], v.shape[3],
+                                                      _lib.dtype_code(q.dtype))
+
+
+def _forward(dev, q, k, v, g, h0, lengths, scale, want_state, train):
+    """y, the final state (or None) and, for training, the states before each run of tokens."""
+    p = _params(q, k, v, g, lengths, scale, dev)
+    y = torch.empty(v.shape, dtype=v.dtype, device=dev)
+    p.y = y.data_ptr()
+    state = states = None
+    if h0 is not None:
+        p.h0 = h0.data_ptr()
+    if want_state:
+        state = torch.empty((q.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=dev)
+        p.state_out = state.data_ptr()
+    if train:
+        states = torch.empty(_states_bytes(q, v), dtype=torch.uint8, device=dev)
+        p.run_states = states.data_ptr() or None
+    _call("mm_decay_attention_fwd", p, 0, dev)
+    return y, state, states
+
+
+class _DecayAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, dev, q, k, v, g, h0, lengths, scale, want_state):
+        y, state, states = _forward(dev, q, k, v, g, h0, lengths, scale, want_state, True)
+        ctx.meta = (dev, q.dtype, q.shape, v.shape, g.dtype, g.shape, scale,
+                    _lib.hooked() and (None if lengths is None else lengths.dtype,))
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, g, lengths, states)
+        return (y, state) if want_state else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dstate=None):
+        if dy is None and dstate is None:
+            return (None,) * 9
+        dev, dtype, qk_shape, v_shape, g_dtype, g_shape, scale, hooked = ctx.meta
+        saved = ctx.saved_tensors
+        if hooked:
+            saved = _checked(saved, dev, dtype, qk_shape, v_shape, g_dtype, g_shape, *hooked)
+        q, k, v, g, lengths, states = saved
+        p = _params(q, k, v, g, lengths, scale, dev)
+        p.run_states = states.data_ptr() or None
+        if dy is None:  # only the final state was used
+            dy = torch.zeros((1, 1, 1, v_shape[3]), dtype=dtype, device=dev).expand(v_shape)
+        elif dy.dtype != dtype or (dy.stride(-1) != 1 and v_shape[3] > 1):
+            dy = dy.to(dtype).contiguous()
+        p.dy, p.dy_stride = dy.data_ptr(), _three(*dy.stride()[:3])
+        if dstate is not None:
+            dstate = dstate.contiguous()
+            p.dstate = dstate.data_ptr()
+        dq, dk = (torch.empty(qk_shape, dtype=dtype, device=dev) for _ in range(2))
+        dv = torch.empty(v_shape, dtype=dtype, device=dev)
+        p.dq, p.dk, p.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        dg = dh0 = None
+        if ctx.needs_input_grad[4]:
+            dg = (torch.empty if v_shape[0] and v_shape[1] else torch.zeros)(g_shape, dtype=torch.float32, device=dev)
+            if len(g_shape) == 1:
+                p.dlog_decay_heads = dg.data_ptr()
+            else:
+                p.dlog_decay = dg.data_ptr() or None
+        if ctx.needs_input_grad[5]:
+            dh0 = torch.empty((v_shape[0], v_shape[2], qk_shape[3], v_shape[3]), dtype=torch.float32, device=dev)
+            p.dh0 = dh0.data_ptr()
+        _call("mm_decay_attention_bwd", p, 1, dev)
+        return None, dq, dk, dv, None if dg is None else dg.to(g_dtype), dh0, None, None, None
+
+
+def _checked(saved, dev, dtype, qk_shape, v_shape, g_dtype, g_shape, lengths_dtype):
+    """The saved tensors, where hooks may have changed them."""
+    q, k, v, g, lengths, states = saved
+    if lengths_dtype is not None:
+        lengths = _lib.saved(lengths, lengths_dtype, (v_shape[0],), dev)
+    q, k = (_lib.saved(t, dtype, qk_shape, dev, rows=True) for t in (q, k))
+    v = _lib.saved(v, dtype, v_shape, dev, rows=True)
+    return q, k, v, _lib.saved(g, g_dtype, g_shape, dev), lengths, _lib.saved(states, torch.uint8, (_states_bytes(q, v),), dev)
+
+
+def _check(q, k, v, g, lead, names):
+    """q and k (*lead, groups, key_dim), v (*lead, heads, value_dim), g (*lead, heads) or (heads,)."""
+    n = len(lead)
+    if q.dim() != n + 2 or v.dim() != n + 2 or v.shape[:n] != q.shape[:n]:
+        raise ValueError(f"q must be {names[:-1]}, groups, key_dim) and v {names[:-1]}, heads, value_dim), got "
+                         f"{tuple(q.shape)} and {tuple(v.shape)}")
+    if k.shape != q.shape:
+        raise ValueError(f"k is {tuple(k.shape)}, q {tuple(q.shape)}")
+    groups, dk = q.shape[n:]
+    heads, dv = v.shape[n:]
+    if groups < 1 or heads < 1 or heads % groups:
+        raise ValueError(f"{heads} heads cannot share {groups} groups of q and k")
+    if not 1 <= dk <= MAX_KEY_DIM or not 1 <= dv <= MAX_VALUE_DIM:
+        raise ValueError(f"key_dim {dk} must be 1 to {MAX_KEY_DIM}, value_dim {dv} 1 to {MAX_VALUE_DIM}")
+    if g.shape != (heads,) and g.shape != (*q.shape[:n], heads):
+        raise ValueError(f"log_decay is {tuple(g.shape)}, expected {(heads,)} or {(*q.shape[:n], heads)}")
+    for name, t in (("k", k), ("v", v)):
+        if t.dtype != q.dtype:
+            raise TypeError(f"{name} is {t.dtype}, q {q.dtype}")
+    _lib.dtype_code(q.dtype)
+    _lib.dtype_code(g.dtype)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        channels_last(t, name)
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, *, scale: float = 1.0,
+                    h0: torch.Tensor | None = None, lengths: torch.Tensor | None = None, return_state: bool = False):
+    """Linear attention with a decay for each head over a batch of sequences (see the module's formulas).
+
+    q, k: (batch, seqlen, groups, key_dim), v: (batch, seqlen, heads, value_dim), of one dtype (float32, float16,
+    bfloat16) with unit channel stride, any other strides; head h uses q and k of group h // (heads // groups).
+    key_dim up to 128, value_dim up to 1024.  log_decay: (batch, seqlen, heads), or (heads,) for a constant, of any of
+    the three dtypes, at most 0 (-inf forgets all before; above 0 the state grows until it overflows).  h0: (batch,
+    heads, key_dim, value_dim), the state before the first token, zeros if not given.  lengths: (batch,) int32 or int64
+    on the same GPU; tokens from lengths[b] on (clamped to 0 .. seqlen) leave the state alone, have y = 0 and zero
+    gradients, whatever their inputs hold.
+
+    Returns y (batch, seqlen, heads, value_dim), contiguous, in v's dtype; with ``return_state`` also the state after
+    each sequence's last token, (batch, heads, key_dim, value_dim) float32.
+
+    With 16-bit inputs the scores of a run of 64 tokens and the state that meets q are rounded to 16 bits, once each,
+    before their products, and so are their gradients; the state itself is not.  The gradient of a float32 log_decay
+    beside 16-bit q, k and v is therefore as exact as theirs.  In float16 the scores scale * q.k and the gradients'
+    dy.v have to stay below 65504.  A NaN or an infinity stays in its sequence and head (in its group, for the gradients
+    of q and k); one in k or v may also reach the up to 63 tokens before it in its run of 64.
+
+    Gradients flow to q, k, v, log_decay and h0 (once, not twice, and not in forward mode).  For them a call that needs
+    any keeps its inputs and, in their dtype, the state before every 64th token.
+
+    To capture a backward pass into a graph, capture the forward pass with it, and let no eager autograd graph of the
+    same leaf tensors be alive at that time."""
+    if q.dim() != 4:
+        raise ValueError(f"q must be (batch, seqlen, groups, key_dim), got {tuple(q.shape)}")
+    _check(q, k, v, log_decay, q.shape[:2], "(batch, seqlen)")
+    b, n, _, dk = q.shape
+    heads, dv = v.shape[2:]
+    if h0 is not None:
+        if h0.shape != (b, heads, dk, dv):
+            raise ValueError(f"h0 is {tuple(h0.shape)}, expected {(b, heads, dk, dv)}")
+        if not h0.is_floating_point():
+            raise TypeError(f"h0 is {h0.dtype}")
+    if lengths is not None:
+        if lengths.shape != (b,):
+            raise ValueError(f"lengths is {tuple(lengths.shape)}, expected ({b},)")
+        if lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"lengths is {lengths.dtype}, expected int32 or int64")
+    _lib.refuse_transforms("decay_attention", q, k, v, log_decay, h0)
+    dev = _lib.require_cuda(q, k, v, log_decay, h0, lengths)
+    h0 = None if h0 is None else (h0 if h0.dtype == torch.float32 else h0.float()).contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, h0)):
+        return _DecayAttention.apply(dev, q, k, v, log_decay, h0, lengths, float(scale), return_state)
+    y, state, _ = _forward(dev, q, k, v, log_decay, h0, lengths, float(scale), return_state, False)
+    return (y, state) if return_state else y
+
+
+def decay_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                         *, scale: float = 1.0, state_out: torch.Tensor | None = None, out: torch.Tensor | None = None):
+    """One token of every sequence: the new state, and y (batch, heads, value_dim) in v's dtype, which is returned.
+
+    state (batch, heads, key_dim, value_dim) contiguous float32 is updated in place, or left as it is where ``state_out``
+    (the same kind of tensor) is given.  q, k: (batch, groups, key_dim), v and ``out``: (batch, heads, value_dim), of one
+    dtype with unit channel stride; log_decay (batch, heads) or (heads,).  Not differentiable: a tensor that requires a
+    gradient is refused while gradients are on, and one with a tangent always."""
+    if q.dim() != 3:
+        raise ValueError(f"q must be (batch, groups, key_dim), got {tuple(q.shape)}")
+    _check(q, k, v, log_decay, q.shape[:1], "(batch)")
+    b, groups, dk = q.shape
+    heads, dv = v.shape[1:]
+    for name, t in (("state", state), ("state_out", state_out)):
+        if t is not None and (t.shape != (b, heads, dk, dv) or t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous float32 {(b, heads, dk, dv)}")
+    if out is not None:
+        if out.shape != v.shape:
+            raise ValueError(f"out is {tuple(out.shape)}, v {tuple(v.shape)}")
+        if out.dtype != v.dtype:
+            raise TypeError(f"out is {out.dtype}, v {v.dtype}")
+        channels_last(out, "out")
+    if torch.is_grad_enabled() and (state.requires_grad or q.requires_grad or k.requires_grad or v.requires_grad
+                                    or log_decay.requires_grad):
+        raise RuntimeError("decay_attention_step has no gradient: call it under no_grad or inference_mode, "
+                           "or train through decay_attention")
+    _lib.refuse_transforms("decay_attention_step", state, q, k, v, log_decay)
+    dev = _lib.require_cuda(state, q, k, v, log_decay, state_out, out)
+    lib = _lib.load()
+    if out is None:
+        out = torch.empty(v.shape, dtype=v.dtype, device=dev)
+    with _lib.on_device(dev):
+        st = lib.mm_decay_attention_step(
+            state.data_ptr(), state.data_ptr() if state_out is None else state_out.data_ptr(), q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), log_decay.data_ptr(), out.data_ptr(), b, heads, groups, dk, dv, _two(*q.stride()[:2]),
+            _two(*k.stride()[:2]), _two(*v.stride()[:2]),
+            _two(0, log_decay.stride(0)) if log_decay.dim() == 1 else _two(*log_decay.stride()), _two(*out.stride()[:2]),
+            float(scale), _lib.dtype_code(q.dtype), _lib.dtype_code(log_decay.dtype), _lib.stream_of(dev))
+    _lib.check(st, "mm_decay_attention_step")
+    return out
