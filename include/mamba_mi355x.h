@@ -558,6 +558,59 @@ int mm_decay_attention_step(const float* state, float* state_out, const void* q,
                             const int64_t y_stride[2], float scale, int32_t dtype,
                             int32_t log_decay_dtype, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Embedding (training; the reference looks rows up through MLX): y[i] = scale * weight[ids[i]], rounded once.
+ * ids (n,) contiguous, int32 (ids_dtype 0) or int64 (1); weight (vocab, dim) with a row stride; y (n, dim) contiguous.
+ * An id outside [0, vocab) gives a row of NaNs. */
+int mm_embedding_fwd(const void* ids, const void* weight, void* y, int64_t n, int64_t vocab, int64_t dim,
+                     int64_t weight_stride, float scale, int32_t ids_dtype, int32_t dtype, void* stream);
+/* Its gradient: dweight[v] = scale * (sum over the i with ids[i] = v, in their order, in fp32), zeros without any; ids
+ * outside [0, vocab) and the id `padding` (-1 = none) have none.  dy (n, dim) with a row stride; dweight (vocab, dim)
+ * contiguous, all of it written. */
+size_t mm_embedding_bwd_workspace_size(int64_t n, int64_t vocab, int64_t dim);
+int mm_embedding_bwd(const void* ids, const void* dy, void* dweight, int64_t n, int64_t vocab, int64_t dim,
+                     int64_t dy_stride, float scale, int64_t padding, int32_t ids_dtype, int32_t dtype,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Softmax cross entropy of the rows before the head, without keeping the logits (no counterpart in the reference, which
+ * has the head's logits alone, mamba_model.py:78):
+ *   l = weight x      loss = log(sum_v exp(l_v)) - l[target]      (0 where target is ignore_index)
+ * x (rows, dim), weight (vocab, dim) in dtype with row strides; targets (rows,) contiguous, int32 (targets_dtype 0) or
+ * int64 (1).  A target outside [0, vocab) that is not ignore_index makes its row's loss NaN, and its gradients.  What an
+ * ignored row of x holds does not matter.  reduction 0: loss (rows,); 1: their mean over the rows that are not ignored
+ * (NaN if there is none), 2: their sum, one float, added in 64 bits.  Logits, maxima, sums and losses are fp32.  The
+ * forward call writes lse (rows,), log(sum_v exp(l_v)), unless it is NULL; the backward call reads it.
+ *
+ * Backward: dl = (softmax(l) - onehot(target)) dloss, computed again from x, weight and lse in pieces of the vocabulary
+ * of at most 512 MB and rounded once to dtype; dx = dl weight (rows, dim), dweight = dl^T x (vocab, dim), contiguous, in
+ * dtype, summed in fp32 in a fixed order (either may be NULL).  dloss: fp32, for reduction 0 with a stride (0: all the same), else one. */
+typedef struct mm_linear_cross_entropy_params {
+  const void* x;
+  const void* weight;
+  const void* targets;
+  float* loss;
+  float* lse;
+  const float* dloss;
+  void* dx;
+  void* dweight;
+  void* workspace;            /* 256-byte aligned, no initial contents */
+  size_t workspace_bytes;
+  int64_t rows, dim, vocab;
+  int64_t x_stride, weight_stride, dloss_stride;
+  int64_t ignore_index;
+  int32_t dtype;
+  int32_t targets_dtype;
+  int32_t reduction;
+  int32_t reserved;
+} mm_linear_cross_entropy_params;
+
+/* Workspace bytes of the forward (backward = 0) or backward call with these parameters (weight's address and stride, the
+ * sizes, types and reduction count). */
+size_t mm_linear_cross_entropy_workspace_size(const mm_linear_cross_entropy_params* p, int32_t backward);
+int mm_linear_cross_entropy_fwd(const mm_linear_cross_entropy_params* p, void* stream);
+int mm_linear_cross_entropy_bwd(const mm_linear_cross_entropy_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,7 +9,9 @@ include/mamba_mi355x.h); projections use torch GEMMs.  There is no CPU fallback.
 from mamba_metal_amd._loader import load_kernel
 from mamba_metal_amd.act8 import Act8, act8_pack, act8_unpack
 from mamba_metal_amd.conv1d import causal_conv1d_train
+from mamba_metal_amd.cross_entropy import linear_cross_entropy
 from mamba_metal_amd.decay_attention import decay_attention, decay_attention_step
+from mamba_metal_amd.embedding import embedding
 from mamba_metal_amd.gated_scan import gated_scan, gated_scan_step
 from mamba_metal_amd.generate import (GraphDecoder, GraphPrefill, generate, generate_fast,
                                       generate_fast_ids)
@@ -37,8 +39,10 @@ __all__ = [
     "causal_conv1d_train",
     "decay_attention",
     "decay_attention_step",
+    "embedding",
     "gated_scan",
     "gated_scan_step",
     "generate_fast_ids",
     "init_weights_",
+    "linear_cross_entropy",
 ]

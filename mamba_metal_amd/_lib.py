@@ -111,6 +111,17 @@ class DecayAttentionParams(ctypes.Structure):
     ]
 
 
+class LinearCrossEntropyParams(ctypes.Structure):
+    """Mirror of ``mm_linear_cross_entropy_params`` (include/mamba_mi355x.h)."""
+
+    _fields_ = [
+        ("x", _vp), ("weight", _vp), ("targets", _vp), ("loss", _vp), ("lse", _vp), ("dloss", _vp), ("dx", _vp),
+        ("dweight", _vp), ("workspace", _vp), ("workspace_bytes", _sz), ("rows", _i64), ("dim", _i64), ("vocab", _i64),
+        ("x_stride", _i64), ("weight_stride", _i64), ("dloss_stride", _i64), ("ignore_index", _i64), ("dtype", _i32),
+        ("targets_dtype", _i32), ("reduction", _i32), ("reserved", _i32),
+    ]
+
+
 ACT8_BLOCK = 16   # MM_ACT8_BLOCK
 
 _SIGNATURES = {
@@ -156,6 +167,13 @@ _SIGNATURES = {
     "mm_decay_attention_bwd": ([ctypes.POINTER(DecayAttentionParams), _vp], ctypes.c_int),
     "mm_decay_attention_step": (
         [_vp] * 7 + [_i64] * 5 + [_i64a2] * 5 + [ctypes.c_float, _i32, _i32, _vp], ctypes.c_int),
+    "mm_embedding_fwd": ([_vp] * 3 + [_i64] * 4 + [ctypes.c_float, _i32, _i32, _vp], ctypes.c_int),
+    "mm_embedding_bwd_workspace_size": ([_i64] * 3, _sz),
+    "mm_embedding_bwd": (
+        [_vp] * 3 + [_i64] * 4 + [ctypes.c_float, _i64, _i32, _i32, _vp, _sz, _vp], ctypes.c_int),
+    "mm_linear_cross_entropy_workspace_size": ([ctypes.POINTER(LinearCrossEntropyParams), _i32], _sz),
+    "mm_linear_cross_entropy_fwd": ([ctypes.POINTER(LinearCrossEntropyParams), _vp], ctypes.c_int),
+    "mm_linear_cross_entropy_bwd": ([ctypes.POINTER(LinearCrossEntropyParams), _vp], ctypes.c_int),
     "mm_act8_pack": ([_vp] * 3 + [_i64] * 3 + [_i64a2, _i32, _vp], ctypes.c_int),
     "mm_act8_unpack": ([_vp] * 3 + [_i64] * 3 + [_i64a2, _i32, _vp], ctypes.c_int),
     "mm_causal_conv1d_fwd_act8": (

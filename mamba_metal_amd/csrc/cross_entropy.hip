@@ -1,0 +1,645 @@
+// Softmax cross entropy of the rows before a language model's head, without keeping the logits.
+//
+//   l = W x      loss = log sum_v exp(l_v) - l_t      dl = (softmax(l) - onehot(t)) dloss      dx = W^T dl   dW = dl x^T
+//
+// Forward: the product W x by tiles, whose epilogue leaves of a tile the maximum and the sum of exponentials of every row
+// (and the target's logit): 8 bytes for 256 logits.  Backward: piece by piece of the vocabulary the logits are computed
+// again, and the epilogue turns them into dl in the inputs' type (its one rounding); the piece is then multiplied with W
+// (adding to dx, in fp32) and with x (its rows of dW).  The four products are the time; everything else is a few percent.
+// A product's tile has the vocabulary along the accumulators' rows, so that the softmax's sums run within a lane.
+//
+// Rows that are ignored take no part: the others are gathered first (their sums over rows are then never touched by what
+// an ignored row holds, and a batch that is mostly ignored costs its share), and workgroups past their count end at once.
+#include "cross_entropy.h"
+
+namespace mm {
+namespace xent {
+
+using slab::Matrix;
+using slab::f32x16;
+using slab::kAcross;
+using slab::kAlong;
+using slab::u32x2;
+using slab::u32x4;
+
+using Big = slab::Tile<256, 256, 2, 4>;
+using Mid = slab::Tile<128, 128, 2, 2>;
+using Thin = slab::Tile<128, 64, 4, 1>;  // few rows of x
+
+constexpr int kThreads = 1024;
+
+__device__ __forceinline__ int64_t target_of(const Loss& p, int64_t i) {
+  return p.targets64 ? static_cast<const int64_t*>(p.targets)[i] : static_cast<const int32_t*>(p.targets)[i];
+}
+
+// A sum (or maximum) over a workgroup of 1024.
+template <typename V, typename F>
+__device__ __forceinline__ V all_of(V v, V* s, F join) {
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) v = join(v, __shfl_xor(v, x, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = s[0];
+  for (int w = 1; w < kThreads / 64; ++w) v = join(v, s[w]);
+  return v;
+}
+
+// The rows that count, in order, and for the backward pass what their gradients are multiplied by.  One workgroup.
+__global__ __launch_bounds__(kThreads) void rows_kernel(const Loss p, bool backward) {
+  __shared__ int32_t s_wave[kThreads / 64];
+  __shared__ float s_f[kThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t base = 0;
+  float top = 0.0f;
+  for (int64_t r0 = 0; r0 < p.rows; r0 += kThreads) {
+    const int64_t r = r0 + threadIdx.x;
+    const int64_t t = r < p.rows ? target_of(p, r) : 0;
+    const bool on = r < p.rows && t != p.ignore;
+    const uint64_t b = __ballot(on);
+    if (lane == 0) s_wave[wave] = __popcll(b);
+    __syncthreads();
+    int32_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+      before += w < wave ? s_wave[w] : 0;
+      all += s_wave[w];
+    }
+    __syncthreads();
+    const int32_t at = base + before + __popcll(b & ((1ull << lane) - 1));
+    if (r < p.rows) p.at[r] = on ? at : -1;
+    if (on) {
+      p.row[at] = static_cast<int32_t>(r);
+      p.target_at[at] = t;
+      if (backward) {
+        const float d = p.dloss[r * p.dloss_stride];
+        p.weights[at] = d;
+        p.lse_at[at] = t < 0 || t >= p.vocab ? __builtin_nanf("") : p.lse[r];
+        top = fmaxf(top, fabsf(d));
+      }
+    }
+    base += all;
+  }
+  if (threadIdx.x == 0) p.count[0] = base;
+  if (threadIdx.x < 4) reinterpret_cast<uint32_t*>(p.zeros)[threadIdx.x] = 0;
+  if (!backward) return;
+  // Mean: every row's share.  fp16: the pieces hold dl times a power of two that puts the largest |dloss| at 2^12, so
+  // that small probabilities are not subnormal; the sums take it back.
+  top = all_of(top, s_f, [](float a, float b) { return fmaxf(a, b); });
+  const float share = p.reduction == 1 ? 1.0f / static_cast<float>(base) : 1.0f;
+  float up = 1.0f;
+  if (p.dtype == MM_F16) {
+    const int e = static_cast<int>(__float_as_uint(top * share) >> 23) - 127;
+    if (top * share > 0.0f && e > -100 && e < 100) up = __builtin_ldexpf(1.0f, 12 - e);
+  }
+  for (int64_t i = threadIdx.x; i < base; i += kThreads) p.weights[i] *= share * up;
+  if (threadIdx.x == 0) p.scalars[0] = 1.0f / up;
+}
+
+// Rows of a matrix to 16-byte aligned ones with zeros behind their end; gather: those that count.
+template <int DT>
+__global__ __launch_bounds__(256) void lay_out_kernel(const void* from, int64_t from_ld, char* to, int64_t to_ld, int64_t rows,
+                                                     int64_t dim, const int32_t* row, const int32_t* count, bool vec) {
+  using T = typename Ty<DT>::T;
+  constexpr int kE = 16 / sizeof(T);
+  const int64_t units = to_ld / 16, n = (count ? *count : rows) * units;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < n; e += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t r = e / units, c = e % units * kE;
+    const T* const p = static_cast<const T*>(from) + (row ? row[r] : r) * from_ld + c;
+    u32x4 v;
+    if (vec) {
+      v = *reinterpret_cast<const u32x4*>(p);
+    } else {
+      T t[kE];
+#pragma unroll
+      for (int j = 0; j < kE; ++j) t[j] = c + j < dim ? p[j] : static_cast<T>(0);
+      __builtin_memcpy(&v, t, 16);
+    }
+    *reinterpret_cast<u32x4*>(to + r * to_ld + c * sizeof(T)) = v;
+  }
+}
+
+__device__ __forceinline__ Matrix vocabulary(const Loss& p, int64_t v0) {
+  const int64_t es = p.dtype == MM_F32 ? 4 : 2;
+  Matrix m;
+  m.base = (p.wc ? p.wc : static_cast<const char*>(p.weight));
+  m.ld = p.wc ? p.ld : p.w_ld * es;
+  m.base += v0 * m.ld;
+  m.rows = p.vocab - v0;
+  m.k = p.ld / es;
+  m.zeros = p.zeros;
+  return m;
+}
+__device__ __forceinline__ Matrix counted(const Loss& p, int32_t count) {
+  Matrix m;
+  m.base = p.xc;
+  m.ld = p.ld;
+  m.rows = count;
+  m.k = p.ld / (p.dtype == MM_F32 ? 4 : 2);
+  m.zeros = p.zeros;
+  return m;
+}
+
+// Logits of a tile of the vocabulary (rows) and of x (columns).  Forward: each column's maximum and sum of exponentials.
+// Backward: dl of the piece.
+template <int DT, typename S, bool GRAD>
+__global__ __launch_bounds__(64 * S::NW) void logits_kernel(const Loss p) {
+  using T = typename Ty<DT>::T;
+  __shared__ __attribute__((aligned(16))) char s0[(S::BM + S::BN) * slab::kSlab];
+  __shared__ __attribute__((aligned(16))) char s1[(S::BM + S::BN) * slab::kSlab];
+  const int32_t count = *p.count;
+  const int64_t vocab = GRAD ? p.piece_n : p.vocab;
+  const uint32_t vt = static_cast<uint32_t>((GRAD ? p.piece_ld / static_cast<int64_t>(sizeof(T)) : vocab) + S::BM - 1) / S::BM;
+  const uint32_t rt = static_cast<uint32_t>((p.rows + S::BN - 1) / S::BN);
+  uint32_t m, n;
+  slab::tile_of(blockIdx.x, vt, rt, m, n);
+  const int64_t v0 = static_cast<int64_t>(m) * S::BM, r0 = static_cast<int64_t>(n) * S::BN;
+  if (r0 >= count) return;
+  f32x16 acc[S::TM][S::TN];
+  slab::clear<S>(acc);
+  const Matrix w = vocabulary(p, GRAD ? p.piece0 : 0), x = counted(p, count);
+  slab::product<DT, kAlong, kAlong, S>(w, x, v0, r0, 0, w.k, s0, s1, acc);
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / S::WN, wn = wave % S::WN;
+  const int64_t vw = v0 + wm * 32 * S::TM + 4 * (lane >> 5);  // of the lane's first accumulator
+  const int here = vocab - vw < 1 << 20 ? static_cast<int>(vocab - vw) : 1 << 20;  // tokens from there on
+  if constexpr (!GRAD) {
+    __syncthreads();
+    float* const s_stat = reinterpret_cast<float*>(s0);  // (WM, BN, 2)
+#pragma unroll
+    for (int j = 0; j < S::TN; ++j) {
+      const int col = wn * 32 * S::TN + 32 * j + (lane & 31);
+      const int64_t r = r0 + col;
+      const int64_t t64 = r < count ? p.target_at[r] - vw : -1;
+      const int t = t64 >= 0 && t64 < here ? static_cast<int>(t64) : -1;
+      float top = -INFINITY, hit = 0.0f;
+      bool bad = false, mine = false;
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int v = 32 * i + 8 * (e >> 2) + (e & 3);
+          const float l = v < here ? acc[i][j][e] : -INFINITY;
+          acc[i][j][e] = l;
+          hit = v == t ? l : hit;
+          mine |= v == t;
+          bad |= l != l;  // (lost by fmaxf and, in fp32, by exp2_acc's clamp)
+          top = fmaxf(top, l);
+        }
+      if (mine) p.hit[r] = hit;
+      top = fmaxf(top, lane_xor(top, 32));
+      float sum = 0.0f;
+      const float from = top == -INFINITY ? 0.0f : top;  // (all logits -inf: a sum of 0, not a NaN)
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum += exp2_decay<DT>((acc[i][j][e] - from) * kLog2e);
+      if (bad || top == INFINITY) sum = __builtin_nanf("");
+      sum += lane_xor(sum, 32);
+      if (lane < 32) {
+        s_stat[(wm * S::BN + col) * 2] = top;
+        s_stat[(wm * S::BN + col) * 2 + 1] = sum;
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < S::BN; c += 64 * S::NW) {
+      if (r0 + c >= count) continue;
+      float top = s_stat[c * 2], sum = s_stat[c * 2 + 1];
+#pragma unroll
+      for (int k = 1; k < S::WM; ++k) {
+        const float t2 = s_stat[(k * S::BN + c) * 2], s2 = s_stat[(k * S::BN + c) * 2 + 1];
+        const float m2 = fmaxf(top, t2), from = m2 == -INFINITY ? 0.0f : m2;
+        sum = sum * exp2_acc((top - from) * kLog2e) + s2 * exp2_acc((t2 - from) * kLog2e);
+        top = m2;
+      }
+      float* const out = p.stats + ((r0 + c) * p.tiles + m) * 2;
+      out[0] = top;
+      out[1] = sum;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < S::TN; ++j) {
+      const int64_t r = r0 + wn * 32 * S::TN + 32 * j + (lane & 31);
+      if (r >= count) continue;
+      const float lse = p.lse_at[r], weight = p.weights[r];
+      const int64_t t64 = p.target_at[r] - p.piece0 - vw;
+      const int t = t64 >= 0 && t64 < here ? static_cast<int>(t64) : -1;
+      char* const to = p.piece + r * p.piece_ld + vw * static_cast<int64_t>(sizeof(T));
+      const int wide = static_cast<int>(p.piece_ld / static_cast<int64_t>(sizeof(T)) - vw);
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int v = 32 * i + 8 * q;
+          if (v >= wide) continue;
+          T d[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float z = (acc[i][j][4 * q + e] - lse) * kLog2e;
+            float g = exp2_decay<DT>(z);
+            if (DT == MM_F32) g = z != z ? z : g;
+            g = (g - (v + e == t ? 1.0f : 0.0f)) * weight;
+            d[e] = Ty<DT>::from(v + e < here ? g : 0.0f);
+          }
+          if constexpr (DT == MM_F32) {
+            *reinterpret_cast<slab::f32x4*>(to + v * 4) = slab::f32x4{d[0], d[1], d[2], d[3]};
+          } else {
+            u32x2 w2;
+            __builtin_memcpy(&w2, d, 8);
+            *reinterpret_cast<u32x2*>(to + v * 2) = w2;
+          }
+        }
+    }
+  }
+}
+
+// A row's loss from its tiles' maxima and sums: a wave a row.
+__global__ __launch_bounds__(256) void merge_kernel(const Loss p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (r >= p.rows) return;
+  const int32_t at = p.at[r];
+  float loss = 0.0f, lse = 0.0f;
+  if (at >= 0) {
+    const float* const s = p.stats + at * p.tiles * 2;
+    float top = -INFINITY;
+    for (int64_t t = lane; t < p.tiles; t += 64) top = fmaxf(top, s[2 * t]);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, lane_xor(top, x));
+    const float from = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    for (int64_t t = lane; t < p.tiles; t += 64) sum += s[2 * t + 1] * exp2_acc((s[2 * t] - from) * kLog2e);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) sum += lane_xor(sum, x);
+    const int64_t t = p.target_at[at];
+    lse = top + logf(sum);
+    loss = t < 0 || t >= p.vocab ? __builtin_nanf("") : (top - p.hit[at]) + logf(sum);
+  }
+  if (lane == 0) {
+    if (p.lse) p.lse[r] = lse;
+    (p.row_loss ? p.row_loss : p.loss)[r] = loss;
+  }
+}
+
+// The rows' sum or mean, in 64 bits and a fixed order.  One workgroup.
+__global__ __launch_bounds__(kThreads) void total_kernel(const Loss p) {
+  __shared__ double s_d[kThreads / 64];
+  double sum = 0.0;
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < p.rows; r += kThreads) sum += p.row_loss[r];
+  sum = all_of(sum, s_d, [](double a, double b) { return a + b; });
+  if (threadIdx.x == 0) p.loss[0] = static_cast<float>(p.reduction == 1 ? sum / static_cast<double>(*p.count) : sum);
+}
+
+// dx's part of this piece: rows that count by channels, a split of the piece's tokens; added in fp32.
+template <int DT, typename S>
+__global__ __launch_bounds__(64 * S::NW) void dx_kernel(const Loss p) {
+  using T = typename Ty<DT>::T;
+  __shared__ __attribute__((aligned(16))) char s0[(S::BM + S::BN) * slab::kSlab];
+  __shared__ __attribute__((aligned(16))) char s1[(S::BM + S::BN) * slab::kSlab];
+  const int32_t count = *p.count;
+  const uint32_t mt = static_cast<uint32_t>((p.rows + S::BM - 1) / S::BM), nt = static_cast<uint32_t>((p.dim + S::BN - 1) / S::BN);
+  uint32_t m, n;
+  slab::tile_of(blockIdx.x % (mt * nt), mt, nt, m, n);
+  const int64_t split = blockIdx.x / (mt * nt);
+  const int64_t r0 = static_cast<int64_t>(m) * S::BM, c0 = static_cast<int64_t>(n) * S::BN;
+  if (r0 >= count) return;
+  const int64_t k0 = split * p.split_k, k1 = k0 + p.split_k < p.piece_n ? k0 + p.split_k : p.piece_n;
+  f32x16 acc[S::TM][S::TN];
+  slab::clear<S>(acc);
+  Matrix dl, w = vocabulary(p, p.piece0);
+  dl.base = p.piece;
+  dl.ld = p.piece_ld;
+  dl.rows = count;
+  dl.zeros = p.zeros;
+  w.rows = p.ld / static_cast<int64_t>(sizeof(T));
+  if (k1 > k0) slab::product<DT, kAlong, kAcross, S>(dl, w, r0, c0, k0, k1 - k0, s0, s1, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float* const out = p.dx_part + split * p.rows * p.dim;
+#pragma unroll
+  for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::TN; ++j) {
+      const int64_t c = c0 + wave % S::WN * 32 * S::TN + 32 * j + (lane & 31);
+      const int64_t rt = r0 + wave / S::WN * 32 * S::TM + 32 * i + 4 * (lane >> 5);
+      const int here = c < p.dim ? static_cast<int>(count - rt) : 0;
+      float* at = out + rt * p.dim + c;
+#pragma unroll
+      for (int q = 0; q < 4; ++q, at += 8 * p.dim)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (8 * q + e < here) {
+            const float v = acc[i][j][4 * q + e];
+            at[e * p.dim] = p.first_piece ? v : at[e * p.dim] + v;
+          }
+    }
+}
+
+// The piece's rows of dW.
+template <int DT, typename S>
+__global__ __launch_bounds__(64 * S::NW) void dw_kernel(const Loss p) {
+  using T = typename Ty<DT>::T;
+  __shared__ __attribute__((aligned(16))) char s0[(S::BM + S::BN) * slab::kSlab];
+  __shared__ __attribute__((aligned(16))) char s1[(S::BM + S::BN) * slab::kSlab];
+  const int32_t count = *p.count;
+  const uint32_t mt = static_cast<uint32_t>((p.piece_n + S::BM - 1) / S::BM), nt = static_cast<uint32_t>((p.dim + S::BN - 1) / S::BN);
+  uint32_t m, n;
+  slab::tile_of(blockIdx.x, mt, nt, m, n);
+  const int64_t v0 = static_cast<int64_t>(m) * S::BM, c0 = static_cast<int64_t>(n) * S::BN;
+  f32x16 acc[S::TM][S::TN];
+  slab::clear<S>(acc);
+  Matrix dl, x;
+  dl.base = p.piece;
+  dl.ld = p.piece_ld;
+  dl.rows = p.piece_ld / static_cast<int64_t>(sizeof(T));
+  dl.zeros = p.zeros;
+  x.base = p.xc;
+  x.ld = p.ld;
+  x.rows = p.ld / static_cast<int64_t>(sizeof(T));
+  x.zeros = p.zeros;
+  slab::product<DT, kAcross, kAcross, S>(dl, x, v0, c0, 0, count, s0, s1, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float down = p.scalars[0];
+#pragma unroll
+  for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::TN; ++j) {
+      const int64_t c = c0 + wave % S::WN * 32 * S::TN + 32 * j + (lane & 31);
+      const int64_t vt = v0 + wave / S::WN * 32 * S::TM + 32 * i + 4 * (lane >> 5);
+      const int here = c < p.dim && vt < p.piece_n ? static_cast<int>(p.piece_n - vt) : 0;
+      T* at = static_cast<T*>(p.dweight) + (p.piece0 + vt) * p.dim + c;
+#pragma unroll
+      for (int q = 0; q < 4; ++q, at += 8 * p.dim)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (8 * q + e < here) at[e * p.dim] = Ty<DT>::from(acc[i][j][4 * q + e] * down);
+    }
+}
+
+// dx: the splits' sums in order, rounded; zeros in the rows that are ignored.
+template <int DT>
+__global__ __launch_bounds__(256) void finish_dx_kernel(const Loss p) {
+  const int64_t r = blockIdx.x;
+  const int32_t at = p.at[r];
+  const float down = p.scalars[0];
+  for (int64_t c = threadIdx.x; c < p.dim; c += 256) {
+    float sum = 0.0f;
+    if (at >= 0) {
+#pragma unroll 4
+      for (int64_t s = 0; s < p.splits; ++s) sum += p.dx_part[(s * p.rows + at) * p.dim + c];
+    }
+    st<DT>(p.dx, r * p.dim + c, sum * down);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------- host
+constexpr int64_t kMaxRows = int64_t{1} << 30, kMaxVocab = int64_t{1} << 30, kMaxDim = int64_t{1} << 20;
+constexpr int64_t kPieceBytes = int64_t{512} << 20;  // of dl kept at a time
+
+enum Size { kBig, kMid, kThin };
+// 256 x 256 tiles where they are enough for the card, else 128 x 128; 128 x 64 for few rows, where the vocabulary's
+// rows are the traffic.
+static Size size_of(int64_t m, int64_t n) {
+  if (ceil_div(m, 256) * ceil_div(n, 256) >= 192) return kBig;
+  return kMid;
+}
+static Size logits_size(int64_t vocab, int64_t rows) { return rows <= 64 ? kThin : size_of(vocab, rows); }
+static int64_t edge(Size s) { return s == kBig ? 256 : 128; }
+
+struct Plan {
+  int64_t ld, tiles, piece_n, pieces, splits, split_k;
+  bool copy_w;
+  Size logits;
+  int64_t at, row, count, scalars, weights, lse_at, target_at, xc, wc, zeros, stats, hit, row_loss, piece, dx_part, total;
+};
+
+static Plan plan_of(const mm_linear_cross_entropy_params* q, bool backward) {
+  Plan s{};
+  const int64_t es = dtype_size(q->dtype);
+  s.ld = round_up(q->dim * es, 16);
+  s.copy_w = s.ld != q->dim * es || q->weight_stride * es % 16 != 0 || !aligned(q->weight, 16);
+  s.logits = logits_size(q->vocab, q->rows);
+  s.tiles = ceil_div(q->vocab, edge(s.logits));
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t was = at;
+    at += round_up(bytes, 256);
+    return was;
+  };
+  s.at = take(q->rows * 4);
+  s.row = take(q->rows * 4);
+  s.count = take(4);
+  s.scalars = take(4);
+  s.zeros = take(16);
+  s.target_at = take(q->rows * 8);
+  s.xc = take(q->rows * s.ld);
+  if (s.copy_w) s.wc = take(q->vocab * s.ld);
+  if (!backward) {
+    s.stats = take(q->rows * s.tiles * 8);
+    s.hit = take(q->rows * 4);
+    s.row_loss = take(q->reduction ? q->rows * 4 : 0);
+  } else {
+    s.weights = take(q->rows * 4);
+    s.lse_at = take(q->rows * 4);
+    // pieces of equal sizes, whole tiles of 256
+    int64_t most = kPieceBytes / (q->rows * es) / 256 * 256;
+    if (most < 256) most = 256;
+    s.pieces = ceil_div(q->vocab, most);
+    s.piece_n = round_up(ceil_div(q->vocab, s.pieces), 256);
+    s.pieces = ceil_div(q->vocab, s.piece_n);
+    s.piece = take(q->rows * s.piece_n * es);
+    // dx has few tiles and a long sum: splits of it until there are 512 workgroups, of 512 tokens at least
+    const int64_t e = edge(size_of(q->rows, q->dim)), tiles = ceil_div(q->rows, e) * ceil_div(q->dim, e);
+    s.splits = tiles >= 256 ? 1 : ceil_div(512, tiles);
+    const int64_t limit = s.piece_n / 512 > 0 ? s.piece_n / 512 : 1;
+    if (s.splits > limit) s.splits = limit;
+    s.split_k = round_up(ceil_div(s.piece_n, s.splits), 64);
+    s.splits = ceil_div(s.piece_n, s.split_k);
+    s.dx_part = take(s.splits * q->rows * q->dim * 4);
+  }
+  s.total = at;
+  return s;
+}
+
+static int check(const mm_linear_cross_entropy_params* q) {
+  if (!q) return fail(MM_ERR_NULL_POINTER, "params is NULL");
+  if (!valid_dtype(q->dtype)) return fail(MM_ERR_DTYPE, "dtype %d", q->dtype);
+  if (q->targets_dtype != 0 && q->targets_dtype != 1) return fail(MM_ERR_DTYPE, "targets_dtype %d", q->targets_dtype);
+  if (q->reduction < 0 || q->reduction > 2) return fail(MM_ERR_SHAPE, "reduction %d", q->reduction);
+  if (q->rows < 0 || q->dim < 1 || q->vocab < 1 || q->rows > kMaxRows || q->dim > kMaxDim || q->vocab > kMaxVocab ||
+      q->rows * q->dim >= (int64_t{1} << 40) || q->vocab * q->dim >= (int64_t{1} << 40) ||
+      ceil_div(q->rows, 64) * ceil_div(q->vocab, 128) >= (int64_t{1} << 31))
+    return fail(MM_ERR_SHAPE, "%lld rows, dim %lld, vocab %lld: empty, negative or too large", (long long)q->rows, (long long)q->dim,
+                (long long)q->vocab);
+  if (q->rows > 0 && (!q->x || !q->weight || !q->targets)) return fail(MM_ERR_NULL_POINTER, "x, weight and targets are required");
+  if (q->x_stride < 0 || q->weight_stride < 0 || q->dloss_stride < 0) return fail(MM_ERR_LAYOUT, "negative stride");
+  return MM_OK;
+}
+static int check_workspace(const mm_linear_cross_entropy_params* q, const Plan& s) {
+  if (q->rows > 0 && (!q->workspace || !aligned(q->workspace, 256) || q->workspace_bytes < static_cast<size_t>(s.total)))
+    return fail(MM_ERR_WORKSPACE, "needs %lld bytes of 256-byte aligned workspace", (long long)s.total);
+  return MM_OK;
+}
+static Loss loss_of(const mm_linear_cross_entropy_params* q, const Plan& s, bool backward) {
+  char* const ws = static_cast<char*>(q->workspace);
+  Loss p{};
+  p.x = q->x;
+  p.weight = q->weight;
+  p.targets = q->targets;
+  p.rows = q->rows;
+  p.dim = q->dim;
+  p.vocab = q->vocab;
+  p.x_ld = q->x_stride;
+  p.w_ld = q->weight_stride;
+  p.ignore = q->ignore_index;
+  p.dloss_stride = q->reduction ? 0 : q->dloss_stride;
+  p.targets64 = q->targets_dtype;
+  p.dtype = q->dtype;
+  p.reduction = q->reduction;
+  p.loss = q->loss;
+  p.lse = q->lse;
+  p.dloss = q->dloss;
+  p.dx = q->dx;
+  p.dweight = q->dweight;
+  p.at = reinterpret_cast<int32_t*>(ws + s.at);
+  p.row = reinterpret_cast<int32_t*>(ws + s.row);
+  p.count = reinterpret_cast<int32_t*>(ws + s.count);
+  p.scalars = reinterpret_cast<float*>(ws + s.scalars);
+  p.target_at = reinterpret_cast<int64_t*>(ws + s.target_at);
+  p.zeros = ws + s.zeros;
+  p.xc = ws + s.xc;
+  p.wc = s.copy_w ? ws + s.wc : nullptr;
+  p.ld = s.ld;
+  p.tiles = s.tiles;
+  if (!backward) {
+    p.stats = reinterpret_cast<float*>(ws + s.stats);
+    p.hit = reinterpret_cast<float*>(ws + s.hit);
+    p.row_loss = q->reduction ? reinterpret_cast<float*>(ws + s.row_loss) : nullptr;
+  } else {
+    p.weights = reinterpret_cast<float*>(ws + s.weights);
+    p.lse_at = reinterpret_cast<float*>(ws + s.lse_at);
+    p.piece = ws + s.piece;
+    p.piece_ld = s.piece_n * dtype_size(q->dtype);
+    p.dx_part = reinterpret_cast<float*>(ws + s.dx_part);
+    p.splits = s.splits;
+    p.split_k = s.split_k;
+  }
+  return p;
+}
+
+template <int DT>
+static void launch_gather(const Loss& p, const Plan& s, bool backward, hipStream_t st) {
+  hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(kThreads), 0, st, p, backward);
+  const int64_t es = dtype_size(DT);
+  auto grid = [&](int64_t rows) {
+    const int64_t n = ceil_div(rows * (s.ld / 16), 256);
+    return dim3(static_cast<unsigned>(n < 4096 ? n : 4096));
+  };
+  const bool vec = s.ld == p.dim * es && p.x_ld * es % 16 == 0 && aligned(p.x, 16);
+  hipLaunchKernelGGL((lay_out_kernel<DT>), grid(p.rows), dim3(256), 0, st, p.x, p.x_ld, p.xc, s.ld, p.rows, p.dim, p.row, p.count, vec);
+  if (p.wc)
+    hipLaunchKernelGGL((lay_out_kernel<DT>), grid(p.vocab), dim3(256), 0, st, p.weight, p.w_ld, p.wc, s.ld, p.vocab, p.dim, nullptr,
+                       nullptr, false);
+}
+template <int DT, typename S, bool GRAD>
+static void launch_logits_t(const Loss& p, int64_t vocab, hipStream_t st) {
+  hipLaunchKernelGGL((logits_kernel<DT, S, GRAD>), dim3(static_cast<unsigned>(ceil_div(vocab, S::BM) * ceil_div(p.rows, S::BN))),
+                     dim3(64 * S::NW), 0, st, p);
+}
+template <int DT, bool GRAD>
+static void launch_logits(const Loss& p, Size size, int64_t vocab, hipStream_t st) {
+  switch (size) {
+    case kBig: launch_logits_t<DT, Big, GRAD>(p, vocab, st); break;
+    case kMid: launch_logits_t<DT, Mid, GRAD>(p, vocab, st); break;
+    default: launch_logits_t<DT, Thin, GRAD>(p, vocab, st); break;
+  }
+}
+template <int DT, typename S>
+static void launch_dx_t(const Loss& p, hipStream_t st) {
+  const int64_t tiles = ceil_div(p.rows, S::BM) * ceil_div(p.dim, S::BN);
+  hipLaunchKernelGGL((dx_kernel<DT, S>), dim3(static_cast<unsigned>(tiles * p.splits)), dim3(64 * S::NW), 0, st, p);
+}
+template <int DT, typename S>
+static void launch_dw_t(const Loss& p, hipStream_t st) {
+  const int64_t tiles = ceil_div(p.piece_n, S::BM) * ceil_div(p.dim, S::BN);
+  hipLaunchKernelGGL((dw_kernel<DT, S>), dim3(static_cast<unsigned>(tiles)), dim3(64 * S::NW), 0, st, p);
+}
+
+template <int DT>
+static void forward(const Loss& p, const Plan& s, hipStream_t st) {
+  launch_gather<DT>(p, s, false, st);
+  launch_logits<DT, false>(p, s.logits, p.vocab, st);
+  hipLaunchKernelGGL(merge_kernel, dim3(static_cast<unsigned>(ceil_div(p.rows, 4))), dim3(256), 0, st, p);
+  if (p.reduction) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(kThreads), 0, st, p);
+}
+template <int DT>
+static void backward(Loss p, const Plan& s, hipStream_t st) {
+  launch_gather<DT>(p, s, true, st);
+  for (int64_t k = 0; k < s.pieces; ++k) {
+    p.piece0 = k * s.piece_n;
+    p.piece_n = p.piece0 + s.piece_n < p.vocab ? s.piece_n : p.vocab - p.piece0;
+    p.first_piece = k == 0;
+    launch_logits<DT, true>(p, logits_size(s.piece_n, p.rows), s.piece_n, st);
+    if (p.dx) {
+      if (size_of(p.rows, p.dim) == kBig) launch_dx_t<DT, Big>(p, st); else launch_dx_t<DT, Mid>(p, st);
+    }
+    if (p.dweight) {
+      if (size_of(p.piece_n, p.dim) == kBig) launch_dw_t<DT, Big>(p, st); else launch_dw_t<DT, Mid>(p, st);
+    }
+  }
+  if (p.dx) hipLaunchKernelGGL((finish_dx_kernel<DT>), dim3(static_cast<unsigned>(p.rows)), dim3(256), 0, st, p);
+}
+
+}  // namespace xent
+}  // namespace mm
+
+extern "C" {
+
+size_t mm_linear_cross_entropy_workspace_size(const mm_linear_cross_entropy_params* p, int32_t backward) {
+  using namespace mm;
+  using namespace mm::xent;
+  if (check(p) != MM_OK || p->rows == 0) return 0;
+  return static_cast<size_t>(plan_of(p, backward != 0).total);
+}
+
+int mm_linear_cross_entropy_fwd(const mm_linear_cross_entropy_params* q, void* stream) {
+  using namespace mm;
+  using namespace mm::xent;
+  clear_error();
+  int e = check(q);
+  if (e != MM_OK || q->rows == 0) return e;
+  if (!q->loss) return fail(MM_ERR_NULL_POINTER, "loss is required");
+  const Plan s = plan_of(q, false);
+  if ((e = check_workspace(q, s)) != MM_OK) return e;
+  const Loss p = loss_of(q, s, false);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (q->dtype) {
+    case MM_F32: forward<MM_F32>(p, s, st); break;
+    case MM_F16: forward<MM_F16>(p, s, st); break;
+    default: forward<MM_BF16>(p, s, st); break;
+  }
+  return check_launch("linear_cross_entropy_fwd");
+}
+
+int mm_linear_cross_entropy_bwd(const mm_linear_cross_entropy_params* q, void* stream) {
+  using namespace mm;
+  using namespace mm::xent;
+  clear_error();
+  int e = check(q);
+  if (e != MM_OK || q->rows == 0) return e;
+  if (!q->lse || !q->dloss) return fail(MM_ERR_NULL_POINTER, "lse and dloss are required");
+  const Plan s = plan_of(q, true);
+  if ((e = check_workspace(q, s)) != MM_OK) return e;
+  if (!q->dx && !q->dweight) return MM_OK;
+  const Loss p = loss_of(q, s, true);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (q->dtype) {
+    case MM_F32: backward<MM_F32>(p, s, st); break;
+    case MM_F16: backward<MM_F16>(p, s, st); break;
+    default: backward<MM_BF16>(p, s, st); break;
+  }
+  return check_launch("linear_cross_entropy_bwd");
+}
+
+}  // extern "C"

@@ -15,6 +15,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from mamba_metal_amd.cross_entropy import linear_cross_entropy
+from mamba_metal_amd.embedding import embedding
 from mamba_metal_amd.mamba_block import NORM_PENDING, MambaBlock
 from mamba_metal_amd.linear import decode_head_argmax, decode_linear, decode_linear_ok
 from mamba_metal_amd.norm import add_rmsnorm
@@ -107,6 +109,19 @@ class MambaModel(nn.Module):
     def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
         """input_ids (B, L) -> logits (B, L, vocab_size)."""
         return self._head(self._run(input_ids, lambda m, h, resid, nrm, nxt: (m(h), None)))
+
+    @torch.no_grad()
+    def loss(self, input_ids: torch.Tensor, targets: torch.Tensor | None = None, *, ignore_index: int = -100,
+             reduction: str = "mean") -> torch.Tensor:
+        """Cross entropy of (B, L) ``targets`` under the model, of the next tokens if none are given (the last one of a
+        sequence then has none), in float32: what a text's perplexity is made of.  The logits are not kept
+        (``linear_cross_entropy``, whose ``ignore_index`` and ``reduction`` these are).  Without gradients: the scan
+        has none."""
+        if targets is None:
+            targets = F.pad(input_ids[:, 1:], (0, 1), value=ignore_index)
+        E = self.embeddings.weight
+        h = self._run(input_ids, lambda m, h, resid, nrm, nxt: (m(h), None), resid=embedding(input_ids, E))
+        return linear_cross_entropy(h, E, targets, ignore_index=ignore_index, reduction=reduction)
 
     def init_state(self, batch_size: int = 1):
         """Zero conv and SSM states (float32, as mamba_model.py:80-91)."""
