@@ -161,13 +161,15 @@ static int check_strides(const int64_t* s, const char* name) {
     if (s[i] < 0) return fail(MM_ERR_LAYOUT, "%s has a negative stride", name);
   return MM_OK;
 }
-// 16 bytes at a time: aligned rows of a width that 16 bytes divide.
-static bool vec_ok(const void* p, const int64_t* s, int n, int64_t width, int32_t dtype) {
+// 16 bytes at a time: aligned rows of a width that 16 bytes divide, a run of them within 32-bit offsets.
+static bool vec_ok(const void* p, const int64_t* s, int64_t width, int32_t dtype) {
   const int64_t e = 16 / dtype_size(dtype);
-  bool ok = aligned(p, 16) && width % e == 0;
-  for (int i = 0; i < n; ++i) ok = ok && s[i] % e == 0;
+  bool ok = aligned(p, 16) && width % e == 0 && s[1] < (int64_t{1} << 23);
+  for (int i = 0; i < 3; ++i) ok = ok && s[i] % e == 0;
   return ok;
 }
+// The pass's output, 4 channels at a time.
+static bool out_ok(const void* p, int64_t width) { return aligned(p, 16) && width % 4 == 0; }
 
 static int check_common(const mm_decay_attention_params* p) {
   if (!p) return fail(MM_ERR_NULL_POINTER, "params is NULL");
@@ -267,8 +269,9 @@ int mm_decay_attention_fwd(const mm_decay_attention_params* p, void* stream) {
   set(k.q, k.q_stride, p->q, p->q_stride);
   set(k.k, k.k_stride, p->k, p->k_stride);
   set(k.v, k.v_stride, p->v, p->v_stride);
-  k.vec = vec_ok(k.q, k.q_stride, 3, k.dk, k.dtype) | vec_ok(k.k, k.k_stride, 3, k.dk, k.dtype) << 1 |
-          vec_ok(k.v, k.v_stride, 3, k.dv, k.dtype) << 2;
+  k.vec = vec_ok(k.q, k.q_stride, k.dk, k.dtype) | vec_ok(k.k, k.k_stride, k.dk, k.dtype) << 1 |
+          vec_ok(k.v, k.v_stride, k.dv, k.dtype) << 2;
+  k.vec |= out_ok(p->y, k.dv) << 4;
   k.init = p->h0;
   k.final_state = p->state_out;
   k.y = p->y;
@@ -302,8 +305,9 @@ int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream) {
   set(k.q, k.q_stride, p->k, p->k_stride);
   set(k.k, k.k_stride, p->q, p->q_stride);
   set(k.v, k.v_stride, p->dy, p->dy_stride);
-  k.vec = vec_ok(k.q, k.q_stride, 3, k.dk, k.dtype) | vec_ok(k.k, k.k_stride, 3, k.dk, k.dtype) << 1 |
-          vec_ok(k.v, k.v_stride, 3, k.dv, k.dtype) << 2;
+  k.vec = vec_ok(k.q, k.q_stride, k.dk, k.dtype) | vec_ok(k.k, k.k_stride, k.dk, k.dtype) << 1 |
+          vec_ok(k.v, k.v_stride, k.dv, k.dtype) << 2;
+  k.vec |= out_ok(p->dv, k.dv) << 4;
   k.init = p->dstate;
   k.final_state = p->dh0;
   k.y = p->dv;
@@ -347,8 +351,8 @@ int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream) {
     d.vblocks = s.vblocks;
     d.sets = s.sets;
     d.set_heads = s.set_heads;
-    d.vec = vec_ok(d.q, d.q_stride, 3, d.dk, p->dtype) | vec_ok(d.k, d.k_stride, 3, d.dk, p->dtype) << 1 |
-            vec_ok(d.v, d.v_stride, 3, d.dv, p->dtype) << 2 | vec_ok(d.dy, d.dy_stride, 3, d.dv, p->dtype) << 3;
+    d.vec = vec_ok(d.q, d.q_stride, d.dk, p->dtype) | vec_ok(d.k, d.k_stride, d.dk, p->dtype) << 1 |
+            vec_ok(d.v, d.v_stride, d.dv, p->dtype) << 2 | vec_ok(d.dy, d.dy_stride, d.dv, p->dtype) << 3;
     d.dtype = p->dtype;
     d.g_dtype = p->log_decay_dtype;
     d.lengths_dtype = p->lengths_dtype;

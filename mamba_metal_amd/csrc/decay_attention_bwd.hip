@@ -17,46 +17,15 @@
 namespace mm {
 namespace dattn {
 
-// As Staged, for 512 threads.
-template <int DT, int W>
-struct Staged512 {
-  using T = typename Ty<DT>::T;
-  static constexpr int kE = Op<DT>::kE, kUnits = W / kE, kSteps = kRun * kUnits / 512 > 0 ? kRun * kUnits / 512 : 1;
-  u32x4 v[kSteps];
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int width, bool vec) {
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int u = s * 512 + static_cast<int>(threadIdx.x), r = u / kUnits, e = u % kUnits * kE;
-      v[s] = u32x4{0, 0, 0, 0};
-      if (r < rows && e < width) {
-        const T* const p = base + r * stride + e;
-        if (vec) {
-          v[s] = *reinterpret_cast<const u32x4*>(p);
-        } else {
-          T t[kE];
-#pragma unroll
-          for (int j = 0; j < kE; ++j) t[j] = e + j < width ? p[j] : static_cast<T>(0);
-          __builtin_memcpy(&v[s], t, 16);
-        }
-      }
-    }
-  }
-  __device__ __forceinline__ void store(T* tile) const {
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int u = s * 512 + static_cast<int>(threadIdx.x), r = u / kUnits, e = u % kUnits * kE;
-      *reinterpret_cast<u32x4*>(tile + r * (W + Op<DT>::kPad) + e) = v[s];
-    }
-  }
-};
-
 template <int DT, int DKP>
 __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
   using T = typename Ty<DT>::T;
   using O = Op<DT>;
-  constexpr int LDK = DKP + O::kPad, LDV = kVBlock + O::kPad, ND = DKP / 16, NU = kVBlock / O::kStep;
-  __shared__ __attribute__((aligned(16))) T s_qk[2][kRun * LDK];  // q, k
-  __shared__ __attribute__((aligned(16))) T s_dv[2][kRun * LDV];  // dy, v
+  using TK = Tile<DT, DKP>;
+  using TV = Tile<DT, kVBlock>;
+  constexpr int ND = DKP / 16, NU = kVBlock / O::kStep;
+  __shared__ __attribute__((aligned(16))) T s_qk[2][kRun * TK::kLd];  // q, k
+  __shared__ __attribute__((aligned(16))) T s_dv[2][kRun * TV::kLd];  // dy, v
   __shared__ Decays s_d;
   __shared__ float s_sum[2][kRun], s_inter[2][kRun];  // M's row and column sums; the states' parts
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
@@ -78,7 +47,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
   for (int t = 0; t < ND; ++t) out[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (rows > 0) {
     {
-      Staged512<DT, DKP> r;
+      Staged<DT, DKP, 512> r;
       r.load(static_cast<const T*>(p.q) + b * p.q_stride[0] + t0 * p.q_stride[1] + group * p.q_stride[2], p.q_stride[1],
              rows, dk, p.vec & 1);
       r.store(s_qk[0]);
@@ -96,11 +65,11 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       A[ot] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int u = 0; u < DKP / O::kStep; ++u)
-        A[ot] = mma<DT>(row_operand<DT>(s_other, LDK, 16 * ot, u * O::kStep, lane),
-                        row_operand<DT>(s_own, LDK, 16 * blk, u * O::kStep, lane), A[ot]);
+        A[ot] = mma<DT>(TK::row(s_other, 16 * ot, u * O::kStep, lane),
+                        TK::row(s_own, 16 * blk, u * O::kStep, lane), A[ot]);
     }
 
-    Staged512<DT, kVBlock> ry, rv;
+    Staged<DT, kVBlock, 512> ry, rv;
     float rg = 0.0f;
     auto fetch = [&](int h, int vb) __attribute__((always_inline)) {
       const int64_t head = group * p.per + h;
@@ -133,7 +102,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         const T* const other_t = s_dv[1 - role];
         u32x4 own[NU];
 #pragma unroll
-        for (int u = 0; u < NU; ++u) own[u] = row_operand_acc<DT>(own_t, LDV, 16 * blk, u * O::kStep, lane);
+        for (int u = 0; u < NU; ++u) own[u] = TV::row_acc(own_t, 16 * blk, u * O::kStep, lane);
         if constexpr (DT == MM_F16) {
           const float f = (role ? p.dfactors : p.factors)[(bh * p.runs + run) * p.vblocks + vb];
 #pragma unroll
@@ -150,7 +119,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         for (int ot = 0; ot < 4; ++ot) {
           if (role ? ot < blk : ot > blk) continue;
 #pragma unroll
-          for (int u = 0; u < NU; ++u) acc[ot] = mma<DT>(row_operand_acc<DT>(other_t, LDV, 16 * ot, u * O::kStep, lane), own[u], acc[ot]);
+          for (int u = 0; u < NU; ++u) acc[ot] = mma<DT>(TV::row_acc(other_t, 16 * ot, u * O::kStep, lane), own[u], acc[ot]);
         }
       }
       // dP and M
@@ -183,14 +152,14 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         out[t] += tmp[t];
         if (p.dg) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) inter[r] += tmp[t][r] * Ty<DT>::f(s_own[(16 * blk + 4 * g + r) * LDK + 16 * t + i]);
+          for (int r = 0; r < 4; ++r) inter[r] += tmp[t][r] * Ty<DT>::f(s_own[TK::at(16 * blk + 4 * g + r, 16 * t + i)]);
         }
       }
 #pragma unroll
       for (int u = 0; u < kRun / O::kStep; ++u) {
         if (role ? (u + 1) * O::kStep <= 16 * blk : u * O::kStep > 16 * blk + 15) continue;
 #pragma unroll
-        for (int t = 0; t < ND; ++t) out[t] = mma<DT>(dp[u], column_operand<DT>(s_other, LDK, u * O::kStep, 16 * t, lane), out[t]);
+        for (int t = 0; t < ND; ++t) out[t] = mma<DT>(dp[u], TK::column(s_other, u * O::kStep, 16 * t, lane), out[t]);
       }
       if (p.dg) {
         sum += lane_xor(sum, 16);

@@ -52,29 +52,32 @@ __device__ __forceinline__ void split_operand(const float (&x)[8], u32x4 (&out)[
 }
 
 template <int DT, int DKP, bool REV, bool OUT>
-__global__ __launch_bounds__(256) void pass_kernel(const Pass p) {
+__global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) void pass_kernel(const Pass p) {
   using T = typename Ty<DT>::T;
   using O = Op<DT>;
-  constexpr int LDK = DKP + O::kPad, LDV = kVBlock + O::kPad, LDP = kRun + O::kPad;
+  using TK = Tile<DT, DKP>;
+  using TV = Tile<DT, kVBlock>;  // (values and scores: both 64 wide)
+  static_assert(kVBlock == kRun, "one tile type for both");
   constexpr int ND = DKP / 16;  // state tiles of a wave
+  constexpr int NU = DKP / O::kStep, NR = kRun / O::kStep;
   constexpr int TERMS = DT == MM_F32 ? 1 : DT == MM_F16 ? 2 : 3;
-  __shared__ __attribute__((aligned(16))) T s_q[OUT ? kRun * LDK : 8];  // what asks: q, or k mirrored
-  __shared__ __attribute__((aligned(16))) T s_k[kRun * LDK];            // what adds to the state: k, or q
-  __shared__ __attribute__((aligned(16))) T s_v[kRun * LDV];            // its values: v, or dy
-  __shared__ __attribute__((aligned(16))) T s_p[OUT ? kRun * LDP : 8];
-  __shared__ __attribute__((aligned(16))) T s_s[OUT ? 4 * 16 * LDK : 8];  // a wave's state columns, to turn them over
-  __shared__ Decays s_d;
-  __shared__ float s_max[4];
-  __shared__ double s_x[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  constexpr int kDecayWave = REV ? 3 : 0;                             // the one with the fewest scores
+  __shared__ __attribute__((aligned(16))) T s_q[OUT ? kRun * TK::kLd : 8];  // what asks: q, or k mirrored
+  __shared__ __attribute__((aligned(16))) T s_k[kRun * TK::kLd];            // what adds to the state: k, or q
+  __shared__ __attribute__((aligned(16))) T s_v[kRun * TV::kLd];            // its values: v, or dy
+  __shared__ __attribute__((aligned(16))) T s_p[OUT ? kRun * TV::kLd : 8];  // scores; 16 rows a wave, first for its own use
+  __shared__ Decays s_d[2];
+  __shared__ float s_max[4], s_x[4];
+  int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
 
   uint32_t id = blockIdx.x;
   const int vb = static_cast<int>(id % p.vblocks);
   id /= p.vblocks;
   const int seg = static_cast<int>(id % p.segments);
   id /= p.segments;
-  const int64_t head = id % p.heads, b = id / p.heads;
-  const int64_t group = head / p.per;
+  const int64_t head = id % static_cast<uint32_t>(p.heads), b = id / static_cast<uint32_t>(p.heads);
+  const int64_t group = static_cast<uint32_t>(head) / static_cast<uint32_t>(p.per);
   const int64_t bh = b * p.heads + head;
   const int64_t len = length_of(p, b);
   const int64_t run0 = static_cast<int64_t>(seg) * p.seg_runs;
@@ -107,46 +110,73 @@ __global__ __launch_bounds__(256) void pass_kernel(const Pass p) {
       }
   }
 
-  Staged<DT, DKP> rq, rk;
-  Staged<DT, kVBlock> rv;
-  float rg = 0.0f;
+  Staged<DT, DKP, 256> rq, rk;
+  Staged<DT, kVBlock, 256> rv;
+  auto rows_of = [&](int64_t run) { return static_cast<int>(len - run * kRun < kRun ? len - run * kRun : kRun); };
   auto fetch = [&](int64_t run) __attribute__((always_inline)) {
     const int64_t t0 = run * kRun;
-    const int rows = static_cast<int>(len - t0 < kRun ? len - t0 : kRun);
+    const int rows = rows_of(run);
     if (OUT) rq.load(qh + t0 * p.q_stride[1], p.q_stride[1], rows, dk, p.vec & 1);
     rk.load(kh + t0 * p.k_stride[1], p.k_stride[1], rows, dk, p.vec & 2);
     rv.load(vh + t0 * p.v_stride[1], p.v_stride[1], rows, vw, p.vec & 4);
-    rg = lane < rows ? load_gate(p, gh + (t0 + lane) * p.g_stride[1]) : 0.0f;
+  };
+  auto gate = [&](int64_t run) {
+    return lane < rows_of(run) ? load_gate(p, gh + (run * kRun + lane) * p.g_stride[1]) : 0.0f;
+  };
+  // fp16: the largest magnitude of the wave's columns
+  auto note_max = [&]() __attribute__((always_inline)) {
+    float m = 0.0f;
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(S[t][r]));
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) m = fmaxf(m, lane_xor(m, x));
+    if (lane == 0) s_max[wave] = m;
   };
   const int64_t live_runs = (len + kRun - 1) / kRun;
   const int64_t walk_end = run_end < live_runs ? run_end : live_runs;  // runs with tokens: [run0, walk_end)
-  double total = 0.0;  // the segment's log decay
-  float factor = 1.0f; // fp16: the state's power of two
-  if (walk_end > run0) {
-    if (DT == MM_F16 && OUT) {
-      float m = 0.0f;
-#pragma unroll
-      for (int t = 0; t < ND; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(S[t][r]));
-#pragma unroll
-      for (int x = 1; x < 64; x *= 2) m = fmaxf(m, lane_xor(m, x));
-      if (lane == 0) s_max[wave] = m;
-    }
-    fetch(REV ? walk_end - 1 : run0);
+  const int64_t walk = walk_end - run0;
+  double total = 0.0;   // the segment's log decay
+  float factor = 1.0f;  // fp16: the state's power of two
+  if (walk > 0) {
+    const int64_t run = REV ? walk_end - 1 : run0;
+    fetch(run);
+    if (DT == MM_F16 && OUT) note_max();
+    if (wave == kDecayWave) run_decays(s_d[0], gate(run), lane);
   }
-  for (int64_t n = 0; n < walk_end - run0; ++n) {
+  for (int64_t n = 0; n < walk; ++n) {
+    // addresses in shared memory are made anew in every run: held over it they would be dozens of registers
+    asm volatile("" : "+v"(lane));
     const int64_t run = REV ? walk_end - 1 - n : run0 + n;
+    const int64_t next = n + 1 < walk ? (REV ? run - 1 : run + 1) : run;
     if (OUT) rq.store(s_q);
     rk.store(s_k);
     rv.store(s_v);
-    if (wave == (REV ? 3 : 0)) run_decays(s_d, rg, lane);
     __syncthreads();
-    if (n + 1 < walk_end - run0) fetch(REV ? run - 1 : run + 1);
-
-    u32x4 vo[kRun / O::kStep];  // this wave's value columns, as operands over the run's tokens
+    const Decays& D = s_d[n & 1];
+    // what the state's product with the saved ones of the forward pass needs, before the next run's loads
+    constexpr int kSaved = OUT && REV ? ND : 1;
+    u32x2 saved2[kSaved];
+    f32x4 saved4[kSaved];
+    const bool dot_wanted = OUT && REV && p.dot;
+    if constexpr (OUT && REV) {
+      if (dot_wanted) {
+        const T* const before = run_state<T>(const_cast<void*>(p.dot_with), p, bh, run, vb, DKP);
 #pragma unroll
-    for (int u = 0; u < kRun / O::kStep; ++u) vo[u] = column_operand<DT>(s_v, LDV, u * O::kStep, 16 * wave, lane);
+        for (int t = 0; t < ND; ++t) {
+          if constexpr (O::kWide) saved4[t] = *reinterpret_cast<const f32x4*>(before + state_at<DT>(wave, t, ND, lane));
+          else saved2[t] = *reinterpret_cast<const u32x2*>(before + state_at<DT>(wave, t, ND, lane));
+        }
+      }
+    }
+    float g_next = 0.0f;
+    if (wave == kDecayWave) g_next = gate(next);
+    if (n + 1 < walk) fetch(next);
+
+    u32x4 vo[NR];  // this wave's value columns, as operands over the run's tokens
+#pragma unroll
+    for (int u = 0; u < NR; ++u) vo[u] = TV::column(s_v, u * O::kStep, 16 * wave, lane);
 
     if constexpr (OUT) {
       if constexpr (DT == MM_F16) {
@@ -157,161 +187,175 @@ __global__ __launch_bounds__(256) void pass_kernel(const Pass p) {
       }
       const float shrink = DT == MM_F16 ? 1.0f / factor : 1.0f;
       // the state as an operand (rounded to 16 bits: products of 16-bit operands, off by half a step each at random)
-      u32x4 so[DKP / O::kStep];
+      u32x4 so[NU];
 #pragma unroll
-      for (int u = 0; u < DKP / O::kStep; ++u) {
+      for (int u = 0; u < NU; ++u) {
         f32x4 part[O::kTiles];
 #pragma unroll
-        for (int n2 = 0; n2 < O::kTiles; ++n2) part[n2] = S[u * O::kTiles + n2] * shrink;
+        for (int c = 0; c < O::kTiles; ++c) part[c] = DT == MM_F16 ? S[u * O::kTiles + c] * shrink : S[u * O::kTiles + c];
         so[u] = from_acc<DT>(part);
       }
       if (p.states) {
-        // for the backward pass: 16 columns turned over, so that its operands over them are whole reads
-        T* const mine = s_s + wave * 16 * LDK;
-#pragma unroll
-        for (int u = 0; u < DKP / O::kStep; ++u) {
-          if constexpr (O::kWide) {
-            *reinterpret_cast<u32x4*>(mine + i * LDK + 16 * u + 4 * g) = so[u];
-          } else {
-            *reinterpret_cast<u32x2*>(mine + i * LDK + 32 * u + 4 * g) = u32x2{so[u][0], so[u][1]};
-            *reinterpret_cast<u32x2*>(mine + i * LDK + 32 * u + 16 + 4 * g) = u32x2{so[u][2], so[u][3]};
-          }
-        }
+        // for the backward pass: the 16 columns turned over, 64 key channels at a time, so that its operands over value
+        // channels are whole reads
         T* const out = run_state<T>(p.states, p, bh, run, vb, DKP);
-        const T* const before = p.dot ? run_state<T>(const_cast<void*>(p.dot_with), p, bh, run, vb, DKP) : nullptr;
         float dot = 0.0f;
-        wave_lds_fence();
+        auto turn_over = [&](const u32x4(&x)[NU], bool keep) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < ND; ++t) {
-          const int64_t at = state_at<DT>(wave, t, ND, lane);
-          if constexpr (O::kWide) {
-            f32x4 v;
+          for (int h = 0; h < DKP / 64; ++h) {
+            wave_lds_fence();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = mine[(4 * g + j) * LDK + 16 * t + i];
-            *reinterpret_cast<f32x4*>(out + at) = v;
-            if (REV && before) {
-              const f32x4 w = *reinterpret_cast<const f32x4*>(before + at);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) dot += v[j] * w[j];
+            for (int c = 0; c < 64 / O::kStep; ++c) {
+              const u32x4 w = x[h * (64 / O::kStep) + c];
+              if constexpr (O::kWide) {
+                *reinterpret_cast<u32x4*>(s_p + TV::at(16 * wave + i, 16 * c + 4 * g)) = w;
+              } else {
+                *reinterpret_cast<u32x2*>(s_p + TV::at(16 * wave + i, 32 * c + 4 * g)) = u32x2{w[0], w[1]};
+                *reinterpret_cast<u32x2*>(s_p + TV::at(16 * wave + i, 32 * c + 16 + 4 * g)) = u32x2{w[2], w[3]};
+              }
             }
-          } else {
-            const u32x2 v = column4<DT>(mine, LDK, 0, 16 * t, lane);
-            *reinterpret_cast<u32x2*>(out + at) = v;
-            if (REV && before) {
-              const u32x2 w = *reinterpret_cast<const u32x2*>(before + at);
+            wave_lds_fence();
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float a, b2, x, y;
-                unpack2<DT>(v[j], a, b2);
-                unpack2<DT>(w[j], x, y);
-                dot += a * x + b2 * y;
+            for (int c = 0; c < 4; ++c) {
+              const int t = 4 * h + c;
+              const int64_t at = state_at<DT>(wave, t, ND, lane);
+              if constexpr (O::kWide) {
+                const f32x4 v = __builtin_bit_cast(f32x4, TV::column(s_p, 16 * wave, 16 * c, lane));
+                if (keep) *reinterpret_cast<f32x4*>(out + at) = v;
+                if (REV && dot_wanted) {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) dot += v[j] * saved4[REV ? t : 0][j];
+                }
+              } else {
+                const u32x2 v = TV::column4(s_p, 16 * wave, 16 * c, lane);
+                if (keep) *reinterpret_cast<u32x2*>(out + at) = v;
+                if (REV && dot_wanted) {
+#pragma unroll
+                  for (int j = 0; j < 2; ++j) {
+                    float a, b2, x2, y2;
+                    unpack2<DT>(v[j], a, b2);
+                    unpack2<DT>(saved2[REV ? t : 0][j], x2, y2);
+                    dot += a * x2 + b2 * y2;
+                  }
+                }
               }
             }
           }
-        }
-        if (REV && before) {
-          if constexpr (!O::kWide) {
+        };
+        turn_over(so, true);
+        if (dot_wanted) {
+          if constexpr (REV && !O::kWide) {
             // what rounding the gradient's state left out, so that the sum has one rounded factor and not two
-            wave_lds_fence();
+            u32x4 rest[NU];
 #pragma unroll
-            for (int u = 0; u < DKP / O::kStep; ++u) {
+            for (int u = 0; u < NU; ++u) {
               f32x4 part[2];
 #pragma unroll
-              for (int n2 = 0; n2 < 2; ++n2)
+              for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                   float a, b2;
-                  unpack2<DT>(so[u][2 * n2 + r], a, b2);
-                  part[n2][2 * r] = S[2 * u + n2][2 * r] * shrink - a;
-                  part[n2][2 * r + 1] = S[2 * u + n2][2 * r + 1] * shrink - b2;
+                  unpack2<DT>(so[u][2 * c + r], a, b2);
+                  part[c][2 * r] = S[2 * u + c][2 * r] * shrink - a;
+                  part[c][2 * r + 1] = S[2 * u + c][2 * r + 1] * shrink - b2;
                 }
-              const u32x4 rest = from_acc<DT>(part);
-              *reinterpret_cast<u32x2*>(mine + i * LDK + 32 * u + 4 * g) = u32x2{rest[0], rest[1]};
-              *reinterpret_cast<u32x2*>(mine + i * LDK + 32 * u + 16 + 4 * g) = u32x2{rest[2], rest[3]};
+              rest[u] = from_acc<DT>(part);
             }
-            wave_lds_fence();
-#pragma unroll
-            for (int t = 0; t < ND; ++t) {
-              const u32x2 v = column4<DT>(mine, LDK, 0, 16 * t, lane);
-              const u32x2 w = *reinterpret_cast<const u32x2*>(before + state_at<DT>(wave, t, ND, lane));
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float a, b2, x, y;
-                unpack2<DT>(v[j], a, b2);
-                unpack2<DT>(w[j], x, y);
-                dot += a * x + b2 * y;
-              }
-            }
+            turn_over(rest, false);
           }
 #pragma unroll
           for (int x = 1; x < 64; x *= 2) dot += lane_xor(dot, x);
           if (lane == 0) s_x[wave] = dot;
         }
         if (DT == MM_F16 && threadIdx.x == 0) p.factors[(bh * p.runs + run) * p.vblocks + vb] = factor;
+        wave_lds_fence();
       }
       // scores of row block `wave`: tiles of (what adds) x (what asks), whose accumulators are rows of p
-      const float hi_r = s_d.hi[16 * wave + i], lo_r = s_d.lo[16 * wave + i];
+      {
+        f32x4 acc[4];
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        if (REV ? st < wave : st > wave) continue;
-        f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int st = 0; st < 4; ++st) acc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int u = 0; u < DKP / O::kStep; ++u)
-          acc = mma<DT>(row_operand<DT>(s_k, LDK, 16 * st, u * O::kStep, lane),
-                        row_operand<DT>(s_q, LDK, 16 * wave, u * O::kStep, lane), acc);
-        const f32x4 hi = *reinterpret_cast<const f32x4*>(s_d.hi + 16 * st + 4 * g);
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(s_d.lo + 16 * st + 4 * g);
-        float v[4];
+        for (int u = 0; u < NU; ++u) {
+          const u32x4 own = TK::row(s_q, 16 * wave, u * O::kStep, lane);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int other = 16 * st + 4 * g + r, row = 16 * wave + i;
-          const bool in = REV ? other >= row : other <= row;
-          const float decay = REV ? between<DT>(hi[r], lo[r], hi_r, lo_r) : between<DT>(hi_r, lo_r, hi[r], lo[r]);
-          v[r] = in ? acc[r] * p.scale * decay : 0.0f;
+          for (int st = 0; st < 4; ++st)
+            if (REV ? st >= wave : st <= wave) acc[st] = mma<DT>(TK::row(s_k, 16 * st, u * O::kStep, lane), own, acc[st]);
         }
-        T* const at = s_p + (16 * wave + i) * LDP + 16 * st + 4 * g;
-        if constexpr (O::kWide) *reinterpret_cast<f32x4*>(at) = f32x4{v[0], v[1], v[2], v[3]};
-        else *reinterpret_cast<u32x2*>(at) = u32x2{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+        const float hi_r = D.hi[16 * wave + i], lo_r = D.lo[16 * wave + i];
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          T* const at = s_p + TV::at(16 * wave + i, 16 * st + 4 * g);
+          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (REV ? st >= wave : st <= wave) {
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(D.hi + 16 * st + 4 * g);
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(D.lo + 16 * st + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float decay = REV ? between<DT>(hi[r], lo[r], hi_r, lo_r) : between<DT>(hi_r, lo_r, hi[r], lo[r]);
+              const float x = acc[st][r] * p.scale * decay;
+              v[r] = st != wave || (REV ? 4 * g + r >= i : 4 * g + r <= i) ? x : 0.0f;
+            }
+          }
+          // (tiles beyond the diagonal: zeros, for the steps of a product that take two tiles at once)
+          if constexpr (O::kWide) *reinterpret_cast<f32x4*>(at) = f32x4{v[0], v[1], v[2], v[3]};
+          else *reinterpret_cast<u32x2*>(at) = u32x2{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+        }
       }
-      // the tiles beside the diagonal that an operand's step takes in with it
-      if constexpr (!O::kWide) {
-        if (REV ? (wave & 1) : !(wave & 1))
-          *reinterpret_cast<u32x2*>(s_p + (16 * wave + i) * LDP + 16 * (REV ? wave - 1 : wave + 1) + 4 * g) = u32x2{0, 0};
-      }
+      if (wave == kDecayWave) run_decays(s_d[(n + 1) & 1], g_next, lane);
       __syncthreads();
-      if (REV && p.dot && threadIdx.x == 0)
-        p.dot[(bh * p.runs + run) * p.vblocks + vb] =
-            (s_x[0] + s_x[1] + s_x[2] + s_x[3]) * s_d.whole * factor *
-            (DT == MM_F16 ? p.factors_with[(bh * p.runs + run) * p.vblocks + vb] : 1.0f);
-      // outputs: row block by row block, this wave's 16 columns
+      if (REV && dot_wanted && threadIdx.x == 0)
+        p.dot[(bh * p.runs + run) * p.vblocks + vb] = (s_x[0] + s_x[1] + s_x[2] + s_x[3]) * D.whole * factor *
+                                                      (DT == MM_F16 ? p.factors_with[(bh * p.runs + run) * p.vblocks + vb] : 1.0f);
+      // outputs, turned over: 4 value channels of a token in a lane
+      f32x4 acc[4];
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) acc[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int rt = 0; rt < 4; ++rt) acc[rt] = mma<DT>(so[u], TK::row_acc(s_q, 16 * rt, u * O::kStep, lane), acc[rt]);
       const float qs = (REV ? 1.0f : p.scale) * factor;
 #pragma unroll
-      for (int rt = 0; rt < 4; ++rt) {
-        f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int rt = 0; rt < 4; ++rt) acc[rt] *= (REV ? D.onward : D.into)[16 * rt + i] * qs;
 #pragma unroll
-        for (int u = 0; u < DKP / O::kStep; ++u)
-          acc = mma<DT>(row_operand_acc<DT>(s_q, LDK, 16 * rt, u * O::kStep, lane), so[u], acc);
-        acc *= *reinterpret_cast<const f32x4*>((REV ? s_d.onward : s_d.into) + 16 * rt + 4 * g) * qs;
+      for (int u = 0; u < NR; ++u)
 #pragma unroll
-        for (int u = 0; u < kRun / O::kStep; ++u) {
+        for (int rt = 0; rt < 4; ++rt) {
           if (REV ? (u + 1) * O::kStep <= 16 * rt : u * O::kStep > 16 * rt + 15) continue;
-          acc = mma<DT>(row_operand_acc<DT>(s_p, LDP, 16 * rt, u * O::kStep, lane), vo[u], acc);
+          acc[rt] = mma<DT>(vo[u], TV::row_acc(s_p, 16 * rt, u * O::kStep, lane), acc[rt]);
         }
-        const int64_t t0 = run * kRun + 16 * rt + 4 * g;
-        T* const y = static_cast<T*>(p.y) + ((b * p.seqlen + t0) * p.heads + head) * p.dv + vcol;
+      const int rows = rows_of(run), left = static_cast<int>(p.seqlen - run * kRun < kRun ? p.seqlen - run * kRun : kRun);
+      const int v0 = 16 * wave + 4 * g;
+      T* const yr = static_cast<T*>(p.y) + ((b * p.seqlen + run * kRun) * p.heads + head) * p.dv + vb * kVBlock;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (t0 + r < p.seqlen && vcol < p.dv) y[r * p.heads * p.dv] = Ty<DT>::from(t0 + r < len ? acc[r] : 0.0f);
+      for (int rt = 0; rt < 4; ++rt) {
+        const int t = 16 * rt + i;
+        if (t >= rows) acc[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (t >= left) continue;
+        T* const y = yr + t * p.heads * p.dv + v0;
+        if (p.vec & 16) {
+          if (v0 < vw) {
+            if constexpr (O::kWide) *reinterpret_cast<f32x4*>(y) = acc[rt];
+            else *reinterpret_cast<u32x2*>(y) = u32x2{pack2<DT>(acc[rt][0], acc[rt][1]), pack2<DT>(acc[rt][2], acc[rt][3])};
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (v0 + r < vw) y[r] = Ty<DT>::from(acc[rt][r]);
+        }
       }
+    } else if (wave == kDecayWave) {
+      run_decays(s_d[(n + 1) & 1], g_next, lane);
     }
     // the state's step
-    const float whole = s_d.whole;
+    const float whole = D.whole;
 #pragma unroll
     for (int t = 0; t < ND; ++t) S[t] *= whole;
-    const float* const weight = REV ? s_d.into : s_d.onward;
+    const float* const weight = REV ? D.into : D.onward;
     const float ws = REV ? p.scale : 1.0f;
 #pragma unroll
-    for (int u = 0; u < kRun / O::kStep; ++u) {
+    for (int u = 0; u < NR; ++u) {
       u32x4 terms[TERMS];
       if constexpr (O::kWide) {
         const f32x4 w = *reinterpret_cast<const f32x4*>(weight + 16 * u + 4 * g) * ws;
@@ -329,29 +373,27 @@ __global__ __launch_bounds__(256) void pass_kernel(const Pass p) {
         }
         split_operand<DT, TERMS>(x, terms);
       }
+      // four state tiles at a time: products that follow each other are independent
 #pragma unroll
-      for (int t = 0; t < ND; ++t) {
-        const u32x4 ko = column_operand<DT>(s_k, LDK, u * O::kStep, 16 * t, lane);
+      for (int t0 = 0; t0 < ND; t0 += 4) {
+        u32x4 ko[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) ko[t] = TK::column(s_k, u * O::kStep, 16 * (t0 + t), lane);
         if constexpr (DT == MM_F16) {
-          S[t] = mma<DT>(ko, terms[0], S[t]);
-          S[t] += mma<DT>(ko, terms[1], f32x4{0.0f, 0.0f, 0.0f, 0.0f}) * (1.0f / kRestUp);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) S[t0 + t] = mma<DT>(ko[t], terms[0], S[t0 + t]);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) S[t0 + t] += mma<DT>(ko[t], terms[1], f32x4{0.0f, 0.0f, 0.0f, 0.0f}) * (1.0f / kRestUp);
         } else {
 #pragma unroll
-          for (int m = TERMS - 1; m >= 0; --m) S[t] = mma<DT>(ko, terms[m], S[t]);
+          for (int m = TERMS - 1; m >= 0; --m)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) S[t0 + t] = mma<DT>(ko[t], terms[m], S[t0 + t]);
         }
       }
     }
-    if (DT == MM_F16 && OUT) {
-      float m = 0.0f;
-#pragma unroll
-      for (int t = 0; t < ND; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(S[t][r]));
-#pragma unroll
-      for (int x = 1; x < 64; x *= 2) m = fmaxf(m, lane_xor(m, x));
-      if (lane == 0) s_max[wave] = m;
-    }
-    if (!OUT) total += static_cast<double>(s_d.hi[63]) + s_d.lo[63];
+    if (DT == MM_F16 && OUT) note_max();
+    if (!OUT) total += static_cast<double>(D.hi[63]) + D.lo[63];
     __syncthreads();
   }
 

@@ -32,7 +32,6 @@ struct Op {
   static constexpr int kE = kWide ? 4 : 8;      // elements of an operand in a lane
   static constexpr int kStep = 4 * kE;          // elements of the sum an operand covers
   static constexpr int kTiles = kWide ? 1 : 2;  // accumulator tiles an operand is made of
-  static constexpr int kPad = kWide ? 4 : 16;   // of a row in shared memory: transposed reads without bank conflicts
 };
 
 template <int DT>
@@ -83,62 +82,81 @@ __device__ __forceinline__ u32x4 from_acc(const f32x4* t) {
                  pack2<DT>(t[1][2], t[1][3])};
 }
 
-// Row r0 + i of a tile in shared memory, elements k0 on, in row order.
-template <int DT>
-__device__ __forceinline__ u32x4 row_operand(const typename Ty<DT>::T* tile, int ld, int r0, int k0, int lane) {
-  return *reinterpret_cast<const u32x4*>(tile + (r0 + (lane & 15)) * ld + k0 + Op<DT>::kE * (lane >> 4));
-}
-// ... in acc order.
-template <int DT>
-__device__ __forceinline__ u32x4 row_operand_acc(const typename Ty<DT>::T* tile, int ld, int r0, int k0, int lane) {
-  const typename Ty<DT>::T* const p = tile + (r0 + (lane & 15)) * ld + k0 + 4 * (lane >> 4);
-  if constexpr (Op<DT>::kWide) {
-    return *reinterpret_cast<const u32x4*>(p);
-  } else {
-    const u32x2 a = *reinterpret_cast<const u32x2*>(p), b = *reinterpret_cast<const u32x2*>(p + 16);
-    return u32x4{a[0], a[1], b[0], b[1]};
-  }
-}
-// Four elements of column c0 + i of rows r0 + 4 g on, 16-bit types: the transposing read, in which each group of 16
-// lanes reads 4 rows of 16 elements, 8 bytes a lane, and gets a column each.
-template <int DT>
-__device__ __forceinline__ u32x2 column4(const typename Ty<DT>::T* tile, int ld, int r0, int c0, int lane) {
-  const typename Ty<DT>::T* const p = tile + (r0 + 4 * (lane >> 4) + ((lane & 15) >> 2)) * ld + c0 + 4 * (lane & 3);
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       (__attribute__((address_space(3))) s16x4*)const_cast<typename Ty<DT>::T*>(p)));
-}
-// Column c0 + i, rows k0 on, in acc order: an operand whose sum runs over a tile's rows.
-template <int DT>
-__device__ __forceinline__ u32x4 column_operand(const typename Ty<DT>::T* tile, int ld, int k0, int c0, int lane) {
-  if constexpr (Op<DT>::kWide) {
-    u32x4 v;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      v[j] = __float_as_uint(tile[(k0 + 4 * (lane >> 4) + j) * ld + c0 + (lane & 15)]);
-    return v;
-  } else {
-    const u32x2 a = column4<DT>(tile, ld, k0, c0, lane), b = column4<DT>(tile, ld, k0 + 16, c0, lane);
-    return u32x4{a[0], a[1], b[0], b[1]};
-  }
-}
-
-// Rows of a (batch, seqlen, heads, width) tensor of one head, as a workgroup of 256 stages them: 64 rows of W elements,
-// 16 bytes a thread and step, held in registers between the load and the write to shared memory.
+// A tile of W columns in shared memory.  16-bit rows are cut into chunks of 16 bytes, and chunk c of row r is kept at
+// place c ^ turn(r), such that the 16 rows that a row read touches, and the pairs of chunks of the 8 rows that a
+// transposing read touches, lie in different banks.  (fp32: rows 4 words longer do the same.)
 template <int DT, int W>
+struct Tile {
+  using T = typename Ty<DT>::T;
+  static constexpr bool kWide = Op<DT>::kWide;
+  static constexpr int kLd = kWide ? W + 4 : W;
+  static __device__ __forceinline__ int turn(int r) {
+    return W == 128 ? (r & 7) << 1 | (r >> 3 & 1) : (r >> 1 & 3) << 1 | (r >> 3 & 1);
+  }
+  static __device__ __forceinline__ int at(int r, int e) {
+    return kWide ? r * kLd + e : r * kLd + (((e >> 3) ^ turn(r)) << 3) + (e & 7);
+  }
+  // Row r0 + i, elements k0 on, in row order.
+  static __device__ __forceinline__ u32x4 row(const T* tile, int r0, int k0, int lane) {
+    return *reinterpret_cast<const u32x4*>(tile + at(r0 + (lane & 15), k0 + Op<DT>::kE * (lane >> 4)));
+  }
+  // ... in acc order.
+  static __device__ __forceinline__ u32x4 row_acc(const T* tile, int r0, int k0, int lane) {
+    const int r = r0 + (lane & 15), e = k0 + 4 * (lane >> 4);
+    if constexpr (kWide) {
+      return *reinterpret_cast<const u32x4*>(tile + at(r, e));
+    } else {
+      const u32x2 a = *reinterpret_cast<const u32x2*>(tile + at(r, e)), b = *reinterpret_cast<const u32x2*>(tile + at(r, e + 16));
+      return u32x4{a[0], a[1], b[0], b[1]};
+    }
+  }
+  // Four elements of column c0 + i of rows r0 + 4 g on, 16-bit types: the transposing read, in which each group of 16
+  // lanes reads 4 rows of 16 elements, 8 bytes a lane, and gets a column each.
+  static __device__ __forceinline__ u32x2 column4(const T* tile, int r0, int c0, int lane) {
+    const T* const p = tile + at(r0 + 4 * (lane >> 4) + ((lane & 15) >> 2), c0 + 4 * (lane & 3));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)const_cast<T*>(p)));
+  }
+  // Column c0 + i, rows k0 on, in acc order: an operand whose sum runs over a tile's rows.
+  static __device__ __forceinline__ u32x4 column(const T* tile, int k0, int c0, int lane) {
+    if constexpr (kWide) {
+      u32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(tile[at(k0 + 4 * (lane >> 4) + j, c0 + (lane & 15))]);
+      return v;
+    } else {
+      const u32x2 a = column4(tile, k0, c0, lane), b = column4(tile, k0 + 16, c0, lane);
+      return u32x4{a[0], a[1], b[0], b[1]};
+    }
+  }
+};
+
+// 64 rows of W elements of one head, as a workgroup of `Threads` stages them, 16 bytes a thread and step, held in
+// registers between the load and the write to shared memory.
+template <int DT, int W, int Threads>
 struct Staged {
   using T = typename Ty<DT>::T;
   static constexpr int kE = Op<DT>::kE;
-  static constexpr int kUnits = W / kE;                 // 16-byte units of a row
-  static constexpr int kSteps = kRun * kUnits / 256;
+  static constexpr int kUnits = W / kE;                  // 16-byte units of a row
+  static constexpr int kSteps = kRun * kUnits / Threads;
+  static constexpr int kRows = Threads / kUnits;         // of a step
+  static_assert(kSteps >= 1, "a unit for every thread");
   u32x4 v[kSteps];
-  // Rows r >= rows and elements >= width come as zeros.  vec: 16-byte aligned rows and a width that 16 bytes divide.
+  // Rows r >= rows and elements >= width come as zeros.  vec: 16-byte aligned rows that 16 bytes divide, and 64 of them
+  // within 4 GB.
   __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int width, bool vec) {
+    const int r = static_cast<int>(threadIdx.x) / kUnits, e = static_cast<int>(threadIdx.x) % kUnits * kE;
+    if (vec && rows == kRun && width == W) {
+      const uint32_t off = static_cast<uint32_t>(r * stride + e) * static_cast<uint32_t>(sizeof(T));
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        v[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base + s * kRows * stride) + off);
+      return;
+    }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int u = s * 256 + static_cast<int>(threadIdx.x), r = u / kUnits, e = u % kUnits * kE;
       v[s] = u32x4{0, 0, 0, 0};
-      if (r < rows && e < width) {
-        const T* const p = base + r * stride + e;
+      if (s * kRows + r < rows && e < width) {
+        const T* const p = base + (s * kRows + r) * stride + e;
         if (vec) {
           v[s] = *reinterpret_cast<const u32x4*>(p);
         } else {
@@ -151,11 +169,9 @@ struct Staged {
     }
   }
   __device__ __forceinline__ void store(T* tile) const {
+    const int r = static_cast<int>(threadIdx.x) / kUnits, e = static_cast<int>(threadIdx.x) % kUnits * kE;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int u = s * 256 + static_cast<int>(threadIdx.x), r = u / kUnits, e = u % kUnits * kE;
-      *reinterpret_cast<u32x4*>(tile + r * (W + Op<DT>::kPad) + e) = v[s];
-    }
+    for (int s = 0; s < kSteps; ++s) *reinterpret_cast<u32x4*>(tile + Tile<DT, W>::at(s * kRows + r, e)) = v[s];
   }
 };
 
