@@ -269,9 +269,8 @@ int mm_decay_attention_fwd(const mm_decay_attention_params* p, void* stream) {
   set(k.q, k.q_stride, p->q, p->q_stride);
   set(k.k, k.k_stride, p->k, p->k_stride);
   set(k.v, k.v_stride, p->v, p->v_stride);
-  k.vec = vec_ok(k.q, k.q_stride, k.dk, k.dtype) | vec_ok(k.k, k.k_stride, k.dk, k.dtype) << 1 |
-          vec_ok(k.v, k.v_stride, k.dv, k.dtype) << 2;
-  k.vec |= out_ok(p->y, k.dv) << 4;
+  k.vec = vec_ok(k.q, k.q_stride, k.dk, k.dtype) && vec_ok(k.k, k.k_stride, k.dk, k.dtype) &&
+          vec_ok(k.v, k.v_stride, k.dv, k.dtype) && out_ok(p->y, k.dv);
   k.init = p->h0;
   k.final_state = p->state_out;
   k.y = p->y;
@@ -305,9 +304,8 @@ int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream) {
   set(k.q, k.q_stride, p->k, p->k_stride);
   set(k.k, k.k_stride, p->q, p->q_stride);
   set(k.v, k.v_stride, p->dy, p->dy_stride);
-  k.vec = vec_ok(k.q, k.q_stride, k.dk, k.dtype) | vec_ok(k.k, k.k_stride, k.dk, k.dtype) << 1 |
-          vec_ok(k.v, k.v_stride, k.dv, k.dtype) << 2;
-  k.vec |= out_ok(p->dv, k.dv) << 4;
+  k.vec = vec_ok(k.q, k.q_stride, k.dk, k.dtype) && vec_ok(k.k, k.k_stride, k.dk, k.dtype) &&
+          vec_ok(k.v, k.v_stride, k.dv, k.dtype) && out_ok(p->dv, k.dv);
   k.init = p->dstate;
   k.final_state = p->dh0;
   k.y = p->dv;
@@ -351,8 +349,8 @@ int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream) {
     d.vblocks = s.vblocks;
     d.sets = s.sets;
     d.set_heads = s.set_heads;
-    d.vec = vec_ok(d.q, d.q_stride, d.dk, p->dtype) | vec_ok(d.k, d.k_stride, d.dk, p->dtype) << 1 |
-            vec_ok(d.v, d.v_stride, d.dv, p->dtype) << 2 | vec_ok(d.dy, d.dy_stride, d.dv, p->dtype) << 3;
+    d.vec = vec_ok(d.q, d.q_stride, d.dk, p->dtype) && vec_ok(d.k, d.k_stride, d.dk, p->dtype) &&
+            vec_ok(d.v, d.v_stride, d.dv, p->dtype) && vec_ok(d.dy, d.dy_stride, d.dv, p->dtype);
     d.dtype = p->dtype;
     d.g_dtype = p->log_decay_dtype;
     d.lengths_dtype = p->lengths_dtype;

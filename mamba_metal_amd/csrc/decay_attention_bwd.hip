@@ -11,32 +11,46 @@
 // A workgroup takes one run and some heads that share q and k, which it stages once and whose gradients it sums over
 // the heads in registers.  Waves 0 to 3 make dq, waves 4 to 7 dk, 16 tokens each: the two are one computation with the
 // roles exchanged (own rows dy, others v, state S, sum over k; or own rows v, others dy, state dS, sum over q).
+// What a head needs, 48 KB with key_dim 128 in 16 bits, is the traffic that bounds it.  It is loaded straight into shared
+// memory while the head before is computed (two buffers, one barrier a head); fp32, whose buffers would not fit twice,
+// and rows off 16 bytes go through registers instead.
 #include "decay_attention.h"
 #include "decay_tiles.h"
 
 namespace mm {
 namespace dattn {
 
-template <int DT, int DKP>
+__device__ const uint32_t kZeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
+
+__device__ __forceinline__ void load_direct(const char* from, char* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+template <int DT, int DKP, bool DIRECT>
 __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
   using T = typename Ty<DT>::T;
   using O = Op<DT>;
   using TK = Tile<DT, DKP>;
   using TV = Tile<DT, kVBlock>;
   constexpr int ND = DKP / 16, NU = kVBlock / O::kStep;
+  constexpr int64_t kEs = sizeof(T);
+  constexpr int kState = DIRECT ? kVBlock * DKP : 0, kRows = kRun * TV::kLd;  // elements of a buffer's parts
   __shared__ __attribute__((aligned(16))) T s_qk[2][kRun * TK::kLd];  // q, k
-  __shared__ __attribute__((aligned(16))) T s_dv[2][kRun * TV::kLd];  // dy, v
-  __shared__ Decays s_d;
-  __shared__ float s_sum[2][kRun], s_inter[2][kRun];  // M's row and column sums; the states' parts
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  __shared__ __attribute__((aligned(16))) T s_b0[2 * kState + 2 * kRows];  // S, dS, dy, v
+  __shared__ __attribute__((aligned(16))) T s_b1[DIRECT ? 2 * kState + 2 * kRows : 8];
+  __shared__ Decays s_d[2];
+  __shared__ float s_sum[2][2][kRun], s_inter[2][2][kRun];  // M's row and column sums; the states' parts
+  int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
   const int role = wave >> 2, blk = wave & 3;  // 0: dq, 1: dk
 
   uint32_t id = blockIdx.x;
   const int set = static_cast<int>(id % p.sets);
   id /= p.sets;
-  const int64_t group = id % p.groups;
+  const int64_t group = id % static_cast<uint32_t>(p.groups);
   id /= static_cast<uint32_t>(p.groups);
-  const int64_t run = id % p.runs, b = id / p.runs;
+  const int64_t run = id % static_cast<uint32_t>(p.runs), b = id / static_cast<uint32_t>(p.runs);
   const int64_t len = length_of(p, b), t0 = run * kRun;
   const int rows = static_cast<int>(len - t0 < 0 ? 0 : len - t0 < kRun ? len - t0 : kRun);
   const int h0 = set * p.set_heads, h1 = h0 + p.set_heads < p.per ? h0 + p.set_heads : static_cast<int>(p.per);
@@ -48,12 +62,20 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
   if (rows > 0) {
     {
       Staged<DT, DKP, 512> r;
-      r.load(static_cast<const T*>(p.q) + b * p.q_stride[0] + t0 * p.q_stride[1] + group * p.q_stride[2], p.q_stride[1],
-             rows, dk, p.vec & 1);
-      r.store(s_qk[0]);
-      r.load(static_cast<const T*>(p.k) + b * p.k_stride[0] + t0 * p.k_stride[1] + group * p.k_stride[2], p.k_stride[1],
-             rows, dk, p.vec & 2);
-      r.store(s_qk[1]);
+      const char* const q = static_cast<const char*>(p.q) + (b * p.q_stride[0] + t0 * p.q_stride[1] + group * p.q_stride[2]) * kEs;
+      const char* const k = static_cast<const char*>(p.k) + (b * p.k_stride[0] + t0 * p.k_stride[1] + group * p.k_stride[2]) * kEs;
+      if (p.vec) {
+        Staged<DT, DKP, 512> r2;
+        r.load(q, static_cast<uint32_t>((r.row() * p.q_stride[1] + r.elem()) * kEs), r.kRows * p.q_stride[1] * kEs, rows, dk);
+        r2.load(k, static_cast<uint32_t>((r.row() * p.k_stride[1] + r.elem()) * kEs), r.kRows * p.k_stride[1] * kEs, rows, dk);
+        r.store(s_qk[0]);
+        r2.store(s_qk[1]);
+      } else {
+        r.load_any(q, p.q_stride[1], rows, dk);
+        r.store(s_qk[0]);
+        r.load_any(k, p.k_stride[1], rows, dk);
+        r.store(s_qk[1]);
+      }
     }
     __syncthreads();
     const T* const s_own = s_qk[role];
@@ -65,75 +87,123 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       A[ot] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int u = 0; u < DKP / O::kStep; ++u)
-        A[ot] = mma<DT>(TK::row(s_other, 16 * ot, u * O::kStep, lane),
-                        TK::row(s_own, 16 * blk, u * O::kStep, lane), A[ot]);
+        A[ot] = mma<DT>(TK::row(s_other, 16 * ot, u * O::kStep, lane), TK::row(s_own, 16 * blk, u * O::kStep, lane), A[ot]);
     }
 
+    // A step is a head's block of value channels.
+    const char* const dy0 = static_cast<const char*>(p.dy) + (b * p.dy_stride[0] + t0 * p.dy_stride[1]) * kEs;
+    const char* const v0 = static_cast<const char*>(p.v) + (b * p.v_stride[0] + t0 * p.v_stride[1]) * kEs;
     Staged<DT, kVBlock, 512> ry, rv;
-    float rg = 0.0f;
-    auto fetch = [&](int h, int vb) __attribute__((always_inline)) {
+    auto fetch = [&](T* buf, int h, int vb) __attribute__((always_inline)) {
       const int64_t head = group * p.per + h;
       const int vw = static_cast<int>(p.dv - vb * kVBlock < kVBlock ? p.dv - vb * kVBlock : kVBlock);
-      ry.load(static_cast<const T*>(p.dy) + b * p.dy_stride[0] + t0 * p.dy_stride[1] + head * p.dy_stride[2] + vb * kVBlock,
-              p.dy_stride[1], rows, vw, p.vec & 8);
-      rv.load(static_cast<const T*>(p.v) + b * p.v_stride[0] + t0 * p.v_stride[1] + head * p.v_stride[2] + vb * kVBlock,
-              p.v_stride[1], rows, vw, p.vec & 4);
-      if (vb == 0) rg = lane < rows ? load_gate(p, b * p.g_stride[0] + (t0 + lane) * p.g_stride[1] + head * p.g_stride[2]) : 0.0f;
-    };
-    fetch(h0, 0);
-    for (int h = h0; h < h1; ++h) {
-      const int64_t head = group * p.per + h, bh = b * p.heads + head;
-      f32x4 acc[4], tmp[ND];
+      const char* const dy = dy0 + (head * p.dy_stride[2] + vb * kVBlock) * kEs;
+      const char* const v = v0 + (head * p.v_stride[2] + vb * kVBlock) * kEs;
+      if constexpr (DIRECT) {
+        char* const to = reinterpret_cast<char*>(buf);
+        constexpr int kBytes = kState * static_cast<int>(kEs);
+        const int64_t block = ((b * p.heads + head) * p.runs + run) * p.vblocks + vb;
 #pragma unroll
-      for (int ot = 0; ot < 4; ++ot) acc[ot] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int which = 0; which < 2; ++which) {
+          const char* const from = static_cast<const char*>(which ? p.dstates : p.states) + block * kBytes;
 #pragma unroll
-      for (int t = 0; t < ND; ++t) tmp[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      float factor = 1.0f;
-      for (int vb = 0; vb < p.vblocks; ++vb) {
-        __syncthreads();
-        ry.store(s_dv[0]);
-        rv.store(s_dv[1]);
-        if (vb == 0 && wave == 0) run_decays(s_d, rg, lane);
-        __syncthreads();
-        const T* const from = run_state<T>(const_cast<void*>(role ? p.dstates : p.states), p, bh, run, vb, DKP);
-        if (vb + 1 < p.vblocks) fetch(h, vb + 1);
-        else if (h + 1 < h1) fetch(h + 1, 0);
-        const T* const own_t = s_dv[role];
-        const T* const other_t = s_dv[1 - role];
-        u32x4 own[NU];
-#pragma unroll
-        for (int u = 0; u < NU; ++u) own[u] = TV::row_acc(own_t, 16 * blk, u * O::kStep, lane);
-        if constexpr (DT == MM_F16) {
-          const float f = (role ? p.dfactors : p.factors)[(bh * p.runs + run) * p.vblocks + vb];
-#pragma unroll
-          for (int t = 0; t < ND; ++t) tmp[t] *= factor / f;
-          factor = f;
+          for (int q = 0; q < kBytes / 8192; ++q) {
+            const int at = (q * 8 + wave) * 1024;
+            load_direct(from + at + lane * 16, to + which * kBytes + at);
+          }
         }
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-          for (int t = 0; t < ND; ++t)
-            tmp[t] = mma<DT>(own[u], *reinterpret_cast<const u32x4*>(from + static_cast<int64_t>((u * ND + t) * 64 + lane) * O::kE),
-                             tmp[t]);
-#pragma unroll
-        for (int ot = 0; ot < 4; ++ot) {
-          if (role ? ot < blk : ot > blk) continue;
-#pragma unroll
-          for (int u = 0; u < NU; ++u) acc[ot] = mma<DT>(TV::row_acc(other_t, 16 * ot, u * O::kStep, lane), own[u], acc[ot]);
+        // a row of 64 channels is 8 chunks; place lane % 8 of it holds chunk place ^ turn(row)
+        const int r = wave * 8 + (lane >> 3), c = (lane & 7) ^ TV::turn(r);
+        const bool in = r < rows && c * 8 < vw;
+        const char* const zeros = reinterpret_cast<const char*>(kZeros);
+        load_direct(in ? dy + r * p.dy_stride[1] * kEs + c * 16 : zeros, to + 2 * kBytes + wave * 1024);
+        load_direct(in ? v + r * p.v_stride[1] * kEs + c * 16 : zeros, to + 2 * kBytes + kRows * kEs + wave * 1024);
+      } else {
+        if (p.vec) {
+          ry.load(dy, static_cast<uint32_t>((ry.row() * p.dy_stride[1] + ry.elem()) * kEs), ry.kRows * p.dy_stride[1] * kEs, rows, vw);
+          rv.load(v, static_cast<uint32_t>((rv.row() * p.v_stride[1] + rv.elem()) * kEs), rv.kRows * p.v_stride[1] * kEs, rows, vw);
+        } else {
+          ry.load_any(dy, p.dy_stride[1], rows, vw);
+          rv.load_any(v, p.v_stride[1], rows, vw);
         }
       }
+    };
+    auto gate = [&](int h) {
+      return lane < rows ? load_gate(p, b * p.g_stride[0] + (t0 + lane) * p.g_stride[1] + (group * p.per + h) * p.g_stride[2]) : 0.0f;
+    };
+    // dg of a head whose parts all waves have left
+    auto finish_dg = [&](int h) __attribute__((always_inline)) {
+      const int64_t head = group * p.per + h;
+      const float* const sum = &s_sum[(h - h0) & 1][0][0];
+      const float* const inter = &s_inter[(h - h0) & 1][0][0];
+      const double u = static_cast<double>(sum[lane]) - sum[kRun + lane] + inter[lane];
+      const double kv = inter[kRun + lane];
+      const double up = prefix_sum(u), all = __shfl(up, 63, 64);
+      double dg = all - up + u + prefix_sum(kv) - kv;
+      for (int vb = 0; vb < p.vblocks; ++vb) dg += p.dot[((b * p.heads + head) * p.runs + run) * p.vblocks + vb];
+      if (lane < rows) p.dg[(b * p.seqlen + t0 + lane) * p.heads + head] = static_cast<float>(dg);
+    };
+
+    f32x4 acc[4], tmp[ND];
+    float factor = 1.0f;
+    auto step = [&](T* cur, T* other, int h, int vb) __attribute__((always_inline)) {
+      asm volatile("" : "+v"(lane));
+      const int64_t head = group * p.per + h, bh = b * p.heads + head;
+      const bool last_block = vb + 1 == p.vblocks, more = !last_block || h + 1 < h1;
+      const int h_next = last_block ? h + 1 : h, vb_next = last_block ? 0 : vb + 1;
+      if constexpr (!DIRECT) {
+        __syncthreads();
+        ry.store(cur + 2 * kState);
+        rv.store(cur + 2 * kState + kRows);
+      }
+      __syncthreads();
+      if (more) fetch(other, h_next, vb_next);
+      float g_next = 0.0f;
+      const bool decays_now = wave == 7 && last_block && h + 1 < h1;
+      if (decays_now) g_next = gate(h + 1);
+      if (p.dg && wave == 0 && vb == 0 && h > h0) finish_dg(h - 1);
+      const Decays& D = s_d[(h - h0) & 1];
+      if (vb == 0) {
+#pragma unroll
+        for (int ot = 0; ot < 4; ++ot) acc[ot] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < ND; ++t) tmp[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        factor = 1.0f;
+      }
+      const T* const own_t = cur + 2 * kState + role * kRows;
+      const T* const other_t = cur + 2 * kState + (1 - role) * kRows;
+      const T* const state = DIRECT ? cur + role * kState : run_state<T>(const_cast<void*>(role ? p.dstates : p.states), p, bh, run, vb, DKP);
+      u32x4 own[NU];
+#pragma unroll
+      for (int u = 0; u < NU; ++u) own[u] = TV::row_acc(own_t, 16 * blk, u * O::kStep, lane);
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int ot = 0; ot < 4; ++ot)
+          if (role ? ot >= blk : ot <= blk) acc[ot] = mma<DT>(TV::row_acc(other_t, 16 * ot, u * O::kStep, lane), own[u], acc[ot]);
+      if constexpr (DT == MM_F16) {
+        const float f = (role ? p.dfactors : p.factors)[(bh * p.runs + run) * p.vblocks + vb];
+#pragma unroll
+        for (int t = 0; t < ND; ++t) tmp[t] *= factor / f;
+        factor = f;
+      }
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+          tmp[t] = mma<DT>(own[u], *reinterpret_cast<const u32x4*>(state + ((u * ND + t) * 64 + lane) * O::kE), tmp[t]);
+      if (!last_block) return;
       // dP and M
-      const float hi_r = s_d.hi[16 * blk + i], lo_r = s_d.lo[16 * blk + i];
+      const float hi_r = D.hi[16 * blk + i], lo_r = D.lo[16 * blk + i];
       float sum = 0.0f;
 #pragma unroll
       for (int ot = 0; ot < 4; ++ot) {
         if (role ? ot < blk : ot > blk) continue;
-        const f32x4 hi = *reinterpret_cast<const f32x4*>(s_d.hi + 16 * ot + 4 * g);
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(s_d.lo + 16 * ot + 4 * g);
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(D.hi + 16 * ot + 4 * g);
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(D.lo + 16 * ot + 4 * g);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int other = 16 * ot + 4 * g + r, row = 16 * blk + i;
-          const bool in = role ? other >= row : other <= row;
+          const bool in = ot != blk || (role ? 4 * g + r >= i : 4 * g + r <= i);
           const float decay = role ? between<DT>(hi[r], lo[r], hi_r, lo_r) : between<DT>(hi_r, lo_r, hi[r], lo[r]);
           acc[ot][r] = in ? acc[ot][r] * p.scale * decay : 0.0f;
           sum += in ? acc[ot][r] * A[ot][r] : 0.0f;
@@ -143,8 +213,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
 #pragma unroll
       for (int u = 0; u < kRun / O::kStep; ++u) dp[u] = from_acc<DT>(acc + u * O::kTiles);
       // the states' part, scaled row by row
-      const f32x4 w = *reinterpret_cast<const f32x4*>((role ? s_d.onward : s_d.into) + 16 * blk + 4 * g) *
-                      ((role ? 1.0f : p.scale) * factor);
+      const f32x4 w = *reinterpret_cast<const f32x4*>((role ? D.onward : D.into) + 16 * blk + 4 * g) * ((role ? 1.0f : p.scale) * factor);
       f32x4 inter = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int t = 0; t < ND; ++t) {
@@ -164,24 +233,43 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       if (p.dg) {
         sum += lane_xor(sum, 16);
         sum += lane_xor(sum, 32);
-        if (g == 0) s_sum[role][16 * blk + i] = sum;
+        if (g == 0) s_sum[(h - h0) & 1][role][16 * blk + i] = sum;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
 #pragma unroll
           for (int x = 1; x < 16; x *= 2) inter[r] += lane_xor(inter[r], x);
-          if (i == 0) s_inter[role][16 * blk + 4 * g + r] = inter[r];
         }
-        __syncthreads();
-        if (wave == 0) {
-          const double u = static_cast<double>(s_sum[0][lane]) - s_sum[1][lane] + s_inter[0][lane];
-          const double kv = s_inter[1][lane];
-          const double up = prefix_sum(u), all = __shfl(up, 63, 64);
-          double dg = all - up + u + prefix_sum(kv) - kv;
-          for (int vb = 0; vb < p.vblocks; ++vb) dg += p.dot[(bh * p.runs + run) * p.vblocks + vb];
-          if (lane < rows) p.dg[(b * p.seqlen + t0 + lane) * p.heads + head] = static_cast<float>(dg);
-        }
+        if (i == 0) *reinterpret_cast<f32x4*>(&s_inter[(h - h0) & 1][role][16 * blk + 4 * g]) = inter;
+      }
+      if (decays_now) run_decays(s_d[(h + 1 - h0) & 1], g_next, lane);
+    };
+    if (wave == 7) run_decays(s_d[0], gate(h0), lane);
+    fetch(s_b0, h0, 0);
+    const int steps = (h1 - h0) * p.vblocks;
+    int h = h0, vb = 0;
+    auto advance = [&] {
+      if (++vb == p.vblocks) {
+        vb = 0;
+        ++h;
+      }
+    };
+    if constexpr (DIRECT) {
+      int n = 0;
+      for (; n + 1 < steps; n += 2) {
+        step(s_b0, s_b1, h, vb);
+        advance();
+        step(s_b1, s_b0, h, vb);
+        advance();
+      }
+      if (n < steps) step(s_b0, s_b1, h, vb);
+    } else {
+      for (int n = 0; n < steps; ++n) {
+        step(s_b0, s_b0, h, vb);
+        advance();
       }
     }
+    __syncthreads();
+    if (p.dg && wave == 0) finish_dg(h1 - 1);
   }
   if (p.dg && wave == 0 && lane >= rows && t0 + lane < p.seqlen)
     for (int h = h0; h < h1; ++h) p.dg[(b * p.seqlen + t0 + lane) * p.heads + group * p.per + h] = 0.0f;
@@ -203,17 +291,21 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
   }
 }
 
-template <int DT>
+template <int DT, int DKP>
 static void launch_grad_t(const Grad& p, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(p.batch * p.runs * p.groups * p.sets));
-  if (padded_dk(p.dk) == 64) hipLaunchKernelGGL((grad_kernel<DT, 64>), grid, dim3(512), 0, s, p);
-  else hipLaunchKernelGGL((grad_kernel<DT, 128>), grid, dim3(512), 0, s, p);
+  if (DT != MM_F32 && p.vec) hipLaunchKernelGGL((grad_kernel<DT, DKP, DT != MM_F32>), grid, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((grad_kernel<DT, DKP, false>), grid, dim3(512), 0, s, p);
+}
+template <int DT>
+static void launch_grad_d(const Grad& p, hipStream_t s) {
+  if (padded_dk(p.dk) == 64) launch_grad_t<DT, 64>(p, s); else launch_grad_t<DT, 128>(p, s);
 }
 void launch_grad(const Grad& p, hipStream_t s) {
   switch (p.dtype) {
-    case MM_F32: launch_grad_t<MM_F32>(p, s); break;
-    case MM_F16: launch_grad_t<MM_F16>(p, s); break;
-    default: launch_grad_t<MM_BF16>(p, s); break;
+    case MM_F32: launch_grad_d<MM_F32>(p, s); break;
+    case MM_F16: launch_grad_d<MM_F16>(p, s); break;
+    default: launch_grad_d<MM_BF16>(p, s); break;
   }
 }
 

@@ -51,7 +51,7 @@ __device__ __forceinline__ void split_operand(const float (&x)[8], u32x4 (&out)[
     }
 }
 
-template <int DT, int DKP, bool REV, bool OUT>
+template <int DT, int DKP, bool REV, bool OUT, bool VEC>
 __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) void pass_kernel(const Pass p) {
   using T = typename Ty<DT>::T;
   using O = Op<DT>;
@@ -85,11 +85,6 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
   const int vw = static_cast<int>(p.dv - vb * kVBlock < kVBlock ? p.dv - vb * kVBlock : kVBlock);
   const int dk = static_cast<int>(p.dk);
 
-  const T* const qh = static_cast<const T*>(p.q) + b * p.q_stride[0] + group * p.q_stride[2];
-  const T* const kh = static_cast<const T*>(p.k) + b * p.k_stride[0] + group * p.k_stride[2];
-  const T* const vh = static_cast<const T*>(p.v) + b * p.v_stride[0] + head * p.v_stride[2] + vb * kVBlock;
-  const int64_t gh = b * p.g_stride[0] + head * p.g_stride[2];
-
   // The state before the first run walked: zeros, the caller's, or what the segments before this one left.
   f32x4 S[ND];
 #pragma unroll
@@ -112,13 +107,35 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
 
   Staged<DT, DKP, 256> rq, rk;
   Staged<DT, kVBlock, 256> rv;
+  // The run to fetch next: its rows' addresses (running ones: few scalar registers), which a step moves on by a run.
+  constexpr int64_t kEs = sizeof(T);
+  const int64_t live_runs = (len + kRun - 1) / kRun;
+  const int64_t walk_end = run_end < live_runs ? run_end : live_runs;  // runs with tokens: [run0, walk_end)
+  const int64_t walk = walk_end - run0;
+  int64_t at_run = REV ? walk_end - 1 : run0;
+  const char* qp = static_cast<const char*>(p.q) + (b * p.q_stride[0] + group * p.q_stride[2] + at_run * kRun * p.q_stride[1]) * kEs;
+  const char* kp = static_cast<const char*>(p.k) + (b * p.k_stride[0] + group * p.k_stride[2] + at_run * kRun * p.k_stride[1]) * kEs;
+  const char* vp = static_cast<const char*>(p.v) + (b * p.v_stride[0] + head * p.v_stride[2] + vb * kVBlock + at_run * kRun * p.v_stride[1]) * kEs;
+  T* yp = static_cast<T*>(p.y) + ((b * p.seqlen + at_run * kRun) * p.heads + head) * p.dv + vb * kVBlock;  // (of the run at hand)
+  const int64_t gh = b * p.g_stride[0] + head * p.g_stride[2];
+  const uint32_t q_off = static_cast<uint32_t>((rq.row() * p.q_stride[1] + rq.elem()) * kEs);
+  const uint32_t k_off = static_cast<uint32_t>((rk.row() * p.k_stride[1] + rk.elem()) * kEs);
+  const uint32_t v_off = static_cast<uint32_t>((rv.row() * p.v_stride[1] + rv.elem()) * kEs);
+  constexpr int kWay = REV ? -1 : 1;
   auto rows_of = [&](int64_t run) { return static_cast<int>(len - run * kRun < kRun ? len - run * kRun : kRun); };
-  auto fetch = [&](int64_t run) __attribute__((always_inline)) {
-    const int64_t t0 = run * kRun;
-    const int rows = rows_of(run);
-    if (OUT) rq.load(qh + t0 * p.q_stride[1], p.q_stride[1], rows, dk, p.vec & 1);
-    rk.load(kh + t0 * p.k_stride[1], p.k_stride[1], rows, dk, p.vec & 2);
-    rv.load(vh + t0 * p.v_stride[1], p.v_stride[1], rows, vw, p.vec & 4);
+  auto fetch = [&](int rows) __attribute__((always_inline)) {
+    if constexpr (VEC) {
+      if (OUT) rq.load(qp, q_off, rq.kRows * p.q_stride[1] * kEs, rows, dk);
+      rk.load(kp, k_off, rk.kRows * p.k_stride[1] * kEs, rows, dk);
+      rv.load(vp, v_off, rv.kRows * p.v_stride[1] * kEs, rows, vw);
+    } else {
+      if (OUT) rq.load_any(qp, p.q_stride[1], rows, dk);
+      rk.load_any(kp, p.k_stride[1], rows, dk);
+      rv.load_any(vp, p.v_stride[1], rows, vw);
+    }
+    if (OUT) qp += kWay * kRun * p.q_stride[1] * kEs;
+    kp += kWay * kRun * p.k_stride[1] * kEs;
+    vp += kWay * kRun * p.v_stride[1] * kEs;
   };
   auto gate = [&](int64_t run) {
     return lane < rows_of(run) ? load_gate(p, gh + (run * kRun + lane) * p.g_stride[1]) : 0.0f;
@@ -134,22 +151,18 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     for (int x = 1; x < 64; x *= 2) m = fmaxf(m, lane_xor(m, x));
     if (lane == 0) s_max[wave] = m;
   };
-  const int64_t live_runs = (len + kRun - 1) / kRun;
-  const int64_t walk_end = run_end < live_runs ? run_end : live_runs;  // runs with tokens: [run0, walk_end)
-  const int64_t walk = walk_end - run0;
   double total = 0.0;   // the segment's log decay
   float factor = 1.0f;  // fp16: the state's power of two
   if (walk > 0) {
-    const int64_t run = REV ? walk_end - 1 : run0;
-    fetch(run);
+    fetch(rows_of(at_run));
     if (DT == MM_F16 && OUT) note_max();
-    if (wave == kDecayWave) run_decays(s_d[0], gate(run), lane);
+    if (wave == kDecayWave) run_decays(s_d[0], gate(at_run), lane);
   }
   for (int64_t n = 0; n < walk; ++n) {
     // addresses in shared memory are made anew in every run: held over it they would be dozens of registers
     asm volatile("" : "+v"(lane));
-    const int64_t run = REV ? walk_end - 1 - n : run0 + n;
-    const int64_t next = n + 1 < walk ? (REV ? run - 1 : run + 1) : run;
+    const int64_t run = at_run, next = n + 1 < walk ? run + kWay : run;
+    at_run = next;
     if (OUT) rq.store(s_q);
     rk.store(s_k);
     rv.store(s_v);
@@ -172,7 +185,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     }
     float g_next = 0.0f;
     if (wave == kDecayWave) g_next = gate(next);
-    if (n + 1 < walk) fetch(next);
+    if (n + 1 < walk) fetch(rows_of(next));
 
     u32x4 vo[NR];  // this wave's value columns, as operands over the run's tokens
 #pragma unroll
@@ -327,14 +340,13 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
         }
       const int rows = rows_of(run), left = static_cast<int>(p.seqlen - run * kRun < kRun ? p.seqlen - run * kRun : kRun);
       const int v0 = 16 * wave + 4 * g;
-      T* const yr = static_cast<T*>(p.y) + ((b * p.seqlen + run * kRun) * p.heads + head) * p.dv + vb * kVBlock;
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
         const int t = 16 * rt + i;
         if (t >= rows) acc[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (t >= left) continue;
-        T* const y = yr + t * p.heads * p.dv + v0;
-        if (p.vec & 16) {
+        T* const y = yp + t * p.heads * p.dv + v0;
+        if constexpr (VEC) {
           if (v0 < vw) {
             if constexpr (O::kWide) *reinterpret_cast<f32x4*>(y) = acc[rt];
             else *reinterpret_cast<u32x2*>(y) = u32x2{pack2<DT>(acc[rt][0], acc[rt][1]), pack2<DT>(acc[rt][2], acc[rt][3])};
@@ -345,6 +357,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
             if (v0 + r < vw) y[r] = Ty<DT>::from(acc[rt][r]);
         }
       }
+      yp += kWay * kRun * p.heads * p.dv;
     } else if (wave == kDecayWave) {
       run_decays(s_d[(n + 1) & 1], g_next, lane);
     }
@@ -451,20 +464,24 @@ __global__ __launch_bounds__(256) void join_kernel(const Pass p) {
   }
 }
 
-template <int DT, int DKP, bool REV>
+template <int DT, int DKP, bool REV, bool VEC>
 static void launch_pass_t(const Pass& p, hipStream_t s) {
   const unsigned per_seg = static_cast<unsigned>(p.batch * p.heads * p.vblocks);
   if (p.segments > 1) {
-    hipLaunchKernelGGL((pass_kernel<DT, DKP, REV, false>), dim3(per_seg * p.segments), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((pass_kernel<DT, DKP, REV, false, VEC>), dim3(per_seg * p.segments), dim3(256), 0, s, p);
     const int64_t n = p.batch * p.heads * p.vblocks * static_cast<int64_t>(kVBlock) * DKP / 4;
     hipLaunchKernelGGL((join_kernel<DKP, REV>), dim3(static_cast<unsigned>(ceil_div(n, 256))), dim3(256), 0, s, p);
   }
-  hipLaunchKernelGGL((pass_kernel<DT, DKP, REV, true>), dim3(per_seg * p.segments), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((pass_kernel<DT, DKP, REV, true, VEC>), dim3(per_seg * p.segments), dim3(256), 0, s, p);
 }
+// vec: 16 bytes at a time where all rows allow it; any other layout element by element.
 template <int DT, bool REV>
 static void launch_pass_d(const Pass& p, hipStream_t s) {
-  if (padded_dk(p.dk) == 64) launch_pass_t<DT, 64, REV>(p, s);
-  else launch_pass_t<DT, 128, REV>(p, s);
+  if (padded_dk(p.dk) == 64) {
+    if (p.vec) launch_pass_t<DT, 64, REV, true>(p, s); else launch_pass_t<DT, 64, REV, false>(p, s);
+  } else {
+    if (p.vec) launch_pass_t<DT, 128, REV, true>(p, s); else launch_pass_t<DT, 128, REV, false>(p, s);
+  }
 }
 template <bool REV>
 static void launch_pass(const Pass& p, hipStream_t s) {

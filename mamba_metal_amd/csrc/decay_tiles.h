@@ -141,37 +141,40 @@ struct Staged {
   static constexpr int kRows = Threads / kUnits;         // of a step
   static_assert(kSteps >= 1, "a unit for every thread");
   u32x4 v[kSteps];
-  // Rows r >= rows and elements >= width come as zeros.  vec: 16-byte aligned rows that 16 bytes divide, and 64 of them
-  // within 4 GB.
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int width, bool vec) {
-    const int r = static_cast<int>(threadIdx.x) / kUnits, e = static_cast<int>(threadIdx.x) % kUnits * kE;
-    if (vec && rows == kRun && width == W) {
-      const uint32_t off = static_cast<uint32_t>(r * stride + e) * static_cast<uint32_t>(sizeof(T));
+  static __device__ __forceinline__ int row() { return static_cast<int>(threadIdx.x) / kUnits; }
+  static __device__ __forceinline__ int elem() { return static_cast<int>(threadIdx.x) % kUnits * kE; }
+  // Rows r >= rows and elements >= width come as zeros.  16-byte aligned rows that 16 bytes divide, 64 of them within
+  // 4 GB: `first` is the first row's (wave-uniform) address, `off` row() and elem() in bytes, `step` kRows rows in bytes.
+  __device__ __forceinline__ void load(const char* first, uint32_t off, int64_t step, int rows, int width) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-        v[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base + s * kRows * stride) + off);
-      return;
+    for (int s = 0; s < kSteps; ++s) v[s] = u32x4{0, 0, 0, 0};
+    if (elem() >= width) return;
+    if (rows == kRun) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s, first += step) v[s] = *reinterpret_cast<const u32x4*>(first + off);
+    } else {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s, first += step)
+        if (s * kRows + row() < rows) v[s] = *reinterpret_cast<const u32x4*>(first + off);
     }
-#pragma unroll
+  }
+  // Any rows.
+  __device__ __forceinline__ void load_any(const char* first, int64_t stride, int rows, int width) {
+    const T* const base = reinterpret_cast<const T*>(first) + row() * stride + elem();
     for (int s = 0; s < kSteps; ++s) {
-      v[s] = u32x4{0, 0, 0, 0};
-      if (s * kRows + r < rows && e < width) {
-        const T* const p = base + (s * kRows + r) * stride + e;
-        if (vec) {
-          v[s] = *reinterpret_cast<const u32x4*>(p);
-        } else {
-          T t[kE];
+      T t[kE];
 #pragma unroll
-          for (int j = 0; j < kE; ++j) t[j] = e + j < width ? p[j] : static_cast<T>(0);
-          __builtin_memcpy(&v[s], t, 16);
-        }
-      }
+      for (int j = 0; j < kE; ++j)
+        t[j] = s * kRows + row() < rows && elem() + j < width ? base[s * kRows * stride + j] : static_cast<T>(0);
+      u32x4 w;
+      __builtin_memcpy(&w, t, 16);
+#pragma unroll
+      for (int q = 0; q < kSteps; ++q) v[q] = q == s ? w : v[q];
     }
   }
   __device__ __forceinline__ void store(T* tile) const {
-    const int r = static_cast<int>(threadIdx.x) / kUnits, e = static_cast<int>(threadIdx.x) % kUnits * kE;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) *reinterpret_cast<u32x4*>(tile + Tile<DT, W>::at(s * kRows + r, e)) = v[s];
+    for (int s = 0; s < kSteps; ++s) *reinterpret_cast<u32x4*>(tile + Tile<DT, W>::at(s * kRows + row(), elem())) = v[s];
   }
 };
 
