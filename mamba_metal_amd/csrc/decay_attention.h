@@ -67,26 +67,11 @@ template <typename P>
 __device__ __forceinline__ float load_gate(const P& p, int64_t at) {
   return p.g_dtype == MM_F32 ? ld<MM_F32>(p.g, at) : p.g_dtype == MM_F16 ? ld<MM_F16>(p.g, at) : ld<MM_BF16>(p.g, at);
 }
-// A run's state of one value block, 64 x DKP elements: operands over the value channels of products with dy or v, a
-// lane's elements together (in acc order of the sum).
-template <typename T, typename P>
-__device__ __forceinline__ T* run_state(void* states, const P& p, int64_t bh, int64_t run, int vb, int dkp) {
-  return static_cast<T*>(states) + ((bh * p.runs + run) * p.vblocks + vb) * 64 * dkp;
-}
-// Where lane's four elements of value channels 16 wave + 4 g .. + 3, key channel 16 t + i lie in it.
-template <int DT>
-__device__ __forceinline__ int64_t state_at(int wave, int t, int nd, int lane) {
-  return DT == MM_F32 ? static_cast<int64_t>((wave * nd + t) * 64 + lane) * 4
-                      : static_cast<int64_t>(((wave >> 1) * nd + t) * 64 + lane) * 8 + (wave & 1) * 4;
-}
+// A run's saved state of one value block: 64 value channels (rows) by DKP key channels, (bh, run, value block) contiguous.
 typedef float seg_f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ seg_f32x4* seg_state(const Pass& p, int64_t bh, int seg, int vb) {
   const int64_t dkp = p.dk <= 64 ? 64 : 128;
   return reinterpret_cast<seg_f32x4*>(p.seg_states) + ((bh * p.segments + seg) * p.vblocks + vb) * 16 * dkp;
 }
-// Between writes and reads of a wave's own shared memory: the wave's accesses are carried out in order, the compiler
-// just has to leave them so.
-__device__ __forceinline__ void wave_lds_fence() { asm volatile("" ::: "memory"); }
-
 }  // namespace dattn
 }  // namespace mm

@@ -108,8 +108,9 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
           const char* const from = static_cast<const char*>(which ? p.dstates : p.states) + block * kBytes;
 #pragma unroll
           for (int q = 0; q < kBytes / 8192; ++q) {
-            const int at = (q * 8 + wave) * 1024;
-            load_direct(from + at + lane * 16, to + which * kBytes + at);
+            // a row of DKP channels is DKP / 8 chunks, and place c of it holds chunk c ^ turn(row)
+            const int at = (q * 8 + wave) * 1024, unit = at / 16 + lane, r = unit / (DKP / 8), c = unit % (DKP / 8) ^ TK::turn(r);
+            load_direct(from + r * (DKP * 2) + c * 16, to + which * kBytes + at);
           }
         }
         // a row of 64 channels is 8 chunks; place lane % 8 of it holds chunk place ^ turn(row)
@@ -172,7 +173,21 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       }
       const T* const own_t = cur + 2 * kState + role * kRows;
       const T* const other_t = cur + 2 * kState + (1 - role) * kRows;
-      const T* const state = DIRECT ? cur + role * kState : run_state<T>(const_cast<void*>(role ? p.dstates : p.states), p, bh, run, vb, DKP);
+      const T* const state = DIRECT ? cur + role * kState
+                                    : static_cast<const T*>(role ? p.dstates : p.states) + ((bh * p.runs + run) * p.vblocks + vb) * kVBlock * DKP;
+      // columns d of the state, 16 t on, over its value channels
+      auto state_operand = [&](int u, int t) __attribute__((always_inline)) {
+        if constexpr (DIRECT) {
+          return TK::column(state, u * O::kStep, 16 * t, lane);
+        } else {
+          T e[O::kE];
+#pragma unroll
+          for (int j = 0; j < O::kE; ++j) e[j] = state[(u * O::kStep + 16 * (j >> 2) + 4 * g + (j & 3)) * DKP + 16 * t + i];
+          u32x4 w;
+          __builtin_memcpy(&w, e, 16);
+          return w;
+        }
+      };
       u32x4 own[NU];
 #pragma unroll
       for (int u = 0; u < NU; ++u) own[u] = TV::row_acc(own_t, 16 * blk, u * O::kStep, lane);
@@ -191,7 +206,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int t = 0; t < ND; ++t)
-          tmp[t] = mma<DT>(own[u], *reinterpret_cast<const u32x4*>(state + ((u * ND + t) * 64 + lane) * O::kE), tmp[t]);
+          tmp[t] = mma<DT>(own[u], state_operand(u, t), tmp[t]);
       if (!last_block) return;
       // dP and M
       const float hi_r = D.hi[16 * blk + i], lo_r = D.lo[16 * blk + i];

@@ -10,7 +10,8 @@
 //   dv_s = sum_{t >= s} scale (k_s . q_t) exp(c_t - c_s) dy_t + exp(c_63 - c_s) dS^T k_s
 //   dS  <- exp(c_63) dS + sum_t scale exp(c_t) q_t dy_t^T
 // A workgroup walks over the runs of one head and 64 value channels; wave w keeps columns 16 w .. 16 w + 15 of the
-// state in registers, fp32, as accumulators whose layout is at once the operand of S^T q.  Where the heads alone do not
+// state in registers, fp32, and leaves them in shared memory as operands of S^T q; token block w is its share of the
+// outputs.  Where the heads alone do not
 // fill the card the tokens are cut into segments: a first pass finds what each segment adds to the state, a small kernel
 // joins them, and the second pass starts each segment from its state.
 #pragma once
@@ -56,16 +57,15 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
   using T = typename Ty<DT>::T;
   using O = Op<DT>;
   using TK = Tile<DT, DKP>;
-  using TV = Tile<DT, kVBlock>;  // (values and scores: both 64 wide)
-  static_assert(kVBlock == kRun, "one tile type for both");
+  using TV = Tile<DT, kVBlock>;
   constexpr int ND = DKP / 16;  // state tiles of a wave
   constexpr int NU = DKP / O::kStep, NR = kRun / O::kStep;
   constexpr int TERMS = DT == MM_F32 ? 1 : DT == MM_F16 ? 2 : 3;
-  constexpr int kDecayWave = REV ? 3 : 0;                             // the one with the fewest scores
-  __shared__ __attribute__((aligned(16))) T s_q[OUT ? kRun * TK::kLd : 8];  // what asks: q, or k mirrored
-  __shared__ __attribute__((aligned(16))) T s_k[kRun * TK::kLd];            // what adds to the state: k, or q
-  __shared__ __attribute__((aligned(16))) T s_v[kRun * TV::kLd];            // its values: v, or dy
-  __shared__ __attribute__((aligned(16))) T s_p[OUT ? kRun * TV::kLd : 8];  // scores; 16 rows a wave, first for its own use
+  constexpr int kDecayWave = REV ? 3 : 0;                                   // the one with the fewest scores
+  __shared__ __attribute__((aligned(16))) T s_q[OUT ? kRun * TK::kLd : 8];     // what asks: q, or k mirrored
+  __shared__ __attribute__((aligned(16))) T s_k[kRun * TK::kLd];               // what adds to the state: k, or q
+  __shared__ __attribute__((aligned(16))) T s_v[kRun * TV::kLd];               // its values: v, or dy
+  __shared__ __attribute__((aligned(16))) T s_s[OUT ? kVBlock * TK::kLd : 8];  // the state as an operand, a value channel a row
   __shared__ Decays s_d[2];
   __shared__ float s_max[4], s_x[4];
   int lane = threadIdx.x & 63;
@@ -151,6 +151,12 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     for (int x = 1; x < 64; x *= 2) m = fmaxf(m, lane_xor(m, x));
     if (lane == 0) s_max[wave] = m;
   };
+  // mirrored: the product of both states of a run, once all waves have left their parts
+  const bool dot_wanted = OUT && REV && p.dot;
+  auto note_dot = [&](int64_t run, const Decays& d) {
+    const int64_t block = (bh * p.runs + run) * p.vblocks + vb;
+    if (threadIdx.x == 0) p.dot[block] = (s_x[0] + s_x[1] + s_x[2] + s_x[3]) * d.whole * (DT == MM_F16 ? p.factors_with[block] : 1.0f);
+  };
   double total = 0.0;   // the segment's log decay
   float factor = 1.0f;  // fp16: the state's power of two
   if (walk > 0) {
@@ -163,34 +169,13 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     asm volatile("" : "+v"(lane));
     const int64_t run = at_run, next = n + 1 < walk ? run + kWay : run;
     at_run = next;
+    __syncthreads();  // nobody reads the tiles of the run before
+    if constexpr (OUT && REV) {
+      if (dot_wanted && n > 0) note_dot(run - kWay, s_d[(n - 1) & 1]);
+    }
     if (OUT) rq.store(s_q);
     rk.store(s_k);
     rv.store(s_v);
-    __syncthreads();
-    const Decays& D = s_d[n & 1];
-    // what the state's product with the saved ones of the forward pass needs, before the next run's loads
-    constexpr int kSaved = OUT && REV ? ND : 1;
-    u32x2 saved2[kSaved];
-    f32x4 saved4[kSaved];
-    const bool dot_wanted = OUT && REV && p.dot;
-    if constexpr (OUT && REV) {
-      if (dot_wanted) {
-        const T* const before = run_state<T>(const_cast<void*>(p.dot_with), p, bh, run, vb, DKP);
-#pragma unroll
-        for (int t = 0; t < ND; ++t) {
-          if constexpr (O::kWide) saved4[t] = *reinterpret_cast<const f32x4*>(before + state_at<DT>(wave, t, ND, lane));
-          else saved2[t] = *reinterpret_cast<const u32x2*>(before + state_at<DT>(wave, t, ND, lane));
-        }
-      }
-    }
-    float g_next = 0.0f;
-    if (wave == kDecayWave) g_next = gate(next);
-    if (n + 1 < walk) fetch(rows_of(next));
-
-    u32x4 vo[NR];  // this wave's value columns, as operands over the run's tokens
-#pragma unroll
-    for (int u = 0; u < NR; ++u) vo[u] = TV::column(s_v, u * O::kStep, 16 * wave, lane);
-
     if constexpr (OUT) {
       if constexpr (DT == MM_F16) {
         // fp16 has 5 exponent bits: the state goes through a power of two that puts its largest element at 2^13
@@ -198,170 +183,139 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
         const int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
         factor = m > 0.0f && e < 128 ? __builtin_ldexpf(1.0f, e - 13 < -120 ? -120 : e - 13) : 1.0f;
       }
+      // (rounded to 16 bits: products of 16-bit operands, off by half a step each at random)
       const float shrink = DT == MM_F16 ? 1.0f / factor : 1.0f;
-      // the state as an operand (rounded to 16 bits: products of 16-bit operands, off by half a step each at random)
-      u32x4 so[NU];
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        f32x4 part[O::kTiles];
-#pragma unroll
-        for (int c = 0; c < O::kTiles; ++c) part[c] = DT == MM_F16 ? S[u * O::kTiles + c] * shrink : S[u * O::kTiles + c];
-        so[u] = from_acc<DT>(part);
+      for (int t = 0; t < ND; ++t) {
+        const f32x4 x = DT == MM_F16 ? S[t] * shrink : S[t];
+        T* const to = s_s + TK::at(16 * wave + i, 16 * t + 4 * g);
+        if constexpr (O::kWide) *reinterpret_cast<f32x4*>(to) = x;
+        else *reinterpret_cast<u32x2*>(to) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
       }
+    }
+    __syncthreads();
+    const Decays& D = s_d[n & 1];
+    const int64_t block = (bh * p.runs + run) * p.vblocks + vb;  // of the saved states
+    // what the state's product with the saved ones of the forward pass needs, before the next run's loads
+    constexpr int kSaved = OUT && REV ? ND : 1;
+    u32x2 saved2[kSaved];
+    f32x4 saved4[kSaved];
+    if constexpr (OUT && REV) {
+      if (dot_wanted) {
+        const T* const before = static_cast<const T*>(p.dot_with) + block * kVBlock * DKP + (16 * wave + i) * DKP + 4 * g;
+#pragma unroll
+        for (int t = 0; t < ND; ++t) {
+          if constexpr (O::kWide) saved4[t] = *reinterpret_cast<const f32x4*>(before + 16 * t);
+          else saved2[t] = *reinterpret_cast<const u32x2*>(before + 16 * t);
+        }
+      }
+    }
+    float g_next = 0.0f;
+    if (wave == kDecayWave) g_next = gate(next);
+    if (n + 1 < walk) fetch(rows_of(next));
+    // What this run adds to the state: this wave's value columns, as operands over the run's tokens.
+    if constexpr (OUT) {
       if (p.states) {
-        // for the backward pass: the 16 columns turned over, 64 key channels at a time, so that its operands over value
-        // channels are whole reads
-        T* const out = run_state<T>(p.states, p, bh, run, vb, DKP);
-        float dot = 0.0f;
-        auto turn_over = [&](const u32x4(&x)[NU], bool keep) __attribute__((always_inline)) {
+        T* const to = static_cast<T*>(p.states) + block * kVBlock * DKP;
+        constexpr int kUnits = DKP / O::kE;
 #pragma unroll
-          for (int h = 0; h < DKP / 64; ++h) {
-            wave_lds_fence();
-#pragma unroll
-            for (int c = 0; c < 64 / O::kStep; ++c) {
-              const u32x4 w = x[h * (64 / O::kStep) + c];
-              if constexpr (O::kWide) {
-                *reinterpret_cast<u32x4*>(s_p + TV::at(16 * wave + i, 16 * c + 4 * g)) = w;
-              } else {
-                *reinterpret_cast<u32x2*>(s_p + TV::at(16 * wave + i, 32 * c + 4 * g)) = u32x2{w[0], w[1]};
-                *reinterpret_cast<u32x2*>(s_p + TV::at(16 * wave + i, 32 * c + 16 + 4 * g)) = u32x2{w[2], w[3]};
-              }
-            }
-            wave_lds_fence();
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int t = 4 * h + c;
-              const int64_t at = state_at<DT>(wave, t, ND, lane);
-              if constexpr (O::kWide) {
-                const f32x4 v = __builtin_bit_cast(f32x4, TV::column(s_p, 16 * wave, 16 * c, lane));
-                if (keep) *reinterpret_cast<f32x4*>(out + at) = v;
-                if (REV && dot_wanted) {
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) dot += v[j] * saved4[REV ? t : 0][j];
-                }
-              } else {
-                const u32x2 v = TV::column4(s_p, 16 * wave, 16 * c, lane);
-                if (keep) *reinterpret_cast<u32x2*>(out + at) = v;
-                if (REV && dot_wanted) {
-#pragma unroll
-                  for (int j = 0; j < 2; ++j) {
-                    float a, b2, x2, y2;
-                    unpack2<DT>(v[j], a, b2);
-                    unpack2<DT>(saved2[REV ? t : 0][j], x2, y2);
-                    dot += a * x2 + b2 * y2;
-                  }
-                }
-              }
-            }
-          }
-        };
-        turn_over(so, true);
+        for (int s = 0; s < kVBlock * kUnits / 256; ++s) {
+          const int u = s * 256 + static_cast<int>(threadIdx.x), r = u / kUnits, e = u % kUnits * O::kE;
+          *reinterpret_cast<u32x4*>(to + r * DKP + e) = *reinterpret_cast<const u32x4*>(s_s + TK::at(r, e));
+        }
+        if (DT == MM_F16 && threadIdx.x == 0) p.factors[block] = factor;
+      }
+      if constexpr (REV) {
         if (dot_wanted) {
-          if constexpr (REV && !O::kWide) {
-            // what rounding the gradient's state left out, so that the sum has one rounded factor and not two
-            u32x4 rest[NU];
+          float dot = 0.0f;
 #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-              f32x4 part[2];
-#pragma unroll
-              for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                  float a, b2;
-                  unpack2<DT>(so[u][2 * c + r], a, b2);
-                  part[c][2 * r] = S[2 * u + c][2 * r] * shrink - a;
-                  part[c][2 * r + 1] = S[2 * u + c][2 * r + 1] * shrink - b2;
-                }
-              rest[u] = from_acc<DT>(part);
+          for (int t = 0; t < ND; ++t) {
+            f32x4 x;
+            if constexpr (O::kWide) {
+              x = saved4[t];
+            } else {
+              float a[4];
+              unpack2<DT>(saved2[t][0], a[0], a[1]);
+              unpack2<DT>(saved2[t][1], a[2], a[3]);
+              x = f32x4{a[0], a[1], a[2], a[3]};
             }
-            turn_over(rest, false);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dot += x[r] * S[t][r];
           }
 #pragma unroll
           for (int x = 1; x < 64; x *= 2) dot += lane_xor(dot, x);
           if (lane == 0) s_x[wave] = dot;
         }
-        if (DT == MM_F16 && threadIdx.x == 0) p.factors[(bh * p.runs + run) * p.vblocks + vb] = factor;
-        wave_lds_fence();
       }
-      // scores of row block `wave`: tiles of (what adds) x (what asks), whose accumulators are rows of p
-      {
-        f32x4 acc[4];
+      // Token block `wave` of the run: its scores, as accumulators (what adds) x (what asks) that are at once operands of
+      // their product with the values.
+      u32x4 own[NU];
 #pragma unroll
-        for (int st = 0; st < 4; ++st) acc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-          const u32x4 own = TK::row(s_q, 16 * wave, u * O::kStep, lane);
-#pragma unroll
-          for (int st = 0; st < 4; ++st)
-            if (REV ? st >= wave : st <= wave) acc[st] = mma<DT>(TK::row(s_k, 16 * st, u * O::kStep, lane), own, acc[st]);
-        }
-        const float hi_r = D.hi[16 * wave + i], lo_r = D.lo[16 * wave + i];
-#pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          T* const at = s_p + TV::at(16 * wave + i, 16 * st + 4 * g);
-          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          if (REV ? st >= wave : st <= wave) {
-            const f32x4 hi = *reinterpret_cast<const f32x4*>(D.hi + 16 * st + 4 * g);
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(D.lo + 16 * st + 4 * g);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float decay = REV ? between<DT>(hi[r], lo[r], hi_r, lo_r) : between<DT>(hi_r, lo_r, hi[r], lo[r]);
-              const float x = acc[st][r] * p.scale * decay;
-              v[r] = st != wave || (REV ? 4 * g + r >= i : 4 * g + r <= i) ? x : 0.0f;
-            }
-          }
-          // (tiles beyond the diagonal: zeros, for the steps of a product that take two tiles at once)
-          if constexpr (O::kWide) *reinterpret_cast<f32x4*>(at) = f32x4{v[0], v[1], v[2], v[3]};
-          else *reinterpret_cast<u32x2*>(at) = u32x2{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
-        }
-      }
-      if (wave == kDecayWave) run_decays(s_d[(n + 1) & 1], g_next, lane);
-      __syncthreads();
-      if (REV && dot_wanted && threadIdx.x == 0)
-        p.dot[(bh * p.runs + run) * p.vblocks + vb] = (s_x[0] + s_x[1] + s_x[2] + s_x[3]) * D.whole * factor *
-                                                      (DT == MM_F16 ? p.factors_with[(bh * p.runs + run) * p.vblocks + vb] : 1.0f);
-      // outputs, turned over: 4 value channels of a token in a lane
+      for (int u = 0; u < NU; ++u) own[u] = TK::row(s_q, 16 * wave, u * O::kStep, lane);
       f32x4 acc[4];
 #pragma unroll
-      for (int rt = 0; rt < 4; ++rt) acc[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int st = 0; st < 4; ++st) {
+        acc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (REV ? st < wave : st > wave) continue;
+#pragma unroll
+        for (int u = 0; u < NU; ++u) acc[st] = mma<DT>(TK::row(s_k, 16 * st, u * O::kStep, lane), own[u], acc[st]);
+      }
+      const float hi_r = D.hi[16 * wave + i], lo_r = D.lo[16 * wave + i];
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        if (REV ? st < wave : st > wave) continue;
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(D.hi + 16 * st + 4 * g);
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(D.lo + 16 * st + 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float decay = REV ? between<DT>(hi[r], lo[r], hi_r, lo_r) : between<DT>(hi_r, lo_r, hi[r], lo[r]);
+          const float x = acc[st][r] * p.scale * decay;
+          acc[st][r] = st != wave || (REV ? 4 * g + r >= i : 4 * g + r <= i) ? x : 0.0f;
+        }
+      }
+      u32x4 po[NR];
+#pragma unroll
+      for (int u = 0; u < NR; ++u) po[u] = from_acc<DT>(acc + u * O::kTiles);
+      // outputs, turned over: 4 value channels of a token in a lane
+      f32x4 y[4];
+#pragma unroll
+      for (int vt = 0; vt < 4; ++vt) y[vt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int rt = 0; rt < 4; ++rt) acc[rt] = mma<DT>(so[u], TK::row_acc(s_q, 16 * rt, u * O::kStep, lane), acc[rt]);
-      const float qs = (REV ? 1.0f : p.scale) * factor;
+        for (int vt = 0; vt < 4; ++vt) y[vt] = mma<DT>(TK::row(s_s, 16 * vt, u * O::kStep, lane), own[u], y[vt]);
+      const float ws = (REV ? D.onward : D.into)[16 * wave + i] * ((REV ? 1.0f : p.scale) * factor);
 #pragma unroll
-      for (int rt = 0; rt < 4; ++rt) acc[rt] *= (REV ? D.onward : D.into)[16 * rt + i] * qs;
+      for (int vt = 0; vt < 4; ++vt) y[vt] *= ws;
 #pragma unroll
-      for (int u = 0; u < NR; ++u)
+      for (int u = 0; u < NR; ++u) {
+        if (REV ? (u + 1) * O::kStep <= 16 * wave : u * O::kStep > 16 * wave + 15) continue;
 #pragma unroll
-        for (int rt = 0; rt < 4; ++rt) {
-          if (REV ? (u + 1) * O::kStep <= 16 * rt : u * O::kStep > 16 * rt + 15) continue;
-          acc[rt] = mma<DT>(vo[u], TV::row_acc(s_p, 16 * rt, u * O::kStep, lane), acc[rt]);
-        }
-      const int rows = rows_of(run), left = static_cast<int>(p.seqlen - run * kRun < kRun ? p.seqlen - run * kRun : kRun);
-      const int v0 = 16 * wave + 4 * g;
+        for (int vt = 0; vt < 4; ++vt) y[vt] = mma<DT>(TV::column(s_v, u * O::kStep, 16 * vt, lane), po[u], y[vt]);
+      }
+      const int left = static_cast<int>(p.seqlen - run * kRun < kRun ? p.seqlen - run * kRun : kRun), t = 16 * wave + i;
+      if (t < left) {
+        T* const to = yp + t * p.heads * p.dv + 4 * g;
+        const bool in = t < rows_of(run);
 #pragma unroll
-      for (int rt = 0; rt < 4; ++rt) {
-        const int t = 16 * rt + i;
-        if (t >= rows) acc[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (t >= left) continue;
-        T* const y = yp + t * p.heads * p.dv + v0;
-        if constexpr (VEC) {
-          if (v0 < vw) {
-            if constexpr (O::kWide) *reinterpret_cast<f32x4*>(y) = acc[rt];
-            else *reinterpret_cast<u32x2*>(y) = u32x2{pack2<DT>(acc[rt][0], acc[rt][1]), pack2<DT>(acc[rt][2], acc[rt][3])};
+        for (int vt = 0; vt < 4; ++vt) {
+          if (!in) y[vt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          if constexpr (VEC) {
+            if (16 * vt + 4 * g < vw) {
+              if constexpr (O::kWide) *reinterpret_cast<f32x4*>(to + 16 * vt) = y[vt];
+              else *reinterpret_cast<u32x2*>(to + 16 * vt) = u32x2{pack2<DT>(y[vt][0], y[vt][1]), pack2<DT>(y[vt][2], y[vt][3])};
+            }
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (16 * vt + 4 * g + r < vw) to[16 * vt + r] = Ty<DT>::from(y[vt][r]);
           }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (v0 + r < vw) y[r] = Ty<DT>::from(acc[rt][r]);
         }
       }
       yp += kWay * kRun * p.heads * p.dv;
-    } else if (wave == kDecayWave) {
-      run_decays(s_d[(n + 1) & 1], g_next, lane);
     }
-    // the state's step
+    if (wave == kDecayWave) run_decays(s_d[(n + 1) & 1], g_next, lane);
+    // the state's step: this wave's value columns, weighted, as operands over the run's tokens
     const float whole = D.whole;
 #pragma unroll
     for (int t = 0; t < ND; ++t) S[t] *= whole;
@@ -369,16 +323,17 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     const float ws = REV ? p.scale : 1.0f;
 #pragma unroll
     for (int u = 0; u < NR; ++u) {
+      const u32x4 vo = TV::column(s_v, u * O::kStep, 16 * wave, lane);
       u32x4 terms[TERMS];
       if constexpr (O::kWide) {
         const f32x4 w = *reinterpret_cast<const f32x4*>(weight + 16 * u + 4 * g) * ws;
-        terms[0] = __builtin_bit_cast(u32x4, __builtin_bit_cast(f32x4, vo[u]) * w);
+        terms[0] = __builtin_bit_cast(u32x4, __builtin_bit_cast(f32x4, vo) * w);
       } else {
         const f32x4 w0 = *reinterpret_cast<const f32x4*>(weight + 32 * u + 4 * g) * ws;
         const f32x4 w1 = *reinterpret_cast<const f32x4*>(weight + 32 * u + 16 + 4 * g) * ws;
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) unpack2<DT>(vo[u][j], x[2 * j], x[2 * j + 1]);
+        for (int j = 0; j < 4; ++j) unpack2<DT>(vo[j], x[2 * j], x[2 * j + 1]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           x[j] *= w0[j];
@@ -407,7 +362,12 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     }
     if (DT == MM_F16 && OUT) note_max();
     if (!OUT) total += static_cast<double>(D.hi[63]) + D.lo[63];
-    __syncthreads();
+  }
+  if constexpr (OUT && REV) {
+    if (walk > 0 && dot_wanted) {
+      __syncthreads();
+      note_dot(run0, s_d[(walk - 1) & 1]);
+    }
   }
 
   if constexpr (OUT) {

@@ -146,16 +146,15 @@ struct Staged {
   // Rows r >= rows and elements >= width come as zeros.  16-byte aligned rows that 16 bytes divide, 64 of them within
   // 4 GB: `first` is the first row's (wave-uniform) address, `off` row() and elem() in bytes, `step` kRows rows in bytes.
   __device__ __forceinline__ void load(const char* first, uint32_t off, int64_t step, int rows, int width) {
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) v[s] = u32x4{0, 0, 0, 0};
-    if (elem() >= width) return;
-    if (rows == kRun) {
+    if (rows == kRun && width == W) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s, first += step) v[s] = *reinterpret_cast<const u32x4*>(first + off);
-    } else {
+      return;
+    }
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s, first += step)
-        if (s * kRows + row() < rows) v[s] = *reinterpret_cast<const u32x4*>(first + off);
+    for (int s = 0; s < kSteps; ++s, first += step) {
+      v[s] = u32x4{0, 0, 0, 0};
+      if (s * kRows + row() < rows && elem() < width) v[s] = *reinterpret_cast<const u32x4*>(first + off);
     }
   }
   // Any rows.
