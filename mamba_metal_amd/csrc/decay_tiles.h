@@ -83,15 +83,16 @@ __device__ __forceinline__ u32x4 from_acc(const f32x4* t) {
 }
 
 // A tile of W columns in shared memory.  16-bit rows are cut into chunks of 16 bytes, and chunk c of row r is kept at
-// place c ^ turn(r), such that the 16 rows that a row read touches, and the pairs of chunks of the 8 rows that a
-// transposing read touches, lie in different banks.  (fp32: rows 4 words longer do the same.)
+// place c ^ turn(r), without bank conflicts: a transposing read touches pairs of chunks of 8 rows, whose turns differ above
+// the lowest bit; a 16-byte row read goes in four parts of 16 lanes, 0-3, 12-15 and 20-27 and so on, so that rows 4 to 11 of
+// one chunk and the other rows of its neighbour meet, and those have both turns of each pair.  (fp32: rows 4 words longer.)
 template <int DT, int W>
 struct Tile {
   using T = typename Ty<DT>::T;
   static constexpr bool kWide = Op<DT>::kWide;
   static constexpr int kLd = kWide ? W + 4 : W;
   static __device__ __forceinline__ int turn(int r) {
-    return W == 128 ? (r & 7) << 1 | (r >> 3 & 1) : (r >> 1 & 3) << 1 | (r >> 3 & 1);
+    return W == 128 ? ((r & 7) ^ (r >> 1 & 4)) << 1 | (r >> 3 & 1) : ((r >> 1 & 3) ^ (r >> 2 & 2)) << 1 | (r >> 3 & 1);
   }
   static __device__ __forceinline__ int at(int r, int e) {
     return kWide ? r * kLd + e : r * kLd + (((e >> 3) ^ turn(r)) << 3) + (e & 7);
