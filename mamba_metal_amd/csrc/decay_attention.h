@@ -63,9 +63,16 @@ __device__ __forceinline__ int64_t length_of(const P& p, int64_t b) {
   const int64_t n = p.lengths_dtype ? static_cast<const int64_t*>(p.lengths)[b] : static_cast<const int32_t*>(p.lengths)[b];
   return n < 0 ? 0 : n < p.seqlen ? n : p.seqlen;
 }
+// A log decay: the load, and what it stands for, apart, so that the load's time can pass between them.
 template <typename P>
-__device__ __forceinline__ float load_gate(const P& p, int64_t at) {
-  return p.g_dtype == MM_F32 ? ld<MM_F32>(p.g, at) : p.g_dtype == MM_F16 ? ld<MM_F16>(p.g, at) : ld<MM_BF16>(p.g, at);
+__device__ __forceinline__ uint32_t load_gate(const P& p, int64_t at) {
+  return p.g_dtype == MM_F32 ? static_cast<const uint32_t*>(p.g)[at] : static_cast<const uint16_t*>(p.g)[at];
+}
+template <typename P>
+__device__ __forceinline__ float gate_value(const P& p, uint32_t raw) {
+  return p.g_dtype == MM_F32   ? __uint_as_float(raw)
+         : p.g_dtype == MM_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(raw)))
+                               : __uint_as_float(raw << 16);
 }
 // A run's saved state of one value block: 64 value channels (rows) by DKP key channels, (bh, run, value block) contiguous.
 typedef float seg_f32x4 __attribute__((ext_vector_type(4)));

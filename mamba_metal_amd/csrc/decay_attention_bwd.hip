@@ -130,7 +130,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       }
     };
     auto gate = [&](int h) {
-      return lane < rows ? load_gate(p, b * p.g_stride[0] + (t0 + lane) * p.g_stride[1] + (group * p.per + h) * p.g_stride[2]) : 0.0f;
+      return lane < rows ? load_gate(p, b * p.g_stride[0] + (t0 + lane) * p.g_stride[1] + (group * p.per + h) * p.g_stride[2]) : 0u;
     };
     // dg of a head whose parts all waves have left
     auto finish_dg = [&](int h) __attribute__((always_inline)) {
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       }
       __syncthreads();
       if (more) fetch(other, h_next, vb_next);
-      float g_next = 0.0f;
+      uint32_t g_next = 0;
       const bool decays_now = wave == 7 && last_block && h + 1 < h1;
       if (decays_now) g_next = gate(h + 1);
       if (p.dg && wave == 0 && vb == 0 && h > h0) finish_dg(h - 1);
@@ -256,9 +256,9 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         }
         if (i == 0) *reinterpret_cast<f32x4*>(&s_inter[(h - h0) & 1][role][16 * blk + 4 * g]) = inter;
       }
-      if (decays_now) run_decays(s_d[(h + 1 - h0) & 1], g_next, lane);
+      if (decays_now) run_decays(s_d[(h + 1 - h0) & 1], gate_value(p, g_next), lane);
     };
-    if (wave == 7) run_decays(s_d[0], gate(h0), lane);
+    if (wave == 7) run_decays(s_d[0], gate_value(p, gate(h0)), lane);
     fetch(s_b0, h0, 0);
     const int steps = (h1 - h0) * p.vblocks;
     int h = h0, vb = 0;

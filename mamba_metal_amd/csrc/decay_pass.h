@@ -123,22 +123,25 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
   const uint32_t v_off = static_cast<uint32_t>((rv.row() * p.v_stride[1] + rv.elem()) * kEs);
   constexpr int kWay = REV ? -1 : 1;
   auto rows_of = [&](int64_t run) { return static_cast<int>(len - run * kRun < kRun ? len - run * kRun : kRun); };
-  auto fetch = [&](int rows) __attribute__((always_inline)) {
-    if constexpr (VEC) {
-      if (OUT) rq.load(qp, q_off, rq.kRows * p.q_stride[1] * kEs, rows, dk);
-      rk.load(kp, k_off, rk.kRows * p.k_stride[1] * kEs, rows, dk);
-      rv.load(vp, v_off, rv.kRows * p.v_stride[1] * kEs, rows, vw);
-    } else {
-      if (OUT) rq.load_any(qp, p.q_stride[1], rows, dk);
-      rk.load_any(kp, p.k_stride[1], rows, dk);
-      rv.load_any(vp, p.v_stride[1], rows, vw);
-    }
-    if (OUT) qp += kWay * kRun * p.q_stride[1] * kEs;
+  // Three parts, spread over a run's computation: issued at once they would wait for each other's way into the cache
+  // (2400 of a run's 12000 cycles).
+  auto fetch_k = [&](int rows) __attribute__((always_inline)) {
+    if constexpr (VEC) rk.load(kp, k_off, rk.kRows * p.k_stride[1] * kEs, rows, dk);
+    else rk.load_any(kp, p.k_stride[1], rows, dk);
     kp += kWay * kRun * p.k_stride[1] * kEs;
+  };
+  auto fetch_v = [&](int rows) __attribute__((always_inline)) {
+    if constexpr (VEC) rv.load(vp, v_off, rv.kRows * p.v_stride[1] * kEs, rows, vw);
+    else rv.load_any(vp, p.v_stride[1], rows, vw);
     vp += kWay * kRun * p.v_stride[1] * kEs;
   };
+  auto fetch_q = [&](int rows) __attribute__((always_inline)) {
+    if constexpr (VEC) rq.load(qp, q_off, rq.kRows * p.q_stride[1] * kEs, rows, dk);
+    else rq.load_any(qp, p.q_stride[1], rows, dk);
+    qp += kWay * kRun * p.q_stride[1] * kEs;
+  };
   auto gate = [&](int64_t run) {
-    return lane < rows_of(run) ? load_gate(p, gh + (run * kRun + lane) * p.g_stride[1]) : 0.0f;
+    return lane < rows_of(run) ? load_gate(p, gh + (run * kRun + lane) * p.g_stride[1]) : 0u;
   };
   // fp16: the largest magnitude of the wave's columns
   auto note_max = [&]() __attribute__((always_inline)) {
@@ -160,9 +163,11 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
   double total = 0.0;   // the segment's log decay
   float factor = 1.0f;  // fp16: the state's power of two
   if (walk > 0) {
-    fetch(rows_of(at_run));
+    fetch_k(rows_of(at_run));
+    fetch_v(rows_of(at_run));
+    if (OUT) fetch_q(rows_of(at_run));
     if (DT == MM_F16 && OUT) note_max();
-    if (wave == kDecayWave) run_decays(s_d[0], gate(at_run), lane);
+    if (wave == kDecayWave) run_decays(s_d[0], gate_value(p, gate(at_run)), lane);
   }
   for (int64_t n = 0; n < walk; ++n) {
     // addresses in shared memory are made anew in every run: held over it they would be dozens of registers
@@ -210,9 +215,10 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
         }
       }
     }
-    float g_next = 0.0f;
+    uint32_t g_next = 0;
     if (wave == kDecayWave) g_next = gate(next);
-    if (n + 1 < walk) fetch(rows_of(next));
+    if (n + 1 < walk) fetch_v(rows_of(next));
+    if (!OUT && n + 1 < walk) fetch_k(rows_of(next));
     // What this run adds to the state: this wave's value columns, as operands over the run's tokens.
     if constexpr (OUT) {
       if (p.states) {
@@ -260,6 +266,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
 #pragma unroll
         for (int u = 0; u < NU; ++u) acc[st] = mma<DT>(TK::row(s_k, 16 * st, u * O::kStep, lane), own[u], acc[st]);
       }
+      if (n + 1 < walk) fetch_k(rows_of(next));
       const float hi_r = D.hi[16 * wave + i], lo_r = D.lo[16 * wave + i];
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
@@ -284,6 +291,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
       for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int vt = 0; vt < 4; ++vt) y[vt] = mma<DT>(TK::row(s_s, 16 * vt, u * O::kStep, lane), own[u], y[vt]);
+      if (n + 1 < walk) fetch_q(rows_of(next));
       const float ws = (REV ? D.onward : D.into)[16 * wave + i] * ((REV ? 1.0f : p.scale) * factor);
 #pragma unroll
       for (int vt = 0; vt < 4; ++vt) y[vt] *= ws;
@@ -314,7 +322,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
       }
       yp += kWay * kRun * p.heads * p.dv;
     }
-    if (wave == kDecayWave) run_decays(s_d[(n + 1) & 1], g_next, lane);
+    if (wave == kDecayWave) run_decays(s_d[(n + 1) & 1], gate_value(p, g_next), lane);
     // the state's step: this wave's value columns, weighted, as operands over the run's tokens
     const float whole = D.whole;
 #pragma unroll

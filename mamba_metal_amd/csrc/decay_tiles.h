@@ -229,8 +229,5 @@ __device__ __forceinline__ float between(float hi_t, float lo_t, float hi_s, flo
   return DT == MM_F32 && x != x ? x : e;  // (exp2_acc's clamp would lose a NaN)
 }
 
-template <int GT>
-__device__ __forceinline__ float load_g(const void* g, int64_t i) { return ld<GT>(g, i); }
-
 }  // namespace dattn
 }  // namespace mm
