@@ -132,16 +132,27 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
     auto gate = [&](int h) {
       return lane < rows ? load_gate(p, b * p.g_stride[0] + (t0 + lane) * p.g_stride[1] + (group * p.per + h) * p.g_stride[2]) : 0u;
     };
+    // what the head needs of its states' product and (fp16) powers of two, a step ahead
+    auto dot_of = [&](int h) {
+      float dot = 0.0f;
+      for (int vb = 0; vb < p.vblocks; ++vb) dot += p.dot[((b * p.heads + group * p.per + h) * p.runs + run) * p.vblocks + vb];
+      return dot;
+    };
+    auto factor_of = [&](int h, int vb) {
+      return (role ? p.dfactors : p.factors)[((b * p.heads + group * p.per + h) * p.runs + run) * p.vblocks + vb];
+    };
+    float dot_here = 0.0f, dot_before = 0.0f, factor_here = 1.0f;
+    if (p.dg && wave == 0) dot_here = dot_of(h0);
+    if (DT == MM_F16) factor_here = factor_of(h0, 0);
     // dg of a head whose parts all waves have left
-    auto finish_dg = [&](int h) __attribute__((always_inline)) {
+    auto finish_dg = [&](int h, float dot) __attribute__((always_inline)) {
       const int64_t head = group * p.per + h;
       const float* const sum = &s_sum[(h - h0) & 1][0][0];
       const float* const inter = &s_inter[(h - h0) & 1][0][0];
       const double u = static_cast<double>(sum[lane]) - sum[kRun + lane] + inter[lane];
       const double kv = inter[kRun + lane];
       const double up = prefix_sum(u), all = __shfl(up, 63, 64);
-      double dg = all - up + u + prefix_sum(kv) - kv;
-      for (int vb = 0; vb < p.vblocks; ++vb) dg += p.dot[((b * p.heads + head) * p.runs + run) * p.vblocks + vb];
+      const double dg = all - up + u + prefix_sum(kv) - kv + dot;
       if (lane < rows) p.dg[(b * p.seqlen + t0 + lane) * p.heads + head] = static_cast<float>(dg);
     };
 
@@ -162,7 +173,14 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       uint32_t g_next = 0;
       const bool decays_now = wave == 7 && last_block && h + 1 < h1;
       if (decays_now) g_next = gate(h + 1);
-      if (p.dg && wave == 0 && vb == 0 && h > h0) finish_dg(h - 1);
+      float factor_next = 1.0f;
+      if (DT == MM_F16 && more) factor_next = factor_of(h_next, vb_next);
+      if (p.dg && wave == 0 && vb == 0) {
+        const float dot_next = h + 1 < h1 ? dot_of(h + 1) : 0.0f;
+        if (h > h0) finish_dg(h - 1, dot_before);
+        dot_before = dot_here;
+        dot_here = dot_next;
+      }
       const Decays& D = s_d[(h - h0) & 1];
       if (vb == 0) {
 #pragma unroll
@@ -197,10 +215,10 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         for (int ot = 0; ot < 4; ++ot)
           if (role ? ot >= blk : ot <= blk) acc[ot] = mma<DT>(TV::row_acc(other_t, 16 * ot, u * O::kStep, lane), own[u], acc[ot]);
       if constexpr (DT == MM_F16) {
-        const float f = (role ? p.dfactors : p.factors)[(bh * p.runs + run) * p.vblocks + vb];
 #pragma unroll
-        for (int t = 0; t < ND; ++t) tmp[t] *= factor / f;
-        factor = f;
+        for (int t = 0; t < ND; ++t) tmp[t] *= factor / factor_here;
+        factor = factor_here;
+        factor_here = factor_next;
       }
 #pragma unroll
       for (int u = 0; u < NU; ++u)
@@ -284,7 +302,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       }
     }
     __syncthreads();
-    if (p.dg && wave == 0) finish_dg(h1 - 1);
+    if (p.dg && wave == 0) finish_dg(h1 - 1, dot_before);
   }
   if (p.dg && wave == 0 && lane >= rows && t0 + lane < p.seqlen)
     for (int h = h0; h < h1; ++h) p.dg[(b * p.seqlen + t0 + lane) * p.heads + group * p.per + h] = 0.0f;

@@ -219,18 +219,20 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     if (wave == kDecayWave) g_next = gate(next);
     if (n + 1 < walk) fetch_v(rows_of(next));
     if (!OUT && n + 1 < walk) fetch_k(rows_of(next));
-    // What this run adds to the state: this wave's value columns, as operands over the run's tokens.
-    if constexpr (OUT) {
-      if (p.states) {
-        T* const to = static_cast<T*>(p.states) + block * kVBlock * DKP;
-        constexpr int kUnits = DKP / O::kE;
+    // The state kept for the backward pass, a quarter at a time, for the same reason as the loads.
+    auto keep_state = [&](int quarter) __attribute__((always_inline)) {
+      if (!OUT || !p.states) return;
+      T* const to = static_cast<T*>(p.states) + block * kVBlock * DKP;
+      constexpr int kUnits = DKP / O::kE, kEach = kVBlock * kUnits / 256 / 4 > 0 ? kVBlock * kUnits / 256 / 4 : 1;
+      if (quarter >= kVBlock * kUnits / 256) return;
 #pragma unroll
-        for (int s = 0; s < kVBlock * kUnits / 256; ++s) {
-          const int u = s * 256 + static_cast<int>(threadIdx.x), r = u / kUnits, e = u % kUnits * O::kE;
-          *reinterpret_cast<u32x4*>(to + r * DKP + e) = *reinterpret_cast<const u32x4*>(s_s + TK::at(r, e));
-        }
-        if (DT == MM_F16 && threadIdx.x == 0) p.factors[block] = factor;
+      for (int s = 0; s < kEach; ++s) {
+        const int u = (quarter * kEach + s) * 256 + static_cast<int>(threadIdx.x), r = u / kUnits, e = u % kUnits * O::kE;
+        *reinterpret_cast<u32x4*>(to + r * DKP + e) = *reinterpret_cast<const u32x4*>(s_s + TK::at(r, e));
       }
+      if (DT == MM_F16 && quarter == 0 && threadIdx.x == 0) p.factors[block] = factor;
+    };
+    if constexpr (OUT) {
       if constexpr (REV) {
         if (dot_wanted) {
           float dot = 0.0f;
@@ -267,6 +269,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
         for (int u = 0; u < NU; ++u) acc[st] = mma<DT>(TK::row(s_k, 16 * st, u * O::kStep, lane), own[u], acc[st]);
       }
       if (n + 1 < walk) fetch_k(rows_of(next));
+      keep_state(0);
       const float hi_r = D.hi[16 * wave + i], lo_r = D.lo[16 * wave + i];
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
@@ -283,6 +286,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
       u32x4 po[NR];
 #pragma unroll
       for (int u = 0; u < NR; ++u) po[u] = from_acc<DT>(acc + u * O::kTiles);
+      keep_state(1);
       // outputs, turned over: 4 value channels of a token in a lane
       f32x4 y[4];
 #pragma unroll
@@ -292,6 +296,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
 #pragma unroll
         for (int vt = 0; vt < 4; ++vt) y[vt] = mma<DT>(TK::row(s_s, 16 * vt, u * O::kStep, lane), own[u], y[vt]);
       if (n + 1 < walk) fetch_q(rows_of(next));
+      keep_state(2);
       const float ws = (REV ? D.onward : D.into)[16 * wave + i] * ((REV ? 1.0f : p.scale) * factor);
 #pragma unroll
       for (int vt = 0; vt < 4; ++vt) y[vt] *= ws;
@@ -331,6 +336,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     const float ws = REV ? p.scale : 1.0f;
 #pragma unroll
     for (int u = 0; u < NR; ++u) {
+      if (u == NR - 1) keep_state(3);
       const u32x4 vo = TV::column(s_v, u * O::kStep, 16 * wave, lane);
       u32x4 terms[TERMS];
       if constexpr (O::kWide) {
