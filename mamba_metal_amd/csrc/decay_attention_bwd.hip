@@ -27,7 +27,7 @@ __device__ __forceinline__ void load_direct(const char* from, char* to) {
                                    (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
-template <int DT, int DKP, bool DIRECT>
+template <int DT, int DKP, bool DIRECT, bool ONE>
 __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
   using T = typename Ty<DT>::T;
   using O = Op<DT>;
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
   const int64_t len = length_of(p, b), t0 = run * kRun;
   const int rows = static_cast<int>(len - t0 < 0 ? 0 : len - t0 < kRun ? len - t0 : kRun);
   const int h0 = set * p.set_heads, h1 = h0 + p.set_heads < p.per ? h0 + p.set_heads : static_cast<int>(p.per);
-  const int dk = static_cast<int>(p.dk);
+  const int dk = static_cast<int>(p.dk), vblocks = ONE ? 1 : p.vblocks;
 
   f32x4 out[ND];
 #pragma unroll
@@ -90,10 +90,30 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         A[ot] = mma<DT>(TK::row(s_other, 16 * ot, u * O::kStep, lane), TK::row(s_own, 16 * blk, u * O::kStep, lane), A[ot]);
     }
 
+    // the own rows of q (or k) as the accumulators of the states' parts hold them (fp32: too many registers)
+    uint32_t held[ND][2];
+    if (p.dg && !O::kWide) {
+#pragma unroll
+      for (int t = 0; t < ND; ++t) {
+        T e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[r] = s_own[TK::at(16 * blk + 4 * g + r, 16 * t + i)];
+        __builtin_memcpy(held[t], e, 8);
+      }
+    }
+
     // A step is a head's block of value channels.
     const char* const dy0 = static_cast<const char*>(p.dy) + (b * p.dy_stride[0] + t0 * p.dy_stride[1]) * kEs;
     const char* const v0 = static_cast<const char*>(p.v) + (b * p.v_stride[0] + t0 * p.v_stride[1]) * kEs;
     Staged<DT, kVBlock, 512> ry, rv;
+    // Where a lane's direct loads come from.  A state's row of DKP channels is DKP / 8 chunks of 16 bytes, and place c of it
+    // holds chunk c ^ turn(row) (the 8 KB that the waves load at once are whole multiples of 16 rows, so that it is the same
+    // for all); a row of 64 value channels is 8 chunks.
+    const int unit = wave * 64 + lane;
+    const uint32_t state_off = static_cast<uint32_t>(unit / (DKP / 8) * DKP * 2 + (unit % (DKP / 8) ^ TK::turn(unit / (DKP / 8))) * 16);
+    const int row_here = unit / 8, chunk_here = unit % 8 ^ TV::turn(unit / 8);
+    const uint32_t dy_off = static_cast<uint32_t>(row_here * p.dy_stride[1] * kEs) + chunk_here * 16;
+    const uint32_t v_off = static_cast<uint32_t>(row_here * p.v_stride[1] * kEs) + chunk_here * 16;
     auto fetch = [&](T* buf, int h, int vb) __attribute__((always_inline)) {
       const int64_t head = group * p.per + h;
       const int vw = static_cast<int>(p.dv - vb * kVBlock < kVBlock ? p.dv - vb * kVBlock : kVBlock);
@@ -102,23 +122,24 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       if constexpr (DIRECT) {
         char* const to = reinterpret_cast<char*>(buf);
         constexpr int kBytes = kState * static_cast<int>(kEs);
-        const int64_t block = ((b * p.heads + head) * p.runs + run) * p.vblocks + vb;
+        const int64_t block = ((b * p.heads + head) * p.runs + run) * vblocks + vb;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
           const char* const from = static_cast<const char*>(which ? p.dstates : p.states) + block * kBytes;
 #pragma unroll
-          for (int q = 0; q < kBytes / 8192; ++q) {
-            // a row of DKP channels is DKP / 8 chunks, and place c of it holds chunk c ^ turn(row)
-            const int at = (q * 8 + wave) * 1024, unit = at / 16 + lane, r = unit / (DKP / 8), c = unit % (DKP / 8) ^ TK::turn(r);
-            load_direct(from + r * (DKP * 2) + c * 16, to + which * kBytes + at);
-          }
+          for (int q = 0; q < kBytes / 8192; ++q) load_direct(from + q * 8192 + state_off, to + which * kBytes + (q * 8 + wave) * 1024);
         }
-        // a row of 64 channels is 8 chunks; place lane % 8 of it holds chunk place ^ turn(row)
-        const int r = wave * 8 + (lane >> 3), c = (lane & 7) ^ TV::turn(r);
-        const bool in = r < rows && c * 8 < vw;
-        const char* const zeros = reinterpret_cast<const char*>(kZeros);
-        load_direct(in ? dy + r * p.dy_stride[1] * kEs + c * 16 : zeros, to + 2 * kBytes + wave * 1024);
-        load_direct(in ? v + r * p.v_stride[1] * kEs + c * 16 : zeros, to + 2 * kBytes + kRows * kEs + wave * 1024);
+        char* const dy_to = to + 2 * kBytes + wave * 1024;
+        char* const v_to = dy_to + kRows * kEs;
+        if (rows == kRun && vw == kVBlock) {
+          load_direct(dy + dy_off, dy_to);
+          load_direct(v + v_off, v_to);
+        } else {
+          const bool in = row_here < rows && chunk_here * 8 < vw;
+          const char* const zeros = reinterpret_cast<const char*>(kZeros);
+          load_direct(in ? dy + dy_off : zeros, dy_to);
+          load_direct(in ? v + v_off : zeros, v_to);
+        }
       } else {
         if (p.vec) {
           ry.load(dy, static_cast<uint32_t>((ry.row() * p.dy_stride[1] + ry.elem()) * kEs), ry.kRows * p.dy_stride[1] * kEs, rows, vw);
@@ -135,11 +156,11 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
     // what the head needs of its states' product and (fp16) powers of two, a step ahead
     auto dot_of = [&](int h) {
       float dot = 0.0f;
-      for (int vb = 0; vb < p.vblocks; ++vb) dot += p.dot[((b * p.heads + group * p.per + h) * p.runs + run) * p.vblocks + vb];
+      for (int vb = 0; vb < vblocks; ++vb) dot += p.dot[((b * p.heads + group * p.per + h) * p.runs + run) * vblocks + vb];
       return dot;
     };
     auto factor_of = [&](int h, int vb) {
-      return (role ? p.dfactors : p.factors)[((b * p.heads + group * p.per + h) * p.runs + run) * p.vblocks + vb];
+      return (role ? p.dfactors : p.factors)[((b * p.heads + group * p.per + h) * p.runs + run) * vblocks + vb];
     };
     float dot_here = 0.0f, dot_before = 0.0f, factor_here = 1.0f;
     if (p.dg && wave == 0) dot_here = dot_of(h0);
@@ -161,7 +182,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
     auto step = [&](T* cur, T* other, int h, int vb) __attribute__((always_inline)) {
       asm volatile("" : "+v"(lane));
       const int64_t head = group * p.per + h, bh = b * p.heads + head;
-      const bool last_block = vb + 1 == p.vblocks, more = !last_block || h + 1 < h1;
+      const bool last_block = vb + 1 == vblocks, more = !last_block || h + 1 < h1;
       const int h_next = last_block ? h + 1 : h, vb_next = last_block ? 0 : vb + 1;
       if constexpr (!DIRECT) {
         __syncthreads();
@@ -182,7 +203,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         dot_here = dot_next;
       }
       const Decays& D = s_d[(h - h0) & 1];
-      if (vb == 0) {
+      if (ONE || vb == 0) {
 #pragma unroll
         for (int ot = 0; ot < 4; ++ot) acc[ot] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -192,7 +213,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       const T* const own_t = cur + 2 * kState + role * kRows;
       const T* const other_t = cur + 2 * kState + (1 - role) * kRows;
       const T* const state = DIRECT ? cur + role * kState
-                                    : static_cast<const T*>(role ? p.dstates : p.states) + ((bh * p.runs + run) * p.vblocks + vb) * kVBlock * DKP;
+                                    : static_cast<const T*>(role ? p.dstates : p.states) + ((bh * p.runs + run) * vblocks + vb) * kVBlock * DKP;
       // columns d of the state, 16 t on, over its value channels
       auto state_operand = [&](int u, int t) __attribute__((always_inline)) {
         if constexpr (DIRECT) {
@@ -234,13 +255,22 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         if (role ? ot < blk : ot > blk) continue;
         const f32x4 hi = *reinterpret_cast<const f32x4*>(D.hi + 16 * ot + 4 * g);
         const f32x4 lo = *reinterpret_cast<const f32x4*>(D.lo + 16 * ot + 4 * g);
+        float x[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const bool in = ot != blk || (role ? 4 * g + r >= i : 4 * g + r <= i);
-          const float decay = role ? between<DT>(hi[r], lo[r], hi_r, lo_r) : between<DT>(hi_r, lo_r, hi[r], lo[r]);
-          acc[ot][r] = in ? acc[ot][r] * p.scale * decay : 0.0f;
-          sum += in ? acc[ot][r] * A[ot][r] : 0.0f;
+          const float decay = between<DT>(hi_r, lo_r, hi[r], lo[r], role != 0);
+          acc[ot][r] *= p.scale * decay;
+          x[r] = acc[ot][r] * A[ot][r];
         }
+        if (ot == blk) {  // the diagonal's tile
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool in = role ? 4 * g + r >= i : 4 * g + r <= i;
+            acc[ot][r] = in ? acc[ot][r] : 0.0f;
+            x[r] = in ? x[r] : 0.0f;
+          }
+        }
+        sum += (x[0] + x[1]) + (x[2] + x[3]);
       }
       u32x4 dp[kRun / O::kStep];
 #pragma unroll
@@ -249,13 +279,24 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       const f32x4 w = *reinterpret_cast<const f32x4*>((role ? D.onward : D.into) + 16 * blk + 4 * g) * ((role ? 1.0f : p.scale) * factor);
       f32x4 inter = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int t = 0; t < ND; ++t) {
-        tmp[t] *= w;
-        out[t] += tmp[t];
-        if (p.dg) {
+      for (int t = 0; t < ND; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) inter[r] += tmp[t][r] * Ty<DT>::f(s_own[TK::at(16 * blk + 4 * g + r, 16 * t + i)]);
+        for (int r = 0; r < 4; ++r) out[t][r] = __builtin_fmaf(tmp[t][r], w[r], out[t][r]);
+      if (p.dg) {
+#pragma unroll
+        for (int t = 0; t < ND; ++t) {
+          float x[4];
+          if constexpr (O::kWide) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = Ty<DT>::f(s_own[TK::at(16 * blk + 4 * g + r, 16 * t + i)]);
+          } else {
+            unpack2<DT>(held[t][0], x[0], x[1]);
+            unpack2<DT>(held[t][1], x[2], x[3]);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) inter[r] = __builtin_fmaf(tmp[t][r], x[r], inter[r]);
         }
+        inter *= w;
       }
 #pragma unroll
       for (int u = 0; u < kRun / O::kStep; ++u) {
@@ -278,10 +319,10 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
     };
     if (wave == 7) run_decays(s_d[0], gate_value(p, gate(h0)), lane);
     fetch(s_b0, h0, 0);
-    const int steps = (h1 - h0) * p.vblocks;
+    const int steps = (h1 - h0) * vblocks;
     int h = h0, vb = 0;
     auto advance = [&] {
-      if (++vb == p.vblocks) {
+      if (++vb == vblocks) {
         vb = 0;
         ++h;
       }
@@ -327,8 +368,15 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
 template <int DT, int DKP>
 static void launch_grad_t(const Grad& p, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(p.batch * p.runs * p.groups * p.sets));
-  if (DT != MM_F32 && p.vec) hipLaunchKernelGGL((grad_kernel<DT, DKP, DT != MM_F32>), grid, dim3(512), 0, s, p);
-  else hipLaunchKernelGGL((grad_kernel<DT, DKP, false>), grid, dim3(512), 0, s, p);
+  constexpr bool kDirect = DT != MM_F32;
+  if constexpr (kDirect) {
+    if (p.vec) {
+      if (p.vblocks == 1) hipLaunchKernelGGL((grad_kernel<DT, DKP, kDirect, true>), grid, dim3(512), 0, s, p);
+      else hipLaunchKernelGGL((grad_kernel<DT, DKP, kDirect, false>), grid, dim3(512), 0, s, p);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((grad_kernel<DT, DKP, false, false>), grid, dim3(512), 0, s, p);
 }
 template <int DT>
 static void launch_grad_d(const Grad& p, hipStream_t s) {

@@ -221,10 +221,10 @@ __device__ __forceinline__ void run_decays(Decays& d, float g, int lane) {
   if (lane == 63) d.whole = exp2_acc(hi) * (1.0f + static_cast<float>(c - hi) * kLn2);
 }
 
-// exp(c_t - c_s)
+// exp(c_t - c_s), or with `back` exp(c_s - c_t)
 template <int DT>
-__device__ __forceinline__ float between(float hi_t, float lo_t, float hi_s, float lo_s) {
-  const float x = (hi_t - hi_s) + (lo_t - lo_s);
+__device__ __forceinline__ float between(float hi_t, float lo_t, float hi_s, float lo_s, bool back = false) {
+  const float d = (hi_t - hi_s) + (lo_t - lo_s), x = back ? -d : d;
   const float e = exp2_decay<DT>(x);
   return DT == MM_F32 && x != x ? x : e;  // (exp2_acc's clamp would lose a NaN)
 }
