@@ -74,7 +74,6 @@ __device__ __forceinline__ float gate_value(const P& p, uint32_t raw) {
          : p.g_dtype == MM_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(raw)))
                                : __uint_as_float(raw << 16);
 }
-// A run's saved state of one value block: 64 value channels (rows) by DKP key channels, (bh, run, value block) contiguous.
 typedef float seg_f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ seg_f32x4* seg_state(const Pass& p, int64_t bh, int seg, int vb) {
   const int64_t dkp = p.dk <= 64 ? 64 : 128;

@@ -218,6 +218,8 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       auto state_operand = [&](int u, int t) __attribute__((always_inline)) {
         if constexpr (DIRECT) {
           return TK::column(state, u * O::kStep, 16 * t, lane);
+        } else if constexpr (O::kWide) {
+          return *reinterpret_cast<const u32x4*>(state + ((u * ND + t) * 64 + lane) * 4);
         } else {
           T e[O::kE];
 #pragma unroll

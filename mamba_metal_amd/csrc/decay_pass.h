@@ -207,11 +207,11 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     f32x4 saved4[kSaved];
     if constexpr (OUT && REV) {
       if (dot_wanted) {
-        const T* const before = static_cast<const T*>(p.dot_with) + block * kVBlock * DKP + (16 * wave + i) * DKP + 4 * g;
+        const T* const before = static_cast<const T*>(p.dot_with) + block * kVBlock * DKP;
 #pragma unroll
         for (int t = 0; t < ND; ++t) {
-          if constexpr (O::kWide) saved4[t] = *reinterpret_cast<const f32x4*>(before + 16 * t);
-          else saved2[t] = *reinterpret_cast<const u32x2*>(before + 16 * t);
+          if constexpr (O::kWide) saved4[t] = *reinterpret_cast<const f32x4*>(before + ((wave * ND + t) * 64 + lane) * 4);
+          else saved2[t] = *reinterpret_cast<const u32x2*>(before + (16 * wave + i) * DKP + 16 * t + 4 * g);
         }
       }
     }
@@ -219,10 +219,25 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     if (wave == kDecayWave) g_next = gate(next);
     if (n + 1 < walk) fetch_v(rows_of(next));
     if (!OUT && n + 1 < walk) fetch_k(rows_of(next));
-    // The state kept for the backward pass, a quarter at a time, for the same reason as the loads.
+    // The state kept for the backward pass, a quarter at a time, for the same reason as the loads.  16 bits: a value
+    // channel a row; fp32: as operands over the value channels, a lane's four together.
+    float dot = 0.0f;
     auto keep_state = [&](int quarter) __attribute__((always_inline)) {
       if (!OUT || !p.states) return;
       T* const to = static_cast<T*>(p.states) + block * kVBlock * DKP;
+      if constexpr (O::kWide) {
+#pragma unroll
+        for (int c = 0; c < ND / 4; ++c) {
+          const int t = quarter * (ND / 4) + c;
+          const f32x4 v = __builtin_bit_cast(f32x4, TK::column(s_s, 16 * wave, 16 * t, lane));
+          *reinterpret_cast<f32x4*>(to + ((wave * ND + t) * 64 + lane) * 4) = v;
+          if (REV && dot_wanted) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dot += v[r] * saved4[REV ? t : 0][r];
+          }
+        }
+        return;
+      }
       constexpr int kUnits = DKP / O::kE, kEach = kVBlock * kUnits / 256 / 4 > 0 ? kVBlock * kUnits / 256 / 4 : 1;
       if (quarter >= kVBlock * kUnits / 256) return;
 #pragma unroll
@@ -233,26 +248,16 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
       if (DT == MM_F16 && quarter == 0 && threadIdx.x == 0) p.factors[block] = factor;
     };
     if constexpr (OUT) {
-      if constexpr (REV) {
+      if constexpr (REV && !O::kWide) {
         if (dot_wanted) {
-          float dot = 0.0f;
 #pragma unroll
           for (int t = 0; t < ND; ++t) {
-            f32x4 x;
-            if constexpr (O::kWide) {
-              x = saved4[t];
-            } else {
-              float a[4];
-              unpack2<DT>(saved2[t][0], a[0], a[1]);
-              unpack2<DT>(saved2[t][1], a[2], a[3]);
-              x = f32x4{a[0], a[1], a[2], a[3]};
-            }
+            float x[4];
+            unpack2<DT>(saved2[t][0], x[0], x[1]);
+            unpack2<DT>(saved2[t][1], x[2], x[3]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) dot += x[r] * S[t][r];
           }
-#pragma unroll
-          for (int x = 1; x < 64; x *= 2) dot += lane_xor(dot, x);
-          if (lane == 0) s_x[wave] = dot;
         }
       }
       // Token block `wave` of the run: its scores, as accumulators (what adds) x (what asks) that are at once operands of
@@ -373,6 +378,11 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
             for (int t = 0; t < 4; ++t) S[t0 + t] = mma<DT>(ko[t], terms[m], S[t0 + t]);
         }
       }
+    }
+    if (OUT && REV && dot_wanted) {
+#pragma unroll
+      for (int x = 1; x < 64; x *= 2) dot += lane_xor(dot, x);
+      if (lane == 0) s_x[wave] = dot;
     }
     if (DT == MM_F16 && OUT) note_max();
     if (!OUT) total += static_cast<double>(D.hi[63]) + D.lo[63];
