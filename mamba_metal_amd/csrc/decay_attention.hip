@@ -95,7 +95,8 @@ struct Shape {
   int32_t vblocks, segments, sets, set_heads;
 };
 
-// Segments: with fewer than 256 workgroups (one a compute unit) the tokens are cut so that there are 512.
+// Segments: with fewer than 256 workgroups (one a compute unit) the tokens are cut so that there are up to 512, which all
+// run at once.
 // Sets of heads in the gradients of q and k: as few as make 768 workgroups, since each set's sums are written and read
 // once more.
 static Shape shape_of(int64_t batch, int64_t seqlen, int64_t heads, int64_t groups, int64_t dv) {
@@ -103,7 +104,7 @@ static Shape shape_of(int64_t batch, int64_t seqlen, int64_t heads, int64_t grou
   s.runs = ceil_div(seqlen, kRun);
   s.vblocks = static_cast<int32_t>(ceil_div(dv, kVBlock));
   const int64_t wgs = batch * heads * s.vblocks, per = heads / groups;
-  int64_t segs = wgs < 256 ? ceil_div(512, wgs) : 1;
+  int64_t segs = wgs < 256 ? 512 / wgs : 1;
   if (segs > s.runs / 2) segs = s.runs / 2;
   if (segs < 1) segs = 1;
   s.seg_runs = ceil_div(s.runs > 0 ? s.runs : 1, segs);
