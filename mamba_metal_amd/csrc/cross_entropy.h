@@ -27,7 +27,6 @@ struct Loss {
   char* xc;               // rows that count, (rows, ld) with zeros behind dim
   char* wc;               // the weight laid out the same, where its rows are not aligned
   int64_t ld;             // bytes of their rows
-  char* zeros;
   float* stats;           // (rows, tiles, 2): maximum and sum of exponentials of a tile of the vocabulary
   float* hit;             // by place: the target's logit
   float* row_loss;        // (rows,), where the loss is one number

@@ -11,6 +11,7 @@
 // Rows that are ignored take no part: the others are gathered first (their sums over rows are then never touched by what
 // an ignored row holds, and a batch that is mostly ignored costs its share), and workgroups past their count end at once.
 #include "cross_entropy.h"
+#include "row_io.h"
 
 namespace mm {
 namespace xent {
@@ -22,9 +23,9 @@ using slab::kAlong;
 using slab::u32x2;
 using slab::u32x4;
 
-using Big = slab::Tile<256, 256, 2, 4>;
-using Mid = slab::Tile<128, 128, 2, 2>;
-using Thin = slab::Tile<128, 64, 4, 1>;  // few rows of x
+using Big = slab::Tile<256, 256, 2, 4, 4>;
+using Mid = slab::Tile<128, 128, 2, 2, 4>;
+using Thin = slab::Tile<128, 64, 4, 1, 4>;  // few rows of x
 
 constexpr int kThreads = 1024;
 
@@ -81,7 +82,6 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Loss p, bool backw
     base += all;
   }
   if (threadIdx.x == 0) p.count[0] = base;
-  if (threadIdx.x < 4) reinterpret_cast<uint32_t*>(p.zeros)[threadIdx.x] = 0;
   if (!backward) return;
   // Mean: every row's share.  fp16: the pieces hold dl times a power of two that puts the largest |dloss| at 2^12, so
   // that small probabilities are not subnormal; the sums take it back.
@@ -127,7 +127,6 @@ __device__ __forceinline__ Matrix vocabulary(const Loss& p, int64_t v0) {
   m.base += v0 * m.ld;
   m.rows = p.vocab - v0;
   m.k = p.ld / es;
-  m.zeros = p.zeros;
   return m;
 }
 __device__ __forceinline__ Matrix counted(const Loss& p, int32_t count) {
@@ -136,7 +135,6 @@ __device__ __forceinline__ Matrix counted(const Loss& p, int32_t count) {
   m.ld = p.ld;
   m.rows = count;
   m.k = p.ld / (p.dtype == MM_F32 ? 4 : 2);
-  m.zeros = p.zeros;
   return m;
 }
 
@@ -145,8 +143,7 @@ __device__ __forceinline__ Matrix counted(const Loss& p, int32_t count) {
 template <int DT, typename S, bool GRAD>
 __global__ __launch_bounds__(64 * S::NW) void logits_kernel(const Loss p) {
   using T = typename Ty<DT>::T;
-  __shared__ __attribute__((aligned(16))) char s0[(S::BM + S::BN) * slab::kSlab];
-  __shared__ __attribute__((aligned(16))) char s1[(S::BM + S::BN) * slab::kSlab];
+  MM_SLAB_STAGES(S, stages)
   const int32_t count = *p.count;
   const int64_t vocab = GRAD ? p.piece_n : p.vocab;
   const uint32_t vt = static_cast<uint32_t>((GRAD ? p.piece_ld / static_cast<int64_t>(sizeof(T)) : vocab) + S::BM - 1) / S::BM;
@@ -155,47 +152,75 @@ __global__ __launch_bounds__(64 * S::NW) void logits_kernel(const Loss p) {
   slab::tile_of(blockIdx.x, vt, rt, m, n);
   const int64_t v0 = static_cast<int64_t>(m) * S::BM, r0 = static_cast<int64_t>(n) * S::BN;
   if (r0 >= count) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / S::WN, wn = wave % S::WN;
+  // what the end needs of this lane's columns
+  int64_t target[S::TN];  // relative to the matrix's first row
+  float lse[S::TN], weight[S::TN];
+#pragma unroll
+  for (int j = 0; j < S::TN; ++j) {
+    const int64_t r = r0 + wn * 32 * S::TN + 32 * j + (lane & 31), in = r < count ? r : 0;
+    const int64_t t = p.target_at[in];
+    target[j] = r < count ? t - (GRAD ? p.piece0 : 0) : -1;
+    lse[j] = GRAD ? p.lse_at[in] : 0.0f;
+    weight[j] = GRAD ? p.weights[in] : 0.0f;
+  }
   f32x16 acc[S::TM][S::TN];
   slab::clear<S>(acc);
   const Matrix w = vocabulary(p, GRAD ? p.piece0 : 0), x = counted(p, count);
-  slab::product<DT, kAlong, kAlong, S>(w, x, v0, r0, 0, w.k, s0, s1, acc);
+  slab::product<DT, kAlong, kAlong, S>(w, x, v0, r0, 0, w.k, stages0, stages1, stages2, stages3, acc);
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = wave / S::WN, wn = wave % S::WN;
   const int64_t vw = v0 + wm * 32 * S::TM + 4 * (lane >> 5);  // of the lane's first accumulator
   const int here = vocab - vw < 1 << 20 ? static_cast<int>(vocab - vw) : 1 << 20;  // tokens from there on
+  const bool edge = v0 + S::BM > vocab;  // (most tiles have none)
   if constexpr (!GRAD) {
-    __syncthreads();
-    float* const s_stat = reinterpret_cast<float*>(s0);  // (WM, BN, 2)
+    float* const s_stat = reinterpret_cast<float*>(stages0);  // (WM, BN, 2)
 #pragma unroll
     for (int j = 0; j < S::TN; ++j) {
       const int col = wn * 32 * S::TN + 32 * j + (lane & 31);
       const int64_t r = r0 + col;
-      const int64_t t64 = r < count ? p.target_at[r] - vw : -1;
-      const int t = t64 >= 0 && t64 < here ? static_cast<int>(t64) : -1;
-      float top = -INFINITY, hit = 0.0f;
-      bool bad = false, mine = false;
+      const int64_t t = target[j] - vw;
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (32 * i + 8 * (e >> 2) + (e & 3) >= here) acc[i][j][e] = -INFINITY;
+      }
+      if (__any(t >= 0 && t < 32 * S::TM && t < here)) {
+#pragma unroll
+        for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (32 * i + 8 * (e >> 2) + (e & 3) == t && r < count) p.hit[r] = acc[i][j][e];
+      }
+      float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int v = 32 * i + 8 * (e >> 2) + (e & 3);
-          const float l = v < here ? acc[i][j][e] : -INFINITY;
-          acc[i][j][e] = l;
-          hit = v == t ? l : hit;
-          mine |= v == t;
-          bad |= l != l;  // (lost by fmaxf and, in fp32, by exp2_acc's clamp)
-          top = fmaxf(top, l);
-        }
-      if (mine) p.hit[r] = hit;
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[i][j][e]);
       top = fmaxf(top, lane_xor(top, 32));
       float sum = 0.0f;
       const float from = top == -INFINITY ? 0.0f : top;  // (all logits -inf: a sum of 0, not a NaN)
+      if constexpr (DT == MM_F32) {
+        bool bad = top == INFINITY;
 #pragma unroll
-      for (int i = 0; i < S::TM; ++i)
+        for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sum += exp2_decay<DT>((acc[i][j][e] - from) * kLog2e);
-      if (bad || top == INFINITY) sum = __builtin_nanf("");
+          for (int e = 0; e < 16; ++e) {
+            const float l = acc[i][j][e];
+            bad |= l != l;  // (lost by fmaxf and exp2_acc's clamp)
+            sum += exp2_acc((l - from) * kLog2e);
+          }
+        if (bad) sum = __builtin_nanf("");
+      } else {
+        // (a NaN, and an infinity less itself, goes through the hardware's exp2)
+        const float base = from * kLog2e;
+#pragma unroll
+        for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum += exp2_hw(__builtin_fmaf(acc[i][j][e], kLog2e, -base));
+      }
       sum += lane_xor(sum, 32);
       if (lane < 32) {
         s_stat[(wm * S::BN + col) * 2] = top;
@@ -220,36 +245,80 @@ __global__ __launch_bounds__(64 * S::NW) void logits_kernel(const Loss p) {
   } else {
 #pragma unroll
     for (int j = 0; j < S::TN; ++j) {
-      const int64_t r = r0 + wn * 32 * S::TN + 32 * j + (lane & 31);
-      if (r >= count) continue;
-      const float lse = p.lse_at[r], weight = p.weights[r];
-      const int64_t t64 = p.target_at[r] - p.piece0 - vw;
-      const int t = t64 >= 0 && t64 < here ? static_cast<int>(t64) : -1;
-      char* const to = p.piece + r * p.piece_ld + vw * static_cast<int64_t>(sizeof(T));
-      const int wide = static_cast<int>(p.piece_ld / static_cast<int64_t>(sizeof(T)) - vw);
+      const int64_t t = target[j] - vw;
 #pragma unroll
       for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int v = 32 * i + 8 * q;
-          if (v >= wide) continue;
-          T d[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float z = (acc[i][j][4 * q + e] - lse) * kLog2e;
-            float g = exp2_decay<DT>(z);
-            if (DT == MM_F32) g = z != z ? z : g;
-            g = (g - (v + e == t ? 1.0f : 0.0f)) * weight;
-            d[e] = Ty<DT>::from(v + e < here ? g : 0.0f);
-          }
+        for (int e = 0; e < 16; ++e) {
           if constexpr (DT == MM_F32) {
-            *reinterpret_cast<slab::f32x4*>(to + v * 4) = slab::f32x4{d[0], d[1], d[2], d[3]};
+            const float z = (acc[i][j][e] - lse[j]) * kLog2e, g = exp2_acc(z);
+            acc[i][j][e] = (z != z ? z : g) * weight[j];
           } else {
-            u32x2 w2;
-            __builtin_memcpy(&w2, d, 8);
-            *reinterpret_cast<u32x2*>(to + v * 2) = w2;
+            acc[i][j][e] = exp2_hw(__builtin_fmaf(acc[i][j][e], kLog2e, -lse[j] * kLog2e)) * weight[j];
           }
         }
+      if (__any(t >= 0 && t < 32 * S::TM)) {
+#pragma unroll
+        for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (32 * i + 8 * (e >> 2) + (e & 3) == t) acc[i][j][e] -= weight[j];
+      }
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (32 * i + 8 * (e >> 2) + (e & 3) >= here) acc[i][j][e] = 0.0f;
+      }
+    }
+    // Out by rows: through the stages, half a tile's rows at a time where it is large, a row's 16-byte chunks turned by its
+    // number.  (A row of the piece is a whole number of tiles of 256; fp32 is stored from the accumulators.)
+    const int wide = static_cast<int>(p.piece_ld / static_cast<int64_t>(sizeof(T)) - v0);  // of this tile's columns
+    if constexpr (DT == MM_F32) {
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j) {
+        const int64_t r = r0 + wn * 32 * S::TN + 32 * j + (lane & 31);
+        if (r >= count) continue;
+#pragma unroll
+        for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int v = wm * 32 * S::TM + 4 * (lane >> 5) + 32 * i + 8 * q;
+            if (v >= wide) continue;
+            float* const to = reinterpret_cast<float*>(p.piece + r * p.piece_ld) + v0 + v;
+            *reinterpret_cast<slab::f32x4*>(to) = slab::f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          }
+      }
+    } else {
+      constexpr int kChunks = S::BM * 2 / 16, kPart = S::BN / 4;  // of a row; rows that a stage holds
+      static_assert(kPart * S::BM * 2 <= S::kStage && kPart % 16 == 0, "a quarter of the tile's rows in a stage");
+      auto stage_of = [&](int row) { return row / kPart == 0 ? stages0 : row / kPart == 1 ? stages1 : row / kPart == 2 ? stages2 : stages3; };
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j) {
+        const int row = wn * 32 * S::TN + 32 * j + (lane & 31);
+        char* const to = stage_of(row) + row % kPart * (S::BM * 2) + 8 * (lane >> 5);
+#pragma unroll
+        for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            T d[4];
+            round2<DT>(acc[i][j][4 * q], acc[i][j][4 * q + 1], d[0], d[1]);
+            round2<DT>(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3], d[2], d[3]);
+            u32x2 w2;
+            __builtin_memcpy(&w2, d, 8);
+            const int chunk = wm * 4 * S::TM + 4 * i + q;
+            *reinterpret_cast<u32x2*>(to + ((chunk ^ (row % kChunks)) << 4)) = w2;
+          }
+      }
+      __syncthreads();
+#pragma unroll 4
+      for (int u = threadIdx.x; u < S::BN * kChunks; u += 64 * S::NW) {
+        const int row = u / kChunks, chunk = u % kChunks;
+        if (r0 + row >= count || chunk * 8 >= wide) continue;
+        *reinterpret_cast<u32x4*>(p.piece + (r0 + row) * p.piece_ld + (v0 + chunk * 8) * 2) =
+            *reinterpret_cast<const u32x4*>(stage_of(row) + row % kPart * (S::BM * 2) + ((chunk ^ (row % kChunks)) << 4));
+      }
     }
   }
 }
@@ -296,8 +365,7 @@ __global__ __launch_bounds__(kThreads) void total_kernel(const Loss p) {
 template <int DT, typename S>
 __global__ __launch_bounds__(64 * S::NW) void dx_kernel(const Loss p) {
   using T = typename Ty<DT>::T;
-  __shared__ __attribute__((aligned(16))) char s0[(S::BM + S::BN) * slab::kSlab];
-  __shared__ __attribute__((aligned(16))) char s1[(S::BM + S::BN) * slab::kSlab];
+  MM_SLAB_STAGES(S, stages)
   const int32_t count = *p.count;
   const uint32_t mt = static_cast<uint32_t>((p.rows + S::BM - 1) / S::BM), nt = static_cast<uint32_t>((p.dim + S::BN - 1) / S::BN);
   uint32_t m, n;
@@ -312,9 +380,8 @@ __global__ __launch_bounds__(64 * S::NW) void dx_kernel(const Loss p) {
   dl.base = p.piece;
   dl.ld = p.piece_ld;
   dl.rows = count;
-  dl.zeros = p.zeros;
   w.rows = p.ld / static_cast<int64_t>(sizeof(T));
-  if (k1 > k0) slab::product<DT, kAlong, kAcross, S>(dl, w, r0, c0, k0, k1 - k0, s0, s1, acc);
+  if (k1 > k0) slab::product<DT, kAlong, kAcross, S>(dl, w, r0, c0, k0, k1 - k0, stages0, stages1, stages2, stages3, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float* const out = p.dx_part + split * p.rows * p.dim;
 #pragma unroll
@@ -340,8 +407,7 @@ __global__ __launch_bounds__(64 * S::NW) void dx_kernel(const Loss p) {
 template <int DT, typename S>
 __global__ __launch_bounds__(64 * S::NW) void dw_kernel(const Loss p) {
   using T = typename Ty<DT>::T;
-  __shared__ __attribute__((aligned(16))) char s0[(S::BM + S::BN) * slab::kSlab];
-  __shared__ __attribute__((aligned(16))) char s1[(S::BM + S::BN) * slab::kSlab];
+  MM_SLAB_STAGES(S, stages)
   const int32_t count = *p.count;
   const uint32_t mt = static_cast<uint32_t>((p.piece_n + S::BM - 1) / S::BM), nt = static_cast<uint32_t>((p.dim + S::BN - 1) / S::BN);
   uint32_t m, n;
@@ -353,12 +419,10 @@ __global__ __launch_bounds__(64 * S::NW) void dw_kernel(const Loss p) {
   dl.base = p.piece;
   dl.ld = p.piece_ld;
   dl.rows = p.piece_ld / static_cast<int64_t>(sizeof(T));
-  dl.zeros = p.zeros;
   x.base = p.xc;
   x.ld = p.ld;
   x.rows = p.ld / static_cast<int64_t>(sizeof(T));
-  x.zeros = p.zeros;
-  slab::product<DT, kAcross, kAcross, S>(dl, x, v0, c0, 0, count, s0, s1, acc);
+  slab::product<DT, kAcross, kAcross, S>(dl, x, v0, c0, 0, count, stages0, stages1, stages2, stages3, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float down = p.scalars[0];
 #pragma unroll
@@ -411,14 +475,14 @@ struct Plan {
   int64_t ld, tiles, piece_n, pieces, splits, split_k;
   bool copy_w;
   Size logits;
-  int64_t at, row, count, scalars, weights, lse_at, target_at, xc, wc, zeros, stats, hit, row_loss, piece, dx_part, total;
+  int64_t at, row, count, scalars, weights, lse_at, target_at, xc, wc, stats, hit, row_loss, piece, dx_part, total;
 };
 
 static Plan plan_of(const mm_linear_cross_entropy_params* q, bool backward) {
   Plan s{};
   const int64_t es = dtype_size(q->dtype);
   s.ld = round_up(q->dim * es, 16);
-  s.copy_w = s.ld != q->dim * es || q->weight_stride * es % 16 != 0 || !aligned(q->weight, 16);
+  s.copy_w = s.ld != q->dim * es || q->weight_stride * es % 16 != 0 || q->weight_stride * es >= (int64_t{1} << 23) || !aligned(q->weight, 16);
   s.logits = logits_size(q->vocab, q->rows);
   s.tiles = ceil_div(q->vocab, edge(s.logits));
   int64_t at = 0;
@@ -431,7 +495,6 @@ static Plan plan_of(const mm_linear_cross_entropy_params* q, bool backward) {
   s.row = take(q->rows * 4);
   s.count = take(4);
   s.scalars = take(4);
-  s.zeros = take(16);
   s.target_at = take(q->rows * 8);
   s.xc = take(q->rows * s.ld);
   if (s.copy_w) s.wc = take(q->vocab * s.ld);
@@ -507,7 +570,6 @@ static Loss loss_of(const mm_linear_cross_entropy_params* q, const Plan& s, bool
   p.count = reinterpret_cast<int32_t*>(ws + s.count);
   p.scalars = reinterpret_cast<float*>(ws + s.scalars);
   p.target_at = reinterpret_cast<int64_t*>(ws + s.target_at);
-  p.zeros = ws + s.zeros;
   p.xc = ws + s.xc;
   p.wc = s.copy_w ? ws + s.wc : nullptr;
   p.ld = s.ld;

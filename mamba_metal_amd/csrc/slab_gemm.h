@@ -1,18 +1,23 @@
 // Products of large tiles on the matrix cores: C[m, n] = sum_k A(m, k) B(n, k), both operands streamed through shared
-// memory by loads that go there directly, two stages deep.
+// memory by loads that go there directly, several stages deep.
 //
-// A stage is a slab of 128 bytes of k (64 16-bit elements, 32 fp32 ones) of the tile's rows.  An operand lies in memory
-// either way:
-//   kAlong   k is contiguous: a row of the slab is 128 bytes of a row of the matrix, eight 16-byte chunks.  Chunk c of
-//            row r is kept at place c ^ (r / 2 % 8), so that 16 rows' reads of one chunk fall into different banks.
-//   kAcross  rows (m or n) are contiguous: the slab is 64 (32) rows of k by the tile's width, read with the transposing
-//            read (fp32: element by element).  Its chunks are kept at c ^ f(k), for the same reason.
-// The direct load writes 16 bytes a lane at consecutive places, so the permutation is of the addresses that the lanes
-// read.  Elements past the matrix's k (and columns past its width, kAcross) come from a block of zeros; rows past its end
-// are its last row again, whose results are not stored.
+// A stage is a slab of 64 bytes of k (32 16-bit elements, 16 fp32 ones) of the tile's rows.  What the 32 units of a die
+// read at once is shared in its cache, so that all of them wait for the same misses: a stage's loads take 1.5 to 2 us,
+// twice what its products take, and it is the bytes under way that keep the matrix cores fed (two stages of 128 bytes of
+// k, half as many bytes under way: 51% of their cycles busy).
+//
+// An operand lies in memory either way:
+//   kAlong   k is contiguous: a row of the slab is 64 bytes of a row of the matrix, four 16-byte chunks.  Chunk c of
+//            row r is kept at place c ^ (r / 4 % 4), so that the rows whose reads meet fall into different banks.
+//   kAcross  rows (m or n) are contiguous: the slab is 32 (16) rows of k by the tile's width, read with the transposing
+//            read (fp32: element by element), which takes 64 bytes of each of 4 rows of k: those lie side by side.
+// The direct load writes 16 bytes a lane at consecutive places, so the arrangement is of the addresses that the lanes
+// read.  They are buffer loads: a lane whose element lies past the matrix's k (or past its width, kAcross) is given an
+// offset past the buffer's end, which loads zeros, and reads of shared memory wait for themselves alone (behind flat ones
+// the compiler waits for all reads under way).  Rows past a matrix's end are its last row again, whose results are not stored.
 //
 // The 32 x 32 tiles' operand layout: lane l holds row l % 32 and 16 bytes of k, chunk 2 s + l / 32 of the slab at step s
-// of 4; an accumulator holds column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4.
+// of 2; an accumulator holds column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4.
 #pragma once
 
 #include "mm_common.h"
@@ -28,7 +33,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kSlab = 128;  // bytes of k
+constexpr int kSlab = 64;  // bytes of k
+constexpr int kSteps = 2;  // of 32 bytes
 enum Lie { kAlong, kAcross };
 
 template <int DT>
@@ -47,15 +53,15 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
 
 struct Matrix {
   const char* base;
-  int64_t ld;       // bytes from one row in memory to the next
+  int64_t ld;       // bytes from one row in memory to the next; a tile's rows lie within 2 GB
   int64_t rows;     // kAlong: rows of the operand; kAcross: its columns, in elements
   int64_t k;        // elements of the sum
-  const char* zeros;  // 16 bytes of them
 };
 
-__device__ __forceinline__ void load_direct(const char* from, char* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+constexpr uint32_t kNowhere = 0x80000000u;  // an offset past a buffer's end
+__device__ __forceinline__ void load_direct(const char* base, uint32_t off, char* to) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7fffffff, 0x00027000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)to, 16, off, 0, 0, 0);
 }
 
 // One operand of a workgroup's tile: R rows, staged by NW waves.
@@ -64,59 +70,71 @@ struct Side {
   using T = typename Ty<DT>::T;
   static constexpr int kEs = sizeof(T);
   static constexpr int kDepth = kSlab / kEs;               // elements of k in a slab
-  static constexpr int kBytes = R * kSlab;
-  static constexpr int kLoads = kBytes / 1024 / NW;        // of a wave, 64 lanes of 16 bytes each
-  static constexpr int kRowChunks = R * kEs / 16;          // kAcross: chunks of a row of k
-  static_assert(kLoads >= 1 && kLoads * 1024 * NW == kBytes, "whole loads");
-  const char* at[kLoads];
-  int32_t k_at[kLoads];  // the lane's first element of k within the slab
+  static constexpr int kLoads = R * kSlab / 1024 / NW;     // of a wave, 64 lanes of 16 bytes each
+  static constexpr int kReads = LIE == kAlong ? 1 : kEs == 2 ? 2 : 4;  // of an operand
+  static_assert(kLoads >= 1 && kLoads * 1024 * NW == R * kSlab, "whole loads");
+  // kAcross: a load is kRows rows of k.  16-bit: 64 bytes of each of kSide rows side by side, then the next 64 bytes of
+  // them; where a load has but 2 rows, the next one's are 128 bytes further on in the banks.
+  static constexpr int kRows = 1024 / (R * kEs), kSide = kRows < 4 ? kRows : 4, kGroups = R * kEs / 64;
+  static constexpr int kLoadBytes = LIE == kAcross && kEs == 2 && kRows == 2 ? 1024 + 128 : 1024;  // a load's place
+  static constexpr int kBytes = kLoads * NW * kLoadBytes;
+  const char* base;       // of the next slab: wave-uniform, and a lane's offset from it fits 32 bits
+  uint32_t off[kLoads];
   int64_t step;
-  const char* zeros;
+  int k_at[kLoads];       // a lane's first element of k in a slab
 
-  static __device__ __forceinline__ int place(int k) {  // kAcross: what a row of k has its chunks permuted by
-    return kEs != 2 ? 0 : kRowChunks >= 16 ? (k & 3) << 2 : kRowChunks == 8 ? (k >> 1 & 1) << 2 : 0;
+  // Lane's row of k (kAcross) or first element of k (kAlong), and column of the tile, in its load q.
+  static __device__ __forceinline__ int k_of(int q, int wave, int lane) {
+    if constexpr (LIE == kAlong) return (lane % 4 ^ (lane >> 4 & 3)) * 16 / kEs;
+    else if constexpr (kEs == 2) return (q * NW + wave) * kRows + lane / 4 / kSide / kGroups * kSide + lane / 4 % kSide;
+    else return (q * NW + wave) * kRows + lane * 16 / (R * kEs);
+  }
+  static __device__ __forceinline__ int col_of(int lane) {
+    if constexpr (kEs == 2) return lane / 4 / kSide % kGroups * 32 + lane % 4 * 8;
+    else return lane * 4 % R;
   }
   __device__ __forceinline__ void init(const Matrix& m, int64_t row0, int64_t k0, int wave, int lane) {
-    zeros = m.zeros;
     step = LIE == kAlong ? kSlab : kDepth * m.ld;
+    // (a tile may lie past the matrix's end: kAlong its rows are all the last one, kAcross its columns all zeros)
+    const int64_t first = LIE == kAlong && row0 >= m.rows ? m.rows - 1 : row0;
+    base = m.base + (LIE == kAlong ? first * m.ld + k0 * kEs : k0 * m.ld + first * kEs);
+    const int64_t over = m.rows - 1 - first;                 // kAlong: not negative
+    const int last = over < R ? static_cast<int>(over) : R;  // row of the tile
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) {
-      const int s = (q * NW + wave) * 64 + lane;
+      const int r = ((q * NW + wave) * 64 + lane) / 4;
+      k_at[q] = k_of(q, wave, lane);
       if constexpr (LIE == kAlong) {
-        const int r = s / 8, c = s % 8 ^ (r >> 1 & 7);
-        const int64_t row = row0 + r < m.rows ? row0 + r : m.rows - 1;
-        k_at[q] = c * 16 / kEs;
-        at[q] = m.base + row * m.ld + k0 * kEs + c * 16;
+        off[q] = static_cast<uint32_t>((r < last ? r : last) * m.ld) + k_at[q] * kEs;
       } else {
-        const int k = s / kRowChunks, c = s % kRowChunks ^ place(k);
-        const int64_t col = row0 + c * (16 / kEs);
-        k_at[q] = col < m.rows ? k : 1 << 30;  // (never within k)
-        at[q] = m.base + (k0 + k) * m.ld + col * kEs;
+        const int col = col_of(lane);
+        off[q] = static_cast<uint32_t>(k_at[q] * m.ld) + col * kEs;
+        if (row0 + col >= m.rows) k_at[q] = kDepth;  // (never within k)
       }
     }
   }
-  // Issues the loads of one slab, of whose k `left` elements are in the matrix, and moves on.
+  // Issues the loads of one slab, of whose k `left` elements are in the matrix, and moves on.  (Without a branch: behind
+  // one the compiler waits for all reads of shared memory instead of the oldest.)
   __device__ __forceinline__ void load(char* tile, int64_t left, int wave) {
-    const bool all = LIE == kAlong && left >= kDepth;
+    const int here = left < kDepth ? static_cast<int>(left < 0 ? 0 : left) : kDepth;
 #pragma unroll
-    for (int q = 0; q < kLoads; ++q) {
-      const char* const from = all || k_at[q] < left ? at[q] : zeros;
-      load_direct(from, tile + (q * NW + wave) * 1024);
-      at[q] += step;
-    }
+    for (int q = 0; q < kLoads; ++q) load_direct(base, k_at[q] < here ? off[q] : kNowhere, tile + (q * NW + wave) * kLoadBytes);
+    base += step;
   }
-  // Rows r0 .. r0 + 31 at step s (of 4), of a staged slab.
+  // Rows r0 .. r0 + 31 at step s of a staged slab.
   static __device__ __forceinline__ u32x4 operand(const char* tile, int r0, int s, int lane) {
     if constexpr (LIE == kAlong) {
       const int r = r0 + (lane & 31), c = 2 * s + (lane >> 5);
-      return *reinterpret_cast<const u32x4*>(tile + r * kSlab + ((c ^ (r >> 1 & 7)) << 4));
+      return *reinterpret_cast<const u32x4*>(tile + r * kSlab + ((c ^ (r >> 2 & 3)) << 4));
     } else if constexpr (kEs == 2) {
       // 16 lanes read 4 rows of k by 16 columns, 8 bytes each, and get a column each
-      const int col = r0 + (lane & 16) + 4 * (lane & 3), k = 16 * s + 8 * (lane >> 5) + ((lane & 15) >> 2);
-      const char* const p = tile + k * R * kEs + (((col >> 3) ^ place(k)) << 4) + (col & 7) * 2;
+      constexpr int four = kRows == 2 ? 2 * kLoadBytes : 4 * R * kEs;  // bytes of 4 rows of k
+      const int row = (lane & 15) >> 2, in = ((lane & 16) >> 3 | (lane & 3) >> 1) * 16 + (lane & 1) * 8;
+      const int lie = kRows == 2 ? (row >> 1) * kLoadBytes + (row & 1) * 64 : row * 64;
+      const char* const p = tile + (r0 >> 5) * (kSide * 64) + (4 * s + 2 * (lane >> 5)) * four + lie + in;
       typedef __attribute__((address_space(3))) s16x4 Lds;
       const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p)));
-      const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p + 4 * R * kEs)));
+      const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p + four)));
       return u32x4{a[0], a[1], b[0], b[1]};
     } else {
       u32x4 v;
@@ -128,17 +146,39 @@ struct Side {
   }
 };
 
-// A tile's shape: BM x BN by WM x WN waves, each TM x TN tiles of 32 x 32.
-template <int BM_, int BN_, int WM_, int WN_>
+// A tile's shape: BM x BN by WM x WN waves, each TM x TN tiles of 32 x 32; ST stages.
+template <int BM_, int BN_, int WM_, int WN_, int ST_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  static constexpr int ST = ST_;                                   // stages, and the bytes of one
+  static constexpr int kStage = (BM + BN) * kSlab / 8 * (BM == 256 || BN == 256 ? 9 : 8);
 };
 
-// acc += the sum over `k` elements from k0 on.  All threads of the workgroup; s0 and s1 are (BM + BN) * 128 bytes each
-// and must be two objects, so that the compiler sees that a stage's reads and the next one's loads do not meet.
+// A tile's stages: separate objects, so that the compiler sees that one's reads and another's loads do not meet.
+#define MM_SLAB_STAGES(S, name)                                                                  \
+  __shared__ __attribute__((aligned(16))) char name##0[S::kStage];                               \
+  __shared__ __attribute__((aligned(16))) char name##1[S::kStage];                               \
+  __shared__ __attribute__((aligned(16))) char name##2[S::kStage];                               \
+  __shared__ __attribute__((aligned(16))) char name##3[S::kStage];
+
+// Waits until all but the wave's last `Left` loads are done and its reads of shared memory too, then for the others.
+template <int Left>
+__device__ __forceinline__ void meet() {
+  static_assert(Left < 64, "the counter's range");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((Left & 15) | (Left >> 4) << 14 | 7 << 4);  // vmcnt, expcnt free, lgkmcnt 0
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// acc += the sum over `k` elements from k0 on.  All threads of the workgroup; returns when nobody reads or loads the
+// stages any more.  (__restrict__: what tells the compiler of the transposing reads that a stage is none of the others;
+// else each would wait for all loads under way.)
 template <int DT, Lie LA, Lie LB, typename S>
-__device__ __forceinline__ void product(const Matrix& A, const Matrix& B, int64_t m0, int64_t n0, int64_t k0, int64_t k, char* s0,
-                                        char* s1, f32x16 (&acc)[S::TM][S::TN]) {
+__device__ __forceinline__ void product(const Matrix& A, const Matrix& B, int64_t m0, int64_t n0, int64_t k0, int64_t k,
+                                        char* __restrict__ s0, char* __restrict__ s1, char* __restrict__ s2,
+                                        char* __restrict__ s3, f32x16 (&acc)[S::TM][S::TN]) {
+  static_assert(S::ST == 4, "as many objects");
   using SA = Side<DT, LA, S::BM, S::NW>;
   using SB = Side<DT, LB, S::BN, S::NW>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -153,34 +193,58 @@ __device__ __forceinline__ void product(const Matrix& A, const Matrix& B, int64_
     a.load(to, left, wave);
     b.load(to + SA::kBytes, left, wave);
   };
-  auto multiply = [&](const char* from) __attribute__((always_inline)) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      u32x4 ao[S::TM], bo[S::TN];
-#pragma unroll
-      for (int i = 0; i < S::TM; ++i) ao[i] = SA::operand(from, wm + 32 * i, s, lane);
-#pragma unroll
-      for (int j = 0; j < S::TN; ++j) bo[j] = SB::operand(from + SA::kBytes, wn + 32 * j, s, lane);
-#pragma unroll
-      for (int i = 0; i < S::TM; ++i)
-#pragma unroll
-        for (int j = 0; j < S::TN; ++j) acc[i][j] = mma<DT>(ao[i], bo[j], acc[i][j]);
-    }
+  // A step's operands, read while the step before is multiplied.
+  struct Step {
+    u32x4 a[S::TM], b[S::TN];
   };
-  if (slabs > 0) load(s0, 0);
+  auto read = [&](const char* from, int s) __attribute__((always_inline)) {
+    Step q;
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i) q.a[i] = SA::operand(from, wm + 32 * i, s, lane);
+#pragma unroll
+    for (int j = 0; j < S::TN; ++j) q.b[j] = SB::operand(from + SA::kBytes, wn + 32 * j, s, lane);
+    return q;
+  };
+  auto multiply = [&](const Step& q) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j) acc[i][j] = mma<DT>(q.a[i], q.b[j], acc[i][j]);
+  };
+  constexpr int kLoads = SA::kLoads + SB::kLoads;
+  static_assert(kSteps == 2, "a slab's first step before the others are met, its second behind it");
+  load(s0, 0);
+  load(s1, 1);
+  load(s2, 2);
+  load(s3, 3);
+  meet<(S::ST - 1) * kLoads>();
+  Step q0 = read(s0, 0), q1;
+  // The slab's second step is multiplied when nobody reads the slab any more and the next one is there: that one's first
+  // operands are read, and the loads that take the slab's place issued, under those products.  (Past the last slab zeros
+  // are loaded, so that the count of loads under way stays the same.)
+  auto slab = [&](char* here, const char* there, int64_t t) __attribute__((always_inline)) {
+    q1 = read(here, 1);
+    __builtin_amdgcn_sched_barrier(0);  // (the reads first: the compiler would put each next to its use)
+    multiply(q0);
+    __builtin_amdgcn_sched_barrier(0);
+    meet<(S::ST - 2) * kLoads>();
+    q0 = read(there, 0);
+    load(here, t + S::ST);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(q1);
+    __builtin_amdgcn_sched_barrier(0);
+  };
   int64_t t = 0;
-  for (; t + 1 < slabs; t += 2) {
-    __syncthreads();  // s0 is loaded, and nobody reads s1
-    load(s1, t + 1);
-    multiply(s0);
-    __syncthreads();
-    if (t + 2 < slabs) load(s0, t + 2);
-    multiply(s1);
+  for (; t + S::ST <= slabs; t += S::ST) {
+    slab(s0, s1, t);
+    slab(s1, s2, t + 1);
+    slab(s2, s3, t + 2);
+    slab(s3, s0, t + 3);
   }
-  if (t < slabs) {
-    __syncthreads();
-    multiply(s0);
-  }
+  if (t < slabs) slab(s0, s1, t);
+  if (t + 1 < slabs) slab(s1, s2, t + 1);
+  if (t + 2 < slabs) slab(s2, s3, t + 2);
+  meet<0>();
 }
 
 template <typename S>
