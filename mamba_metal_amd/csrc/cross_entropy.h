@@ -20,7 +20,7 @@ struct Loss {
   int32_t* at;            // (rows,) a row's place among those that count, -1 for an ignored one
   int32_t* row;           // the row of each place
   int32_t* count;         // [0] how many count
-  float* scalars;         // [0] 1 / the power of two of the gradients' pieces
+  float* scalars;         // [0] what the sums of the pieces are multiplied by
   float* weights;         // by place: what multiplies a row's gradient, and
   float* lse_at;          // its lse
   int64_t* target_at;     // and target
@@ -33,8 +33,9 @@ struct Loss {
   char* piece;            // dl of a piece of the vocabulary, (rows, piece_ld bytes)
   float* dx_part;         // (splits, rows, dim) sums of dx
   int64_t piece_ld, piece0, piece_n;      // bytes; this piece's tokens
-  int64_t tiles, splits, split_k;
+  int64_t tiles, splits, split_k;         // of the vocabulary in stats; of dx's sums over a piece, and a split's tokens
   int32_t first_piece;
+  uint32_t dx_tiles;                      // workgroups of dx, before dW's
 };
 
 }  // namespace xent

@@ -46,53 +46,82 @@ __device__ __forceinline__ V all_of(V v, V* s, F join) {
   return v;
 }
 
-// The rows that count, in order, and for the backward pass what their gradients are multiplied by.  One workgroup.
+// The rows that count, in order, and for the backward pass what their gradients are multiplied by.  One workgroup: 8192 rows
+// a turn, their loads all under way at once.
 __global__ __launch_bounds__(kThreads) void rows_kernel(const Loss p, bool backward) {
-  __shared__ int32_t s_wave[kThreads / 64];
+  constexpr int kTurn = 8;
+  __shared__ int32_t s_wave[kTurn * kThreads / 64];
   __shared__ float s_f[kThreads / 64];
+  static_assert(kTurn * kThreads / 64 == 128, "two counts a lane");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int32_t base = 0;
   float top = 0.0f;
-  for (int64_t r0 = 0; r0 < p.rows; r0 += kThreads) {
-    const int64_t r = r0 + threadIdx.x;
-    const int64_t t = r < p.rows ? target_of(p, r) : 0;
-    const bool on = r < p.rows && t != p.ignore;
-    const uint64_t b = __ballot(on);
-    if (lane == 0) s_wave[wave] = __popcll(b);
-    __syncthreads();
-    int32_t before = 0, all = 0;
+  for (int64_t r0 = 0; r0 < p.rows; r0 += kTurn * kThreads) {
+    int64_t t[kTurn];
+    float d[kTurn], lse[kTurn];
+    uint64_t on[kTurn];
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) {
-      before += w < wave ? s_wave[w] : 0;
-      all += s_wave[w];
+    for (int j = 0; j < kTurn; ++j) {
+      const int64_t r = r0 + j * kThreads + threadIdx.x, in = r < p.rows ? r : p.rows - 1;
+      t[j] = target_of(p, in);
+      d[j] = backward && !p.reduction ? p.dloss[in * p.dloss_stride] : 0.0f;
+      lse[j] = backward ? p.lse[in] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < kTurn; ++j) {
+      on[j] = __ballot(r0 + j * kThreads + threadIdx.x < p.rows && t[j] != p.ignore);
+      if (lane == 0) s_wave[j * (kThreads / 64) + wave] = __popcll(on[j]);
     }
     __syncthreads();
-    const int32_t at = base + before + __popcll(b & ((1ull << lane) - 1));
-    if (r < p.rows) p.at[r] = on ? at : -1;
-    if (on) {
-      p.row[at] = static_cast<int32_t>(r);
-      p.target_at[at] = t;
-      if (backward) {
-        const float d = p.dloss[r * p.dloss_stride];
-        p.weights[at] = d;
-        p.lse_at[at] = t < 0 || t >= p.vocab ? __builtin_nanf("") : p.lse[r];
-        top = fmaxf(top, fabsf(d));
+    int32_t lo = s_wave[lane], hi = s_wave[64 + lane];
+    const int32_t own_lo = lo, own_hi = hi;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) {
+      const int32_t a = __shfl_up(lo, x, 64), c = __shfl_up(hi, x, 64);
+      lo += lane >= x ? a : 0;
+      hi += lane >= x ? c : 0;
+    }
+    const int32_t half = __shfl(lo, 63, 64), all = half + __shfl(hi, 63, 64);
+    lo -= own_lo;
+    hi += half - own_hi;
+#pragma unroll
+    for (int j = 0; j < kTurn; ++j) {
+      const int64_t r = r0 + j * kThreads + threadIdx.x;
+      const int32_t at = base + __shfl(j < kTurn / 2 ? lo : hi, j % (kTurn / 2) * (kThreads / 64) + wave, 64) +
+                         __popcll(on[j] & ((1ull << lane) - 1));
+      const bool mine = on[j] >> lane & 1;
+      if (r < p.rows) p.at[r] = mine ? at : -1;
+      if (mine) {
+        p.row[at] = static_cast<int32_t>(r);
+        p.target_at[at] = t[j];
+        if (backward) {
+          p.weights[at] = d[j];
+          p.lse_at[at] = t[j] < 0 || t[j] >= p.vocab ? __builtin_nanf("") : lse[j];
+          top = fmaxf(top, fabsf(d[j]));
+        }
       }
     }
     base += all;
+    __syncthreads();
   }
   if (threadIdx.x == 0) p.count[0] = base;
   if (!backward) return;
-  // Mean: every row's share.  fp16: the pieces hold dl times a power of two that puts the largest |dloss| at 2^12, so
-  // that small probabilities are not subnormal; the sums take it back.
+  // One number for all rows is left out of the pieces and multiplies the sums: what a target's dl is nearly is then a power
+  // of two, which its rounding keeps.  fp16: the pieces hold dl times a power of two that puts the largest at 2^12, so that
+  // small probabilities are not subnormal; the sums take it back.
+  if (p.reduction) {
+    const float up = p.dtype == MM_F16 ? 4096.0f : 1.0f;
+    for (int64_t i = threadIdx.x; i < base; i += kThreads) p.weights[i] = up;
+    if (threadIdx.x == 0) p.scalars[0] = base == 0 ? 0.0f : *p.dloss * (p.reduction == 1 ? 1.0f / static_cast<float>(base) : 1.0f) / up;
+    return;
+  }
   top = all_of(top, s_f, [](float a, float b) { return fmaxf(a, b); });
-  const float share = p.reduction == 1 ? 1.0f / static_cast<float>(base) : 1.0f;
   float up = 1.0f;
   if (p.dtype == MM_F16) {
-    const int e = static_cast<int>(__float_as_uint(top * share) >> 23) - 127;
-    if (top * share > 0.0f && e > -100 && e < 100) up = __builtin_ldexpf(1.0f, 12 - e);
+    const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+    if (top > 0.0f && e > -100 && e < 100) up = __builtin_ldexpf(1.0f, 12 - e);
+    for (int64_t i = threadIdx.x; i < base; i += kThreads) p.weights[i] *= up;  // (a thread's own or behind all_of's barrier)
   }
-  for (int64_t i = threadIdx.x; i < base; i += kThreads) p.weights[i] *= share * up;
   if (threadIdx.x == 0) p.scalars[0] = 1.0f / up;
 }
 
@@ -361,16 +390,14 @@ __global__ __launch_bounds__(kThreads) void total_kernel(const Loss p) {
   if (threadIdx.x == 0) p.loss[0] = static_cast<float>(p.reduction == 1 ? sum / static_cast<double>(*p.count) : sum);
 }
 
-// dx's part of this piece: rows that count by channels, a split of the piece's tokens; added in fp32.
+// A tile of dx's part of this piece: rows that count by channels, a split of the piece's tokens; added in fp32.
 template <int DT, typename S>
-__global__ __launch_bounds__(64 * S::NW) void dx_kernel(const Loss p) {
+__device__ __forceinline__ void dx_tile(const Loss& p, uint32_t id, int32_t count, char* s0, char* s1, char* s2, char* s3) {
   using T = typename Ty<DT>::T;
-  MM_SLAB_STAGES(S, stages)
-  const int32_t count = *p.count;
   const uint32_t mt = static_cast<uint32_t>((p.rows + S::BM - 1) / S::BM), nt = static_cast<uint32_t>((p.dim + S::BN - 1) / S::BN);
   uint32_t m, n;
-  slab::tile_of(blockIdx.x % (mt * nt), mt, nt, m, n);
-  const int64_t split = blockIdx.x / (mt * nt);
+  slab::tile_of(id % (mt * nt), mt, nt, m, n);
+  const int64_t split = id / (mt * nt);
   const int64_t r0 = static_cast<int64_t>(m) * S::BM, c0 = static_cast<int64_t>(n) * S::BN;
   if (r0 >= count) return;
   const int64_t k0 = split * p.split_k, k1 = k0 + p.split_k < p.piece_n ? k0 + p.split_k : p.piece_n;
@@ -381,7 +408,7 @@ __global__ __launch_bounds__(64 * S::NW) void dx_kernel(const Loss p) {
   dl.ld = p.piece_ld;
   dl.rows = count;
   w.rows = p.ld / static_cast<int64_t>(sizeof(T));
-  if (k1 > k0) slab::product<DT, kAlong, kAcross, S>(dl, w, r0, c0, k0, k1 - k0, stages0, stages1, stages2, stages3, acc);
+  if (k1 > k0) slab::product<DT, kAlong, kAcross, S>(dl, w, r0, c0, k0, k1 - k0, s0, s1, s2, s3, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float* const out = p.dx_part + split * p.rows * p.dim;
 #pragma unroll
@@ -403,15 +430,13 @@ __global__ __launch_bounds__(64 * S::NW) void dx_kernel(const Loss p) {
     }
 }
 
-// The piece's rows of dW.
+// A tile of the piece's rows of dW.
 template <int DT, typename S>
-__global__ __launch_bounds__(64 * S::NW) void dw_kernel(const Loss p) {
+__device__ __forceinline__ void dw_tile(const Loss& p, uint32_t id, int32_t count, char* s0, char* s1, char* s2, char* s3) {
   using T = typename Ty<DT>::T;
-  MM_SLAB_STAGES(S, stages)
-  const int32_t count = *p.count;
   const uint32_t mt = static_cast<uint32_t>((p.piece_n + S::BM - 1) / S::BM), nt = static_cast<uint32_t>((p.dim + S::BN - 1) / S::BN);
   uint32_t m, n;
-  slab::tile_of(blockIdx.x, mt, nt, m, n);
+  slab::tile_of(id, mt, nt, m, n);
   const int64_t v0 = static_cast<int64_t>(m) * S::BM, c0 = static_cast<int64_t>(n) * S::BN;
   f32x16 acc[S::TM][S::TN];
   slab::clear<S>(acc);
@@ -422,7 +447,7 @@ __global__ __launch_bounds__(64 * S::NW) void dw_kernel(const Loss p) {
   x.base = p.xc;
   x.ld = p.ld;
   x.rows = p.ld / static_cast<int64_t>(sizeof(T));
-  slab::product<DT, kAcross, kAcross, S>(dl, x, v0, c0, 0, count, stages0, stages1, stages2, stages3, acc);
+  slab::product<DT, kAcross, kAcross, S>(dl, x, v0, c0, 0, count, s0, s1, s2, s3, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float down = p.scalars[0];
 #pragma unroll
@@ -439,6 +464,15 @@ __global__ __launch_bounds__(64 * S::NW) void dw_kernel(const Loss p) {
         for (int e = 0; e < 4; ++e)
           if (8 * q + e < here) at[e * p.dim] = Ty<DT>::from(acc[i][j][4 * q + e] * down);
     }
+}
+
+// Both gradients of a piece in one launch, dx's longer sums first: the card is full until the last of dW's tiles.
+template <int DT, typename S>
+__global__ __launch_bounds__(64 * S::NW) void grads_kernel(const Loss p) {
+  MM_SLAB_STAGES(S, stages)
+  const int32_t count = *p.count;
+  if (blockIdx.x < p.dx_tiles) dx_tile<DT, S>(p, blockIdx.x, count, stages0, stages1, stages2, stages3);
+  else dw_tile<DT, S>(p, blockIdx.x - p.dx_tiles, count, stages0, stages1, stages2, stages3);
 }
 
 // dx: the splits' sums in order, rounded; zeros in the rows that are ignored.
@@ -462,19 +496,56 @@ constexpr int64_t kMaxRows = int64_t{1} << 30, kMaxVocab = int64_t{1} << 30, kMa
 constexpr int64_t kPieceBytes = int64_t{512} << 20;  // of dl kept at a time
 
 enum Size { kBig, kMid, kThin };
-// 256 x 256 tiles where they are enough for the card, else 128 x 128; 128 x 64 for few rows, where the vocabulary's
-// rows are the traffic.
-static Size size_of(int64_t m, int64_t n) {
-  if (ceil_div(m, 256) * ceil_div(n, 256) >= 192) return kBig;
-  return kMid;
+static int64_t high(Size s) { return s == kBig ? 256 : 128; }
+static int64_t wide(Size s) { return s == kBig ? 256 : s == kMid ? 128 : 64; }
+static int64_t tiles_of(Size s, int64_t m, int64_t n) { return ceil_div(m, high(s)) * ceil_div(n, wide(s)); }
+// 256 x 256 where there are enough of them to fill the card's rounds, else 128 x 128, and in fp32, whose products take
+// longer than their operands, 128 x 64.  (bf16, 1024 rows of 1024 by 8192 tokens, 128 large tiles: 27 us against 33;
+// 2048 rows, 256 of them: 47 us against 39.  fp32, 999 by 10007 of 1001, 160 large tiles: 192 us, 208 in tiles of 128 x 128,
+// 261 large; 2048 by 16384 of 1024, 512 of them: 595 us against 549.)
+static Size size_of(int dtype, int64_t big_tiles) {
+  if (dtype == MM_F32) return big_tiles >= 512 ? kBig : kThin;
+  return big_tiles >= 192 ? kBig : kMid;
 }
-static Size logits_size(int64_t vocab, int64_t rows) { return rows <= 64 ? kThin : size_of(vocab, rows); }
-static int64_t edge(Size s) { return s == kBig ? 256 : 128; }
+// 128 x 64 also for few rows, where the vocabulary's rows are the traffic.
+static Size logits_size(int dtype, int64_t vocab, int64_t rows) { return rows <= 64 ? kThin : size_of(dtype, tiles_of(kBig, vocab, rows)); }
+
+// The gradients of a piece of n tokens: tiles, and the splits of dx's few, long sums.
+struct Grads {
+  Size size;
+  int64_t splits, split_k;
+};
+static Grads grads_of(int dtype, int64_t rows, int64_t dim, int64_t n, bool dx, bool dw) {
+  // in products of a tile's row and column
+  auto work = [&](Size s) { return (dx ? tiles_of(s, rows, dim) * n : 0) + (dw ? tiles_of(s, n, dim) * rows : 0); };
+  const int64_t sum = dw && rows > 512 ? rows : 512;
+  Grads g{size_of(dtype, work(kBig) / sum), 1, n};
+  if (!dx) return g;
+  const int64_t most = n / 512 < 1 ? 1 : n / 512 < 16 ? n / 512 : 16, tiles = tiles_of(g.size, rows, dim);
+  if (dw) {
+    // none longer than the share of one place on the card (bf16, 2048 rows of 1024 by 8192 tokens: 195 us whole, 110 in
+    // two, 85 in three and in four; 8192 of 2560 by 25344: 2.06 ms whole and in four; fp32 as above: 384 us in four)
+    const int64_t places = 256 * (g.size == kBig ? 1 : g.size == kMid ? 2 : 3);
+    g.splits = ceil_div(n * places, work(g.size));
+  } else {
+    // alone: the rounds that end first, a tile's ends counted as 512 tokens
+    int64_t least = INT64_MAX;
+    for (int64_t s = 1; s <= most; ++s) {
+      const int64_t t = ceil_div(tiles * s, 256) * (ceil_div(n, s) + 512);
+      if (t < least) least = t, g.splits = s;
+    }
+  }
+  if (g.splits > most) g.splits = most;
+  g.split_k = round_up(ceil_div(n, g.splits), 64);
+  g.splits = ceil_div(n, g.split_k);
+  return g;
+}
 
 struct Plan {
-  int64_t ld, tiles, piece_n, pieces, splits, split_k;
+  int64_t ld, tiles, piece_n, pieces;
   bool copy_w;
   Size logits;
+  Grads grads;
   int64_t at, row, count, scalars, weights, lse_at, target_at, xc, wc, stats, hit, row_loss, piece, dx_part, total;
 };
 
@@ -483,8 +554,8 @@ static Plan plan_of(const mm_linear_cross_entropy_params* q, bool backward) {
   const int64_t es = dtype_size(q->dtype);
   s.ld = round_up(q->dim * es, 16);
   s.copy_w = s.ld != q->dim * es || q->weight_stride * es % 16 != 0 || q->weight_stride * es >= (int64_t{1} << 23) || !aligned(q->weight, 16);
-  s.logits = logits_size(q->vocab, q->rows);
-  s.tiles = ceil_div(q->vocab, edge(s.logits));
+  s.logits = logits_size(q->dtype, q->vocab, q->rows);
+  s.tiles = ceil_div(q->vocab, high(s.logits));
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t was = at;
@@ -512,14 +583,11 @@ static Plan plan_of(const mm_linear_cross_entropy_params* q, bool backward) {
     s.piece_n = round_up(ceil_div(q->vocab, s.pieces), 256);
     s.pieces = ceil_div(q->vocab, s.piece_n);
     s.piece = take(q->rows * s.piece_n * es);
-    // dx has few tiles and a long sum: splits of it until there are 512 workgroups, of 512 tokens at least
-    const int64_t e = edge(size_of(q->rows, q->dim)), tiles = ceil_div(q->rows, e) * ceil_div(q->dim, e);
-    s.splits = tiles >= 256 ? 1 : ceil_div(512, tiles);
-    const int64_t limit = s.piece_n / 512 > 0 ? s.piece_n / 512 : 1;
-    if (s.splits > limit) s.splits = limit;
-    s.split_k = round_up(ceil_div(s.piece_n, s.splits), 64);
-    s.splits = ceil_div(s.piece_n, s.split_k);
-    s.dx_part = take(s.splits * q->rows * q->dim * 4);
+    s.logits = logits_size(q->dtype, s.piece_n, q->rows);
+    // (the workspace's size does not hang on which of the gradients are asked for)
+    const Grads both = grads_of(q->dtype, q->rows, q->dim, s.piece_n, true, true), one = grads_of(q->dtype, q->rows, q->dim, s.piece_n, true, false);
+    s.grads = !q->dx ? grads_of(q->dtype, q->rows, q->dim, s.piece_n, false, true) : q->dweight ? both : one;
+    s.dx_part = take((both.splits > one.splits ? both.splits : one.splits) * q->rows * q->dim * 4);
   }
   s.total = at;
   return s;
@@ -584,8 +652,8 @@ static Loss loss_of(const mm_linear_cross_entropy_params* q, const Plan& s, bool
     p.piece = ws + s.piece;
     p.piece_ld = s.piece_n * dtype_size(q->dtype);
     p.dx_part = reinterpret_cast<float*>(ws + s.dx_part);
-    p.splits = s.splits;
-    p.split_k = s.split_k;
+    p.splits = s.grads.splits;
+    p.split_k = s.grads.split_k;
   }
   return p;
 }
@@ -613,19 +681,22 @@ template <int DT, bool GRAD>
 static void launch_logits(const Loss& p, Size size, int64_t vocab, hipStream_t st) {
   switch (size) {
     case kBig: launch_logits_t<DT, Big, GRAD>(p, vocab, st); break;
-    case kMid: launch_logits_t<DT, Mid, GRAD>(p, vocab, st); break;
-    default: launch_logits_t<DT, Thin, GRAD>(p, vocab, st); break;
+    case kMid:
+      if constexpr (DT != MM_F32) launch_logits_t<DT, Mid, GRAD>(p, vocab, st);
+      break;
+    case kThin: launch_logits_t<DT, Thin, GRAD>(p, vocab, st); break;
   }
 }
 template <int DT, typename S>
-static void launch_dx_t(const Loss& p, hipStream_t st) {
-  const int64_t tiles = ceil_div(p.rows, S::BM) * ceil_div(p.dim, S::BN);
-  hipLaunchKernelGGL((dx_kernel<DT, S>), dim3(static_cast<unsigned>(tiles * p.splits)), dim3(64 * S::NW), 0, st, p);
+static void launch_grads_t(Loss p, hipStream_t st) {
+  p.dx_tiles = p.dx ? static_cast<uint32_t>(ceil_div(p.rows, S::BM) * ceil_div(p.dim, S::BN) * p.splits) : 0;
+  const int64_t dw = p.dweight ? ceil_div(p.piece_n, S::BM) * ceil_div(p.dim, S::BN) : 0;
+  hipLaunchKernelGGL((grads_kernel<DT, S>), dim3(static_cast<unsigned>(p.dx_tiles + dw)), dim3(64 * S::NW), 0, st, p);
 }
-template <int DT, typename S>
-static void launch_dw_t(const Loss& p, hipStream_t st) {
-  const int64_t tiles = ceil_div(p.piece_n, S::BM) * ceil_div(p.dim, S::BN);
-  hipLaunchKernelGGL((dw_kernel<DT, S>), dim3(static_cast<unsigned>(tiles)), dim3(64 * S::NW), 0, st, p);
+template <int DT>
+static void launch_grads(const Loss& p, Size size, hipStream_t st) {
+  if (size == kBig) return launch_grads_t<DT, Big>(p, st);
+  if constexpr (DT == MM_F32) launch_grads_t<DT, Thin>(p, st); else launch_grads_t<DT, Mid>(p, st);
 }
 
 template <int DT>
@@ -642,13 +713,8 @@ static void backward(Loss p, const Plan& s, hipStream_t st) {
     p.piece0 = k * s.piece_n;
     p.piece_n = p.piece0 + s.piece_n < p.vocab ? s.piece_n : p.vocab - p.piece0;
     p.first_piece = k == 0;
-    launch_logits<DT, true>(p, logits_size(s.piece_n, p.rows), s.piece_n, st);
-    if (p.dx) {
-      if (size_of(p.rows, p.dim) == kBig) launch_dx_t<DT, Big>(p, st); else launch_dx_t<DT, Mid>(p, st);
-    }
-    if (p.dweight) {
-      if (size_of(p.piece_n, p.dim) == kBig) launch_dw_t<DT, Big>(p, st); else launch_dw_t<DT, Mid>(p, st);
-    }
+    launch_logits<DT, true>(p, s.logits, s.piece_n, st);
+    if (p.dx || p.dweight) launch_grads<DT>(p, s.grads.size, st);
   }
   if (p.dx) hipLaunchKernelGGL((finish_dx_kernel<DT>), dim3(static_cast<unsigned>(p.rows)), dim3(256), 0, st, p);
 }

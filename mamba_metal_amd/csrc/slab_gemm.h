@@ -20,6 +20,8 @@
 // of 2; an accumulator holds column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4.
 #pragma once
 
+#include <type_traits>
+
 #include "mm_common.h"
 
 namespace mm {
@@ -38,16 +40,15 @@ constexpr int kSteps = 2;  // of 32 bytes
 enum Lie { kAlong, kAcross };
 
 template <int DT>
-__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+constexpr int kParts = DT == MM_F32 ? 4 : 1;  // products that 16 bytes of each operand make
+template <int DT>
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, int part, f32x16 c) {
   if constexpr (DT == MM_F16) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   } else if constexpr (DT == MM_BF16) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
-    return c;
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[part]), __uint_as_float(b[part]), c, 0, 0, 0);
   }
 }
 
@@ -68,7 +69,7 @@ __device__ __forceinline__ void load_direct(const char* base, uint32_t off, char
 template <int DT, Lie LIE, int R, int NW>
 struct Side {
   using T = typename Ty<DT>::T;
-  static constexpr int kEs = sizeof(T);
+  static constexpr int kEs = sizeof(T), kWidth = R;
   static constexpr int kDepth = kSlab / kEs;               // elements of k in a slab
   static constexpr int kLoads = R * kSlab / 1024 / NW;     // of a wave, 64 lanes of 16 bytes each
   static constexpr int kReads = LIE == kAlong ? 1 : kEs == 2 ? 2 : 4;  // of an operand
@@ -126,16 +127,6 @@ struct Side {
     if constexpr (LIE == kAlong) {
       const int r = r0 + (lane & 31), c = 2 * s + (lane >> 5);
       return *reinterpret_cast<const u32x4*>(tile + r * kSlab + ((c ^ (r >> 2 & 3)) << 4));
-    } else if constexpr (kEs == 2) {
-      // 16 lanes read 4 rows of k by 16 columns, 8 bytes each, and get a column each
-      constexpr int four = kRows == 2 ? 2 * kLoadBytes : 4 * R * kEs;  // bytes of 4 rows of k
-      const int row = (lane & 15) >> 2, in = ((lane & 16) >> 3 | (lane & 3) >> 1) * 16 + (lane & 1) * 8;
-      const int lie = kRows == 2 ? (row >> 1) * kLoadBytes + (row & 1) * 64 : row * 64;
-      const char* const p = tile + (r0 >> 5) * (kSide * 64) + (4 * s + 2 * (lane >> 5)) * four + lie + in;
-      typedef __attribute__((address_space(3))) s16x4 Lds;
-      const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p)));
-      const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p + four)));
-      return u32x4{a[0], a[1], b[0], b[1]};
     } else {
       u32x4 v;
       const char* const p = tile + (8 * s + 4 * (lane >> 5)) * R * kEs + (r0 + (lane & 31)) * kEs;
@@ -145,6 +136,66 @@ struct Side {
     }
   }
 };
+
+// 16-bit kAcross: where a lane's reads of columns r0 on begin, and what a column tile, a step and 4 rows of k are further.
+// 16 lanes read 4 rows of k by 16 columns, 8 bytes each, and get a column each.
+template <typename SIDE>
+struct Across {
+  static constexpr int kFour = SIDE::kRows == 2 ? 2 * SIDE::kLoadBytes : 4 * SIDE::kWidth * 2, kStep = 4 * kFour, kTile = SIDE::kSide * 64;
+  static __device__ __forceinline__ uint32_t lane_at(int r0, int lane) {
+    const int row = (lane & 15) >> 2, in = ((lane & 16) >> 3 | (lane & 3) >> 1) * 16 + (lane & 1) * 8;
+    return (r0 >> 5) * kTile + 2 * (lane >> 5) * kFour + (SIDE::kRows == 2 ? (row >> 1) * SIDE::kLoadBytes + (row & 1) * 64 : row * 64) + in;
+  }
+};
+// The operands of N column tiles, or of N and M of both sides, at step S: all reads and their wait in one piece.  (The
+// compiler knows of no address in a transposing read, and would have each wait for all loads that fill other stages.)
+#define MM_TR "ds_read_b64_tr_b16 "
+template <typename C, int S>
+__device__ __forceinline__ void across2(uint32_t at, u32x4 (&o)[2]) {
+  u32x2 r[4];
+  constexpr int s = S * C::kStep, f = C::kFour, t = C::kTile;
+  asm volatile(MM_TR "%0, %4 offset:%5\n" MM_TR "%1, %4 offset:%6\n" MM_TR "%2, %4 offset:%7\n" MM_TR "%3, %4 offset:%8\n"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+               : "v"(at), "n"(s), "n"(s + f), "n"(s + t), "n"(s + t + f)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 2; ++i) o[i] = u32x4{r[2 * i][0], r[2 * i][1], r[2 * i + 1][0], r[2 * i + 1][1]};
+}
+template <typename C, typename D, int S>
+__device__ __forceinline__ void across22(uint32_t at, uint32_t bt, u32x4 (&o)[2], u32x4 (&p)[2]) {
+  u32x2 r[8];
+  constexpr int s = S * C::kStep, f = C::kFour, t = C::kTile, s2 = S * D::kStep, f2 = D::kFour, t2 = D::kTile;
+  asm volatile(MM_TR "%0, %8 offset:%10\n" MM_TR "%1, %8 offset:%11\n" MM_TR "%2, %8 offset:%12\n" MM_TR "%3, %8 offset:%13\n"
+               MM_TR "%4, %9 offset:%14\n" MM_TR "%5, %9 offset:%15\n" MM_TR "%6, %9 offset:%16\n" MM_TR "%7, %9 offset:%17\n"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+               : "v"(at), "v"(bt), "n"(s), "n"(s + f), "n"(s + t), "n"(s + t + f), "n"(s2), "n"(s2 + f2), "n"(s2 + t2), "n"(s2 + t2 + f2)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 2; ++i) o[i] = u32x4{r[2 * i][0], r[2 * i][1], r[2 * i + 1][0], r[2 * i + 1][1]};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) p[i] = u32x4{r[4 + 2 * i][0], r[4 + 2 * i][1], r[5 + 2 * i][0], r[5 + 2 * i][1]};
+}
+template <typename C, typename D, int S>
+__device__ __forceinline__ void across42(uint32_t at, uint32_t bt, u32x4 (&o)[4], u32x4 (&p)[2]) {
+  u32x2 r[12];
+  constexpr int s = S * C::kStep, f = C::kFour, t = C::kTile, s2 = S * D::kStep, f2 = D::kFour, t2 = D::kTile;
+  asm volatile(MM_TR "%0, %12 offset:%14\n" MM_TR "%1, %12 offset:%15\n" MM_TR "%2, %12 offset:%16\n" MM_TR "%3, %12 offset:%17\n"
+               MM_TR "%4, %12 offset:%18\n" MM_TR "%5, %12 offset:%19\n" MM_TR "%6, %12 offset:%20\n" MM_TR "%7, %12 offset:%21\n"
+               MM_TR "%8, %13 offset:%22\n" MM_TR "%9, %13 offset:%23\n" MM_TR "%10, %13 offset:%24\n" MM_TR "%11, %13 offset:%25\n"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]), "=&v"(r[8]),
+                 "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11])
+               : "v"(at), "v"(bt), "n"(s), "n"(s + f), "n"(s + t), "n"(s + t + f), "n"(s + 2 * t), "n"(s + 2 * t + f), "n"(s + 3 * t),
+                 "n"(s + 3 * t + f), "n"(s2), "n"(s2 + f2), "n"(s2 + t2), "n"(s2 + t2 + f2)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = u32x4{r[2 * i][0], r[2 * i][1], r[2 * i + 1][0], r[2 * i + 1][1]};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) p[i] = u32x4{r[8 + 2 * i][0], r[8 + 2 * i][1], r[9 + 2 * i][0], r[9 + 2 * i][1]};
+}
+#undef MM_TR
 
 // A tile's shape: BM x BN by WM x WN waves, each TM x TN tiles of 32 x 32; ST stages.
 template <int BM_, int BN_, int WM_, int WN_, int ST_>
@@ -172,12 +223,11 @@ __device__ __forceinline__ void meet() {
 }
 
 // acc += the sum over `k` elements from k0 on.  All threads of the workgroup; returns when nobody reads or loads the
-// stages any more.  (__restrict__: what tells the compiler of the transposing reads that a stage is none of the others;
-// else each would wait for all loads under way.)
+// stages any more.
 template <int DT, Lie LA, Lie LB, typename S>
 __device__ __forceinline__ void product(const Matrix& A, const Matrix& B, int64_t m0, int64_t n0, int64_t k0, int64_t k,
-                                        char* __restrict__ s0, char* __restrict__ s1, char* __restrict__ s2,
-                                        char* __restrict__ s3, f32x16 (&acc)[S::TM][S::TN]) {
+                                        char* s0, char* s1, char* s2, char* s3,
+                                         f32x16 (&acc)[S::TM][S::TN]) {
   static_assert(S::ST == 4, "as many objects");
   using SA = Side<DT, LA, S::BM, S::NW>;
   using SB = Side<DT, LB, S::BN, S::NW>;
@@ -197,19 +247,37 @@ __device__ __forceinline__ void product(const Matrix& A, const Matrix& B, int64_
   struct Step {
     u32x4 a[S::TM], b[S::TN];
   };
-  auto read = [&](const char* from, int s) __attribute__((always_inline)) {
+  constexpr bool kTrA = LA == kAcross && SA::kEs == 2, kTrB = LB == kAcross && SB::kEs == 2;
+  uint32_t tr_a = 0, tr_b = 0;
+  if constexpr (kTrA) tr_a = Across<SA>::lane_at(wm, lane);
+  if constexpr (kTrB) tr_b = Across<SB>::lane_at(wn, lane) + SA::kBytes;
+  auto read = [&](const char* from, auto step) __attribute__((always_inline)) {
+    constexpr int s = decltype(step)::value;
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)from));
     Step q;
+    if constexpr (!kTrA) {
 #pragma unroll
-    for (int i = 0; i < S::TM; ++i) q.a[i] = SA::operand(from, wm + 32 * i, s, lane);
+      for (int i = 0; i < S::TM; ++i) q.a[i] = SA::operand(from, wm + 32 * i, s, lane);
+    }
+    if constexpr (!kTrB) {
 #pragma unroll
-    for (int j = 0; j < S::TN; ++j) q.b[j] = SB::operand(from + SA::kBytes, wn + 32 * j, s, lane);
+      for (int j = 0; j < S::TN; ++j) q.b[j] = SB::operand(from + SA::kBytes, wn + 32 * j, s, lane);
+    }
+    if constexpr (kTrA && S::TM == 4) across42<Across<SA>, Across<SB>, s>(at + tr_a, at + tr_b, q.a, q.b);
+    else if constexpr (kTrA) across22<Across<SA>, Across<SB>, s>(at + tr_a, at + tr_b, q.a, q.b);
+    else if constexpr (kTrB) across2<Across<SB>, s>(at + tr_b, q.b);
+    static_assert(!kTrA || kTrB, "both, or B alone");
     return q;
   };
+  using First = std::integral_constant<int, 0>;
+  using Second = std::integral_constant<int, 1>;
   auto multiply = [&](const Step& q) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < S::TM; ++i)
+    for (int part = 0; part < kParts<DT>; ++part)  // (neighbours in time add to different sums)
 #pragma unroll
-      for (int j = 0; j < S::TN; ++j) acc[i][j] = mma<DT>(q.a[i], q.b[j], acc[i][j]);
+      for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc[i][j] = mma<DT>(q.a[i], q.b[j], part, acc[i][j]);
   };
   constexpr int kLoads = SA::kLoads + SB::kLoads;
   static_assert(kSteps == 2, "a slab's first step before the others are met, its second behind it");
@@ -218,21 +286,35 @@ __device__ __forceinline__ void product(const Matrix& A, const Matrix& B, int64_
   load(s2, 2);
   load(s3, 3);
   meet<(S::ST - 1) * kLoads>();
-  Step q0 = read(s0, 0), q1;
+  Step q0 = read(s0, First{}), q1;
   // The slab's second step is multiplied when nobody reads the slab any more and the next one is there: that one's first
   // operands are read, and the loads that take the slab's place issued, under those products.  (Past the last slab zeros
   // are loaded, so that the count of loads under way stays the same.)
   auto slab = [&](char* here, const char* there, int64_t t) __attribute__((always_inline)) {
-    q1 = read(here, 1);
-    __builtin_amdgcn_sched_barrier(0);  // (the reads first: the compiler would put each next to its use)
-    multiply(q0);
-    __builtin_amdgcn_sched_barrier(0);
-    meet<(S::ST - 2) * kLoads>();
-    q0 = read(there, 0);
-    load(here, t + S::ST);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(q1);
-    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kTrB) {
+      // (these reads end with a wait: under it the other wave's products, and this one's that are under way)
+      multiply(q0);
+      __builtin_amdgcn_sched_barrier(0);
+      q1 = read(here, Second{});
+      meet<(S::ST - 2) * kLoads>();
+      load(here, t + S::ST);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(q1);
+      __builtin_amdgcn_sched_barrier(0);
+      q0 = read(there, First{});
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      q1 = read(here, Second{});
+      __builtin_amdgcn_sched_barrier(0);  // (the reads first: the compiler would put each next to its use)
+      multiply(q0);
+      __builtin_amdgcn_sched_barrier(0);
+      meet<(S::ST - 2) * kLoads>();
+      q0 = read(there, First{});
+      load(here, t + S::ST);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(q1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   int64_t t = 0;
   for (; t + S::ST <= slabs; t += S::ST) {
