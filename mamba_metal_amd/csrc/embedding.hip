@@ -5,9 +5,12 @@
 // All of it is memory traffic.  The gradient's rows are sums in a fixed order, so that calls repeat bit for bit: the
 // tokens are sorted by id (a stable radix sort, least digit first, of up to 9 bits a pass), runs of equal ids are
 // summed in fp32 in the order of their positions, and rounded once.  A run may be any length (the commonest token of a
-// text takes several percent of it): the sorted tokens are cut into tiles of 32, and what a run leaves in the tiles it
+// text takes several percent of it): the sorted tokens are cut into tiles of 16, and what a run leaves in the tiles it
 // crosses is joined by a last kernel.  Rows without a token are zeros; the whole table is cleared by workgroups that run
-// beside the sort's (whose few workgroups would leave the card idle), at no cost of their own.
+// beside the sort's (whose few workgroups would leave the card idle), at no cost of their own.  Up to 16384 tokens are
+// sorted by one workgroup in its LDS, in one launch; more by counting and scattering, a launch for each digit.
+#include <type_traits>
+
 #include "mm_common.h"
 
 namespace mm {
@@ -19,7 +22,9 @@ constexpr int kBlock = 2048;     // tokens a workgroup of the sort
 constexpr int kWaveItems = kBlock / 4;
 constexpr int kRounds = kWaveItems / 64;
 constexpr int kMaxBits = 9;      // of a digit
-constexpr int kTile = 32;        // sorted tokens a wave sums
+constexpr int kTile = 16;        // sorted tokens a wave sums
+constexpr int kOne = 16384, kOneThreads = 1024;  // tokens that one workgroup sorts: a key and a place of 14 bits in a word
+constexpr int64_t kOneVocab = int64_t{1} << 18;
 constexpr int64_t kClear = 64 << 10;  // bytes a clearing workgroup writes
 
 struct Params {
@@ -48,18 +53,17 @@ __device__ __forceinline__ uint32_t key_of(const Params& p, int64_t i) {
 
 // kV elements at once: 16 bytes, or single elements where rows are not aligned.
 template <int DT, int kV>
-__device__ __forceinline__ void load_elems(const void* base, int64_t at, float (&x)[kV]) {
-  using T = typename Ty<DT>::T;
-  const T* const p = static_cast<const T*>(base) + at;
-  if constexpr (kV == 1) {
-    x[0] = Ty<DT>::f(*p);
-  } else {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
-    T t[kV];
-    __builtin_memcpy(t, &w, 16);
+using Raw = std::conditional_t<kV == 1, typename Ty<DT>::T, u32x4>;
+template <int DT, int kV>
+__device__ __forceinline__ Raw<DT, kV> load_raw(const void* base, int64_t at) {
+  return *reinterpret_cast<const Raw<DT, kV>*>(static_cast<const typename Ty<DT>::T*>(base) + at);
+}
+template <int DT, int kV>
+__device__ __forceinline__ void elems_of(const Raw<DT, kV>& w, float (&x)[kV]) {
+  typename Ty<DT>::T t[kV];
+  __builtin_memcpy(t, &w, sizeof(t));
 #pragma unroll
-    for (int j = 0; j < kV; ++j) x[j] = Ty<DT>::f(t[j]);
-  }
+  for (int j = 0; j < kV; ++j) x[j] = Ty<DT>::f(t[j]);
 }
 // (x scale) as an fp32 product, then rounded: the empty asm keeps the two from becoming one mixed-precision instruction in
 // some kernels and not in others.
@@ -98,7 +102,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const Params p, int lanes) {
   for (int64_t u = lane & (lanes - 1); u < units; u += lanes) {
     float x[kV];
     if (in) {
-      load_elems<DT, kV>(p.weight, id * p.ld + u * kV, x);
+      elems_of<DT, kV>(load_raw<DT, kV>(p.weight, id * p.ld + u * kV), x);
     } else {
 #pragma unroll
       for (int j = 0; j < kV; ++j) x[j] = __builtin_nanf("");
@@ -108,6 +112,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const Params p, int lanes) {
 }
 
 // This launch's share of clearing the table: share `part` of `parts`, by the workgroups from p.sort_blocks on.
+template <int NT>
 __device__ __forceinline__ void clear_share(const Params& p, int64_t bytes0, int64_t bytes1) {
   const int64_t b0 = bytes0 + (blockIdx.x - p.sort_blocks) * kClear;
   const int64_t b1 = b0 + kClear < bytes1 ? b0 + kClear : bytes1;
@@ -116,17 +121,108 @@ __device__ __forceinline__ void clear_share(const Params& p, int64_t bytes0, int
   if ((reinterpret_cast<uintptr_t>(base) & 15) == 0) {
     int64_t at = b0 + threadIdx.x * 16;
 #pragma unroll 4
-    for (; at + 16 <= b1; at += 256 * 16) *reinterpret_cast<u32x4*>(base + at) = u32x4{0, 0, 0, 0};
+    for (; at + 16 <= b1; at += NT * 16) *reinterpret_cast<u32x4*>(base + at) = u32x4{0, 0, 0, 0};
     if (at < b1)
       for (; at < b1; at += 2) *reinterpret_cast<uint16_t*>(base + at) = 0;
   } else {
-    for (int64_t at = b0 + threadIdx.x * 2; at < b1; at += 512) *reinterpret_cast<uint16_t*>(base + at) = 0;
+    for (int64_t at = b0 + threadIdx.x * 2; at < b1; at += 2 * NT) *reinterpret_cast<uint16_t*>(base + at) = 0;
+  }
+}
+
+// Lanes of a wave with this lane's digit among those of `in`.
+__device__ __forceinline__ uint64_t equals(uint64_t in, uint32_t d, int bits) {
+  uint64_t same = in;
+#pragma unroll
+  for (int b = 0; b < kMaxBits; ++b) {
+    if (b >= bits) break;
+    const bool one = d >> b & 1;
+    const uint64_t on = __ballot(one);
+    same &= one ? on : ~on;
+  }
+  return same;
+}
+
+// The whole sort, by workgroup 0; the others clear the table.  A wave holds 64 `rounds` neighbouring tokens in registers; a
+// pass ranks them among its own, a round at a time, joins the waves' counts, and sends them through the LDS.
+__global__ __launch_bounds__(kOneThreads) void sort_kernel(const Params p, int passes, int bits, int rounds, int64_t clear1) {
+  if (blockIdx.x >= p.sort_blocks) return clear_share<kOneThreads>(p, 0, clear1);
+  constexpr int kWaves = kOneThreads / 64, kRegs = kOne / kOneThreads;
+  __shared__ uint32_t s_item[kOne];
+  __shared__ uint32_t s_wave[kWaves][1 << kMaxBits];
+  __shared__ uint32_t s_sum[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = static_cast<int>(p.n), digits = 1 << bits, i0 = wave * 64 * rounds + lane;
+  const uint32_t mask = digits - 1;
+  uint32_t item[kRegs], at[kRegs];
+#pragma unroll
+  for (int r = 0; r < kRegs; ++r) {
+    const int i = i0 + r * 64;
+    item[r] = r < rounds && i < n ? key_of(p, i) << 14 | i : 0;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = 14 + pass * bits;
+    for (int d = lane; d < digits; d += 64) s_wave[wave][d] = 0;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < kRegs; ++r) {
+      if (r >= rounds) break;
+      const bool in = i0 + r * 64 < n;
+      const uint32_t d = item[r] >> shift & mask;
+      const uint64_t same = equals(__ballot(in), d, bits), below = same & ((1ull << lane) - 1);
+      const uint32_t first = s_wave[wave][d];
+      __builtin_amdgcn_wave_barrier();
+      if (in && below == 0) s_wave[wave][d] = first + __popcll(same);
+      __builtin_amdgcn_wave_barrier();
+      at[r] = first + __popcll(below);
+    }
+    __syncthreads();
+    // where a digit's tokens of a wave begin: behind all smaller digits, and this one's in the waves before
+    uint32_t count[kWaves], total = 0;
+    if (tid < digits) {
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        count[w] = s_wave[w][tid];
+        total += count[w];
+      }
+    }
+    uint32_t incl = total;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) {
+      const uint32_t up = __shfl_up(incl, x, 64);
+      incl += lane >= x ? up : 0;
+    }
+    if (lane == 63) s_sum[wave] = incl;
+    __syncthreads();
+    if (tid < digits) {
+      uint32_t start = incl - total;
+      for (int w = 0; w < wave; ++w) start += s_sum[w];
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        s_wave[w][tid] = start;
+        start += count[w];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRegs; ++r)
+      if (r < rounds && i0 + r * 64 < n) s_item[s_wave[wave][item[r] >> shift & mask] + at[r]] = item[r];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRegs; ++r)
+      if (r < rounds && i0 + r * 64 < n) item[r] = s_item[i0 + r * 64];
+  }
+#pragma unroll
+  for (int r = 0; r < kRegs; ++r) {
+    const int i = i0 + r * 64;
+    if (r >= rounds || i >= n) break;
+    p.key[0][i] = item[r] >> 14;
+    p.pos[0][i] = item[r] & (kOne - 1);
   }
 }
 
 // First launch: how often each value of the first digit occurs in each block of tokens; clears the second's counts.
 __global__ __launch_bounds__(256) void count_kernel(const Params p, int bits, int64_t hist_words, int64_t clear1) {
-  if (blockIdx.x >= p.sort_blocks) return clear_share(p, 0, clear1);
+  if (blockIdx.x >= p.sort_blocks) return clear_share<256>(p, 0, clear1);
   __shared__ uint32_t s_hist[1 << kMaxBits];
   const int digits = 1 << bits;
   for (int d = threadIdx.x; d < digits; d += 256) s_hist[d] = 0;
@@ -146,7 +242,7 @@ __global__ __launch_bounds__(256) void count_kernel(const Params p, int bits, in
 // One pass: each block's tokens to their places by one digit, stably, and the counts of the next digit at the new
 // places (integer atomics: their order does not matter).  hist `in` belongs to this pass; `out` is cleared for use.
 __global__ __launch_bounds__(256) void scatter_kernel(const Params p, int pass, int passes, int bits, int64_t clear0, int64_t clear1) {
-  if (blockIdx.x >= p.sort_blocks) return clear_share(p, clear0, clear1);
+  if (blockIdx.x >= p.sort_blocks) return clear_share<256>(p, clear0, clear1);
   __shared__ uint32_t s_base[1 << kMaxBits];
   __shared__ uint32_t s_wave[4][1 << kMaxBits];
   __shared__ uint32_t s_sum[4];
@@ -196,12 +292,7 @@ __global__ __launch_bounds__(256) void scatter_kernel(const Params p, int pass, 
   for (int r = 0; r < kRounds; ++r) {
     const bool in = i0 + r * 64 + lane < p.n;
     const uint32_t d = key[r] >> (pass * bits) & mask;
-    uint64_t same = __ballot(in);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t on = __ballot(d >> b & 1);
-      same &= d >> b & 1 ? on : ~on;
-    }
-    const uint64_t below = same & ((1ull << lane) - 1);
+    const uint64_t same = equals(__ballot(in), d, bits), below = same & ((1ull << lane) - 1);
     uint32_t first = 0;
     if (in) first = s_wave[wave][d];
     __builtin_amdgcn_wave_barrier();
@@ -230,99 +321,92 @@ __global__ __launch_bounds__(256) void clear_counts_kernel(uint32_t* hist, int64
   if (i < words) hist[i] = 0;
 }
 
-// A wave sums 32 sorted tokens over 64 kV columns: whole runs go to the table, the parts of runs that reach over an
-// edge of the tile to the workspace (first: one that began before; last: one that goes on, if it is not the first).
+// A wave sums 16 sorted tokens over 64 kV columns, all their rows under way at once: whole runs go to the table, the parts
+// of runs that reach over an edge of the tile to the workspace (first: one that began before; last: one that goes on, if it
+// is not the first).
 template <int DT, int kV>
 __global__ __launch_bounds__(256) void sum_kernel(const Params p, int last, int64_t chunks) {
   const int lane = threadIdx.x & 63;
   const int64_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   const int64_t tile = wave / chunks, c0 = (wave % chunks) * 64 * kV + lane * kV;
   if (tile >= p.tiles) return;
-  const uint32_t* const key = p.key[last];
-  const uint32_t* const pos = p.pos[last];
-  const int64_t i0 = tile * kTile, i1 = i0 + kTile < p.n ? i0 + kTile : p.n;
+  const uint32_t vocab = static_cast<uint32_t>(p.vocab);
+  const int64_t i0 = tile * kTile;
   const bool on = c0 < p.dim;
+  // lanes 0 .. 17: the keys from the token before the tile to the one behind it (beyond the tokens: of none)
+  const int64_t in = i0 - 1 + lane;
+  const bool there = lane < kTile + 2 && in >= 0 && in < p.n;
+  const uint32_t own_key = there ? p.key[last][in] : ~0u, own_pos = there ? p.pos[last][in] : 0;
+  uint32_t k[kTile + 2];
+  Raw<DT, kV> x[kTile];
+#pragma unroll
+  for (int e = 0; e < kTile + 2; ++e) k[e] = __builtin_amdgcn_readlane(own_key, e);
+#pragma unroll
+  for (int e = 0; e < kTile; ++e) {
+    const int64_t row = static_cast<uint32_t>(__builtin_amdgcn_readlane(own_pos, e + 1));
+    x[e] = Raw<DT, kV>{};
+    if (k[e + 1] < vocab && on) x[e] = load_raw<DT, kV>(p.dy, row * p.dy_ld + c0);
+  }
   float sum[kV];
 #pragma unroll
   for (int j = 0; j < kV; ++j) sum[j] = 0.0f;
-  uint32_t run = key[i0];
-  bool began = i0 == 0 || key[i0 - 1] != run;  // in this tile
-  for (int64_t i = i0; i < i1; i += 8) {
-    uint32_t k[8];
-    float x[8][kV];
+  bool began = k[0] != k[1];  // the run, in this tile
 #pragma unroll
-    for (int e = 0; e < 8; ++e) k[e] = i + e < i1 ? key[i + e] : static_cast<uint32_t>(p.vocab);
+  for (int e = 0; e < kTile; ++e) {
+    float f[kV];
+    elems_of<DT, kV>(x[e], f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int j = 0; j < kV; ++j) sum[j] += f[j];
+    const bool ends = k[e + 2] != k[e + 1];
+    if ((ends || e == kTile - 1) && k[e + 1] < vocab) {
+      if (on) {
+        if (began && ends) {
+          store_elems<DT, kV>(p.out, k[e + 1] * p.dim + c0, sum, p.scale);
+        } else {
 #pragma unroll
-      for (int j = 0; j < kV; ++j) x[e][j] = 0.0f;
-      if (k[e] < p.vocab && on) load_elems<DT, kV>(p.dy, static_cast<int64_t>(pos[i + e]) * p.dy_ld + c0, x[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (i + e < i1 && k[e] != run) {
-        if (run < p.vocab && on) {
-          if (began) {
-            store_elems<DT, kV>(p.out, run * p.dim + c0, sum, p.scale);
-          } else {
-#pragma unroll
-            for (int j = 0; j < kV; ++j) p.part[(tile * 2) * p.dim + c0 + j] = sum[j];
-          }
+          for (int j = 0; j < kV; ++j) p.part[(tile * 2 + (began ? 1 : 0)) * p.dim + c0 + j] = sum[j];
         }
-        run = k[e];
-        began = true;
-#pragma unroll
-        for (int j = 0; j < kV; ++j) sum[j] = 0.0f;
       }
-#pragma unroll
-      for (int j = 0; j < kV; ++j) sum[j] += x[e][j];
     }
-  }
-  if (run >= p.vocab || !on) return;
-  const bool ends = i1 == p.n || key[i1] != run;
-  if (began && ends) {
-    store_elems<DT, kV>(p.out, run * p.dim + c0, sum, p.scale);
-  } else {
+    if (ends) {
+      began = true;
 #pragma unroll
-    for (int j = 0; j < kV; ++j) p.part[(tile * 2 + (began ? 1 : 0)) * p.dim + c0 + j] = sum[j];
+      for (int j = 0; j < kV; ++j) sum[j] = 0.0f;
+    }
   }
 }
 
-// Joins the run that begins in a tile and goes on behind it.
-template <int DT, int kV>
+// Joins the run that begins in a tile and goes on behind it: a wave for 64 columns (few runs are long, and a long one's
+// sum is a chain of loads: narrow waves make many chains).
+template <int DT>
 __global__ __launch_bounds__(256) void join_kernel(const Params p, int last, int64_t chunks) {
   const int lane = threadIdx.x & 63;
   const int64_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int64_t tile = wave / chunks, c0 = (wave % chunks) * 64 * kV + lane * kV;
-  const uint32_t* const key = p.key[last];
-  const int64_t next = (tile + 1) * kTile;
+  const int64_t tile = wave / chunks, c = (wave % chunks) * 64 + lane, next = (tile + 1) * kTile;
   if (next >= p.n) return;
-  const uint32_t run = key[next - 1];
-  if (run >= p.vocab || key[next] != run) return;
-  if (key[tile * kTile] == run && tile > 0 && key[tile * kTile - 1] == run) return;  // began before this tile
-  if (c0 >= p.dim) return;
-  float sum[kV];
+  const uint32_t* const key = p.key[last];
+  const uint32_t run = key[next - 1], behind = key[next], first = key[tile * kTile], before = tile > 0 ? key[tile * kTile - 1] : ~0u;
+  if (run >= static_cast<uint32_t>(p.vocab) || behind != run || (first == run && before == run)) return;
+  const bool on = c < p.dim;
+  const float* const part = p.part + (on ? c : 0);
+  float sum = part[(tile * 2 + 1) * p.dim];
+  // tiles wholly of this run, and the last one, whose first run it is: a lane looks at each edge of the next 64
+  for (int64_t t = tile + 1, some = 64; some == 64; t += 64) {
+    const int64_t edge = (t + 1 + lane) * kTile;
+    const bool in = edge < p.n;
+    const uint32_t k0 = key[in ? edge - 1 : 0], k1 = key[in ? edge : 0];
+    const uint64_t over = __ballot(in && k0 == run && k1 == run);
+    some = over == ~0ull ? 64 : __builtin_ctzll(~over);
+    const int64_t upto = some < 64 ? some + 1 : 64;
+    for (int64_t e = 0; e < upto; e += 16) {
+      float x[16];
 #pragma unroll
-  for (int j = 0; j < kV; ++j) sum[j] = p.part[(tile * 2 + 1) * p.dim + c0 + j];
-  // tiles wholly of this run, and the last one, whose first run it is
-  int64_t t = tile + 1;
-  for (bool more = true; more;) {
-    int64_t t1 = t;
-    // as far as the next eight tiles go on
-#pragma unroll 1
-    for (int e = 0; e < 8; ++e) {
-      ++t1;
-      if (t1 * kTile >= p.n || key[t1 * kTile - 1] != run || key[t1 * kTile] != run) {
-        more = false;
-        break;
-      }
+      for (int j = 0; j < 16; ++j) x[j] = part[(t + (e + j < upto ? e + j : e)) * 2 * p.dim];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum += e + j < upto ? x[j] : 0.0f;
     }
-#pragma unroll 8
-    for (; t < t1; ++t)
-#pragma unroll
-      for (int j = 0; j < kV; ++j) sum[j] += p.part[(t * 2) * p.dim + c0 + j];
   }
-  store_elems<DT, kV>(p.out, run * p.dim + c0, sum, p.scale);
+  if (on) static_cast<typename Ty<DT>::T*>(p.out)[run * p.dim + c] = scaled<DT>(sum, p.scale);
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
@@ -331,6 +415,7 @@ constexpr int64_t kMaxTokens = int64_t{1} << 31, kMaxVocab = int64_t{1} << 30, k
 struct Plan {
   int64_t blocks, tiles, hist_words, key_at[2], pos_at[2], hist_at[2], part_at, total;
   int bits, passes;
+  bool one;
 };
 // The digits of the keys 0 .. vocab: as few passes as digits of 9 bits allow, of equal widths.
 static Plan plan_of(int64_t n, int64_t vocab, int64_t dim) {
@@ -339,16 +424,17 @@ static Plan plan_of(int64_t n, int64_t vocab, int64_t dim) {
   while ((vocab >> width) != 0) ++width;
   s.passes = (width + kMaxBits - 1) / kMaxBits;
   s.bits = (width + s.passes - 1) / s.passes;
-  s.blocks = ceil_div(n, kBlock);
+  s.one = n <= kOne && vocab < kOneVocab;
+  s.blocks = s.one ? n > 0 : ceil_div(n, kBlock);
   s.tiles = ceil_div(n, kTile);
-  s.hist_words = s.blocks << s.bits;
+  s.hist_words = s.one ? 0 : s.blocks << s.bits;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t was = at;
     at += round_up(bytes, 256);
     return was;
   };
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < (s.one ? 1 : 2); ++k) {
     s.key_at[k] = take(n * 4);
     s.pos_at[k] = take(n * 4);
     s.hist_at[k] = take(s.hist_words * 4);
@@ -383,7 +469,9 @@ static void launch_sums(const Params& p, int last, hipStream_t s) {
   const int64_t chunks = ceil_div(p.dim, 64 * kV);
   const dim3 grid(static_cast<unsigned>(ceil_div(p.tiles * chunks, 4)));
   hipLaunchKernelGGL((sum_kernel<DT, kV>), grid, dim3(256), 0, s, p, last, chunks);
-  if (p.tiles > 1) hipLaunchKernelGGL((join_kernel<DT, kV>), grid, dim3(256), 0, s, p, last, chunks);
+  const int64_t narrow = ceil_div(p.dim, 64);
+  if (p.tiles > 1)
+    hipLaunchKernelGGL((join_kernel<DT>), dim3(static_cast<unsigned>(ceil_div((p.tiles - 1) * narrow, 4))), dim3(256), 0, s, p, last, narrow);
 }
 
 }  // namespace embed
@@ -471,22 +559,27 @@ int mm_embedding_bwd(const void* ids, const void* dy, void* dweight, int64_t n, 
   p.clear_bytes = vocab * dim * dtype_size(dtype);
   hipStream_t st = static_cast<hipStream_t>(stream);
   // the launches of the sort share the clearing, in whole pieces
-  const int launches = n > 0 ? s.passes + 1 : 1;
+  const int launches = s.one ? 1 : s.passes + 1;
   auto upto = [&](int k) {
     const int64_t pieces = ceil_div(p.clear_bytes, kClear);
     const int64_t b = pieces * k / launches * kClear;
     return b < p.clear_bytes ? b : p.clear_bytes;
   };
   auto grid = [&](int k) { return dim3(static_cast<unsigned>(s.blocks + ceil_div(upto(k + 1) - upto(k), kClear))); };
-  if (grid(0).x) hipLaunchKernelGGL(count_kernel, grid(0), dim3(256), 0, st, p, s.bits, s.hist_words, upto(1));
-  if (n > 0) {
+  if (s.one) {
+    hipLaunchKernelGGL(sort_kernel, grid(0), dim3(kOneThreads), 0, st, p, s.passes, s.bits, static_cast<int>(ceil_div(n, kOneThreads)),
+                       upto(1));
+  } else {
+    hipLaunchKernelGGL(count_kernel, grid(0), dim3(256), 0, st, p, s.bits, s.hist_words, upto(1));
     for (int k = 0; k < s.passes; ++k) {
       hipLaunchKernelGGL(scatter_kernel, grid(k + 1), dim3(256), 0, st, p, k, s.passes, s.bits, upto(k + 1), upto(k + 2));
       if (k + 2 < s.passes)
         hipLaunchKernelGGL(clear_counts_kernel, dim3(static_cast<unsigned>(ceil_div(s.hist_words, 256))), dim3(256), 0, st, p.hist[k & 1],
                            s.hist_words);
     }
-    const int last = (s.passes - 1) & 1;
+  }
+  if (n > 0) {
+    const int last = s.one ? 0 : (s.passes - 1) & 1;
     const int64_t per = 16 / dtype_size(dtype);
     const bool vec = dim % per == 0 && dy_stride % per == 0 && aligned(dy, 16) && aligned(dweight, 16);
     MM_EMBED(launch_sums, p, last, st);
