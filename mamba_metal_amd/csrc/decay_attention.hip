@@ -99,12 +99,12 @@ struct Shape {
 // run at once.
 // Sets of heads in the gradients of q and k: as few as make 768 workgroups, since each set's sums are written and read
 // once more.
-static Shape shape_of(int64_t batch, int64_t seqlen, int64_t heads, int64_t groups, int64_t dv) {
+static Shape shape_of(int64_t batch, int64_t seqlen, int64_t heads, int64_t groups, int64_t dv, int32_t dtype) {
   Shape s;
   s.runs = ceil_div(seqlen, kRun);
   s.vblocks = static_cast<int32_t>(ceil_div(dv, kVBlock));
   const int64_t wgs = batch * heads * s.vblocks, per = heads / groups;
-  int64_t segs = wgs < 256 ? 512 / wgs : 1;
+  int64_t segs = wgs < 256 ? (dtype == MM_F32 ? 512 : 768) / wgs : 1;
   if (segs > s.runs / 2) segs = s.runs / 2;
   if (segs < 1) segs = 1;
   s.seg_runs = ceil_div(s.runs > 0 ? s.runs : 1, segs);
@@ -238,7 +238,7 @@ size_t mm_decay_attention_states_size(int64_t batch, int64_t seqlen, int64_t hea
   using namespace mm;
   using namespace mm::dattn;
   if (!valid_dtype(dtype) || !sizes_ok(batch, seqlen, heads, 1, key_dim, value_dim)) return 0;
-  const Shape s = shape_of(batch, seqlen, heads, 1, value_dim);
+  const Shape s = shape_of(batch, seqlen, heads, 1, value_dim, dtype);
   return static_cast<size_t>(states_bytes(s, batch, heads, key_dim, dtype) +
                              (dtype == MM_F16 ? batch * heads * s.runs * s.vblocks * 4 : 0));
 }
@@ -248,7 +248,7 @@ size_t mm_decay_attention_workspace_size(int64_t batch, int64_t seqlen, int64_t 
   using namespace mm;
   using namespace mm::dattn;
   if (!valid_dtype(dtype) || !sizes_ok(batch, seqlen, heads, groups, key_dim, value_dim) || batch == 0) return 0;
-  const Shape s = shape_of(batch, seqlen, heads, groups, value_dim);
+  const Shape s = shape_of(batch, seqlen, heads, groups, value_dim, dtype);
   return static_cast<size_t>(layout_of(s, batch, seqlen, heads, groups, key_dim, value_dim, dtype, backward != 0).total);
 }
 
@@ -263,7 +263,7 @@ int mm_decay_attention_fwd(const mm_decay_attention_params* p, void* stream) {
     if (!p->y) return fail(MM_ERR_NULL_POINTER, "y is required");
   }
   if (p->run_states && !aligned(p->run_states, 256)) return fail(MM_ERR_LAYOUT, "run_states must be 256-byte aligned");
-  const Shape s = shape_of(p->batch, p->seqlen, p->heads, p->groups, p->value_dim);
+  const Shape s = shape_of(p->batch, p->seqlen, p->heads, p->groups, p->value_dim, p->dtype);
   const Layout l = layout_of(s, p->batch, p->seqlen, p->heads, p->groups, p->key_dim, p->value_dim, p->dtype, false);
   if ((e = check_workspace(p, l.total)) != MM_OK) return e;
   Pass k = pass_of(p, s, l);
@@ -296,7 +296,7 @@ int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream) {
     if ((e = check_strides(p->dy_stride, "dy")) != MM_OK) return e;
     if (!aligned(p->run_states, 256)) return fail(MM_ERR_LAYOUT, "run_states must be 256-byte aligned");
   }
-  const Shape s = shape_of(p->batch, p->seqlen, p->heads, p->groups, p->value_dim);
+  const Shape s = shape_of(p->batch, p->seqlen, p->heads, p->groups, p->value_dim, p->dtype);
   const Layout l = layout_of(s, p->batch, p->seqlen, p->heads, p->groups, p->key_dim, p->value_dim, p->dtype, true);
   if ((e = check_workspace(p, l.total)) != MM_OK) return e;
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -68,13 +68,13 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         Staged<DT, DKP, 512> r2;
         r.load(q, static_cast<uint32_t>((r.row() * p.q_stride[1] + r.elem()) * kEs), r.kRows * p.q_stride[1] * kEs, rows, dk);
         r2.load(k, static_cast<uint32_t>((r.row() * p.k_stride[1] + r.elem()) * kEs), r.kRows * p.k_stride[1] * kEs, rows, dk);
-        r.store(s_qk[0]);
-        r2.store(s_qk[1]);
+        r.store(s_qk[0], static_cast<int>(threadIdx.x));
+        r2.store(s_qk[1], static_cast<int>(threadIdx.x));
       } else {
         r.load_any(q, p.q_stride[1], rows, dk);
-        r.store(s_qk[0]);
+        r.store(s_qk[0], static_cast<int>(threadIdx.x));
         r.load_any(k, p.k_stride[1], rows, dk);
-        r.store(s_qk[1]);
+        r.store(s_qk[1], static_cast<int>(threadIdx.x));
       }
     }
     __syncthreads();
@@ -186,8 +186,8 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       const int h_next = last_block ? h + 1 : h, vb_next = last_block ? 0 : vb + 1;
       if constexpr (!DIRECT) {
         __syncthreads();
-        ry.store(cur + 2 * kState);
-        rv.store(cur + 2 * kState + kRows);
+        ry.store(cur + 2 * kState, static_cast<int>(threadIdx.x));
+        rv.store(cur + 2 * kState + kRows, static_cast<int>(threadIdx.x));
       }
       __syncthreads();
       if (more) fetch(other, h_next, vb_next);

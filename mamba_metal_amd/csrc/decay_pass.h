@@ -53,7 +53,7 @@ __device__ __forceinline__ void split_operand(const float (&x)[8], u32x4 (&out)[
 }
 
 template <int DT, int DKP, bool REV, bool OUT, bool VEC>
-__global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) void pass_kernel(const Pass p) {
+__global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : VEC ? 3 : 2) void pass_kernel(const Pass p) {
   using T = typename Ty<DT>::T;
   using O = Op<DT>;
   using TK = Tile<DT, DKP>;
@@ -62,13 +62,12 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
   constexpr int NU = DKP / O::kStep, NR = kRun / O::kStep;
   constexpr int TERMS = DT == MM_F32 ? 1 : DT == MM_F16 ? 2 : 3;
   constexpr int kDecayWave = REV ? 3 : 0;                                   // the one with the fewest scores
-  __shared__ __attribute__((aligned(16))) T s_q[OUT ? kRun * TK::kLd : 8];     // what asks: q, or k mirrored
   __shared__ __attribute__((aligned(16))) T s_k[kRun * TK::kLd];               // what adds to the state: k, or q
   __shared__ __attribute__((aligned(16))) T s_v[kRun * TV::kLd];               // its values: v, or dy
   __shared__ __attribute__((aligned(16))) T s_s[OUT ? kVBlock * TK::kLd : 8];  // the state as an operand, a value channel a row
   __shared__ Decays s_d[2];
   __shared__ float s_max[4], s_x[4];
-  int lane = threadIdx.x & 63;
+  int lane = threadIdx.x & 63, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
 
   uint32_t id = blockIdx.x;
@@ -105,7 +104,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
       }
   }
 
-  Staged<DT, DKP, 256> rq, rk;
+  Staged<DT, DKP, 256> rk;
   Staged<DT, kVBlock, 256> rv;
   // The run to fetch next: its rows' addresses (running ones: few scalar registers), which a step moves on by a run.
   constexpr int64_t kEs = sizeof(T);
@@ -118,7 +117,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
   const char* vp = static_cast<const char*>(p.v) + (b * p.v_stride[0] + head * p.v_stride[2] + vb * kVBlock + at_run * kRun * p.v_stride[1]) * kEs;
   T* yp = static_cast<T*>(p.y) + ((b * p.seqlen + at_run * kRun) * p.heads + head) * p.dv + vb * kVBlock;  // (of the run at hand)
   const int64_t gh = b * p.g_stride[0] + head * p.g_stride[2];
-  const uint32_t q_off = static_cast<uint32_t>((rq.row() * p.q_stride[1] + rq.elem()) * kEs);
+  const uint32_t q_off = static_cast<uint32_t>(((16 * wave + i) * p.q_stride[1] + O::kE * g) * kEs);
   const uint32_t k_off = static_cast<uint32_t>((rk.row() * p.k_stride[1] + rk.elem()) * kEs);
   const uint32_t v_off = static_cast<uint32_t>((rv.row() * p.v_stride[1] + rv.elem()) * kEs);
   constexpr int kWay = REV ? -1 : 1;
@@ -135,9 +134,24 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
     else rv.load_any(vp, p.v_stride[1], rows, vw);
     vp += kWay * kRun * p.v_stride[1] * kEs;
   };
+  // What asks (q, or k mirrored): token 16 wave + i as operands, which no other wave needs.
+  u32x4 own[OUT ? NU : 1];
   auto fetch_q = [&](int rows) __attribute__((always_inline)) {
-    if constexpr (VEC) rq.load(qp, q_off, rq.kRows * p.q_stride[1] * kEs, rows, dk);
-    else rq.load_any(qp, p.q_stride[1], rows, dk);
+    const bool in = 16 * wave + i < rows;
+#pragma unroll
+    for (int u = 0; u < (OUT ? NU : 0); ++u) {
+      const int e = u * O::kStep + O::kE * g;
+      const T* const from = reinterpret_cast<const T*>(qp + q_off) + u * O::kStep;
+      if constexpr (VEC) {
+        own[u] = u32x4{0, 0, 0, 0};
+        if (in && e < dk) own[u] = *reinterpret_cast<const u32x4*>(from);
+      } else {
+        T t[O::kE];
+#pragma unroll
+        for (int j = 0; j < O::kE; ++j) t[j] = in && e + j < dk ? from[j] : static_cast<T>(0);
+        __builtin_memcpy(&own[u], t, 16);
+      }
+    }
     qp += kWay * kRun * p.q_stride[1] * kEs;
   };
   auto gate = [&](int64_t run) {
@@ -171,16 +185,16 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
   }
   for (int64_t n = 0; n < walk; ++n) {
     // addresses in shared memory are made anew in every run: held over it they would be dozens of registers
-    asm volatile("" : "+v"(lane));
+    asm volatile("" : "+v"(lane), "+v"(tid));
+    const int g = lane >> 4, i = lane & 15;
     const int64_t run = at_run, next = n + 1 < walk ? run + kWay : run;
     at_run = next;
     __syncthreads();  // nobody reads the tiles of the run before
     if constexpr (OUT && REV) {
       if (dot_wanted && n > 0) note_dot(run - kWay, s_d[(n - 1) & 1]);
     }
-    if (OUT) rq.store(s_q);
-    rk.store(s_k);
-    rv.store(s_v);
+    rk.store(s_k, tid);
+    rv.store(s_v, tid);
     if constexpr (OUT) {
       if constexpr (DT == MM_F16) {
         // fp16 has 5 exponent bits: the state goes through a power of two that puts its largest element at 2^13
@@ -242,7 +256,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
       if (quarter >= kVBlock * kUnits / 256) return;
 #pragma unroll
       for (int s = 0; s < kEach; ++s) {
-        const int u = (quarter * kEach + s) * 256 + static_cast<int>(threadIdx.x), r = u / kUnits, e = u % kUnits * O::kE;
+        const int u = (quarter * kEach + s) * 256 + tid, r = u / kUnits, e = u % kUnits * O::kE;
         *reinterpret_cast<u32x4*>(to + r * DKP + e) = *reinterpret_cast<const u32x4*>(s_s + TK::at(r, e));
       }
       if (DT == MM_F16 && quarter == 0 && threadIdx.x == 0) p.factors[block] = factor;
@@ -262,9 +276,6 @@ __global__ __launch_bounds__(256, DT == MM_F32 && DKP == 128 && OUT ? 1 : 2) voi
       }
       // Token block `wave` of the run: its scores, as accumulators (what adds) x (what asks) that are at once operands of
       // their product with the values.
-      u32x4 own[NU];
-#pragma unroll
-      for (int u = 0; u < NU; ++u) own[u] = TK::row(s_q, 16 * wave, u * O::kStep, lane);
       f32x4 acc[4];
 #pragma unroll
       for (int st = 0; st < 4; ++st) {

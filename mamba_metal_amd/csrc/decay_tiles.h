@@ -172,9 +172,9 @@ struct Staged {
       for (int q = 0; q < kSteps; ++q) v[q] = q == s ? w : v[q];
     }
   }
-  __device__ __forceinline__ void store(T* tile) const {
+  __device__ __forceinline__ void store(T* tile, int tid) const {  // tid: threadIdx.x
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) *reinterpret_cast<u32x4*>(tile + Tile<DT, W>::at(s * kRows + row(), elem())) = v[s];
+    for (int s = 0; s < kSteps; ++s) *reinterpret_cast<u32x4*>(tile + Tile<DT, W>::at(s * kRows + tid / kUnits, tid % kUnits * kE)) = v[s];
   }
 };
 
