@@ -14,17 +14,55 @@
 // What a head needs, 48 KB with key_dim 128 in 16 bits, is the traffic that bounds it.  It is loaded straight into shared
 // memory while the head before is computed (two buffers, one barrier a head); fp32, whose buffers would not fit twice,
 // and rows off 16 bytes go through registers instead.
+#include <type_traits>
+
 #include "decay_attention.h"
 #include "decay_tiles.h"
+#include "direct_load.h"
 
 namespace mm {
 namespace dattn {
 
-__device__ const uint32_t kZeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
-
-__device__ __forceinline__ void load_direct(const char* from, char* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+// 16-bit types: operands of columns 16 t + i, over 32 rows of a tile, for N of t (Tile's column).  at[t]: where a lane's reads
+// begin; ROWS: the first row.  The reads and their wait are one piece: of a transposing read in the compiler's hands it is not
+// known where it reads, and each would wait for all direct loads under way.
+#define MM_TR "ds_read_b64_tr_b16 "
+template <typename TILE, int ROWS>
+__device__ __forceinline__ void columns(const uint32_t (&at)[4], u32x4 (&o)[4]) {
+  u32x2 r[8];
+  constexpr int kA = ROWS * TILE::kLd * 2, kB = kA + 16 * TILE::kLd * 2;
+  asm volatile(MM_TR "%0, %8 offset:%12\n" MM_TR "%1, %8 offset:%13\n" MM_TR "%2, %9 offset:%12\n" MM_TR "%3, %9 offset:%13\n"
+               MM_TR "%4, %10 offset:%12\n" MM_TR "%5, %10 offset:%13\n" MM_TR "%6, %11 offset:%12\n" MM_TR "%7, %11 offset:%13\n"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(kA), "n"(kB)
+               : "memory");
+#pragma unroll
+  for (int t = 0; t < 4; ++t) o[t] = u32x4{r[2 * t][0], r[2 * t][1], r[2 * t + 1][0], r[2 * t + 1][1]};
+}
+template <typename TILE, int ROWS>
+__device__ __forceinline__ void columns(const uint32_t (&at)[8], u32x4 (&o)[8]) {
+  u32x2 r[16];
+  constexpr int kA = ROWS * TILE::kLd * 2, kB = kA + 16 * TILE::kLd * 2;
+  asm volatile(MM_TR "%0, %16 offset:%24\n" MM_TR "%1, %16 offset:%25\n" MM_TR "%2, %17 offset:%24\n" MM_TR "%3, %17 offset:%25\n"
+               MM_TR "%4, %18 offset:%24\n" MM_TR "%5, %18 offset:%25\n" MM_TR "%6, %19 offset:%24\n" MM_TR "%7, %19 offset:%25\n"
+               MM_TR "%8, %20 offset:%24\n" MM_TR "%9, %20 offset:%25\n" MM_TR "%10, %21 offset:%24\n" MM_TR "%11, %21 offset:%25\n"
+               MM_TR "%12, %22 offset:%24\n" MM_TR "%13, %22 offset:%25\n" MM_TR "%14, %23 offset:%24\n" MM_TR "%15, %23 offset:%25\n"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]), "=&v"(r[8]),
+                 "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
+               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7]), "n"(kA), "n"(kB)
+               : "memory");
+#pragma unroll
+  for (int t = 0; t < 8; ++t) o[t] = u32x4{r[2 * t][0], r[2 * t][1], r[2 * t + 1][0], r[2 * t + 1][1]};
+}
+#undef MM_TR
+// Where column4 of row 0 and column 16 t begins in a tile.  The rows' turn is the same 16 rows further on.
+template <typename TILE, typename T, int N>
+__device__ __forceinline__ void columns_at(const T* tile, int lane, uint32_t (&at)[N]) {
+  const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const T*)tile));
+#pragma unroll
+  for (int t = 0; t < N; ++t) at[t] = base + TILE::at(4 * (lane >> 4) + ((lane & 15) >> 2), 16 * t + 4 * (lane & 3)) * 2;
 }
 
 template <int DT, int DKP, bool DIRECT, bool ONE>
@@ -127,19 +165,12 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         for (int which = 0; which < 2; ++which) {
           const char* const from = static_cast<const char*>(which ? p.dstates : p.states) + block * kBytes;
 #pragma unroll
-          for (int q = 0; q < kBytes / 8192; ++q) load_direct(from + q * 8192 + state_off, to + which * kBytes + (q * 8 + wave) * 1024);
+          for (int q = 0; q < kBytes / 8192; ++q) load_direct(from, q * 8192 + state_off, to + which * kBytes + (q * 8 + wave) * 1024);
         }
         char* const dy_to = to + 2 * kBytes + wave * 1024;
-        char* const v_to = dy_to + kRows * kEs;
-        if (rows == kRun && vw == kVBlock) {
-          load_direct(dy + dy_off, dy_to);
-          load_direct(v + v_off, v_to);
-        } else {
-          const bool in = row_here < rows && chunk_here * 8 < vw;
-          const char* const zeros = reinterpret_cast<const char*>(kZeros);
-          load_direct(in ? dy + dy_off : zeros, dy_to);
-          load_direct(in ? v + v_off : zeros, v_to);
-        }
+        const bool in = row_here < rows && chunk_here * 8 < vw;
+        load_direct(dy, in ? dy_off : kNowhere, dy_to);
+        load_direct(v, in ? v_off : kNowhere, dy_to + kRows * kEs);
       } else {
         if (p.vec) {
           ry.load(dy, static_cast<uint32_t>((ry.row() * p.dy_stride[1] + ry.elem()) * kEs), ry.kRows * p.dy_stride[1] * kEs, rows, vw);
@@ -155,13 +186,16 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
     };
     // what the head needs of its states' product and (fp16) powers of two, a step ahead
     auto dot_of = [&](int h) {
-      float dot = 0.0f;
-      for (int vb = 0; vb < vblocks; ++vb) dot += p.dot[((b * p.heads + group * p.per + h) * p.runs + run) * vblocks + vb];
+      const float* const from = p.dot + ((b * p.heads + group * p.per + h) * p.runs + run) * vblocks;
+      float dot = from[0];
+      for (int vb = 1; vb < vblocks; ++vb) dot += from[vb];
       return dot;
     };
     auto factor_of = [&](int h, int vb) {
       return (role ? p.dfactors : p.factors)[((b * p.heads + group * p.per + h) * p.runs + run) * vblocks + vb];
     };
+    uint32_t g_ahead = 0;  // the next head's log decays
+    if (wave == 7 && h0 + 1 < h1) g_ahead = gate(h0 + 1);
     float dot_here = 0.0f, dot_before = 0.0f, factor_here = 1.0f;
     if (p.dg && wave == 0) dot_here = dot_of(h0);
     if (DT == MM_F16) factor_here = factor_of(h0, 0);
@@ -189,11 +223,11 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         ry.store(cur + 2 * kState, static_cast<int>(threadIdx.x));
         rv.store(cur + 2 * kState + kRows, static_cast<int>(threadIdx.x));
       }
+      if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's direct loads of the step
       __syncthreads();
-      if (more) fetch(other, h_next, vb_next);
-      uint32_t g_next = 0;
       const bool decays_now = wave == 7 && last_block && h + 1 < h1;
-      if (decays_now) g_next = gate(h + 1);
+      const uint32_t g_next = g_ahead;
+      if (decays_now && h + 2 < h1) g_ahead = gate(h + 2);
       float factor_next = 1.0f;
       if (DT == MM_F16 && more) factor_next = factor_of(h_next, vb_next);
       if (p.dg && wave == 0 && vb == 0) {
@@ -202,6 +236,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         dot_before = dot_here;
         dot_here = dot_next;
       }
+      if (more) fetch(other, h_next, vb_next);  // (behind the loads that are waited for first)
       const Decays& D = s_d[(h - h0) & 1];
       if (ONE || vb == 0) {
 #pragma unroll
@@ -216,9 +251,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
                                     : static_cast<const T*>(role ? p.dstates : p.states) + ((bh * p.runs + run) * vblocks + vb) * kVBlock * DKP;
       // columns d of the state, 16 t on, over its value channels
       auto state_operand = [&](int u, int t) __attribute__((always_inline)) {
-        if constexpr (DIRECT) {
-          return TK::column(state, u * O::kStep, 16 * t, lane);
-        } else if constexpr (O::kWide) {
+        if constexpr (O::kWide) {
           return *reinterpret_cast<const u32x4*>(state + ((u * ND + t) * 64 + lane) * 4);
         } else {
           T e[O::kE];
@@ -243,11 +276,26 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         factor = factor_here;
         factor_here = factor_next;
       }
+      auto add_state = [&](auto first) __attribute__((always_inline)) {
+        constexpr int u = decltype(first)::value;
+        if constexpr (DIRECT) {
+          u32x4 o[ND];
+          uint32_t at[ND];
+          columns_at<TK>(state, lane, at);
+          columns<TK, u * 32>(at, o);
 #pragma unroll
-      for (int u = 0; u < NU; ++u)
+          for (int t = 0; t < ND; ++t) tmp[t] = mma<DT>(own[u], o[t], tmp[t]);
+        } else {
 #pragma unroll
-        for (int t = 0; t < ND; ++t)
-          tmp[t] = mma<DT>(own[u], state_operand(u, t), tmp[t]);
+          for (int t = 0; t < ND; ++t) tmp[t] = mma<DT>(own[u], state_operand(u, t), tmp[t]);
+        }
+      };
+      add_state(std::integral_constant<int, 0>{});
+      add_state(std::integral_constant<int, 1>{});
+      if constexpr (NU == 4) {
+        add_state(std::integral_constant<int, 2>{});
+        add_state(std::integral_constant<int, 3>{});
+      }
       if (!last_block) return;
       // dP and M
       const float hi_r = D.hi[16 * blk + i], lo_r = D.lo[16 * blk + i];
@@ -300,11 +348,26 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         }
         inter *= w;
       }
+      auto add_rows = [&](auto first) __attribute__((always_inline)) {
+        constexpr int u = decltype(first)::value;
+        if (role ? (u + 1) * O::kStep <= 16 * blk : u * O::kStep > 16 * blk + 15) return;
+        if constexpr (DIRECT) {
+          u32x4 o[ND];
+          uint32_t at[ND];
+          columns_at<TK>(s_other, lane, at);
+          columns<TK, u * 32>(at, o);
 #pragma unroll
-      for (int u = 0; u < kRun / O::kStep; ++u) {
-        if (role ? (u + 1) * O::kStep <= 16 * blk : u * O::kStep > 16 * blk + 15) continue;
+          for (int t = 0; t < ND; ++t) out[t] = mma<DT>(dp[u], o[t], out[t]);
+        } else {
 #pragma unroll
-        for (int t = 0; t < ND; ++t) out[t] = mma<DT>(dp[u], TK::column(s_other, u * O::kStep, 16 * t, lane), out[t]);
+          for (int t = 0; t < ND; ++t) out[t] = mma<DT>(dp[u], TK::column(s_other, u * O::kStep, 16 * t, lane), out[t]);
+        }
+      };
+      add_rows(std::integral_constant<int, 0>{});
+      add_rows(std::integral_constant<int, 1>{});
+      if constexpr (NU == 4) {
+        add_rows(std::integral_constant<int, 2>{});
+        add_rows(std::integral_constant<int, 3>{});
       }
       if (p.dg) {
         sum += lane_xor(sum, 16);

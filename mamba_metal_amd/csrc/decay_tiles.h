@@ -180,7 +180,7 @@ struct Staged {
 
 // A run's decays: c_t, the running sum of the log decays to token t and with it, in log2 units.  Sums are 64-bit and
 // kept as two floats, so that a difference is exact to fp32 however far both lie down.
-struct Decays {
+struct alignas(16) Decays {
   float hi[kRun], lo[kRun];
   float into[kRun];    // exp(c_t): what the state before the run still counts at t
   float onward[kRun];  // exp(c_last - c_t): what token t still counts at the run's end

@@ -22,6 +22,7 @@
 
 #include <type_traits>
 
+#include "direct_load.h"
 #include "mm_common.h"
 
 namespace mm {
@@ -58,12 +59,6 @@ struct Matrix {
   int64_t rows;     // kAlong: rows of the operand; kAcross: its columns, in elements
   int64_t k;        // elements of the sum
 };
-
-constexpr uint32_t kNowhere = 0x80000000u;  // an offset past a buffer's end
-__device__ __forceinline__ void load_direct(const char* base, uint32_t off, char* to) {
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7fffffff, 0x00027000);
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)to, 16, off, 0, 0, 0);
-}
 
 // One operand of a workgroup's tile: R rows, staged by NW waves.
 template <int DT, Lie LIE, int R, int NW>
