@@ -62,7 +62,7 @@ template <typename TILE, typename T, int N>
 __device__ __forceinline__ void columns_at(const T* tile, int lane, uint32_t (&at)[N]) {
   const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const T*)tile));
 #pragma unroll
-  for (int t = 0; t < N; ++t) at[t] = base + TILE::at(4 * (lane >> 4) + ((lane & 15) >> 2), 16 * t + 4 * (lane & 3)) * 2;
+  for (int t = 0; t < N; ++t) at[t] = base + TILE::at(0, 16 * t, 4 * (lane >> 4) + ((lane & 15) >> 2), 4 * (lane & 3)) * 2;
 }
 
 template <int DT, int DKP, bool DIRECT, bool ONE>

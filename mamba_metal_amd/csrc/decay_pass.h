@@ -207,7 +207,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
 #pragma unroll
       for (int t = 0; t < ND; ++t) {
         const f32x4 x = DT == MM_F16 ? S[t] * shrink : S[t];
-        T* const to = s_s + TK::at(16 * wave + i, 16 * t + 4 * g);
+        T* const to = s_s + TK::at(16 * wave, 16 * t, i, 4 * g);
         if constexpr (O::kWide) *reinterpret_cast<f32x4*>(to) = x;
         else *reinterpret_cast<u32x2*>(to) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
       }

@@ -97,24 +97,30 @@ struct Tile {
   static __device__ __forceinline__ int at(int r, int e) {
     return kWide ? r * kLd + e : r * kLd + (((e >> 3) ^ turn(r)) << 3) + (e & 7);
   }
+  // at(r0 + r, e0 + e) for r0 and e0 that 16 divides, r < 16 and e < 16 (or e < e0's lowest bit): r0 does not turn, and e0
+  // only flips bits of what is the same for all of a lane's accesses, an instruction each where `at` would take four.
+  static __device__ __forceinline__ int at(int r0, int e0, int r, int e) {
+    return kWide ? (r0 + r) * kLd + e0 + e : r0 * kLd + ((r * kLd + (((e >> 3) ^ turn(r)) << 3) + (e & 7)) ^ e0);
+  }
   // Row r0 + i, elements k0 on, in row order.
   static __device__ __forceinline__ u32x4 row(const T* tile, int r0, int k0, int lane) {
-    return *reinterpret_cast<const u32x4*>(tile + at(r0 + (lane & 15), k0 + Op<DT>::kE * (lane >> 4)));
+    return *reinterpret_cast<const u32x4*>(tile + at(r0, k0, lane & 15, Op<DT>::kE * (lane >> 4)));
   }
   // ... in acc order.
   static __device__ __forceinline__ u32x4 row_acc(const T* tile, int r0, int k0, int lane) {
-    const int r = r0 + (lane & 15), e = k0 + 4 * (lane >> 4);
+    const int r = lane & 15, e = 4 * (lane >> 4);
     if constexpr (kWide) {
-      return *reinterpret_cast<const u32x4*>(tile + at(r, e));
+      return *reinterpret_cast<const u32x4*>(tile + at(r0, k0, r, e));
     } else {
-      const u32x2 a = *reinterpret_cast<const u32x2*>(tile + at(r, e)), b = *reinterpret_cast<const u32x2*>(tile + at(r, e + 16));
+      const u32x2 a = *reinterpret_cast<const u32x2*>(tile + at(r0, k0, r, e));
+      const u32x2 b = *reinterpret_cast<const u32x2*>(tile + at(r0, k0 + 16, r, e));
       return u32x4{a[0], a[1], b[0], b[1]};
     }
   }
   // Four elements of column c0 + i of rows r0 + 4 g on, 16-bit types: the transposing read, in which each group of 16
   // lanes reads 4 rows of 16 elements, 8 bytes a lane, and gets a column each.
   static __device__ __forceinline__ u32x2 column4(const T* tile, int r0, int c0, int lane) {
-    const T* const p = tile + at(r0 + 4 * (lane >> 4) + ((lane & 15) >> 2), c0 + 4 * (lane & 3));
+    const T* const p = tile + at(r0, c0, 4 * (lane >> 4) + ((lane & 15) >> 2), 4 * (lane & 3));
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)const_cast<T*>(p)));
   }
   // Column c0 + i, rows k0 on, in acc order: an operand whose sum runs over a tile's rows.
