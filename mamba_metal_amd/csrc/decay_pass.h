@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
   const char* kp = static_cast<const char*>(p.k) + (b * p.k_stride[0] + group * p.k_stride[2] + at_run * kRun * p.k_stride[1]) * kEs;
   const char* vp = static_cast<const char*>(p.v) + (b * p.v_stride[0] + head * p.v_stride[2] + vb * kVBlock + at_run * kRun * p.v_stride[1]) * kEs;
   T* yp = static_cast<T*>(p.y) + ((b * p.seqlen + at_run * kRun) * p.heads + head) * p.dv + vb * kVBlock;  // (of the run at hand)
-  const int64_t gh = b * p.g_stride[0] + head * p.g_stride[2];
+  int64_t g_at = b * p.g_stride[0] + head * p.g_stride[2] + at_run * kRun * p.g_stride[1];
   const uint32_t q_off = static_cast<uint32_t>(((16 * wave + i) * p.q_stride[1] + O::kE * g) * kEs);
   const uint32_t k_off = static_cast<uint32_t>((rk.row() * p.k_stride[1] + rk.elem()) * kEs);
   const uint32_t v_off = static_cast<uint32_t>((rv.row() * p.v_stride[1] + rv.elem()) * kEs);
@@ -154,8 +154,10 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
     }
     qp += kWay * kRun * p.q_stride[1] * kEs;
   };
-  auto gate = [&](int64_t run) {
-    return lane < rows_of(run) ? load_gate(p, gh + (run * kRun + lane) * p.g_stride[1]) : 0u;
+  auto gate = [&](int rows) __attribute__((always_inline)) {
+    const uint32_t raw = lane < rows ? load_gate(p, g_at + lane * p.g_stride[1]) : 0u;
+    g_at += kWay * kRun * p.g_stride[1];
+    return raw;
   };
   // fp16: the largest magnitude of the wave's columns
   auto note_max = [&]() __attribute__((always_inline)) {
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
     fetch_v(rows_of(at_run));
     if (OUT) fetch_q(rows_of(at_run));
     if (DT == MM_F16 && OUT) note_max();
-    if (wave == kDecayWave) run_decays(s_d[0], gate_value(p, gate(at_run)), lane);
+    if (wave == kDecayWave) run_decays(s_d[0], gate_value(p, gate(rows_of(at_run))), lane);
   }
   for (int64_t n = 0; n < walk; ++n) {
     // addresses in shared memory are made anew in every run: held over it they would be dozens of registers
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
       }
     }
     uint32_t g_next = 0;
-    if (wave == kDecayWave) g_next = gate(next);
+    if (wave == kDecayWave && n + 1 < walk) g_next = gate(rows_of(next));
     if (n + 1 < walk) fetch_v(rows_of(next));
     if (!OUT && n + 1 < walk) fetch_k(rows_of(next));
     // The state kept for the backward pass, a quarter at a time, for the same reason as the loads.  16 bits: a value
@@ -343,7 +345,7 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
       }
       yp += kWay * kRun * p.heads * p.dv;
     }
-    if (wave == kDecayWave) run_decays(s_d[(n + 1) & 1], gate_value(p, g_next), lane);
+    if (wave == kDecayWave && n + 1 < walk) run_decays(s_d[(n + 1) & 1], gate_value(p, g_next), lane);
     // the state's step: this wave's value columns, weighted, as operands over the run's tokens
     const float whole = D.whole;
 #pragma unroll

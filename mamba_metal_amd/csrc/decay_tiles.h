@@ -97,8 +97,8 @@ struct Tile {
   static __device__ __forceinline__ int at(int r, int e) {
     return kWide ? r * kLd + e : r * kLd + (((e >> 3) ^ turn(r)) << 3) + (e & 7);
   }
-  // at(r0 + r, e0 + e) for r0 and e0 that 16 divides, r < 16 and e < 16 (or e < e0's lowest bit): r0 does not turn, and e0
-  // only flips bits of what is the same for all of a lane's accesses, an instruction each where `at` would take four.
+  // at(r0 + r, e0 + e) for an r0 that 16 divides, which does not turn, and an e0 that has no bit of e's: it only flips bits of
+  // what is the same for all of a lane's accesses, an instruction each where `at` would take four.
   static __device__ __forceinline__ int at(int r0, int e0, int r, int e) {
     return kWide ? (r0 + r) * kLd + e0 + e : r0 * kLd + ((r * kLd + (((e >> 3) ^ turn(r)) << 3) + (e & 7)) ^ e0);
   }
@@ -147,6 +147,7 @@ struct Staged {
   static constexpr int kSteps = kRun * kUnits / Threads;
   static constexpr int kRows = Threads / kUnits;         // of a step
   static_assert(kSteps >= 1, "a unit for every thread");
+  static_assert(Op<DT>::kWide || kRows % 16 == 0, "steps do not turn");
   u32x4 v[kSteps];
   static __device__ __forceinline__ int row() { return static_cast<int>(threadIdx.x) / kUnits; }
   static __device__ __forceinline__ int elem() { return static_cast<int>(threadIdx.x) % kUnits * kE; }
@@ -180,7 +181,7 @@ struct Staged {
   }
   __device__ __forceinline__ void store(T* tile, int tid) const {  // tid: threadIdx.x
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) *reinterpret_cast<u32x4*>(tile + Tile<DT, W>::at(s * kRows + tid / kUnits, tid % kUnits * kE)) = v[s];
+    for (int s = 0; s < kSteps; ++s) *reinterpret_cast<u32x4*>(tile + Tile<DT, W>::at(s * kRows, 0, tid / kUnits, tid % kUnits * kE)) = v[s];
   }
 };
 
