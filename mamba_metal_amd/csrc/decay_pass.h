@@ -451,13 +451,26 @@ __global__ __launch_bounds__(256) void join_kernel(const Pass p) {
       if (d < p.dk && vcol < p.dv) S[r] = p.init[(bh * p.dk + d) * p.dv + vcol];
     }
   }
-  for (int n = 0; n + 1 < p.segments; ++n) {
-    const int seg = REV ? p.segments - 1 - n : n;
-    const double c = p.seg_decay[bh * p.segments + seg];
-    f32x4* const slot = seg_state(p, bh, seg, vb) + in;
-    const float hi = static_cast<float>(c);
-    S = S * (exp2_acc(hi) * (1.0f + static_cast<float>(c - hi) * kLn2)) + *slot;
-    *slot = S;
+  f32x4* const slots = seg_state(p, bh, 0, vb) + in;
+  const int64_t step = seg_state(p, bh, 1, vb) - seg_state(p, bh, 0, vb);
+  const double* const decays = p.seg_decay + bh * p.segments;
+  for (int n0 = 0; n0 + 1 < p.segments; n0 += 8) {
+    f32x4 adds[8];
+    double c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {  // (eight at a time under way; the last one's own is not used)
+      const int n = n0 + j < p.segments ? n0 + j : n0, seg = REV ? p.segments - 1 - n : n;
+      adds[j] = slots[seg * step];
+      c[j] = decays[seg];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int n = n0 + j, seg = REV ? p.segments - 1 - n : n;
+      if (n + 1 >= p.segments) break;
+      const float hi = static_cast<float>(c[j]);
+      S = S * (exp2_acc(hi) * (1.0f + static_cast<float>(c[j] - hi) * kLn2)) + adds[j];
+      slots[seg * step] = S;
+    }
   }
 }
 
