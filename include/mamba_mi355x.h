@@ -583,8 +583,9 @@ int mm_embedding_bwd(const void* ids, const void* dy, void* dweight, int64_t n, 
  * forward call writes lse (rows,), log(sum_v exp(l_v)), unless it is NULL; the backward call reads it.
  *
  * Backward: dl = (softmax(l) - onehot(target)) dloss, computed again from x, weight and lse in pieces of the vocabulary
- * of at most 512 MB and rounded once to dtype; dx = dl weight (rows, dim), dweight = dl^T x (vocab, dim), contiguous, in
- * dtype, summed in fp32 in a fixed order (either may be NULL).  dloss: fp32, for reduction 0 with a stride (0: all the same), else one. */
+ * of at most 512 MB (or of 256 tokens) and rounded once to dtype (reduction 1 and 2: without dloss and the mean's 1 / n,
+ * which multiply the sums); dx = dl weight (rows, dim), dweight = dl^T x (vocab, dim), contiguous, in dtype, summed in fp32
+ * in a fixed order (either may be NULL).  dloss: fp32, for reduction 0 with a stride (0: all the same), else one. */
 typedef struct mm_linear_cross_entropy_params {
   const void* x;
   const void* weight;

@@ -102,8 +102,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     "sum".
 
     Logits and their sums are float32.  Gradients flow to x and weight (once, not twice, and not in forward mode): the
-    gradient of the logits is rounded once to x's dtype (in float16 times a power of two that keeps it in range), in
-    pieces of at most 512 MB, and sums over the vocabulary and the rows are float32, in a fixed order.
+    gradient of the logits is rounded once to x's dtype (in float16 times a power of two that keeps it in range; of a
+    "mean" or "sum" before its one factor), in pieces of at most 512 MB (or of 256 tokens), and sums over the vocabulary and
+    the rows are float32, in a fixed order.
 
     To capture a backward pass into a graph, capture the forward pass with it, and let no eager autograd graph of the
     same leaf tensors be alive at that time."""

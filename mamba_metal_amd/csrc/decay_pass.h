@@ -11,9 +11,15 @@
 //   dS  <- exp(c_63) dS + sum_t scale exp(c_t) q_t dy_t^T
 // A workgroup walks over the runs of one head and 64 value channels; wave w keeps columns 16 w .. 16 w + 15 of the
 // state in registers, fp32, and leaves them in shared memory as operands of S^T q; token block w is its share of the
-// outputs.  Where the heads alone do not
-// fill the card the tokens are cut into segments: a first pass finds what each segment adds to the state, a small kernel
-// joins them, and the second pass starts each segment from its state.
+// outputs.  Where the heads alone do not fill the card the tokens are cut into segments: a first pass finds what each segment
+// adds to the state, a small kernel joins them, and the second pass starts each segment from its state.
+//
+// A run is a chain (shared memory, scores, outputs, state) of which a workgroup's own instructions take less than half: it
+// is hidden by other workgroups, so that registers and shared memory are held to what lets three share a compute unit in 16
+// bits (q goes straight from memory to operands, addresses are made anew in every run).  bf16, 80 heads of 128 by 64 and one
+// q and k: 8192 tokens of one sequence take 53 us for what the segments add, 8 to join them and 98 for the outputs; 8
+// sequences of 2048 tokens 280 us (0.7 GB with the states that are kept, 2.4 TB/s), mirrored 375 us (1.0 GB, 2.7 TB/s).  Two
+// workgroups a unit: 339 and 498 us.
 #pragma once
 
 #include "decay_attention.h"
@@ -432,7 +438,8 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
   }
 }
 
-// What the segments add, joined: slot `seg` gets the state after it (mirrored: before it).
+// What the segments add, joined: slot `seg` gets the state after it (mirrored: before it).  Memory traffic: 9 segments of 80
+// heads, 45 MB in 8 us.
 template <int DKP, bool REV>
 __global__ __launch_bounds__(256) void join_kernel(const Pass p) {
   constexpr int ND = DKP / 16;

@@ -2,7 +2,7 @@
 //
 //   y[i] = scale * weight[ids[i]]          dweight[v] = scale * sum_{i : ids[i] = v} dy[i]
 //
-// All of it is memory traffic.  The gradient's rows are sums in a fixed order, so that calls repeat bit for bit: the
+// All of it is memory traffic.  Forward, 16384 rows of 2560 in bf16: 33 us, 5.1 TB/s.  The gradient's rows are sums in a fixed order, so that calls repeat bit for bit: the
 // tokens are sorted by id (a stable radix sort, least digit first, of up to 9 bits a pass), runs of equal ids are
 // summed in fp32 in the order of their positions, and rounded once.  A run may be any length (the commonest token of a
 // text takes several percent of it): the sorted tokens are cut into tiles of 16, and what a run leaves in the tiles it
@@ -142,7 +142,8 @@ __device__ __forceinline__ uint64_t equals(uint64_t in, uint32_t d, int bits) {
   return same;
 }
 
-// The whole sort, by workgroup 0; the others clear the table.  A wave holds 64 `rounds` neighbouring tokens in registers; a
+// The whole sort, by workgroup 0; the others clear the table (50280 x 2560 in bf16: 257 MB in 39 us, the sort of 16384
+// tokens under it).  A wave holds 64 `rounds` neighbouring tokens in registers; a
 // pass ranks them among its own, a round at a time, joins the waves' counts, and sends them through the LDS.
 __global__ __launch_bounds__(kOneThreads) void sort_kernel(const Params p, int passes, int bits, int rounds, int64_t clear1) {
   if (blockIdx.x >= p.sort_blocks) return clear_share<kOneThreads>(p, 0, clear1);
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(256) void clear_counts_kernel(uint32_t* hist, int64
 
 // A wave sums 16 sorted tokens over 64 kV columns, all their rows under way at once: whole runs go to the table, the parts
 // of runs that reach over an edge of the tile to the workspace (first: one that began before; last: one that goes on, if it
-// is not the first).
+// is not the first).  16384 tokens of 2560 in bf16: 42 us, 3.1 TB/s (tiles of 32, eight rows at a time: 76).
 template <int DT, int kV>
 __global__ __launch_bounds__(256) void sum_kernel(const Params p, int last, int64_t chunks) {
   const int lane = threadIdx.x & 63;
@@ -377,7 +378,7 @@ __global__ __launch_bounds__(256) void sum_kernel(const Params p, int last, int6
 }
 
 // Joins the run that begins in a tile and goes on behind it: a wave for 64 columns (few runs are long, and a long one's
-// sum is a chain of loads: narrow waves make many chains).
+// sum is a chain of loads: narrow waves make many chains; 13 us there, 62 with 512 columns a wave).
 template <int DT>
 __global__ __launch_bounds__(256) void join_kernel(const Params p, int last, int64_t chunks) {
   const int lane = threadIdx.x & 63;

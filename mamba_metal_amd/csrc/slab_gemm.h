@@ -1,10 +1,12 @@
 // Products of large tiles on the matrix cores: C[m, n] = sum_k A(m, k) B(n, k), both operands streamed through shared
 // memory by loads that go there directly, several stages deep.
 //
-// A stage is a slab of 64 bytes of k (32 16-bit elements, 16 fp32 ones) of the tile's rows.  What the 32 units of a die
-// read at once is shared in its cache, so that all of them wait for the same misses: a stage's loads take 1.5 to 2 us,
-// twice what its products take, and it is the bytes under way that keep the matrix cores fed (two stages of 128 bytes of
-// k, half as many bytes under way: 51% of their cycles busy).
+// A stage is a slab of 64 bytes of k (32 16-bit elements, 16 fp32 ones) of the tile's rows, and four are under way.  What
+// the 32 units of a die read at once is shared in its cache, so that all of them wait for the same misses: a stage's loads
+// take 1.5 to 2 us, twice what its products take, and it is the bytes under way that keep the matrix cores fed.  bf16, 8192
+// rows (7377 of them counted) of 2560 by 50280: 1890 us with two stages of 128 bytes behind flat loads, 1.67 to 1.72 ms now,
+// 1.12 PFLOP/s; the cores' cycles are 58% busy at the 1.9 GHz that the card holds under it (a library product of the whole
+// shape reaches 1.19).  fp32, 2048 by 16384 of 4096: 126 TFLOP/s, 89% busy (library: 136).
 //
 // An operand lies in memory either way:
 //   kAlong   k is contiguous: a row of the slab is 64 bytes of a row of the matrix, four 16-byte chunks.  Chunk c of
@@ -57,7 +59,7 @@ struct Matrix {
   const char* base;
   int64_t ld;       // bytes from one row in memory to the next; a tile's rows lie within 2 GB
   int64_t rows;     // kAlong: rows of the operand; kAcross: its columns, in elements
-  int64_t k;        // elements of the sum
+  int64_t k;        // elements of a row
 };
 
 // One operand of a workgroup's tile: R rows, staged by NW waves.
@@ -67,7 +69,6 @@ struct Side {
   static constexpr int kEs = sizeof(T), kWidth = R;
   static constexpr int kDepth = kSlab / kEs;               // elements of k in a slab
   static constexpr int kLoads = R * kSlab / 1024 / NW;     // of a wave, 64 lanes of 16 bytes each
-  static constexpr int kReads = LIE == kAlong ? 1 : kEs == 2 ? 2 : 4;  // of an operand
   static_assert(kLoads >= 1 && kLoads * 1024 * NW == R * kSlab, "whole loads");
   // kAcross: a load is kRows rows of k.  16-bit: 64 bytes of each of kSide rows side by side, then the next 64 bytes of
   // them; where a load has but 2 rows, the next one's are 128 bytes further on in the banks.
