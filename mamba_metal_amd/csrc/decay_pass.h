@@ -22,6 +22,8 @@
 // workgroups a unit: 339 and 498 us.
 #pragma once
 
+#include <type_traits>
+
 #include "decay_attention.h"
 #include "decay_tiles.h"
 
@@ -123,7 +125,8 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
   const char* vp = static_cast<const char*>(p.v) + (b * p.v_stride[0] + head * p.v_stride[2] + vb * kVBlock + at_run * kRun * p.v_stride[1]) * kEs;
   T* yp = static_cast<T*>(p.y) + ((b * p.seqlen + at_run * kRun) * p.heads + head) * p.dv + vb * kVBlock;  // (of the run at hand)
   int64_t g_at = b * p.g_stride[0] + head * p.g_stride[2] + at_run * kRun * p.g_stride[1];
-  const uint32_t q_off = static_cast<uint32_t>(((16 * wave + i) * p.q_stride[1] + O::kE * g) * kEs);
+  using Offset = std::conditional_t<VEC, uint32_t, int64_t>;  // (any rows: they may lie further apart)
+  const Offset q_off = static_cast<Offset>(((16 * wave + i) * p.q_stride[1] + O::kE * g) * kEs);
   const uint32_t k_off = static_cast<uint32_t>((rk.row() * p.k_stride[1] + rk.elem()) * kEs);
   const uint32_t v_off = static_cast<uint32_t>((rv.row() * p.v_stride[1] + rv.elem()) * kEs);
   constexpr int kWay = REV ? -1 : 1;

@@ -160,3 +160,9 @@ def test_params_layout_matches_header(tmp_path):
     subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(exe)], check=True)
     got = dict(l.split() for l in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines())
     assert all(int(got[f]) == getattr(cls, f).offset for f in fields) and int(got["sizeof"]) == ctypes.sizeof(cls)
+
+
+@pytest.mark.parametrize("value", [1 << 63, -(1 << 63) - 1])
+def test_ignore_index_is_64_bit(value):
+    with pytest.raises(ValueError, match="64-bit"):
+        loss(ignore_index=value)
