@@ -118,6 +118,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
         raise ValueError(f"targets is {tuple(targets.shape)}, expected {tuple(x.shape[:-1])}")
     if targets.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"targets is {targets.dtype}, expected int32 or int64")
+    if not -2 ** 63 <= int(ignore_index) < 2 ** 63:
+        raise ValueError(f"ignore_index {ignore_index} is no 64-bit integer")
     _lib.dtype_code(x.dtype)
     if weight.dtype != x.dtype:
         raise TypeError(f"weight is {weight.dtype}, x {x.dtype}")
