@@ -81,8 +81,10 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
   uint32_t id = blockIdx.x;
   const int vb = static_cast<int>(id % p.vblocks);
   id /= p.vblocks;
-  const int seg = static_cast<int>(id % p.segments);
-  id /= p.segments;
+  // (what the last segment walked adds is asked for by nobody: the states-only pass leaves it out)
+  const uint32_t segs = p.segments - (OUT ? 0 : 1);
+  const int seg = static_cast<int>(id % segs) + (REV && !OUT ? 1 : 0);
+  id /= segs;
   const int64_t head = id % static_cast<uint32_t>(p.heads), b = id / static_cast<uint32_t>(p.heads);
   const int64_t group = static_cast<uint32_t>(head) / static_cast<uint32_t>(p.per);
   const int64_t bh = b * p.heads + head;
@@ -468,8 +470,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Pass p) {
     f32x4 adds[8];
     double c[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {  // (eight at a time under way; the last one's own is not used)
-      const int n = n0 + j < p.segments ? n0 + j : n0, seg = REV ? p.segments - 1 - n : n;
+    for (int j = 0; j < 8; ++j) {  // (eight at a time under way)
+      const int n = n0 + j + 1 < p.segments ? n0 + j : n0, seg = REV ? p.segments - 1 - n : n;
       adds[j] = slots[seg * step];
       c[j] = decays[seg];
     }
@@ -488,7 +490,7 @@ template <int DT, int DKP, bool REV, bool VEC>
 static void launch_pass_t(const Pass& p, hipStream_t s) {
   const unsigned per_seg = static_cast<unsigned>(p.batch * p.heads * p.vblocks);
   if (p.segments > 1) {
-    hipLaunchKernelGGL((pass_kernel<DT, DKP, REV, false, VEC>), dim3(per_seg * p.segments), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((pass_kernel<DT, DKP, REV, false, VEC>), dim3(per_seg * (p.segments - 1)), dim3(256), 0, s, p);
     const int64_t n = p.batch * p.heads * p.vblocks * static_cast<int64_t>(kVBlock) * DKP / 4;
     hipLaunchKernelGGL((join_kernel<DKP, REV>), dim3(static_cast<unsigned>(ceil_div(n, 256))), dim3(256), 0, s, p);
   }
