@@ -20,7 +20,11 @@ MAX_VALUE_DIM = 1024  # MM_DECAY_MAX_VALUE_DIM
 _two, _three = _lib._i64a2, _lib._i64a3
 
 
-def _params(q, k, v, g, lengths, scale, dev):
+def _empty_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _params(q, k, v, g, lengths, scale):
     p = _lib.DecayAttentionParams()
     p.batch, p.seqlen, p.groups, p.key_dim = q.shape
     p.heads, p.value_dim = v.shape[2:]
@@ -55,9 +59,10 @@ def _states_bytes(q, v):
 
 
 def _forward(dev, q, k, v, g, h0, lengths, scale, want_state, train):
-    """y, the final state (or None) and, for training, the states before each run of tokens."""
-    p = _params(q, k, v, g, lengths, scale, dev)
-    y = torch.empty(v.shape, dtype=v.dtype, device=dev)
+    """y, the final state (or None), for training the states before each run of tokens, and the inputs' parameters."""
+    inputs = _params(q, k, v, g, lengths, scale)
+    p = _lib.DecayAttentionParams.from_buffer_copy(inputs)
+    y = _empty_like(v)
     p.y = y.data_ptr()
     state = states = None
     if h0 is not None:
@@ -69,13 +74,13 @@ def _forward(dev, q, k, v, g, h0, lengths, scale, want_state, train):
         states = torch.empty(_states_bytes(q, v), dtype=torch.uint8, device=dev)
         p.run_states = states.data_ptr() or None
     _call("mm_decay_attention_fwd", p, 0, dev)
-    return y, state, states
+    return y, state, states, inputs
 
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, dev, q, k, v, g, h0, lengths, scale, want_state):
-        y, state, states = _forward(dev, q, k, v, g, h0, lengths, scale, want_state, True)
+        y, state, states, ctx.inputs = _forward(dev, q, k, v, g, h0, lengths, scale, want_state, True)
         ctx.meta = (dev, q.dtype, q.shape, v.shape, g.dtype, g.shape, scale,
                     _lib.hooked() and (None if lengths is None else lengths.dtype,))
         ctx.set_materialize_grads(False)
@@ -92,7 +97,8 @@ class _DecayAttention(torch.autograd.Function):
         if hooked:
             saved = _checked(saved, dev, dtype, qk_shape, v_shape, g_dtype, g_shape, *hooked)
         q, k, v, g, lengths, states = saved
-        p = _params(q, k, v, g, lengths, scale, dev)
+        # (without hooks the saved tensors are the forward pass's; each backward pass has parameters of its own)
+        p = _params(q, k, v, g, lengths, scale) if hooked else _lib.DecayAttentionParams.from_buffer_copy(ctx.inputs)
         p.run_states = states.data_ptr() or None
         if dy is None:  # only the final state was used
             dy = torch.zeros((1, 1, 1, v_shape[3]), dtype=dtype, device=dev).expand(v_shape)
@@ -102,8 +108,7 @@ class _DecayAttention(torch.autograd.Function):
         if dstate is not None:
             dstate = dstate.contiguous()
             p.dstate = dstate.data_ptr()
-        dq, dk = (torch.empty(qk_shape, dtype=dtype, device=dev) for _ in range(2))
-        dv = torch.empty(v_shape, dtype=dtype, device=dev)
+        dq, dk, dv = _empty_like(q), _empty_like(k), _empty_like(v)
         p.dq, p.dk, p.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         dg = dh0 = None
         if ctx.needs_input_grad[4]:
@@ -131,24 +136,25 @@ def _checked(saved, dev, dtype, qk_shape, v_shape, g_dtype, g_shape, lengths_dty
 
 def _check(q, k, v, g, lead, names):
     """q and k (*lead, groups, key_dim), v (*lead, heads, value_dim), g (*lead, heads) or (heads,)."""
-    n = len(lead)
-    if q.dim() != n + 2 or v.dim() != n + 2 or v.shape[:n] != q.shape[:n]:
+    n, qs, vs, gs = len(lead), q.shape, v.shape, g.shape
+    if len(qs) != n + 2 or len(vs) != n + 2 or vs[:n] != lead:
         raise ValueError(f"q must be {names[:-1]}, groups, key_dim) and v {names[:-1]}, heads, value_dim), got "
-                         f"{tuple(q.shape)} and {tuple(v.shape)}")
-    if k.shape != q.shape:
-        raise ValueError(f"k is {tuple(k.shape)}, q {tuple(q.shape)}")
-    groups, dk = q.shape[n:]
-    heads, dv = v.shape[n:]
+                         f"{tuple(qs)} and {tuple(vs)}")
+    if k.shape != qs:
+        raise ValueError(f"k is {tuple(k.shape)}, q {tuple(qs)}")
+    groups, dk = qs[n:]
+    heads, dv = vs[n:]
     if groups < 1 or heads < 1 or heads % groups:
         raise ValueError(f"{heads} heads cannot share {groups} groups of q and k")
     if not 1 <= dk <= MAX_KEY_DIM or not 1 <= dv <= MAX_VALUE_DIM:
         raise ValueError(f"key_dim {dk} must be 1 to {MAX_KEY_DIM}, value_dim {dv} 1 to {MAX_VALUE_DIM}")
-    if g.shape != (heads,) and g.shape != (*q.shape[:n], heads):
-        raise ValueError(f"log_decay is {tuple(g.shape)}, expected {(heads,)} or {(*q.shape[:n], heads)}")
+    if gs != (heads,) and gs != (*lead, heads):
+        raise ValueError(f"log_decay is {tuple(gs)}, expected {(heads,)} or {(*lead, heads)}")
+    dtype = q.dtype
     for name, t in (("k", k), ("v", v)):
-        if t.dtype != q.dtype:
-            raise TypeError(f"{name} is {t.dtype}, q {q.dtype}")
-    _lib.dtype_code(q.dtype)
+        if t.dtype != dtype:
+            raise TypeError(f"{name} is {t.dtype}, q {dtype}")
+    _lib.dtype_code(dtype)
     _lib.dtype_code(g.dtype)
     for name, t in (("q", q), ("k", k), ("v", v)):
         channels_last(t, name)
@@ -201,7 +207,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     lengths = None if lengths is None else lengths.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, h0)):
         return _DecayAttention.apply(dev, q, k, v, log_decay, h0, lengths, float(scale), return_state)
-    y, state, _ = _forward(dev, q, k, v, log_decay, h0, lengths, float(scale), return_state, False)
+    y, state, *_ = _forward(dev, q, k, v, log_decay, h0, lengths, float(scale), return_state, False)
     return (y, state) if return_state else y
 
 
@@ -235,7 +241,7 @@ def decay_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, 
     dev = _lib.require_cuda(state, q, k, v, log_decay, state_out, out)
     lib = _lib.load()
     if out is None:
-        out = torch.empty(v.shape, dtype=v.dtype, device=dev)
+        out = _empty_like(v)
     with _lib.on_device(dev):
         st = lib.mm_decay_attention_step(
             state.data_ptr(), state.data_ptr() if state_out is None else state_out.data_ptr(), q.data_ptr(), k.data_ptr(),

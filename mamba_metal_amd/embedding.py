@@ -18,7 +18,7 @@ from mamba_metal_amd.act8 import channels_last
 
 def _forward(dev, ids, weight, scale):
     lib = _lib.load()
-    y = torch.empty((*ids.shape, weight.shape[1]), dtype=weight.dtype, device=dev)
+    y = weight.new_empty((*ids.shape, weight.shape[1]))
     with _lib.on_device(dev):
         st = lib.mm_embedding_fwd(ids.data_ptr(), weight.data_ptr(), y.data_ptr(), ids.numel(), *weight.shape, weight.stride(0),
                                   scale, 1 if ids.dtype == torch.int64 else 0, _lib.dtype_code(weight.dtype), _lib.stream_of(dev))
@@ -40,12 +40,12 @@ class _Embedding(torch.autograd.Function):
         ids, = ctx.saved_tensors
         if hooked:
             ids = _lib.saved(ids, *hooked, dev)
-        dy = dy.to(dtype).reshape(-1, dim)
+        dy = (dy if dy.dtype == dtype else dy.to(dtype)).reshape(-1, dim)
         if dy.stride(1) != 1 and dim > 1:
             dy = dy.contiguous()
         lib = _lib.load()
         n = dy.shape[0]
-        dweight = torch.empty((vocab, dim), dtype=dtype, device=dev)
+        dweight = dy.new_empty((vocab, dim))
         nbytes = lib.mm_embedding_bwd_workspace_size(n, vocab, dim)
         work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         with _lib.on_device(dev):
