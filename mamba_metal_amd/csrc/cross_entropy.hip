@@ -59,6 +59,10 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Loss p, bool backw
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int32_t base = 0;
   float top = 0.0f;
+  // One number for all rows is left out of the pieces and multiplies the sums: what a target's dl is nearly is then a power
+  // of two, which its rounding keeps.  fp16: the pieces hold dl times a power of two that puts the largest at 2^12, so that
+  // small probabilities are not subnormal; the sums take it back.
+  const float uniform = p.dtype == MM_F16 ? 4096.0f : 1.0f;
   for (int64_t r0 = 0; r0 < p.rows; r0 += kTurn * kThreads) {
     int64_t t[kTurn];
     float d[kTurn], lse[kTurn];
@@ -98,7 +102,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Loss p, bool backw
         p.row[at] = static_cast<int32_t>(r);
         p.target_at[at] = t[j];
         if (backward) {
-          p.weights[at] = d[j];
+          p.weights[at] = p.reduction ? uniform : d[j];
           p.lse_at[at] = t[j] < 0 || t[j] >= p.vocab ? __builtin_nanf("") : lse[j];
           top = fmaxf(top, fabsf(d[j]));
         }
@@ -109,13 +113,9 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Loss p, bool backw
   }
   if (threadIdx.x == 0) p.count[0] = base;
   if (!backward) return;
-  // One number for all rows is left out of the pieces and multiplies the sums: what a target's dl is nearly is then a power
-  // of two, which its rounding keeps.  fp16: the pieces hold dl times a power of two that puts the largest at 2^12, so that
-  // small probabilities are not subnormal; the sums take it back.
   if (p.reduction) {
-    const float up = p.dtype == MM_F16 ? 4096.0f : 1.0f;
-    for (int64_t i = threadIdx.x; i < base; i += kThreads) p.weights[i] = up;
-    if (threadIdx.x == 0) p.scalars[0] = base == 0 ? 0.0f : *p.dloss * (p.reduction == 1 ? 1.0f / static_cast<float>(base) : 1.0f) / up;
+    if (threadIdx.x == 0)
+      p.scalars[0] = base == 0 ? 0.0f : *p.dloss * (p.reduction == 1 ? 1.0f / static_cast<float>(base) : 1.0f) / uniform;
     return;
   }
   top = all_of(top, s_f, [](float a, float b) { return fmaxf(a, b); });

@@ -164,6 +164,7 @@ __global__ __launch_bounds__(kOneThreads) void sort_kernel(const Params p, int p
     const int shift = 14 + pass * bits;
     for (int d = lane; d < digits; d += 64) s_wave[wave][d] = 0;
     __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int r = 0; r < kRegs; ++r) {
       if (r >= rounds) break;
@@ -174,6 +175,7 @@ __global__ __launch_bounds__(kOneThreads) void sort_kernel(const Params p, int p
       __builtin_amdgcn_wave_barrier();
       if (in && below == 0) s_wave[wave][d] = first + __popcll(same);
       __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
       at[r] = first + __popcll(below);
     }
     __syncthreads();
