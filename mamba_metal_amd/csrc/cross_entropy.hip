@@ -9,7 +9,7 @@
 // A product's tile has the vocabulary along the accumulators' rows, so that the softmax's sums run within a lane.
 // bf16, 8192 rows (7377 counted) of 2560 by 50280 tokens: 1.72 ms forward; backward in two pieces, each 0.92 ms for dl and
 // 1.93 ms for dx and dW (0.98 PFLOP/s); 7.2 ms in all, where three library products of whole matrices would take 5.3 and
-// logits of 0.8 GB.  fp32, 999 (894) of 1001 by 10007: 190 us, 197 and 367, and 20 to lay the odd rows out.
+// logits of 0.8 GB.  fp32, 999 (894) of 1001 by 10007: 198 us, 202 and 384, and 20 to lay the odd rows out.
 //
 // Rows that are ignored take no part: the others are gathered first (their sums over rows are then never touched by what
 // an ignored row holds, and a batch that is mostly ignored costs its share), and workgroups past their count end at once.
@@ -506,12 +506,12 @@ enum Size { kBig, kMid, kThin };
 static int64_t high(Size s) { return s == kBig ? 256 : 128; }
 static int64_t wide(Size s) { return s == kBig ? 256 : s == kMid ? 128 : 64; }
 static int64_t tiles_of(Size s, int64_t m, int64_t n) { return ceil_div(m, high(s)) * ceil_div(n, wide(s)); }
-// 256 x 256 where there are enough of them to fill the card's rounds, else 128 x 128, and in fp32, whose products take
-// longer than their operands, 128 x 64.  (bf16, 1024 rows of 1024 by 8192 tokens, 128 large tiles: 27 us against 33;
-// 2048 rows, 256 of them: 47 us against 39.  fp32, 999 by 10007 of 1001, 160 large tiles: 192 us, 208 in tiles of 128 x 128,
-// 261 large; 2048 by 16384 of 1024, 512 of them: 595 us against 549.)
+// 256 x 256 where there are enough of them to fill the card's rounds, else 128 x 128.  (bf16, 1024 rows of 1024 by 8192
+// tokens, 128 large tiles: 33 us, 27 in small ones; 2048 rows, 256 of them: 39 us, 47 in small ones.)  fp32: 128 x 128, whose
+// sums leave room for a second set of them, or 128 x 64.  (2048 rows of 1024 by 16384 tokens, 512 large tiles: 559 us, 595
+// in small ones; 999 of 1001 by 10007, 160 of them: 208 us, 192 in small ones.)
 static Size size_of(int dtype, int64_t big_tiles) {
-  if (dtype == MM_F32) return big_tiles >= 512 ? kBig : kThin;
+  if (dtype == MM_F32) return big_tiles >= 512 ? kMid : kThin;
   return big_tiles >= 192 ? kBig : kMid;
 }
 // 128 x 64 also for few rows, where the vocabulary's rows are the traffic.
@@ -687,10 +687,10 @@ static void launch_logits_t(const Loss& p, int64_t vocab, hipStream_t st) {
 template <int DT, bool GRAD>
 static void launch_logits(const Loss& p, Size size, int64_t vocab, hipStream_t st) {
   switch (size) {
-    case kBig: launch_logits_t<DT, Big, GRAD>(p, vocab, st); break;
-    case kMid:
-      if constexpr (DT != MM_F32) launch_logits_t<DT, Mid, GRAD>(p, vocab, st);
+    case kBig:
+      if constexpr (DT != MM_F32) launch_logits_t<DT, Big, GRAD>(p, vocab, st);
       break;
+    case kMid: launch_logits_t<DT, Mid, GRAD>(p, vocab, st); break;
     case kThin: launch_logits_t<DT, Thin, GRAD>(p, vocab, st); break;
   }
 }
@@ -702,8 +702,8 @@ static void launch_grads_t(Loss p, hipStream_t st) {
 }
 template <int DT>
 static void launch_grads(const Loss& p, Size size, hipStream_t st) {
-  if (size == kBig) return launch_grads_t<DT, Big>(p, st);
-  if constexpr (DT == MM_F32) launch_grads_t<DT, Thin>(p, st); else launch_grads_t<DT, Mid>(p, st);
+  if (size == kMid) return launch_grads_t<DT, Mid>(p, st);
+  if constexpr (DT == MM_F32) launch_grads_t<DT, Thin>(p, st); else launch_grads_t<DT, Big>(p, st);
 }
 
 template <int DT>

@@ -23,7 +23,7 @@ struct Pass {
   double* seg_decay;
   int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3];  // batch, time, head
   int64_t batch, seqlen, heads, per, dk, dv, runs, seg_runs;
-  int32_t vblocks, segments, vec, dtype, g_dtype, lengths_dtype;
+  int32_t vblocks, segments, vec, dtype, g_dtype, lengths_dtype, fine;
   float scale;
 };
 
@@ -36,7 +36,7 @@ struct Grad {
   float* dg;              // (batch, seqlen, heads) or NULL
   int64_t q_stride[3], k_stride[3], v_stride[3], dy_stride[3], g_stride[3];
   int64_t batch, seqlen, heads, groups, per, dk, dv, runs;
-  int32_t vblocks, sets, set_heads, vec, dtype, g_dtype, lengths_dtype;
+  int32_t vblocks, sets, set_heads, vec, dtype, g_dtype, lengths_dtype, fine;
   float scale;
 };
 
@@ -51,6 +51,10 @@ struct Step {
   float scale;
 };
 
+// Whether the scores of 16-bit types take a second term (decay_tiles.h, score_operand).
+inline bool fine_scores(int64_t batch, int64_t seqlen, int64_t heads, int32_t dtype) {
+  return dtype != MM_F32 && batch * seqlen * heads <= 32768;
+}
 inline int padded_dk(int64_t dk) { return dk <= 64 ? 64 : 128; }
 
 void launch_pass_forward(const Pass& p, hipStream_t s);

@@ -99,8 +99,9 @@ struct Shape {
 // Segments: with fewer than 256 workgroups (one a compute unit) the tokens are cut so that there are as many as run at once,
 // 3 a compute unit in 16 bits, else 2 (80 heads, 8192 tokens in bf16: 161 us in 9 segments, 178 in 6).  Two runs are not cut:
 // fp32, 8 heads: 17 us whole, 20 in two segments and three launches; four runs: 30 us in two segments, 20 in four.
-// Sets of heads in the gradients of q and k: as few as make 768 workgroups, since each set's sums are written and read
-// once more.
+// Sets of heads in the gradients of q and k, which have a compute unit each: as many as end first, a set's own work (q, k,
+// their scores, its sums written and read once more) counted as four heads of a unit.  (80 heads, 256
+// runs of 64 tokens, bf16: 307 us in one set, 310 to 330 and 17 more for the sums in three.)
 static Shape shape_of(int64_t batch, int64_t seqlen, int64_t heads, int64_t groups, int64_t dv, int32_t dtype) {
   Shape s;
   s.runs = ceil_div(seqlen, kRun);
@@ -112,8 +113,11 @@ static Shape shape_of(int64_t batch, int64_t seqlen, int64_t heads, int64_t grou
   s.seg_runs = ceil_div(s.runs > 0 ? s.runs : 1, segs);
   s.segments = static_cast<int32_t>(ceil_div(s.runs > 0 ? s.runs : 1, s.seg_runs));
   const int64_t grads = batch * groups * (s.runs > 0 ? s.runs : 1);
-  int64_t sets = ceil_div(768, grads);
-  if (sets > per) sets = per;
+  int64_t sets = 1, least = INT64_MAX;
+  for (int64_t n = 1; n <= per && n <= 64; ++n) {
+    const int64_t t = ceil_div(grads * n, 256) * (ceil_div(per, n) + 4);
+    if (t < least) least = t, sets = n;
+  }
   s.set_heads = static_cast<int32_t>(ceil_div(per, sets));
   s.sets = static_cast<int32_t>(ceil_div(per, s.set_heads));
   return s;
@@ -219,6 +223,7 @@ static Pass pass_of(const mm_decay_attention_params* p, const Shape& s, const La
   k.g_dtype = p->log_decay_dtype;
   k.lengths_dtype = p->lengths_dtype;
   k.scale = p->scale;
+  k.fine = fine_scores(p->batch, p->seqlen, p->heads, p->dtype);
   if (s.segments > 1) {
     k.seg_states = reinterpret_cast<float*>(ws + l.seg_states);
     k.seg_decay = reinterpret_cast<double*>(ws + l.seg_decay);
@@ -358,6 +363,7 @@ int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream) {
     d.g_dtype = p->log_decay_dtype;
     d.lengths_dtype = p->lengths_dtype;
     d.scale = p->scale;
+    d.fine = fine_scores(p->batch, p->seqlen, p->heads, p->dtype);
     launch_grad(d, st);
     if (s.sets > 1) {
       const dim3 grid(static_cast<unsigned>(ceil_div(n, 256)));

@@ -323,9 +323,10 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         }
         sum += (x[0] + x[1]) + (x[2] + x[3]);
       }
-      u32x4 dp[kRun / O::kStep];
+      const bool fine = !O::kWide && p.fine;
+      u32x4 dp[kRun / O::kStep], rest[kRun / O::kStep];
 #pragma unroll
-      for (int u = 0; u < kRun / O::kStep; ++u) dp[u] = from_acc<DT>(acc + u * O::kTiles);
+      for (int u = 0; u < kRun / O::kStep; ++u) score_operand<DT>(acc + u * O::kTiles, fine, dp[u], rest[u]);
       // the states' part, scaled row by row
       const f32x4 w = *reinterpret_cast<const f32x4*>((role ? D.onward : D.into) + 16 * blk + 4 * g) * ((role ? 1.0f : p.scale) * factor);
       f32x4 inter = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -359,9 +360,17 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
           columns<TK, u * 32>(at, o);
 #pragma unroll
           for (int t = 0; t < ND; ++t) out[t] = mma<DT>(dp[u], o[t], out[t]);
+          if (fine) {
+#pragma unroll
+            for (int t = 0; t < ND; ++t) out[t] = mma_rest<DT>(rest[u], o[t], out[t]);
+          }
         } else {
 #pragma unroll
           for (int t = 0; t < ND; ++t) out[t] = mma<DT>(dp[u], TK::column(s_other, u * O::kStep, 16 * t, lane), out[t]);
+          if (fine) {
+#pragma unroll
+            for (int t = 0; t < ND; ++t) out[t] = mma_rest<DT>(rest[u], TK::column(s_other, u * O::kStep, 16 * t, lane), out[t]);
+          }
         }
       };
       add_rows(std::integral_constant<int, 0>{});

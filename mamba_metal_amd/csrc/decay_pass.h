@@ -30,36 +30,6 @@
 namespace mm {
 namespace dattn {
 
-// 16-bit operands of a product whose result is a state in fp32: the value as a sum of TERMS of them.  bf16: three are
-// fp32's own 24 bits.  fp16: two hold 22 bits, the second one 2^11 times too large (and summed by itself), since the rest of a
-// value below 1/8 would be subnormal, which the matrix cores take as 0; so would be values below 2^-14, which therefore
-// are all rest.
-constexpr float kRestUp = 2048.0f;
-template <int DT, int TERMS>
-__device__ __forceinline__ void split_operand(const float (&x)[8], u32x4 (&out)[TERMS]) {
-  float rest[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) rest[j] = x[j];
-#pragma unroll
-  for (int n = 0; n < TERMS; ++n)
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      float c[2] = {rest[j], rest[j + 1]};
-      if (DT == MM_F16) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) c[e] = n == 0 ? (fabsf(c[e]) < 6.103515625e-05f ? 0.0f : c[e]) : c[e] * kRestUp;
-      }
-      const uint32_t w = pack2<DT>(c[0], c[1]);
-      out[n][j / 2] = w;
-      if (n + 1 < TERMS) {
-        float a, b;
-        unpack2<DT>(w, a, b);
-        rest[j] -= a;
-        rest[j + 1] -= b;
-      }
-    }
-}
-
 template <int DT, int DKP, bool REV, bool OUT, bool VEC>
 __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : VEC ? 3 : 2) void pass_kernel(const Pass p) {
   using T = typename Ty<DT>::T;
@@ -312,9 +282,10 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
           acc[st][r] = st != wave || (REV ? 4 * g + r >= i : 4 * g + r <= i) ? x : 0.0f;
         }
       }
-      u32x4 po[NR];
+      const bool fine = !O::kWide && p.fine;
+      u32x4 po[NR], rest[NR];
 #pragma unroll
-      for (int u = 0; u < NR; ++u) po[u] = from_acc<DT>(acc + u * O::kTiles);
+      for (int u = 0; u < NR; ++u) score_operand<DT>(acc + u * O::kTiles, fine, po[u], rest[u]);
       keep_state(1);
       // outputs, turned over: 4 value channels of a token in a lane
       f32x4 y[4];
@@ -334,6 +305,10 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
         if (REV ? (u + 1) * O::kStep <= 16 * wave : u * O::kStep > 16 * wave + 15) continue;
 #pragma unroll
         for (int vt = 0; vt < 4; ++vt) y[vt] = mma<DT>(TV::column(s_v, u * O::kStep, 16 * vt, lane), po[u], y[vt]);
+        if (fine) {
+#pragma unroll
+          for (int vt = 0; vt < 4; ++vt) y[vt] = mma_rest<DT>(TV::column(s_v, u * O::kStep, 16 * vt, lane), rest[u], y[vt]);
+        }
       }
       const int left = static_cast<int>(p.seqlen - run * kRun < kRun ? p.seqlen - run * kRun : kRun), t = 16 * wave + i;
       if (t < left) {

@@ -82,6 +82,59 @@ __device__ __forceinline__ u32x4 from_acc(const f32x4* t) {
                  pack2<DT>(t[1][2], t[1][3])};
 }
 
+// 16-bit operands of a product whose result is a state in fp32: the value as a sum of TERMS of them.  bf16: three are
+// fp32's own 24 bits.  fp16: two hold 22 bits, the second one 2^11 times too large (and summed by itself), since the rest of a
+// value below 1/8 would be subnormal, which the matrix cores take as 0; so would be values below 2^-14, which therefore
+// are all rest.
+constexpr float kRestUp = 2048.0f;
+template <int DT, int TERMS>
+__device__ __forceinline__ void split_operand(const float (&x)[8], u32x4 (&out)[TERMS]) {
+  float rest[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) rest[j] = x[j];
+#pragma unroll
+  for (int n = 0; n < TERMS; ++n)
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      float c[2] = {rest[j], rest[j + 1]};
+      if (DT == MM_F16) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) c[e] = n == 0 ? (fabsf(c[e]) < 6.103515625e-05f ? 0.0f : c[e]) : c[e] * kRestUp;
+      }
+      const uint32_t w = pack2<DT>(c[0], c[1]);
+      out[n][j / 2] = w;
+      if (n + 1 < TERMS) {
+        float a, b;
+        unpack2<DT>(w, a, b);
+        rest[j] -= a;
+        rest[j + 1] -= b;
+      }
+    }
+}
+
+// Scores (accumulator tiles, in acc order) as operands, rounded once.  A score's rounding is the same in all channels of its
+// token, so that few tokens may all be off by nearly half a step where many are by a third: `fine` ones, of calls of few
+// tokens, take a second term, the rest.  (Of many it would take 4% of a pass.)
+template <int DT>
+__device__ __forceinline__ void score_operand(const f32x4* t, bool fine, u32x4& whole, u32x4& rest) {
+  whole = from_acc<DT>(t);
+  if constexpr (!Op<DT>::kWide) {
+    if (fine) {
+      const float x[8] = {t[0][0], t[0][1], t[0][2], t[0][3], t[1][0], t[1][1], t[1][2], t[1][3]};
+      u32x4 terms[2];
+      split_operand<DT, 2>(x, terms);
+      whole = terms[0];
+      rest = terms[1];
+    }
+  }
+}
+// The product with the rest.
+template <int DT>
+__device__ __forceinline__ f32x4 mma_rest(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (DT == MM_F16) return c + mma<DT>(a, b, f32x4{0.0f, 0.0f, 0.0f, 0.0f}) * (1.0f / kRestUp);
+  else return mma<DT>(a, b, c);
+}
+
 // A tile of W columns in shared memory.  16-bit rows are cut into chunks of 16 bytes, and chunk c of row r is kept at
 // place c ^ turn(r), without bank conflicts: a transposing read touches pairs of chunks of 8 rows, whose turns differ above
 // the lowest bit; a 16-byte row read goes in four parts of 16 lanes, 0-3, 12-15 and 20-27 and so on, so that rows 4 to 11 of

@@ -6,7 +6,7 @@
 // take 1.5 to 2 us, twice what its products take, and it is the bytes under way that keep the matrix cores fed.  bf16, 8192
 // rows (7377 of them counted) of 2560 by 50280: 1890 us with two stages of 128 bytes behind flat loads, 1.67 to 1.72 ms now,
 // 1.12 PFLOP/s; the cores' cycles are 58% busy at the 1.9 GHz that the card holds under it (a library product of the whole
-// shape reaches 1.19).  fp32, 2048 by 16384 of 4096: 126 TFLOP/s, 89% busy (library: 136).
+// shape reaches 1.19).  fp32, 2048 by 16384 of 1024: 117 TFLOP/s (123 without the short sums below).
 //
 // An operand lies in memory either way:
 //   kAlong   k is contiguous: a row of the slab is 64 bytes of a row of the matrix, four 16-byte chunks.  Chunk c of
@@ -267,13 +267,35 @@ __device__ __forceinline__ void product(const Matrix& A, const Matrix& B, int64_
   };
   using First = std::integral_constant<int, 0>;
   using Second = std::integral_constant<int, 1>;
+  // fp32: 256 elements at a time are summed by themselves and then added.  (A sum's own rounding grows with the root of the
+  // addends behind one another: gradients of 700 rows of 4000 by 9000 tokens are off by 3e-7, in one chain by over 1e-6;
+  // it costs 5%.  16-bit inputs bring more than that with them.)
+  constexpr bool kShort = DT == MM_F32;
+  f32x16 part_sum[kShort ? S::TM : 1][kShort ? S::TN : 1];
+  auto& sum = [&]() -> auto& {
+    if constexpr (kShort) return part_sum;
+    else return acc;
+  }();
+  auto flush = [&](bool go_on) __attribute__((always_inline)) {
+    if constexpr (kShort) {
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) {
+          if (go_on) acc[i][j] += part_sum[i][j];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) part_sum[i][j][r] = 0.0f;
+        }
+    }
+  };
+  flush(false);
   auto multiply = [&](const Step& q) __attribute__((always_inline)) {
 #pragma unroll
     for (int part = 0; part < kParts<DT>; ++part)  // (neighbours in time add to different sums)
 #pragma unroll
       for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-        for (int j = 0; j < S::TN; ++j) acc[i][j] = mma<DT>(q.a[i], q.b[j], part, acc[i][j]);
+        for (int j = 0; j < S::TN; ++j) sum[i][j] = mma<DT>(q.a[i], q.b[j], part, sum[i][j]);
   };
   constexpr int kLoads = SA::kLoads + SB::kLoads;
   static_assert(kSteps == 2, "a slab's first step before the others are met, its second behind it");
@@ -318,10 +340,12 @@ __device__ __forceinline__ void product(const Matrix& A, const Matrix& B, int64_
     slab(s1, s2, t + 1);
     slab(s2, s3, t + 2);
     slab(s3, s0, t + 3);
+    if (kShort && t % (256 / SA::kDepth) == 256 / SA::kDepth - S::ST) flush(true);
   }
   if (t < slabs) slab(s0, s1, t);
   if (t + 1 < slabs) slab(s1, s2, t + 1);
   if (t + 2 < slabs) slab(s2, s3, t + 2);
+  flush(true);
   meet<0>();
 }
 
