@@ -36,6 +36,8 @@ struct Loss {
   int64_t tiles, splits, split_k;         // of the vocabulary in stats; of dx's sums over a piece, and a split's tokens
   int32_t first_piece;
   uint32_t dx_tiles;                      // workgroups of dx, before dW's
+  float* logit_part;      // (logit_splits, rows, logit_ld), where few tiles of logits are cut along their sums
+  int64_t logit_splits, logit_k, logit_ld;
 };
 
 }  // namespace xent

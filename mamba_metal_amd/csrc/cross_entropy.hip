@@ -357,6 +357,85 @@ __global__ __launch_bounds__(64 * S::NW) void logits_kernel(const Loss p) {
   }
 }
 
+// fp32, where tiles of logits are so few that most of the card would wait for their long sums: a split of them, kept as it is.
+template <int DT>
+__global__ __launch_bounds__(64 * Thin::NW) void split_logits_kernel(const Loss p, bool grad) {
+  MM_SLAB_STAGES(Thin, stages)
+  const int32_t count = *p.count;
+  const uint32_t vt = static_cast<uint32_t>(p.logit_ld / Thin::BM), rt = static_cast<uint32_t>((p.rows + Thin::BN - 1) / Thin::BN);
+  uint32_t m, n;
+  slab::tile_of(blockIdx.x % (vt * rt), vt, rt, m, n);
+  const int64_t split = blockIdx.x / (vt * rt), v0 = static_cast<int64_t>(m) * Thin::BM, r0 = static_cast<int64_t>(n) * Thin::BN;
+  if (r0 >= count) return;
+  f32x16 acc[Thin::TM][Thin::TN];
+  slab::clear<Thin>(acc);
+  const Matrix w = vocabulary(p, grad ? p.piece0 : 0), x = counted(p, count);
+  const int64_t k0 = split * p.logit_k, k = w.k - k0 < p.logit_k ? w.k - k0 : p.logit_k;
+  slab::product<DT, kAlong, kAlong, Thin>(w, x, v0, r0, k0, k, stages0, stages1, stages2, stages3, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / Thin::WN, wn = wave % Thin::WN;
+#pragma unroll
+  for (int j = 0; j < Thin::TN; ++j) {
+    const int64_t r = r0 + wn * 32 * Thin::TN + 32 * j + (lane & 31);
+    if (r >= count) continue;
+    float* const to = p.logit_part + (split * p.rows + r) * p.logit_ld + v0 + wm * 32 * Thin::TM + 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < Thin::TM; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<slab::f32x4*>(to + 32 * i + 8 * q) = slab::f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+  }
+}
+// Their sums, in order, and what logits_kernel makes of them: a wave takes 128 tokens of a row.
+template <bool GRAD>
+__global__ __launch_bounds__(256) void join_logits_kernel(const Loss p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t tiles = p.logit_ld / 128, unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t r = unit / tiles, m = unit % tiles, v = m * 128 + 2 * lane;
+  if (r >= *p.count) return;
+  float l[2] = {0.0f, 0.0f};
+#pragma unroll 4
+  for (int64_t s = 0; s < p.logit_splits; ++s) {
+    const float* const from = p.logit_part + (s * p.rows + r) * p.logit_ld + v;
+    l[0] += from[0];
+    l[1] += from[1];
+  }
+  const int64_t vocab = GRAD ? p.piece_n : p.vocab, target = p.target_at[r] - (GRAD ? p.piece0 : 0);
+  if constexpr (!GRAD) {
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (v + e >= vocab) l[e] = -INFINITY;
+      else if (v + e == target) p.hit[r] = l[e];
+      top = fmaxf(top, l[e]);
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, lane_xor(top, x));
+    const float from = top == -INFINITY ? 0.0f : top;
+    bool bad = top == INFINITY;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      bad |= l[e] != l[e];
+      sum += exp2_acc((l[e] - from) * kLog2e);
+    }
+    if (bad) sum = __builtin_nanf("");
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) sum += lane_xor(sum, x);
+    if (lane == 0 && m < p.tiles) {
+      p.stats[(r * p.tiles + m) * 2] = top;
+      p.stats[(r * p.tiles + m) * 2 + 1] = sum;
+    }
+  } else {
+    const float lse = p.lse_at[r], weight = p.weights[r];
+    float* const to = reinterpret_cast<float*>(p.piece + r * p.piece_ld) + v;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float z = (l[e] - lse) * kLog2e, g = exp2_acc(z);
+      const float d = (z != z ? z : g) * weight - (v + e == target ? weight : 0.0f);
+      to[e] = v + e < vocab ? d : 0.0f;
+    }
+  }
+}
+
 // A row's loss from its tiles' maxima and sums: a wave a row.  (8192 rows, 197 tiles: 9 us.)
 __global__ __launch_bounds__(256) void merge_kernel(const Loss p) {
   const int lane = threadIdx.x & 63;
@@ -553,6 +632,7 @@ struct Plan {
   bool copy_w;
   Size logits;
   Grads grads;
+  int64_t logit_splits, logit_k, logit_ld, logit_part;
   int64_t at, row, count, scalars, weights, lse_at, target_at, xc, wc, stats, hit, row_loss, piece, dx_part, total;
 };
 
@@ -595,6 +675,20 @@ static Plan plan_of(const mm_linear_cross_entropy_params* q, bool backward) {
     const Grads both = grads_of(q->dtype, q->rows, q->dim, s.piece_n, true, true), one = grads_of(q->dtype, q->rows, q->dim, s.piece_n, true, false);
     s.grads = !q->dx ? grads_of(q->dtype, q->rows, q->dim, s.piece_n, false, true) : q->dweight ? both : one;
     s.dx_part = take((both.splits > one.splits ? both.splits : one.splits) * q->rows * q->dim * 4);
+  }
+  // (the piece's columns are whole tiles of 256)
+  s.logit_splits = 1;
+  s.logit_ld = backward ? s.piece_n : round_up(q->vocab, 128);
+  if (q->dtype == MM_F32 && s.logits == kThin) {
+    // 512 workgroups of 256 elements of the sum at least (a pass over the loss, 30 rows of 4000 by 5000 tokens: 155 us whole,
+    // 49 in 13; 64 of 7000 by 8000: 258, and 92 in 9.  300 of 2000 by 5000, 200 tiles: 86 us whole, 88 in three.)
+    const int64_t tiles = tiles_of(kThin, s.logit_ld, q->rows), most = s.ld / 4 / 256;
+    if (tiles < 192 && most > 1) {
+      s.logit_splits = ceil_div(512, tiles) < most ? ceil_div(512, tiles) : most;
+      s.logit_k = round_up(ceil_div(s.ld / 4, s.logit_splits), 64);
+      s.logit_splits = ceil_div(s.ld / 4, s.logit_k);
+      s.logit_part = take(s.logit_splits * q->rows * s.logit_ld * 4);
+    }
   }
   s.total = at;
   return s;
@@ -649,6 +743,10 @@ static Loss loss_of(const mm_linear_cross_entropy_params* q, const Plan& s, bool
   p.wc = s.copy_w ? ws + s.wc : nullptr;
   p.ld = s.ld;
   p.tiles = s.tiles;
+  p.logit_splits = s.logit_splits;
+  p.logit_k = s.logit_k;
+  p.logit_ld = s.logit_ld;
+  p.logit_part = reinterpret_cast<float*>(ws + s.logit_part);
   if (!backward) {
     p.stats = reinterpret_cast<float*>(ws + s.stats);
     p.hit = reinterpret_cast<float*>(ws + s.hit);
@@ -686,6 +784,15 @@ static void launch_logits_t(const Loss& p, int64_t vocab, hipStream_t st) {
 }
 template <int DT, bool GRAD>
 static void launch_logits(const Loss& p, Size size, int64_t vocab, hipStream_t st) {
+  if constexpr (DT == MM_F32) {
+    if (p.logit_splits > 1) {
+      hipLaunchKernelGGL((split_logits_kernel<DT>), dim3(static_cast<unsigned>(tiles_of(kThin, p.logit_ld, p.rows) * p.logit_splits)),
+                         dim3(64 * Thin::NW), 0, st, p, GRAD);
+      hipLaunchKernelGGL((join_logits_kernel<GRAD>), dim3(static_cast<unsigned>(ceil_div(p.rows * (p.logit_ld / 128), 4))), dim3(256),
+                         0, st, p);
+      return;
+    }
+  }
   switch (size) {
     case kBig:
       if constexpr (DT != MM_F32) launch_logits_t<DT, Big, GRAD>(p, vocab, st);
