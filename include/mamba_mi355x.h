@@ -505,8 +505,8 @@ int mm_causal_conv1d_fwd_act8(const void* x, const void* weight, const void* bia
  * forgets; above 0 the state grows until it overflows).  States (batch, heads, key_dim, value_dim) contiguous fp32.
  * lengths as in mm_gated_scan_params: tokens from lengths[b] on leave the state as it is, have y = 0 and gradients 0,
  * and their inputs do not matter.  key_dim <= 128, value_dim <= 1024.  Sums and states are fp32; 16-bit types round
- * the scores of a run of 64 tokens and the state that meets q, each once, to dtype before their products (the scores of
- * calls of up to 32768 tokens, batch * seqlen * heads, to the sum of two).
+ * the scores of a run of 64 tokens and the state that meets q, each once, to dtype before their products (in calls of up
+ * to 32768 tokens, batch * seqlen * heads, the scores to the sum of two, and so the states in gradients of q, k and g).
  *
  * Training: the forward call given run_states (mm_decay_attention_states_size bytes, 256-byte aligned) writes there, in
  * dtype, the states that the backward call reads.  Sums are taken in a fixed order: calls repeat bit for bit. */

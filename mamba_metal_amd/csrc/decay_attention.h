@@ -16,6 +16,8 @@ struct Pass {
   const void* lengths;
   void* states;           // the state before (mirrored: its gradient after) each run, or NULL
   float* factors;         // fp16: the power of two each of them was divided by
+  void* state_rests;      // `fine`: what the 16-bit states leave of the fp32 ones, or NULL
+  const void* rests_with; // mirrored, `fine`: the forward pass's, for the products
   const void* dot_with;   // mirrored: the forward pass's states and their factors, and where their products with
   const float* factors_with;  // this pass's go, (batch, heads, runs, vblocks); NULL = not wanted
   float* dot;
@@ -30,13 +32,13 @@ struct Pass {
 // Gradients of q, k and the log decays from the states on both sides of each run (decay_attention_bwd.hip).
 struct Grad {
   const void *q, *k, *v, *dy, *g, *lengths;
-  const void *states, *dstates;
+  const void *states, *dstates, *rests, *drests;  // the last two: `fine`, or NULL
   const float *factors, *dfactors, *dot;
   void *dq, *dk_out;      // (batch, seqlen, groups, dk) contiguous; with sets > 1 fp32 (sets, batch, seqlen, groups, dk)
   float* dg;              // (batch, seqlen, heads) or NULL
   int64_t q_stride[3], k_stride[3], v_stride[3], dy_stride[3], g_stride[3];
   int64_t batch, seqlen, heads, groups, per, dk, dv, runs;
-  int32_t vblocks, sets, set_heads, vec, dtype, g_dtype, lengths_dtype, fine;
+  int32_t vblocks, sets, set_heads, vec, dtype, g_dtype, lengths_dtype;
   float scale;
 };
 

@@ -132,7 +132,7 @@ static bool sizes_ok(int64_t batch, int64_t seqlen, int64_t heads, int64_t group
 
 // The regions of a call's workspace.
 struct Layout {
-  int64_t seg_states, seg_decay, dstates, dfactors, dot, parts, dg, total;
+  int64_t seg_states, seg_decay, dstates, dfactors, drests, dot, parts, dg, total;
 };
 static Layout layout_of(const Shape& s, int64_t batch, int64_t seqlen, int64_t heads, int64_t groups, int64_t dk, int64_t dv,
                         int32_t dtype, bool backward) {
@@ -151,6 +151,7 @@ static Layout layout_of(const Shape& s, int64_t batch, int64_t seqlen, int64_t h
   if (backward) {
     l.dstates = take(bh * s.runs * block * dtype_size(dtype));
     l.dfactors = take(dtype == MM_F16 ? bh * s.runs * s.vblocks * 4 : 0);
+    l.drests = take(fine_scores(batch, seqlen, heads, dtype) ? bh * s.runs * block * dtype_size(dtype) : 0);
     l.dot = take(bh * s.runs * s.vblocks * 4);
     l.parts = take(s.sets > 1 ? 2 * s.sets * batch * seqlen * groups * dk * 4 : 0);
     l.dg = take(rows::floats(batch * seqlen, heads) * 4);
@@ -161,6 +162,11 @@ static Layout layout_of(const Shape& s, int64_t batch, int64_t seqlen, int64_t h
 
 static int64_t states_bytes(const Shape& s, int64_t batch, int64_t heads, int64_t dk, int32_t dtype) {
   return round_up(batch * heads * s.runs * s.vblocks * kVBlock * padded_dk(dk) * dtype_size(dtype), 256);
+}
+
+// Behind the states: fp16's powers of two, and the rests of calls with fine scores.
+static int64_t rests_at(const Shape& s, int64_t batch, int64_t heads, int64_t dk, int32_t dtype) {
+  return states_bytes(s, batch, heads, dk, dtype) + (dtype == MM_F16 ? round_up(batch * heads * s.runs * s.vblocks * 4, 256) : 0);
 }
 
 static int check_strides(const int64_t* s, const char* name) {
@@ -246,8 +252,8 @@ size_t mm_decay_attention_states_size(int64_t batch, int64_t seqlen, int64_t hea
   using namespace mm::dattn;
   if (!valid_dtype(dtype) || !sizes_ok(batch, seqlen, heads, 1, key_dim, value_dim)) return 0;
   const Shape s = shape_of(batch, seqlen, heads, 1, value_dim, dtype);
-  return static_cast<size_t>(states_bytes(s, batch, heads, key_dim, dtype) +
-                             (dtype == MM_F16 ? batch * heads * s.runs * s.vblocks * 4 : 0));
+  return static_cast<size_t>(rests_at(s, batch, heads, key_dim, dtype) +
+                             (fine_scores(batch, seqlen, heads, dtype) ? states_bytes(s, batch, heads, key_dim, dtype) : 0));
 }
 
 size_t mm_decay_attention_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t groups, int64_t key_dim,
@@ -285,6 +291,7 @@ int mm_decay_attention_fwd(const mm_decay_attention_params* p, void* stream) {
   k.states = p->run_states;
   if (k.states && p->dtype == MM_F16)
     k.factors = reinterpret_cast<float*>(static_cast<char*>(k.states) + states_bytes(s, p->batch, p->heads, p->key_dim, p->dtype));
+  if (k.states && k.fine) k.state_rests = static_cast<char*>(k.states) + rests_at(s, p->batch, p->heads, p->key_dim, p->dtype);
   launch_pass_forward(k, static_cast<hipStream_t>(stream));
   return check_launch("decay_attention_fwd");
 }
@@ -321,9 +328,12 @@ int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream) {
   k.factors = reinterpret_cast<float*>(ws + l.dfactors);
   const float* const factors = reinterpret_cast<const float*>(
       static_cast<const char*>(p->run_states) + states_bytes(s, p->batch, p->heads, p->key_dim, p->dtype));
+  const char* const rests = static_cast<const char*>(p->run_states) + rests_at(s, p->batch, p->heads, p->key_dim, p->dtype);
+  if (k.fine) k.state_rests = ws + l.drests;
   float* const dg = p->dlog_decay_heads ? reinterpret_cast<float*>(ws + l.dg) : p->dlog_decay;
   if (dg) {
     k.dot_with = p->run_states;
+    if (k.fine) k.rests_with = rests;
     k.factors_with = factors;
     k.dot = reinterpret_cast<float*>(ws + l.dot);
   }
@@ -338,6 +348,7 @@ int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream) {
     d.lengths = p->lengths;
     d.states = p->run_states;
     d.dstates = k.states;
+    if (k.fine) d.rests = rests, d.drests = k.state_rests;
     d.factors = factors;
     d.dfactors = k.factors;
     d.dot = k.dot;
@@ -363,7 +374,6 @@ int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream) {
     d.g_dtype = p->log_decay_dtype;
     d.lengths_dtype = p->lengths_dtype;
     d.scale = p->scale;
-    d.fine = fine_scores(p->batch, p->seqlen, p->heads, p->dtype);
     launch_grad(d, st);
     if (s.sets > 1) {
       const dim3 grid(static_cast<unsigned>(ceil_div(n, 256)));

@@ -66,7 +66,9 @@ __device__ __forceinline__ void columns_at(const T* tile, int lane, uint32_t (&a
   for (int t = 0; t < N; ++t) at[t] = base + TILE::at(0, 16 * t, 4 * (lane >> 4) + ((lane & 15) >> 2), 4 * (lane & 3)) * 2;
 }
 
-template <int DT, int DKP, bool DIRECT, bool ONE>
+// FINE: of few tokens (decay_tiles.h, score_operand), with the rests of the states' roundings, which a run's tokens share: registers
+// go to memory for it (310 us would be 650).
+template <int DT, int DKP, bool DIRECT, bool ONE, bool FINE>
 __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
   using T = typename Ty<DT>::T;
   using O = Op<DT>;
@@ -297,6 +299,24 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         add_state(std::integral_constant<int, 2>{});
         add_state(std::integral_constant<int, 3>{});
       }
+      if constexpr (FINE) {
+        const T* const from = static_cast<const T*>(role ? p.drests : p.rests) + ((bh * p.runs + run) * vblocks + vb) * kVBlock * DKP;
+#pragma unroll 1
+        for (int t = 0; t < ND; ++t) {
+          f32x4 more = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int u = 0; u < NU; ++u) {
+            T e[O::kE];
+#pragma unroll
+            for (int j = 0; j < O::kE; ++j) e[j] = from[(u * O::kStep + 16 * (j >> 2) + 4 * g + (j & 3)) * DKP + 16 * t + i];
+            u32x4 w;
+            __builtin_memcpy(&w, e, 16);
+            more = mma<DT>(own[u], w, more);
+          }
+#pragma unroll
+          for (int k = 0; k < ND; ++k) tmp[k] += k == t ? more * (1.0f / kRestUp) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+      }
       if (!last_block) return;
       // dP and M
       const float hi_r = D.hi[16 * blk + i], lo_r = D.lo[16 * blk + i];
@@ -323,7 +343,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         }
         sum += (x[0] + x[1]) + (x[2] + x[3]);
       }
-      const bool fine = !O::kWide && p.fine;
+      constexpr bool fine = FINE;
       u32x4 dp[kRun / O::kStep], rest[kRun / O::kStep];
 #pragma unroll
       for (int u = 0; u < kRun / O::kStep; ++u) score_operand<DT>(acc + u * O::kTiles, fine, dp[u], rest[u]);
@@ -440,18 +460,25 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
   }
 }
 
-template <int DT, int DKP>
-static void launch_grad_t(const Grad& p, hipStream_t s) {
+template <int DT, int DKP, bool FINE>
+static void launch_grad_f(const Grad& p, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(p.batch * p.runs * p.groups * p.sets));
   constexpr bool kDirect = DT != MM_F32;
   if constexpr (kDirect) {
     if (p.vec) {
-      if (p.vblocks == 1) hipLaunchKernelGGL((grad_kernel<DT, DKP, kDirect, true>), grid, dim3(512), 0, s, p);
-      else hipLaunchKernelGGL((grad_kernel<DT, DKP, kDirect, false>), grid, dim3(512), 0, s, p);
+      if (p.vblocks == 1) hipLaunchKernelGGL((grad_kernel<DT, DKP, kDirect, true, FINE>), grid, dim3(512), 0, s, p);
+      else hipLaunchKernelGGL((grad_kernel<DT, DKP, kDirect, false, FINE>), grid, dim3(512), 0, s, p);
       return;
     }
   }
-  hipLaunchKernelGGL((grad_kernel<DT, DKP, false, false>), grid, dim3(512), 0, s, p);
+  hipLaunchKernelGGL((grad_kernel<DT, DKP, false, false, FINE>), grid, dim3(512), 0, s, p);
+}
+template <int DT, int DKP>
+static void launch_grad_t(const Grad& p, hipStream_t s) {
+  if constexpr (DT != MM_F32) {
+    if (p.rests) return launch_grad_f<DT, DKP, true>(p, s);
+  }
+  launch_grad_f<DT, DKP, false>(p, s);
 }
 template <int DT>
 static void launch_grad_d(const Grad& p, hipStream_t s) {

@@ -193,6 +193,18 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
         T* const to = s_s + TK::at(16 * wave, 16 * t, i, 4 * g);
         if constexpr (O::kWide) *reinterpret_cast<f32x4*>(to) = x;
         else *reinterpret_cast<u32x2*>(to) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+        if constexpr (!O::kWide) {
+          // (a run's tokens share the roundings of its states: few of them get the rests, too)
+          if (p.state_rests) {
+            float a[4];
+            unpack2<DT>(pack2<DT>(x[0], x[1]), a[0], a[1]);
+            unpack2<DT>(pack2<DT>(x[2], x[3]), a[2], a[3]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a[r] = (x[r] - a[r]) * kRestUp;
+            *reinterpret_cast<u32x2*>(static_cast<T*>(p.state_rests) + ((bh * p.runs + run) * p.vblocks + vb) * kVBlock * DKP +
+                                      (16 * wave + i) * DKP + 16 * t + 4 * g) = u32x2{pack2<DT>(a[0], a[1]), pack2<DT>(a[2], a[3])};
+          }
+        }
       }
     }
     __syncthreads();
@@ -254,6 +266,20 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
             unpack2<DT>(saved2[t][1], x[2], x[3]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) dot += x[r] * S[t][r];
+          }
+          if (p.rests_with) {
+            const T* const rest = static_cast<const T*>(p.rests_with) + block * kVBlock * DKP + (16 * wave + i) * DKP + 4 * g;
+            float more = 0.0f;
+#pragma unroll
+            for (int t = 0; t < ND; ++t) {
+              const u32x2 w = *reinterpret_cast<const u32x2*>(rest + 16 * t);
+              float x[4];
+              unpack2<DT>(w[0], x[0], x[1]);
+              unpack2<DT>(w[1], x[2], x[3]);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) more += x[r] * S[t][r];
+            }
+            dot += more * (1.0f / kRestUp);
           }
         }
       }

@@ -163,9 +163,11 @@ def test_step_validation():
 
 def test_sizes():
     lib = _lib.load()
-    # 2 runs of 4 heads, one value block each of 64 x 64 states; float16 keeps a power of two beside each
+    # 2 runs of 4 heads, one value block each of 64 x 64 states; float16 keeps a power of two beside each, and 16-bit calls of
+    # few tokens what the states' roundings leave
     assert lib.mm_decay_attention_states_size(2, 100, 4, 64, 64, _lib.F32) == 2 * 4 * 2 * 64 * 64 * 4
-    assert lib.mm_decay_attention_states_size(2, 100, 4, 65, 65, _lib.F16) == 2 * 4 * 2 * 2 * (64 * 128 * 2 + 4)
+    assert lib.mm_decay_attention_states_size(2, 100, 4, 65, 65, _lib.F16) == 2 * 4 * 2 * 2 * (2 * 64 * 128 * 2) + 256
+    assert lib.mm_decay_attention_states_size(2, 6400, 4, 64, 64, _lib.BF16) == 2 * 4 * 100 * 64 * 64 * 2
     assert lib.mm_decay_attention_states_size(0, 100, 4, 64, 64, 0) == 0
     assert lib.mm_decay_attention_states_size(2, 100, 4, 129, 64, 0) == 0
     assert lib.mm_decay_attention_workspace_size(64, 100, 4, 4, 64, 64, 0, 0) == 0  # enough heads: no segments
