@@ -259,14 +259,14 @@ def hooked() -> bool:
     return _hooks is None or _hooks(False) is not None
 
 
-def saved(t, dtype, shape, device, rows=False):
-    """A backward pass's saved tensor after hooks, which can hand back anything: another type, shape or device than was
-    saved raises, since a kernel would read past its end.  Contiguous; with ``rows``, for an activation, with unit channel
-    stride."""
+def saved(t, dtype, shape, device, rows=False, strided=False):
+    """A backward pass's saved tensor after hooks, which can hand back anything, or after its ``.data`` was replaced:
+    another type, shape or device than was saved raises, since a kernel would read past its end.  Contiguous; with
+    ``rows``, for an activation, with unit channel stride; with ``strided`` as it lies."""
     if t is None or t.dtype != dtype or t.shape != shape or t.get_device() != device.index:
         raise RuntimeError(f"a saved tensor came back as {None if t is None else (t.dtype, tuple(t.shape), str(t.device))}, "
                            f"not as {(dtype, tuple(shape), str(device))}")
-    return t if rows and (t.stride(-1) == 1 or shape[-1] == 1) else t.contiguous()
+    return t if strided or rows and (t.stride(-1) == 1 or shape[-1] == 1) else t.contiguous()
 
 
 _is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)

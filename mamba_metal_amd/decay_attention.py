@@ -59,9 +59,8 @@ def _states_bytes(q, v):
 
 
 def _forward(dev, q, k, v, g, h0, lengths, scale, want_state, train):
-    """y, the final state (or None), for training the states before each run of tokens, and the inputs' parameters."""
-    inputs = _params(q, k, v, g, lengths, scale)
-    p = _lib.DecayAttentionParams.from_buffer_copy(inputs)
+    """y, the final state (or None) and, for training, the states before each run of tokens."""
+    p = _params(q, k, v, g, lengths, scale)
     y = _empty_like(v)
     p.y = y.data_ptr()
     state = states = None
@@ -74,15 +73,15 @@ def _forward(dev, q, k, v, g, h0, lengths, scale, want_state, train):
         states = torch.empty(_states_bytes(q, v), dtype=torch.uint8, device=dev)
         p.run_states = states.data_ptr() or None
     _call("mm_decay_attention_fwd", p, 0, dev)
-    return y, state, states, inputs
+    return y, state, states
 
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, dev, q, k, v, g, h0, lengths, scale, want_state):
-        y, state, states, ctx.inputs = _forward(dev, q, k, v, g, h0, lengths, scale, want_state, True)
+        y, state, states = _forward(dev, q, k, v, g, h0, lengths, scale, want_state, True)
         ctx.meta = (dev, q.dtype, q.shape, v.shape, g.dtype, g.shape, scale,
-                    _lib.hooked() and (None if lengths is None else lengths.dtype,))
+                    (None if lengths is None else lengths.dtype,))
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, v, g, lengths, states)
         return (y, state) if want_state else y
@@ -92,13 +91,11 @@ class _DecayAttention(torch.autograd.Function):
     def backward(ctx, dy, dstate=None):
         if dy is None and dstate is None:
             return (None,) * 9
-        dev, dtype, qk_shape, v_shape, g_dtype, g_shape, scale, hooked = ctx.meta
-        saved = ctx.saved_tensors
-        if hooked:
-            saved = _checked(saved, dev, dtype, qk_shape, v_shape, g_dtype, g_shape, *hooked)
-        q, k, v, g, lengths, states = saved
-        # (without hooks the saved tensors are the forward pass's; each backward pass has parameters of its own)
-        p = _params(q, k, v, g, lengths, scale) if hooked else _lib.DecayAttentionParams.from_buffer_copy(ctx.inputs)
+        dev, dtype, qk_shape, v_shape, g_dtype, g_shape, scale, lengths_dtype = ctx.meta
+        # (A leaf's memory, type and size may be others than in the forward pass: its data replaced, its storage freed and
+        # allocated again.)
+        q, k, v, g, lengths, states = _checked(ctx.saved_tensors, dev, dtype, qk_shape, v_shape, g_dtype, g_shape, *lengths_dtype)
+        p = _params(q, k, v, g, lengths, scale)
         p.run_states = states.data_ptr() or None
         if dy is None:  # only the final state was used
             dy = torch.zeros((1, 1, 1, v_shape[3]), dtype=dtype, device=dev).expand(v_shape)
@@ -125,13 +122,14 @@ class _DecayAttention(torch.autograd.Function):
 
 
 def _checked(saved, dev, dtype, qk_shape, v_shape, g_dtype, g_shape, lengths_dtype):
-    """The saved tensors, where hooks may have changed them."""
+    """The saved tensors, which hooks or a new ``.data`` may have changed."""
     q, k, v, g, lengths, states = saved
     if lengths_dtype is not None:
         lengths = _lib.saved(lengths, lengths_dtype, (v_shape[0],), dev)
     q, k = (_lib.saved(t, dtype, qk_shape, dev, rows=True) for t in (q, k))
     v = _lib.saved(v, dtype, v_shape, dev, rows=True)
-    return q, k, v, _lib.saved(g, g_dtype, g_shape, dev), lengths, _lib.saved(states, torch.uint8, (_states_bytes(q, v),), dev)
+    g = _lib.saved(g, g_dtype, g_shape, dev, strided=True)
+    return q, k, v, g, lengths, _lib.saved(states, torch.uint8, (_states_bytes(q, v),), dev)
 
 
 def _check(q, k, v, g, lead, names):
