@@ -126,7 +126,7 @@ def _conv1d_act8(x, weight, bias, apply_silu):
 
 
 def _checked(saved, dev, dtype, shape, w_dtype, w_shape, has_bias):
-    """The saved tensors, where hooks may have changed them."""
+    """The saved tensors, which hooks or a new ``.data`` may have changed."""
     (b, n, d), (weight, bias, *kept) = shape, saved
     if has_bias:
         bias = _lib.saved(bias, w_dtype, (d,), dev)
@@ -135,14 +135,14 @@ def _checked(saved, dev, dtype, shape, w_dtype, w_shape, has_bias):
     else:
         nblk = -(-n // BLOCK)
         kept = (_lib.saved(kept[0], torch.int8, (b, nblk, d, BLOCK), dev), _lib.saved(kept[1], torch.uint8, (b, nblk, d), dev))
-    return _lib.saved(weight, w_dtype, w_shape, dev), bias, *kept
+    return _lib.saved(weight, w_dtype, w_shape, dev, strided=True), bias, *kept
 
 
 class _CausalConv1d(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, apply_silu, checkpoint):
         ctx.meta = (x.device, x.dtype, x.shape, apply_silu,
-                    _lib.hooked() and (weight.dtype, weight.shape, bias is not None))
+                    (weight.dtype, weight.shape, bias is not None))
         if checkpoint == "int8":
             out, packed = _conv1d_act8(x, weight, bias, apply_silu)
             ctx.save_for_backward(weight, bias, packed.codes, packed.exps)
@@ -154,11 +154,8 @@ class _CausalConv1d(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        dev, dtype, shape, apply_silu, hooked = ctx.meta
-        saved = ctx.saved_tensors
-        if hooked:
-            saved = _checked(saved, dev, dtype, shape, *hooked)
-        weight, bias, *kept = saved
+        dev, dtype, shape, apply_silu, params = ctx.meta
+        weight, bias, *kept = _checked(ctx.saved_tensors, dev, dtype, shape, *params)
         x, packed = (kept[0], None) if len(kept) == 1 else (None, Act8(*kept, shape, dtype))
         if dout.dtype != dtype or (dout.stride(-1) != 1 and shape[2] > 1):
             dout = dout.to(dtype).contiguous()

@@ -64,18 +64,17 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, dev, x, weight, targets, ignore_index, reduction):
         loss, lse = _forward(dev, x, weight, targets, ignore_index, reduction, True)
-        ctx.meta = (dev, x.dtype, x.shape, weight.shape, ignore_index, reduction, _lib.hooked() and (targets.dtype, targets.shape))
+        ctx.meta = (dev, x.dtype, x.shape, weight.shape, ignore_index, reduction, (targets.dtype, targets.shape))
         ctx.save_for_backward(x, weight, targets, lse)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        dev, dtype, x_shape, w_shape, ignore_index, reduction, hooked = ctx.meta
-        x, weight, targets, lse = ctx.saved_tensors
-        if hooked:
-            x, weight = (_lib.saved(t, dtype, s, dev, rows=True) for t, s in ((x, x_shape), (weight, w_shape)))
-            targets, lse = _lib.saved(targets, *hooked, dev), _lib.saved(lse, torch.float32, x_shape[:1], dev)
+        dev, dtype, x_shape, w_shape, ignore_index, reduction, kind = ctx.meta
+        x, weight, targets, lse = ctx.saved_tensors  # (which hooks or a new .data may have changed)
+        x, weight = (_lib.saved(t, dtype, s, dev, rows=True) for t, s in ((x, x_shape), (weight, w_shape)))
+        targets, lse = _lib.saved(targets, *kind, dev), _lib.saved(lse, torch.float32, x_shape[:1], dev)
         p = _params(x, weight, targets, ignore_index, reduction)
         p.lse = lse.data_ptr()
         dloss = dloss.float().reshape(-1)

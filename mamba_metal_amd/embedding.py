@@ -29,17 +29,15 @@ def _forward(dev, ids, weight, scale):
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, dev, ids, weight, scale, padding_idx):
-        ctx.meta = (dev, weight.dtype, weight.shape, scale, padding_idx, _lib.hooked() and (ids.dtype, ids.shape))
+        ctx.meta = (dev, weight.dtype, weight.shape, scale, padding_idx, (ids.dtype, ids.shape))
         ctx.save_for_backward(ids)
         return _forward(dev, ids, weight, scale)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        dev, dtype, (vocab, dim), scale, padding_idx, hooked = ctx.meta
-        ids, = ctx.saved_tensors
-        if hooked:
-            ids = _lib.saved(ids, *hooked, dev)
+        dev, dtype, (vocab, dim), scale, padding_idx, kind = ctx.meta
+        ids = _lib.saved(*ctx.saved_tensors, *kind, dev)  # (which hooks or a new .data may have changed)
         dy = (dy if dy.dtype == dtype else dy.to(dtype)).reshape(-1, dim)
         if dy.stride(1) != 1 and dim > 1:
             dy = dy.contiguous()

@@ -122,7 +122,7 @@ def _backward(dev, inputs, codes, exps, A, lengths, blocks, dtype, shape, gated,
 
 
 def _checked(saved, dev, dtype, shape, gated, lengths_dtype):
-    """The saved tensors, where hooks may have changed them."""
+    """The saved tensors, which hooks or a new ``.data`` may have changed."""
     (b, n, d), (A, lengths, blocks, *kept) = shape, saved
     nblk, k = -(-n // BLOCK), 4 if gated else 3
     if lengths_dtype is not None:
@@ -140,7 +140,7 @@ class _GatedScan(torch.autograd.Function):
     def forward(ctx, dev, x, a_gate, x_gate, A, z, h0, lengths, want_state, checkpoint):
         y, state, blocks, codes, exps = _forward(dev, x, a_gate, x_gate, A, z, h0, lengths, want_state, True, checkpoint)
         ctx.meta = (dev, x.dtype, x.shape, z is not None,
-                    _lib.hooked() and (None if lengths is None else lengths.dtype,))
+                    (None if lengths is None else lengths.dtype,))
         ctx.set_materialize_grads(False)
         if codes is not None:
             ctx.save_for_backward(A, lengths, blocks, codes, exps)
@@ -153,11 +153,8 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dy, dstate=None):
         if dy is None and dstate is None:
             return (None,) * 10
-        dev, dtype, shape, gated, hooked = ctx.meta
-        saved = ctx.saved_tensors
-        if hooked:
-            saved = _checked(saved, dev, dtype, shape, gated, *hooked)
-        A, lengths, blocks, *kept = saved
+        dev, dtype, shape, gated, lengths_dtype = ctx.meta
+        A, lengths, blocks, *kept = _checked(ctx.saved_tensors, dev, dtype, shape, gated, *lengths_dtype)
         inputs, codes, exps = (None, *kept) if len(kept) == 2 else (kept, None, None)
         grads = _backward(dev, inputs, codes, exps, A, lengths, blocks, dtype, shape, gated, dy, dstate,
                           ctx.needs_input_grad[6])
