@@ -246,7 +246,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         for (int ot = 0; ot < 4; ++ot) acc[ot] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < ND; ++t) tmp[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        factor = 1.0f;
+        factor = DT == MM_F16 ? 0.0f : 1.0f;
       }
       const T* const own_t = cur + 2 * kState + role * kRows;
       const T* const other_t = cur + 2 * kState + (1 - role) * kRows;
@@ -273,12 +273,26 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
 #pragma unroll
         for (int ot = 0; ot < 4; ++ot)
           if (role ? ot >= blk : ot <= blk) acc[ot] = mma<DT>(TV::row_acc(other_t, 16 * ot, u * O::kStep, lane), own[u], acc[ot]);
+      // fp16: the sum over blocks stands in the largest of their powers of two, to which the other blocks' parts come down.  (Up to
+      // a smaller one, of a block whose states have decayed to nearly nothing, finite sums would overflow.)
+      constexpr bool kJoin = DT == MM_F16 && !ONE;
+      float part = 1.0f;
       if constexpr (DT == MM_F16) {
+        if constexpr (kJoin) {
+          const float top = fmaxf(factor, factor_here), down = factor / top;
 #pragma unroll
-        for (int t = 0; t < ND; ++t) tmp[t] *= factor / factor_here;
-        factor = factor_here;
+          for (int t = 0; t < ND; ++t) tmp[t] *= down;
+          part = factor_here / top;
+          factor = top;
+        } else {
+          factor = factor_here;
+        }
         factor_here = factor_next;
       }
+      auto add_block = [&](u32x4 a, u32x4 o, f32x4& to) __attribute__((always_inline)) {
+        if constexpr (kJoin) to += mma<DT>(a, o, f32x4{0.0f, 0.0f, 0.0f, 0.0f}) * part;
+        else to = mma<DT>(a, o, to);
+      };
       auto add_state = [&](auto first) __attribute__((always_inline)) {
         constexpr int u = decltype(first)::value;
         if constexpr (DIRECT) {
@@ -287,10 +301,10 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
           columns_at<TK>(state, lane, at);
           columns<TK, u * 32>(at, o);
 #pragma unroll
-          for (int t = 0; t < ND; ++t) tmp[t] = mma<DT>(own[u], o[t], tmp[t]);
+          for (int t = 0; t < ND; ++t) add_block(own[u], o[t], tmp[t]);
         } else {
 #pragma unroll
-          for (int t = 0; t < ND; ++t) tmp[t] = mma<DT>(own[u], state_operand(u, t), tmp[t]);
+          for (int t = 0; t < ND; ++t) add_block(own[u], state_operand(u, t), tmp[t]);
         }
       };
       add_state(std::integral_constant<int, 0>{});
@@ -314,7 +328,7 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
             more = mma<DT>(own[u], w, more);
           }
 #pragma unroll
-          for (int k = 0; k < ND; ++k) tmp[k] += k == t ? more * (1.0f / kRestUp) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          for (int k = 0; k < ND; ++k) tmp[k] += k == t ? more * (part / kRestUp) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
       }
       if (!last_block) return;

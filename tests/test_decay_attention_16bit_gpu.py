@@ -1,0 +1,74 @@
+"""decay_attention in 16 bits: both of its variants (calls of up to 32768 tokens, batch * seqlen * heads, and larger ones),
+blocks of value channels whose states lie far apart, and float16's small numbers.
+
+Tolerances as derived in test_decay_attention_gpu.py, and one addend: below 2^-14 float16's numbers are 2^-24 apart, so that
+an output rounded once is off by up to 2^-25 however small it is."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import decay_ref
+from test_decay_attention_gpu import F16, F32, RUN, half_step, inputs, near, run
+
+pytestmark = pytest.mark.gpu
+# batch and heads a group at 200 tokens: 400 (batch * seqlen * heads), and 38400
+SIZES = [(2, 1), (3, 64)]
+
+
+def check(s, scale, outs, grads):
+    """Outputs and gradients (of log decays in float32, or in the inputs' type) against the recurrence."""
+    dt = s["q"].dtype
+    u, n = half_step(dt), s["q"].shape[1]
+    f = (400 + 2 * (-(-n // RUN))) * 2.0 ** -24
+    least = 2.0 ** -25 if dt == F16 else 0.0
+    args = (s["q"], s["k"], s["v"], s["g"])
+    mags = tuple(t.abs().double() for t in args[:3]) + (s["g"],)
+    ah0 = None if s["h0"] is None else s["h0"].abs()
+    y, states = decay_ref.forward(*args, scale, s["h0"], s["lengths"])
+    ay, astates = decay_ref.forward(*mags, scale, ah0, s["lengths"])
+    near(outs[0], y, u * y.abs() + (u + f) * ay + least, "y")
+    if len(outs) > 1:
+        near(outs[1], states[:, -1], f * astates[:, -1], "state")
+    del states, astates
+    dstate = s["dstate"] if len(outs) > 1 else None
+    want = decay_ref.backward(*args, s["dy"], scale, s["h0"], s["lengths"], dstate)
+    ab = decay_ref.backward(*mags, s["dy"].abs(), scale, ah0, s["lengths"], None if dstate is None else dstate.abs())
+    for k, (name, got) in enumerate(zip(("dq", "dk", "dv"), grads)):
+        near(got, want[k], u * want[k].abs() + (u + f) * ab[k] + least, name)
+    per = s["v"].shape[2] // s["q"].shape[2]
+    crossing = (s["q"].abs().double() * ab[0]).sum(3) + (s["k"].abs().double() * ab[1]).sum(3)
+    whole = torch.zeros_like(crossing)
+    for t in range(0, n, RUN):
+        whole[:, t:t + RUN] = crossing[:, t:t + RUN].sum(1, keepdim=True)
+    whole = whole.repeat_interleave(per, 2)
+    tol = half_step(s["g"].dtype) * want[3].abs() + (u + f) * ab[3] + f * whole + (least if s["g"].dtype == F16 else 0.0)
+    if s["g"].dim() == 1:
+        near(grads[3], want[3].sum((0, 1)), (tol + 2.0 ** -22 * want[3].abs()).sum((0, 1)), "dg")
+    else:
+        near(grads[3], want[3], tol, "dg")
+    if s["h0"] is not None:
+        near(grads[4], want[4], f * ab[4], "dh0")
+
+
+@pytest.mark.parametrize("b,per", SIZES)
+@pytest.mark.parametrize("what", ["dq", "dk"])
+@pytest.mark.parametrize("odd", [False, True])
+@pytest.mark.parametrize("far", [0, 1])
+def test_blocks_far_apart(dev, b, per, what, odd, far):
+    """Two blocks of value channels, of which one's states (their gradients) have decayed to 1e-34 where the other's are near
+    1, with what they are multiplied with in the thousands."""
+    n, dv = 200, 127 if odd else 128
+    s = inputs(dev, F16, b, n, 1, per, 16, dv, g_dtype=F32)
+    s["g"].fill_(-1.2)
+    block = slice(64 * far, 64 * far + 64)
+    if what == "dq":  # the states before tokens 128 on
+        s["v"][:, 64:, :, block] = 0
+        s["dy"] = s["dy"] * 1024
+    else:             # the gradients of the states behind tokens 0 to 63
+        s["dy"][:, :128, :, block] = 0
+        s["v"] = s["v"] * 4096  # (the largest true gradient, of 64 heads that share k: 33800)
+    outs, grads = run(s, 0.01, with_state=False)
+    assert all(bool(t.isfinite().all()) for t in (*outs, *grads))
+    check(s, 0.01, outs, grads)
