@@ -84,24 +84,25 @@ __device__ __forceinline__ u32x4 from_acc(const f32x4* t) {
 
 // 16-bit operands of a product whose result is a state in fp32: the value as a sum of TERMS of them.  bf16: three are
 // fp32's own 24 bits.  fp16: two hold 22 bits, the second one 2^11 times too large (and summed by itself), since the rest of a
-// value below 1/8 would be subnormal, which the matrix cores take as 0; so would be values below 2^-14, which therefore
-// are all rest.
+// value below 1/8 would be subnormal.  The matrix cores take subnormals as they are, but those hold fewer bits: a value below
+// 2^-14 is off by up to 2^-36.
 constexpr float kRestUp = 2048.0f;
 template <int DT, int TERMS>
 __device__ __forceinline__ void split_operand(const float (&x)[8], u32x4 (&out)[TERMS]) {
   float rest[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) rest[j] = x[j];
+  for (int j = 0; j < 8; ++j) {
+    rest[j] = x[j];
+    // (x, a product, as it is in fp32: its first term would else be one rounding of the exact product in the operand and the
+    // rounding of an fp32 one where it is subtracted, next to a tie two numbers that are a step apart)
+    if (DT == MM_F16) asm("" : "+v"(rest[j]));
+  }
 #pragma unroll
   for (int n = 0; n < TERMS; ++n)
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-      float c[2] = {rest[j], rest[j + 1]};
-      if (DT == MM_F16) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) c[e] = n == 0 ? (fabsf(c[e]) < 6.103515625e-05f ? 0.0f : c[e]) : c[e] * kRestUp;
-      }
-      const uint32_t w = pack2<DT>(c[0], c[1]);
+      const float up = DT == MM_F16 && n == 1 ? kRestUp : 1.0f;
+      const uint32_t w = pack2<DT>(rest[j] * up, rest[j + 1] * up);
       out[n][j / 2] = w;
       if (n + 1 < TERMS) {
         float a, b;

@@ -72,3 +72,47 @@ def test_blocks_far_apart(dev, b, per, what, odd, far):
     outs, grads = run(s, 0.01, with_state=False)
     assert all(bool(t.isfinite().all()) for t in (*outs, *grads))
     check(s, 0.01, outs, grads)
+
+
+def added(k, g, lengths, mirrored=False):
+    """What a state would be if each token added |k|, but decayed by whole runs behind (mirrored: before) its own alone."""
+    b, n, heads = g.shape
+    live = torch.arange(n, device=g.device)[None] < lengths[:, None]
+    k = (k.abs().double() * live[..., None, None]).repeat_interleave(heads // k.shape[2], 2)
+    g = g.double() * live[..., None]
+    total = k.new_zeros((b, heads, k.shape[3]))
+    starts = range(0, n, RUN)
+    for t in reversed(starts) if mirrored else starts:
+        total = torch.exp(g[:, t:t + RUN].sum(1))[..., None] * total + k[:, t:t + RUN].sum(1)
+    return total[..., None]
+
+
+@pytest.mark.parametrize("b,per", SIZES)
+@pytest.mark.parametrize("down", [12, 17, 20])
+def test_states_of_small_numbers(dev, b, per, down):
+    """float16's values and gradients near 2^-down, below 2^-14 subnormal numbers: the state and its gradient are float32 all the
+    same.  A run's values are weighted by their decay to its end, and a sum of two float16 numbers, the second times 2^11, stands
+    for each: off by 2^-23 of it (among f's), or by 2^-36 where it is small, which then no decay within the run makes less."""
+    s = inputs(dev, F16, b, 200, 1, per, 32, 48, h0=True, ragged=True, g_dtype=F32)
+    for k in ("v", "dy"):
+        s[k] = s[k] * 2.0 ** -down
+    s["h0"], s["dstate"] = s["h0"] * 2.0 ** -down, s["dstate"] * 2.0 ** -down
+    outs, grads = run(s, 0.6)
+    f = (400 + 2 * 4) * 2.0 ** -24
+    mags = [s[k].abs() for k in ("q", "k", "v")] + [s["g"]]
+    _, states = decay_ref.forward(s["q"], s["k"], s["v"], s["g"], 0.6, s["h0"], s["lengths"])
+    _, a = decay_ref.forward(*mags, 0.6, s["h0"].abs(), s["lengths"])
+    near(outs[1], states[:, -1], f * a[:, -1] + 2.0 ** -36 * added(s["k"], s["g"], s["lengths"]), "state")
+    want = decay_ref.backward(s["q"], s["k"], s["v"], s["g"], s["dy"], 0.6, s["h0"], s["lengths"], s["dstate"])[4]
+    a = decay_ref.backward(*mags, s["dy"].abs(), 0.6, s["h0"].abs(), s["lengths"], s["dstate"].abs())[4]
+    near(grads[4], want, f * a + 2.0 ** -36 * added(s["q"], s["g"], s["lengths"], mirrored=True), "dh0")
+
+
+def test_states_where_products_round_to_ties(dev):
+    """A weighted value whose product is next to the middle of two float16 numbers: its two terms belong together.  (So many
+    tokens that some are; each of the state's elements is near its sum.)"""
+    s = inputs(dev, F16, 4, 250, 1, 64, 16, 64, g_dtype=F32, seed=2)
+    outs, _ = run(s, 1.0)
+    _, states = decay_ref.forward(s["q"], s["k"], s["v"], s["g"])
+    _, a = decay_ref.forward(s["q"].abs(), s["k"].abs(), s["v"].abs(), s["g"])
+    near(outs[1], states[:, -1], (400 + 2 * 4) * 2.0 ** -24 * a[:, -1], "state")
