@@ -357,6 +357,13 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         }
         sum += (x[0] + x[1]) + (x[2] + x[3]);
       }
+      constexpr bool kRange = DT == MM_F16;
+      float up = 1.0f, down = 1.0f;
+      if constexpr (kRange) {
+        score_range(largest(acc), up, down);
+#pragma unroll
+        for (int ot = 0; ot < 4; ++ot) acc[ot] *= up;
+      }
       constexpr bool fine = FINE;
       u32x4 dp[kRun / O::kStep], rest[kRun / O::kStep];
 #pragma unroll
@@ -364,10 +371,12 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       // the states' part, scaled row by row
       const f32x4 w = *reinterpret_cast<const f32x4*>((role ? D.onward : D.into) + 16 * blk + 4 * g) * ((role ? 1.0f : p.scale) * factor);
       f32x4 inter = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (!kRange) {
 #pragma unroll
-      for (int t = 0; t < ND; ++t)
+        for (int t = 0; t < ND; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) out[t][r] = __builtin_fmaf(tmp[t][r], w[r], out[t][r]);
+          for (int r = 0; r < 4; ++r) out[t][r] = __builtin_fmaf(tmp[t][r], w[r], out[t][r]);
+      }
       if (p.dg) {
 #pragma unroll
         for (int t = 0; t < ND; ++t) {
@@ -384,6 +393,21 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         }
         inter *= w;
       }
+      // fp16: the head's gradients gather in the states' part, in the units of each row's scores
+      f32x4 back;
+      if constexpr (kRange) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          back[r] = __shfl(down, 4 * g + r, 64);
+          const float to = w[r] * __uint_as_float(0x7f000000u - __float_as_uint(back[r]));  // (a power of two's inverse)
+#pragma unroll
+          for (int t = 0; t < ND; ++t) tmp[t][r] *= to;
+        }
+      }
+      auto& gather = [&]() -> auto& {
+        if constexpr (kRange) return tmp;
+        else return out;
+      }();
       auto add_rows = [&](auto first) __attribute__((always_inline)) {
         constexpr int u = decltype(first)::value;
         if (role ? (u + 1) * O::kStep <= 16 * blk : u * O::kStep > 16 * blk + 15) return;
@@ -393,17 +417,17 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
           columns_at<TK>(s_other, lane, at);
           columns<TK, u * 32>(at, o);
 #pragma unroll
-          for (int t = 0; t < ND; ++t) out[t] = mma<DT>(dp[u], o[t], out[t]);
+          for (int t = 0; t < ND; ++t) gather[t] = mma<DT>(dp[u], o[t], gather[t]);
           if (fine) {
 #pragma unroll
-            for (int t = 0; t < ND; ++t) out[t] = mma_rest<DT>(rest[u], o[t], out[t]);
+            for (int t = 0; t < ND; ++t) gather[t] = mma_rest<DT>(rest[u], o[t], gather[t]);
           }
         } else {
 #pragma unroll
-          for (int t = 0; t < ND; ++t) out[t] = mma<DT>(dp[u], TK::column(s_other, u * O::kStep, 16 * t, lane), out[t]);
+          for (int t = 0; t < ND; ++t) gather[t] = mma<DT>(dp[u], TK::column(s_other, u * O::kStep, 16 * t, lane), gather[t]);
           if (fine) {
 #pragma unroll
-            for (int t = 0; t < ND; ++t) out[t] = mma_rest<DT>(rest[u], TK::column(s_other, u * O::kStep, 16 * t, lane), out[t]);
+            for (int t = 0; t < ND; ++t) gather[t] = mma_rest<DT>(rest[u], TK::column(s_other, u * O::kStep, 16 * t, lane), gather[t]);
           }
         }
       };
@@ -412,6 +436,12 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       if constexpr (NU == 4) {
         add_rows(std::integral_constant<int, 2>{});
         add_rows(std::integral_constant<int, 3>{});
+      }
+      if constexpr (kRange) {
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) out[t][r] = __builtin_fmaf(tmp[t][r], back[r], out[t][r]);
       }
       if (p.dg) {
         sum += lane_xor(sum, 16);

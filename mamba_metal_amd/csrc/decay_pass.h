@@ -308,6 +308,12 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
           acc[st][r] = st != wave || (REV ? 4 * g + r >= i : 4 * g + r <= i) ? x : 0.0f;
         }
       }
+      float up = 1.0f, down = 1.0f;  // fp16: what the token's outputs stand in until the end
+      if constexpr (DT == MM_F16) {
+        score_range(largest(acc), up, down);
+#pragma unroll
+        for (int st = 0; st < 4; ++st) acc[st] *= up;
+      }
       const bool fine = !O::kWide && p.fine;
       u32x4 po[NR], rest[NR];
 #pragma unroll
@@ -323,7 +329,8 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
         for (int vt = 0; vt < 4; ++vt) y[vt] = mma<DT>(TK::row(s_s, 16 * vt, u * O::kStep, lane), own[u], y[vt]);
       if (n + 1 < walk) fetch_q(rows_of(next));
       keep_state(2);
-      const float ws = (REV ? D.onward : D.into)[16 * wave + i] * ((REV ? 1.0f : p.scale) * factor);
+      float ws = (REV ? D.onward : D.into)[16 * wave + i] * ((REV ? 1.0f : p.scale) * factor);
+      if constexpr (DT == MM_F16) ws *= up;
 #pragma unroll
       for (int vt = 0; vt < 4; ++vt) y[vt] *= ws;
 #pragma unroll
@@ -335,6 +342,10 @@ __global__ __launch_bounds__(256, DT == MM_F32 ? (DKP == 128 && OUT ? 1 : 2) : V
 #pragma unroll
           for (int vt = 0; vt < 4; ++vt) y[vt] = mma_rest<DT>(TV::column(s_v, u * O::kStep, 16 * vt, lane), rest[u], y[vt]);
         }
+      }
+      if constexpr (DT == MM_F16) {
+#pragma unroll
+        for (int vt = 0; vt < 4; ++vt) y[vt] *= down;
       }
       const int left = static_cast<int>(p.seqlen - run * kRun < kRun ? p.seqlen - run * kRun : kRun), t = 16 * wave + i;
       if (t < left) {

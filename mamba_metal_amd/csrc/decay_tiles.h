@@ -129,6 +129,25 @@ __device__ __forceinline__ void score_operand(const f32x4* t, bool fine, u32x4& 
     }
   }
 }
+// fp16 has 5 exponent bits: a token's scores go through a power of two that puts the largest of them, m, at 2^13, and what
+// they are added to with them (2^40 at most, which leaves an output's other parts in fp32's range).  All of scores near 1e-5
+// would be subnormal, and off by 2^-8 of them and more.
+__device__ __forceinline__ void score_range(float m, float& up, float& down) {
+  const int e = static_cast<int>(__float_as_uint(m) >> 23) - 127, k = e > 53 ? -40 : e < -27 ? 40 : 13 - e;
+  const bool ok = m > 0.0f && e < 128;
+  up = ok ? __uint_as_float((127 + k) << 23) : 1.0f;
+  down = ok ? __uint_as_float((127 - k) << 23) : 1.0f;
+}
+template <int N>
+__device__ __forceinline__ float largest(const f32x4 (&t)[N]) {  // of a column of accumulator tiles, in its four lanes
+  float m = 0.0f;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(t[n][r]));
+  m = fmaxf(m, lane_xor(m, 16));
+  return fmaxf(m, lane_xor(m, 32));
+}
 // The product with the rest.
 template <int DT>
 __device__ __forceinline__ f32x4 mma_rest(u32x4 a, u32x4 b, f32x4 c) {

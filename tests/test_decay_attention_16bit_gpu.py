@@ -116,3 +116,16 @@ def test_states_where_products_round_to_ties(dev):
     _, states = decay_ref.forward(s["q"], s["k"], s["v"], s["g"])
     _, a = decay_ref.forward(s["q"].abs(), s["k"].abs(), s["v"].abs(), s["g"])
     near(outs[1], states[:, -1], (400 + 2 * 4) * 2.0 ** -24 * a[:, -1], "state")
+
+
+@pytest.mark.parametrize("b,per", SIZES)
+@pytest.mark.parametrize("dk,dv", [(32, 48), (100, 72)])
+@pytest.mark.parametrize("q,k,v,dy", [(0, 0, 0, -14), (0, 0, -14, 0), (-10, -9, 9, 5), (-14, 0, 14, -5), (9, 8, -12, -12), (-14, -14, 8, 14)])
+def test_scores_of_any_size(dev, b, per, dk, dv, q, k, v, dy):
+    """float16's scores, and dy.v of the gradients, far below 2^-14 and far above 65504, where the outputs are neither."""
+    s = inputs(dev, F16, b, 200, 1, per, dk, dv, ragged=True, g_dtype=F32)
+    for name, up in (("q", q), ("k", k), ("v", v), ("dy", dy)):
+        s[name] = (s[name].clamp(-2, 2) * 2.0 ** up).contiguous()
+    outs, grads = run(s, 0.125, with_state=False)
+    assert all(bool(t.isfinite().all()) for t in (*outs, *grads))
+    check(s, 0.125, outs, grads)
