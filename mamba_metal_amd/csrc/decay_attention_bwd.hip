@@ -394,12 +394,10 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
         inter *= w;
       }
       // fp16: the head's gradients gather in the states' part, in the units of each row's scores
-      f32x4 back;
       if constexpr (kRange) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          back[r] = __shfl(down, 4 * g + r, 64);
-          const float to = w[r] * __uint_as_float(0x7f000000u - __float_as_uint(back[r]));  // (a power of two's inverse)
+          const float to = w[r] * __shfl(up, 4 * g + r, 64);
 #pragma unroll
           for (int t = 0; t < ND; ++t) tmp[t][r] *= to;
         }
@@ -439,9 +437,11 @@ __global__ __launch_bounds__(512) void grad_kernel(const Grad p) {
       }
       if constexpr (kRange) {
 #pragma unroll
-        for (int t = 0; t < ND; ++t)
+        for (int r = 0; r < 4; ++r) {
+          const float back = __shfl(down, 4 * g + r, 64);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) out[t][r] = __builtin_fmaf(tmp[t][r], back[r], out[t][r]);
+          for (int t = 0; t < ND; ++t) out[t][r] = __builtin_fmaf(tmp[t][r], back, out[t][r]);
+        }
       }
       if (p.dg) {
         sum += lane_xor(sum, 16);

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import decay_ref
-from test_decay_attention_gpu import F16, F32, RUN, half_step, inputs, near, run
+from test_decay_attention_gpu import BF16, F16, F32, RUN, half_step, inputs, near, run
 
 pytestmark = pytest.mark.gpu
 # batch and heads a group at 200 tokens: 400 (batch * seqlen * heads), and 38400
@@ -129,3 +129,30 @@ def test_scores_of_any_size(dev, b, per, dk, dv, q, k, v, dy):
     outs, grads = run(s, 0.125, with_state=False)
     assert all(bool(t.isfinite().all()) for t in (*outs, *grads))
     check(s, 0.125, outs, grads)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("shape", [  # batch, seqlen, groups, heads a group, key_dim, value_dim: above 32768 tokens
+    (4, 300, 2, 16, 128, 64), (3, 350, 1, 32, 96, 96), (3, 350, 1, 32, 72, 130), (3, 351, 2, 16, 33, 65), (2, 130, 64, 2, 127, 32),
+    (5, 65, 103, 1, 128, 128), (1, 2100, 1, 16, 128, 24)])
+@pytest.mark.parametrize("fixed", [False, True])
+def test_large_calls(dev, dt, shape, fixed):
+    """The variant of ordinary sizes: wide keys, several blocks of value channels, rows off 16 bytes, shared and single heads."""
+    assert shape[0] * shape[1] * shape[2] * shape[3] > 32768
+    s = inputs(dev, dt, *shape, fixed=fixed, h0=True, ragged=True, g_dtype=F32 if fixed else None, seed=sum(shape))
+    outs, grads = run(s, 0.6)
+    check(s, 0.6, outs, grads)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("shape", [(1, 300, 1, 2, 64, 64), (2, 150, 1, 24, 128, 64), (1, 333, 2, 2, 65, 96)])
+def test_gradients_of_few_tokens_are_rounded_once(dev, dt, shape):
+    """Calls of few tokens: dq, dk and dlog_decay are as far from the truth as its rounding.  What else is rounded there, scores
+    and states, is to two terms, 2^-16 of a sum's magnitudes and less, which here are some 20 times the sum's root mean
+    square: with a rounding of 2^-9 times 0.58 at the root of the mean square, under 0.1 of it, and 1.005 times it together."""
+    s = inputs(dev, dt, *shape, h0=True, seed=sum(shape))
+    _, grads = run(s, 0.6)
+    want = decay_ref.backward(s["q"], s["k"], s["v"], s["g"], s["dy"], 0.6, s["h0"], None, s["dstate"])
+    for name, at in (("dq", 0), ("dk", 1), ("dg", 3)):
+        rounding = (want[at].to(dt).double() - want[at]).norm()
+        assert float((grads[at].double() - want[at]).norm() / rounding) < 1.05, name
