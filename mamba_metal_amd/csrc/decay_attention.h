@@ -3,6 +3,8 @@
 
 #include "mm_common.h"
 
+#include "decay_shape.h"
+
 namespace mm {
 namespace dattn {
 
@@ -53,10 +55,6 @@ struct Step {
   float scale;
 };
 
-// Whether the scores of 16-bit types take a second term (decay_tiles.h, score_operand).
-inline bool fine_scores(int64_t batch, int64_t seqlen, int64_t heads, int32_t dtype) {
-  return dtype != MM_F32 && batch * seqlen * heads <= 32768;
-}
 inline int padded_dk(int64_t dk) { return dk <= 64 ? 64 : 128; }
 
 void launch_pass_forward(const Pass& p, hipStream_t s);

@@ -11,6 +11,8 @@
 
 #include "mm_common.h"
 
+#include "decay_shape.h"
+
 namespace mm {
 namespace dattn {
 
@@ -20,10 +22,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-constexpr int kRun = 64;    // tokens a run
-constexpr int kVBlock = 64; // value channels a workgroup
-constexpr int kMaxDk = 128;
 
 template <int DT>
 struct Op {
