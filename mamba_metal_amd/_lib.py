@@ -18,6 +18,7 @@ from pathlib import Path
 
 import torch  # noqa: F401  (must be loaded before the HIP library; see module docstring)
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 LIB_NAME = "libmamba_mi355x.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
@@ -267,6 +268,13 @@ def saved(t, dtype, shape, device, rows=False, strided=False):
         raise RuntimeError(f"a saved tensor came back as {None if t is None else (t.dtype, tuple(t.shape), str(t.device))}, "
                            f"not as {(dtype, tuple(shape), str(device))}")
     return t if strided or rows and (t.stride(-1) == 1 or shape[-1] == 1) else t.contiguous()
+
+
+def wrote(t) -> None:
+    """Tells autograd that a call wrote the caller's tensor, so that a backward pass that saved it refuses it instead of
+    reading what it holds now.  (Inference tensors count no versions; None is skipped.)"""
+    if t is not None and not t.is_inference():
+        increment_version((t,))
 
 
 _is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)

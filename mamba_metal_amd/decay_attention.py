@@ -239,6 +239,7 @@ def decay_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, 
     _lib.refuse_transforms("decay_attention_step", state, q, k, v, log_decay)
     dev = _lib.require_cuda(state, q, k, v, log_decay, state_out, out)
     lib = _lib.load()
+    given = out
     if out is None:
         out = _empty_like(v)
     with _lib.on_device(dev):
@@ -249,4 +250,6 @@ def decay_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, 
             _two(0, log_decay.stride(0)) if log_decay.dim() == 1 else _two(*log_decay.stride()), _two(*out.stride()[:2]),
             float(scale), _lib.dtype_code(q.dtype), _lib.dtype_code(log_decay.dtype), _lib.stream_of(dev))
     _lib.check(st, "mm_decay_attention_step")
+    _lib.wrote(state if state_out is None else state_out)
+    _lib.wrote(given)
     return out

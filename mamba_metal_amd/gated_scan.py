@@ -268,6 +268,7 @@ def gated_scan_step(state: torch.Tensor, x: torch.Tensor, a_gate: torch.Tensor, 
     lib = _lib.load()
     if A.dtype != torch.float32 or not A.is_contiguous():
         A = A.float().contiguous()
+    given = out
     if out is None:
         out = x.new_empty((b, d))
     with _lib.on_device(dev):
@@ -277,4 +278,6 @@ def gated_scan_step(state: torch.Tensor, x: torch.Tensor, a_gate: torch.Tensor, 
             a_gate.stride(0), x_gate.stride(0), z.stride(0) if z is not None else 0, out.stride(0), code,
             _lib.stream_of(dev))
     _lib.check(st, "mm_gated_scan_step")
+    _lib.wrote(state if state_out is None else state_out)
+    _lib.wrote(given)
     return out
