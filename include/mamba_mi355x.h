@@ -445,7 +445,7 @@ int mm_gated_scan_fwd(const mm_gated_scan_params* p, void* stream);
  * The sums of dA are taken in a fixed order: calls repeat bit for bit. */
 int mm_gated_scan_bwd(const mm_gated_scan_params* p, void* stream);
 
-/* One token of the recurrence: state_out = a * state + sqrt(1 - a^2) * i * x (state_out may be state),
+/* One token of the recurrence: state_out = a * state + sqrt(1 - a^2) * i * x (state_out may be state, but not a part of it),
  * y = state_out * silu(z).  state, state_out (batch, dim) contiguous fp32; the others (batch, dim) in
  * dtype with batch strides and unit channel stride; z may be NULL. */
 int mm_gated_scan_step(const float* state, float* state_out, const void* x, const void* a_gate,
@@ -549,7 +549,7 @@ int mm_decay_attention_fwd(const mm_decay_attention_params* p, void* stream);
  * dh0 = exp(g_1) dS_1. */
 int mm_decay_attention_bwd(const mm_decay_attention_params* p, void* stream);
 
-/* One token: state_out = exp(g) state + k v^T (state_out may be state), y = scale * state_out^T q.  Strides of batch
+/* One token: state_out = exp(g) state + k v^T (state_out may be state, but not a part of it), y = scale * state_out^T q.  Strides of batch
  * and head in elements, unit channel stride; the states contiguous. */
 int mm_decay_attention_step(const float* state, float* state_out, const void* q, const void* k,
                             const void* v, const void* log_decay, void* y, int64_t batch,

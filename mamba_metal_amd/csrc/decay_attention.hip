@@ -376,6 +376,7 @@ int mm_decay_attention_step(const float* state, float* state_out, const void* q,
   for (const int64_t* s : all)
     if (s[0] < 0 || s[1] < 0) return fail(MM_ERR_LAYOUT, "negative stride");
   if (rows_overlap(batch, heads, value_dim, y_stride)) return fail(MM_ERR_LAYOUT, "rows of y overlap");
+  if (partly_same(state, state_out, batch * heads * key_dim * value_dim * 4)) return fail(MM_ERR_LAYOUT, "state_out overlaps state");
   Step p{};
   p.state = state;
   p.state_out = state_out;

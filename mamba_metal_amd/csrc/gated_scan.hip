@@ -819,6 +819,7 @@ int mm_gated_scan_step(const float* state, float* state_out, const void* x, cons
   if (x_stride_b < 0 || a_gate_stride_b < 0 || x_gate_stride_b < 0 || (z && z_stride_b < 0) || y_stride_b < 0)
     return fail(MM_ERR_LAYOUT, "negative stride");
   if (batch > 1 && y_stride_b < dim) return fail(MM_ERR_LAYOUT, "rows of y overlap");
+  if (partly_same(state, state_out, batch * dim * 4)) return fail(MM_ERR_LAYOUT, "state_out overlaps state");
   const dim3 grid(static_cast<unsigned>(ceil_div(dim, kStepThreads)), static_cast<unsigned>(batch));
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define MM_GS(D)                                                                                       \

@@ -47,6 +47,13 @@ inline bool rows_overlap(int64_t n0, int64_t n1, int64_t dim, const int64_t s[2]
   return false;
 }
 
+// Whether two pieces of memory of as many bytes share some but are not one: a kernel that reads the one and writes the other
+// has no order among its workgroups.
+inline bool partly_same(const void* a, const void* b, int64_t bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x != y && (x < y ? y - x : x - y) < static_cast<uintptr_t>(bytes);
+}
+
 // Per-device cache of a launch constant (CU count, resident workgroups per CU of one
 // kernel).  The value is computed on first use on each device and published with an
 // atomic store; racing threads compute and store the same value, so no lock is needed.
