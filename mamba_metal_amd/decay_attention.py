@@ -233,7 +233,7 @@ def decay_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, 
             raise TypeError(f"out is {out.dtype}, v {v.dtype}")
         channels_last(out, "out")
     if torch.is_grad_enabled() and (state.requires_grad or q.requires_grad or k.requires_grad or v.requires_grad
-                                    or log_decay.requires_grad):
+                                    or log_decay.requires_grad or any(t is not None and t.requires_grad for t in (state_out, out))):
         raise RuntimeError("decay_attention_step has no gradient: call it under no_grad or inference_mode, "
                            "or train through decay_attention")
     _lib.refuse_transforms("decay_attention_step", state, q, k, v, log_decay)

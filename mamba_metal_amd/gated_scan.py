@@ -260,7 +260,8 @@ def gated_scan_step(state: torch.Tensor, x: torch.Tensor, a_gate: torch.Tensor, 
     code = _lib.dtype_code(x.dtype)
     _check_rest(A, None, None, b, d)
     if torch.is_grad_enabled() and (state.requires_grad or x.requires_grad or a_gate.requires_grad
-                                    or x_gate.requires_grad or A.requires_grad or (z is not None and z.requires_grad)):
+                                    or x_gate.requires_grad or A.requires_grad
+                                    or any(t is not None and t.requires_grad for t in (z, state_out, out))):
         raise RuntimeError("gated_scan_step has no gradient: call it under no_grad or inference_mode, "
                            "or train through gated_scan")
     _lib.refuse_transforms("gated_scan_step", state, x, a_gate, x_gate, A, z)

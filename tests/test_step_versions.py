@@ -62,3 +62,14 @@ def test_inference_tensors(step, state, out):
     with torch.inference_mode():
         step(normal)
     assert normal._version == 1
+
+
+@pytest.mark.parametrize("step,state,out", STEPS, ids=["attention", "scan"])
+@pytest.mark.parametrize("name", ["state_out", "out"])
+def test_outputs_that_require_a_gradient(step, state, out, name):
+    """Refused while gradients are on, like the inputs: what is written there has none."""
+    t = torch.ones(out if name == "out" else state, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        step(torch.ones(state), **{name: t})
+    with torch.no_grad():
+        step(torch.ones(state), **{name: t})
