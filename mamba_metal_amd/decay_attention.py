@@ -9,6 +9,8 @@ token.  It stands beside ``selective_scan`` and ``gated_scan``, whose states bel
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -20,19 +22,39 @@ MAX_VALUE_DIM = 1024  # MM_DECAY_MAX_VALUE_DIM
 _two, _three = _lib._i64a2, _lib._i64a3
 
 
+# What a call's sizes and strides are to the library, whose conversions cost a microsecond and more each.
+@functools.lru_cache(maxsize=4096)
+def _strides(stride):
+    """The first three of a tensor's strides; of the decays of heads (1-d), the heads' alone."""
+    return _three(0, 0, *stride) if len(stride) == 1 else _three(*stride[:3])
+
+
+@functools.lru_cache(maxsize=4096)
+def _step_strides(stride):
+    """The same of the token step's: batch and head."""
+    return _two(0, *stride) if len(stride) == 1 else _two(*stride[:2])
+
+
+@functools.lru_cache(maxsize=1024)
+def _bytes(qk_shape, v_shape, dtype):
+    """Bytes of the states that are kept, and of the forward and the backward pass's workspaces."""
+    (b, n, groups, dk), (heads, dv), lib = qk_shape, v_shape[2:], _lib.load()
+    return (lib.mm_decay_attention_states_size(b, n, heads, dk, dv, dtype),
+            *(lib.mm_decay_attention_workspace_size(b, n, heads, groups, dk, dv, dtype, back) for back in (0, 1)))
+
+
 def _empty_like(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def _params(q, k, v, g, lengths, scale):
+def _params(q, k, v, g, lengths, scale, qk_shape, v_shape):
     p = _lib.DecayAttentionParams()
-    p.batch, p.seqlen, p.groups, p.key_dim = q.shape
-    p.heads, p.value_dim = v.shape[2:]
-    p.q, p.q_stride = q.data_ptr(), _three(*q.stride()[:3])
-    p.k, p.k_stride = k.data_ptr(), _three(*k.stride()[:3])
-    p.v, p.v_stride = v.data_ptr(), _three(*v.stride()[:3])
-    p.log_decay = g.data_ptr()
-    p.log_decay_stride = _three(0, 0, g.stride(0)) if g.dim() == 1 else _three(*g.stride())
+    p.batch, p.seqlen, p.groups, p.key_dim = qk_shape
+    p.heads, p.value_dim = v_shape[2:]
+    p.q, p.q_stride = q.data_ptr(), _strides(q.stride())
+    p.k, p.k_stride = k.data_ptr(), _strides(k.stride())
+    p.v, p.v_stride = v.data_ptr(), _strides(v.stride())
+    p.log_decay, p.log_decay_stride = g.data_ptr(), _strides(g.stride())
     if lengths is not None:
         p.lengths = lengths.data_ptr()
         p.lengths_dtype = 1 if lengths.dtype == torch.int64 else 0
@@ -41,38 +63,32 @@ def _params(q, k, v, g, lengths, scale):
     return p
 
 
-def _call(name, p, backward, dev):
-    lib = _lib.load()
-    nbytes = lib.mm_decay_attention_workspace_size(p.batch, p.seqlen, p.heads, p.groups, p.key_dim, p.value_dim, p.dtype,
-                                                   backward)
+def _call(name, p, nbytes, dev):
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
     with _lib.on_device(dev):
-        st = getattr(lib, name)(p, _lib.stream_of(dev))
+        st = getattr(_lib.load(), name)(p, _lib.stream_of(dev))
     _lib.check(st, name)
-
-
-def _states_bytes(q, v):
-    return _lib.load().mm_decay_attention_states_size(q.shape[0], q.shape[1], v.shape[2], q.shape[3], v.shape[3],
-                                                      _lib.dtype_code(q.dtype))
 
 
 def _forward(dev, q, k, v, g, h0, lengths, scale, want_state, train):
     """y, the final state (or None) and, for training, the states before each run of tokens."""
-    p = _params(q, k, v, g, lengths, scale)
+    qk_shape, v_shape = q.shape, v.shape
+    p = _params(q, k, v, g, lengths, scale, qk_shape, v_shape)
+    states_bytes, workspace, _ = _bytes(qk_shape, v_shape, p.dtype)
     y = _empty_like(v)
     p.y = y.data_ptr()
     state = states = None
     if h0 is not None:
         p.h0 = h0.data_ptr()
     if want_state:
-        state = torch.empty((q.shape[0], v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=dev)
+        state = torch.empty((v_shape[0], v_shape[2], qk_shape[3], v_shape[3]), dtype=torch.float32, device=dev)
         p.state_out = state.data_ptr()
     if train:
-        states = torch.empty(_states_bytes(q, v), dtype=torch.uint8, device=dev)
+        states = torch.empty(states_bytes, dtype=torch.uint8, device=dev)
         p.run_states = states.data_ptr() or None
-    _call("mm_decay_attention_fwd", p, 0, dev)
+    _call("mm_decay_attention_fwd", p, workspace, dev)
     return y, state, states
 
 
@@ -95,13 +111,13 @@ class _DecayAttention(torch.autograd.Function):
         # (A leaf's memory, type and size may be others than in the forward pass: its data replaced, its storage freed and
         # allocated again.)
         q, k, v, g, lengths, states = _checked(ctx.saved_tensors, dev, dtype, qk_shape, v_shape, g_dtype, g_shape, *lengths_dtype)
-        p = _params(q, k, v, g, lengths, scale)
+        p = _params(q, k, v, g, lengths, scale, qk_shape, v_shape)
         p.run_states = states.data_ptr() or None
         if dy is None:  # only the final state was used
             dy = torch.zeros((1, 1, 1, v_shape[3]), dtype=dtype, device=dev).expand(v_shape)
         elif dy.dtype != dtype or (dy.stride(-1) != 1 and v_shape[3] > 1):
             dy = dy.to(dtype).contiguous()
-        p.dy, p.dy_stride = dy.data_ptr(), _three(*dy.stride()[:3])
+        p.dy, p.dy_stride = dy.data_ptr(), _strides(dy.stride())
         if dstate is not None:
             dstate = dstate.contiguous()
             p.dstate = dstate.data_ptr()
@@ -117,7 +133,7 @@ class _DecayAttention(torch.autograd.Function):
         if ctx.needs_input_grad[5]:
             dh0 = torch.empty((v_shape[0], v_shape[2], qk_shape[3], v_shape[3]), dtype=torch.float32, device=dev)
             p.dh0 = dh0.data_ptr()
-        _call("mm_decay_attention_bwd", p, 1, dev)
+        _call("mm_decay_attention_bwd", p, _bytes(qk_shape, v_shape, p.dtype)[2], dev)
         return None, dq, dk, dv, None if dg is None else dg.to(g_dtype), dh0, None, None, None
 
 
@@ -129,7 +145,8 @@ def _checked(saved, dev, dtype, qk_shape, v_shape, g_dtype, g_shape, lengths_dty
     q, k = (_lib.saved(t, dtype, qk_shape, dev, rows=True) for t in (q, k))
     v = _lib.saved(v, dtype, v_shape, dev, rows=True)
     g = _lib.saved(g, g_dtype, g_shape, dev, strided=True)
-    return q, k, v, g, lengths, _lib.saved(states, torch.uint8, (_states_bytes(q, v),), dev)
+    nbytes = _bytes(qk_shape, v_shape, _lib.dtype_code(dtype))[0]
+    return q, k, v, g, lengths, _lib.saved(states, torch.uint8, (nbytes,), dev)
 
 
 def _check(q, k, v, g, lead, names):
@@ -245,9 +262,8 @@ def decay_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, 
     with _lib.on_device(dev):
         st = lib.mm_decay_attention_step(
             state.data_ptr(), state.data_ptr() if state_out is None else state_out.data_ptr(), q.data_ptr(), k.data_ptr(),
-            v.data_ptr(), log_decay.data_ptr(), out.data_ptr(), b, heads, groups, dk, dv, _two(*q.stride()[:2]),
-            _two(*k.stride()[:2]), _two(*v.stride()[:2]),
-            _two(0, log_decay.stride(0)) if log_decay.dim() == 1 else _two(*log_decay.stride()), _two(*out.stride()[:2]),
+            v.data_ptr(), log_decay.data_ptr(), out.data_ptr(), b, heads, groups, dk, dv, _step_strides(q.stride()),
+            _step_strides(k.stride()), _step_strides(v.stride()), _step_strides(log_decay.stride()), _step_strides(out.stride()),
             float(scale), _lib.dtype_code(q.dtype), _lib.dtype_code(log_decay.dtype), _lib.stream_of(dev))
     _lib.check(st, "mm_decay_attention_step")
     _lib.wrote(state if state_out is None else state_out)
