@@ -507,6 +507,7 @@ int mm_causal_conv1d_fwd_act8(const void* x, const void* weight, const void* bia
  * and their inputs do not matter.  key_dim <= 128, value_dim <= 1024.  Sums and states are fp32; 16-bit types round
  * the scores of a run of 64 tokens and the state that meets q, each once, to dtype before their products (in calls of up
  * to 32768 tokens, batch * seqlen * heads, the scores to the sum of two, and so the states in gradients of q, k and g).
+ * fp16: a token's scores and a run's states go through powers of two; scale * dy has to stay below 65504.
  *
  * Training: the forward call given run_states (mm_decay_attention_states_size bytes, 256-byte aligned) writes there, in
  * dtype, the states that the backward call reads.  Sums are taken in a fixed order: calls repeat bit for bit. */

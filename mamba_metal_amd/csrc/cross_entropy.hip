@@ -7,9 +7,10 @@
 // again, and the epilogue turns them into dl in the inputs' type (its one rounding); the piece is then multiplied with W
 // (adding to dx, in fp32) and with x (its rows of dW).  The four products are the time; everything else is 3%.
 // A product's tile has the vocabulary along the accumulators' rows, so that the softmax's sums run within a lane.
-// bf16, 8192 rows (7377 counted) of 2560 by 50280 tokens: 1.72 ms forward; backward in two pieces, each 0.92 ms for dl and
-// 1.93 ms for dx and dW (0.98 PFLOP/s); 7.2 ms in all, where three library products of whole matrices would take 5.3 and
-// logits of 0.8 GB.  fp32, 999 (894) of 1001 by 10007: 198 us, 202 and 384, and 20 to lay the odd rows out.
+// bf16, 8192 rows (7377 counted) of 2560 by 50280 tokens, in a kernel trace: 1.73 ms forward; backward in two pieces, each 0.92 ms
+// for dl and 1.93 to 1.96 ms for dx and dW (0.98 PFLOP/s), and 0.11 for all else: 7.6 ms.  Untraced the pass takes 7.1 to 7.3,
+// where three library products of whole matrices would take 5.3 and logits of 0.8 GB.  fp32, 999 (894) of 1001 by 10007, in a
+// trace: 195 us, 209 and 381, and 20 a pass to lay the odd rows out; 716 us untraced.
 //
 // Rows that are ignored take no part: the others are gathered first (their sums over rows are then never touched by what
 // an ignored row holds, and a batch that is mostly ignored costs its share), and workgroups past their count end at once.

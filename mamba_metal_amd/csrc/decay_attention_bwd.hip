@@ -13,7 +13,7 @@
 // roles exchanged (own rows dy, others v, state S, sum over k; or own rows v, others dy, state dS, sum over q).
 // What a head needs, 48 KB with key_dim 128 in 16 bits, is loaded straight into shared memory while the head before is
 // computed (two buffers, one barrier a head); fp32, whose buffers would not fit twice, and rows off 16 bytes go through
-// registers instead.  8 sequences of 2048 tokens of 80 heads in bf16: 1.0 GB in 310 to 330 us, 3.2 TB/s; a head takes 4 us of a
+// registers instead.  8 sequences of 2048 tokens of 80 heads in bf16: 1.0 GB in 308 us, 3.3 TB/s; a head takes 4 us of a
 // compute unit, of which its loads are 2.4 (reads that waited for the loads under way: 420 us).
 #include <type_traits>
 

@@ -17,8 +17,9 @@
 // A run is a chain (shared memory, scores, outputs, state) of which a workgroup's own instructions take less than half: it
 // is hidden by other workgroups, so that registers and shared memory are held to what lets three share a compute unit in 16
 // bits (q goes straight from memory to operands, addresses are made anew in every run).  bf16, 80 heads of 128 by 64 and one
-// q and k: 8192 tokens of one sequence take 53 us for what the segments add, 8 to join them and 98 for the outputs; 8
-// sequences of 2048 tokens 280 us (0.7 GB with the states that are kept, 2.4 TB/s), mirrored 375 us (1.0 GB, 2.7 TB/s).  Two
+// q and k, in a kernel trace: 8192 tokens of one sequence take 52 us for what the segments add, 8 to join them and 98 to 103 for
+// the outputs; 8 sequences of 2048 tokens 280 to 290 us (0.7 GB with the states that are kept, 2.4 TB/s), mirrored 375 to 384 us
+// (1.0 GB, 2.7 TB/s).  (Traced, kernels stand alone: with the gradients' 308 these are 970, and the pass takes 900.)  Two
 // workgroups a unit: 339 and 498 us.
 #pragma once
 

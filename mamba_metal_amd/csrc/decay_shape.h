@@ -14,7 +14,15 @@ constexpr int kVBlock = 64; // value channels a workgroup
 constexpr int kMaxDk = 128;
 constexpr int64_t kMaxBatch = 65535, kMaxHeads = 65535, kMaxDv = 1024, kMaxTokens = int64_t{1} << 30;
 
-// Whether the scores of 16-bit types take a second term (decay_tiles.h, score_operand).
+// Whether a call of 16-bit types is `fine`: its scores take a second term (decay_tiles.h, score_operand), and the states that
+// gradients of q, k and the decays read the rests of their roundings.  It costs little where launches and few workgroups are most
+// of the time, and much where the work is.  16 to 32 heads of 128 by 64 that share q and k, bf16 (fp16), a forward and backward
+// pass in us, as it is here and the other way:
+//   tokens x heads      8192         16384        32768          65536          262144
+//   fine                83 (87)      85 (91)      122 (142)      167 (199)      508 (654)
+//   not                 78 (84)      77 (83)      97 (102)       117 (127)      241 (287)
+// (32768 of 32 heads with a q and k each: 109 (112), and 96 (96).)  Off by, in roundings of the output: dq and dk 1.0 and 1.41, the
+// decays' gradient 1.0 and 1.3 to 1.5, y and dv 1.22 to 1.27 and 1.41, at every one of the sizes.
 inline bool fine_scores(int64_t batch, int64_t seqlen, int64_t heads, int32_t dtype) {
   return dtype != MM_F32 && batch * seqlen * heads <= 32768;
 }

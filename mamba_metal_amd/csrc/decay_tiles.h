@@ -113,7 +113,8 @@ __device__ __forceinline__ void split_operand(const float (&x)[8], u32x4 (&out)[
 
 // Scores (accumulator tiles, in acc order) as operands, rounded once.  A score's rounding is the same in all channels of its
 // token, so that few tokens may all be off by nearly half a step where many are by a third: `fine` ones, of calls of few
-// tokens, take a second term, the rest.  (Of many it would take 4% of a pass.)
+// tokens, take a second term, the rest.  (Forward pass of 32 heads of 128 by 64 in bf16 (fp16), 65536 tokens x heads: 41.1 us
+// and 42.0 with it (42.7 and 43.7); 262144: 70 and 75 (78 and 87).)
 template <int DT>
 __device__ __forceinline__ void score_operand(const f32x4* t, bool fine, u32x4& whole, u32x4& rest) {
   whole = from_acc<DT>(t);

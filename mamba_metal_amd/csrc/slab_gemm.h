@@ -358,7 +358,6 @@ __device__ __forceinline__ void clear(f32x16 (&acc)[S::TM][S::TN]) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 }
-__device__ __forceinline__ int acc_row(int r, int lane) { return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
 
 // Workgroup `id` of `total` to a tile of mt x nt: each die (workgroup ids go round the 8) takes a contiguous share, in
 // bands of 8 rows of tiles, so that what runs there at once shares its operands in the die's cache.

@@ -192,10 +192,11 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
 
     With 16-bit inputs the scores of a run of 64 tokens and the state that meets q are rounded to 16 bits, once each,
     before their products, and so are their gradients; the state itself is not, nor are, in calls of up to 32768 tokens
-    (batch * seqlen * heads), the scores and the states in gradients of q, k and log_decay.  The gradient of a float32 log_decay
-    beside 16-bit q, k and v is therefore as exact as theirs.  In float16 scale * dy has to
-    stay below 65504; a token's scores go through a power of two and may be any numbers.  A NaN or an infinity stays in its sequence and head (in its group, for the gradients
-    of q and k); one in k or v may also reach the up to 63 tokens before it in its run of 64.
+    (batch * seqlen * heads), the scores and the states in gradients of q, k and log_decay.  The gradient of a float32
+    log_decay beside 16-bit q, k and v is therefore as exact as theirs; a sequence's last bits may change with how many
+    share its batch.  In float16 scale * dy has to stay below 65504; a token's scores go through a power of two and may be
+    any numbers.  A NaN or an infinity stays in its sequence and head (in its group, for the gradients of q and k); one in
+    k or v may also reach the up to 63 tokens before it in its run of 64.
 
     Gradients flow to q, k, v, log_decay and h0 (once, not twice, and not in forward mode).  For them a call that needs
     any keeps its inputs and, in their dtype, the state before every 64th token.
