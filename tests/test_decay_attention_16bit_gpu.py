@@ -156,3 +156,24 @@ def test_gradients_of_few_tokens_are_rounded_once(dev, dt, shape):
     for name, at in (("dq", 0), ("dk", 1), ("dg", 3)):
         rounding = (want[at].to(dt).double() - want[at]).norm()
         assert float((grads[at].double() - want[at]).norm() / rounding) < 1.05, name
+
+
+@pytest.mark.parametrize("b,per", [(3, 2), (3, 80)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_is_broken_stays_in_its_head(dev, b, per, bad):
+    """A NaN or an infinity in float16, whose powers of two are taken over many numbers: other sequences, and other heads (for dq
+    and dk other groups), are the same bits."""
+    s = inputs(dev, F16, b, 200, 2, per, 64, 72, h0=True, g_dtype=F32)
+    base, clean = run(s, 1.0)
+    for name, at in (("q", (1, 100, 1)), ("k", (1, 100, 1)), ("v", (1, 100, 2 * per - 1)), ("dy", (1, 100, 2 * per - 1))):
+        t = {**s, name: s[name].clone()}
+        t[name][at] = bad
+        outs, grads = run(t, 1.0)
+        heads = slice(0, per) if name in ("q", "k") else slice(0, 2 * per - 1)
+        for a, c in zip([*outs, grads[2], grads[3], grads[4]], [*base, clean[2], clean[3], clean[4]]):
+            at_heads = (slice(None), heads) if a.shape[1] == 2 * per else (slice(None), slice(None), heads)
+            assert torch.equal(a[0::2], c[0::2]) and torch.equal(a[at_heads], c[at_heads]), name
+        for a, c in zip(grads[:2], clean[:2]):
+            assert torch.equal(a[0::2], c[0::2]) and torch.equal(a[:, :, 0], c[:, :, 0]), name
+        of = grads[0 if name == "k" else 1]  # (dk = dS v holds no k)
+        assert bool(of[1, :, 1].isfinite().logical_not().any()), name
